@@ -124,20 +124,28 @@ def build_torch_binding(verbose: bool = True) -> Path:
     from torch.utils import cpp_extension
 
     library = build_library(verbose)
-    source = PACKAGE / "torch" / "csrc" / "flash_train_torch.cpp"
+    folder = PACKAGE / "torch" / "csrc"
+    sources = sorted(folder.glob("*.cpp"))
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     target = PACKAGE / "torch" / ("_flash_train_torch" + suffix)
-    if not _stale(target, [source, library], _newest_header()):
+    headers = max([_newest_header(), *(p.stat().st_mtime for p in folder.glob("*.hpp"))])
+    if not _stale(target, [*sources, library], headers):
         return target
     torch_lib = Path(torch.__file__).resolve().parent / "lib"
     includes = [f"-I{p}" for p in cpp_extension.include_paths()]
     includes += [f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}", f"-I{CUDA_HOME / 'include'}"]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
-          "-DTORCH_EXTENSION_NAME=_flash_train_torch", "-DTORCH_API_INCLUDE_EXTENSION_H",
-          f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *includes, str(source), "-o", str(target),
-          f"-L{PACKAGE}", "-lflash_train", f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10",
-          "-lc10_cuda", "-Wl,-rpath,$ORIGIN/..", f"-Wl,-rpath,{torch_lib}"])
+    flags = ["-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_flash_train_torch",
+             "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *includes]
+    objects, jobs = [], []
+    for source in sources:
+        objects.append(OBJ / f"torch__{source.name}.o")
+        if _stale(objects[-1], [source], headers):
+            jobs.append(["g++", *flags, "-c", str(source), "-o", str(objects[-1])])
+    with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as pool:
+        list(pool.map(_run, jobs))
+    _run(["g++", "-shared", *map(str, objects), "-o", str(target), f"-L{PACKAGE}", "-lflash_train", f"-L{torch_lib}", "-ltorch",
+          "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN/..", f"-Wl,-rpath,{torch_lib}"])
     if verbose:
         print(f"[build] built {target.relative_to(REPO)}", flush=True)
     return target

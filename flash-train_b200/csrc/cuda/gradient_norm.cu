@@ -1,0 +1,523 @@
+// The norm over many gradients and their clipping (ftcuda/training.h).
+//
+//   n = (sum of all x^2)^(1/2)  or  max |x|,     out = x * min(1, max_norm / (n + 1e-6))
+//
+// Two passes over the gradients, since the factor depends on every element: the first reads them, the second
+// reads and writes them. Both are bound by HBM. A pass is one launch for up to kTensors tensors, whose
+// table travels in the kernel's parameters (no copy to the device, so that a captured graph holds it). The tensors are cut into
+// chunks of kChunk elements, and every CTA takes a contiguous run of about as many chunks as any other, whatever tensors they are
+// of: one of a thousand small tensors costs what its bytes cost. Runs instead of single chunks spare the search for a chunk's tensor.
+// The second pass walks every run backwards, as what the first pass read last is still in L2.
+//
+// The first pass leaves one partial sum for each CTA; every CTA of the second adds them all up again, always in the same order, rather
+// than wait for one that does it (a few thousand bytes out of L2), so two launches are all that a clip takes.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <new>
+#include <vector>
+
+#include "ptx.cuh"
+#include "training_common.cuh"
+
+namespace ftcuda {
+namespace {
+
+using training::Element;
+
+constexpr int kThreads            = 256;
+constexpr int kSumCtasPerSm       = 8;
+constexpr int kScaleCtasPerSm     = 4;  // what a thread holds between its loads and its stores takes twice the registers
+constexpr std::uint32_t kChunk    = 16 * kThreads;  // elements: 16 a thread, 64 bytes of FP32 in flight
+constexpr std::uint32_t kTensors  = 480;            // of one launch: 30 KiB of the nearly 32 that a kernel's parameters may take
+constexpr std::uint32_t kFew      = 64;             // ... of the launch for few tensors, whose parameters are quicker to hand over
+constexpr std::uint64_t kMaxGrid  = 2048;           // CTAs of one launch at most (and room for their sums)
+
+struct Entry {
+    const void* data;
+    void* out;
+    std::uint64_t rows, cols;
+    std::int64_t row_stride, out_row_stride;
+    std::uint64_t first;  // chunks of the tensors before
+    std::int32_t element, out_element;
+};
+
+template<std::uint32_t kCapacity> struct Table {
+    Entry entries[kCapacity];
+    std::uint64_t chunks;
+    std::uint32_t count;
+};
+
+// Largest and smallest sum of squares that FP32 holds as well as 64 bits would: with a sum of up to 16 squares in here, none overflowed, and what
+// underflowed in one (2^-150) is under 2^-60 of the sum.
+constexpr float kLargestSum  = 0x1p+120F;
+constexpr float kSmallestSum = 0x1p-90F;
+
+struct Sum2 {
+    double total = 0.0;
+    // n <= 16 neighbouring elements.
+    template<int n> __device__ __forceinline__ void add(const float (&x)[n]) {
+        float sum = 0.0F;
+#pragma unroll
+        for (int i = 0; i < n; ++i) { sum = fmaf(x[i], x[i], sum); }
+        if (sum >= kSmallestSum && sum <= kLargestSum) {
+            total += static_cast<double>(sum);
+        } else {
+#pragma unroll
+            for (int i = 0; i < n; ++i) { total = fma(static_cast<double>(x[i]), static_cast<double>(x[i]), total); }
+        }
+    }
+    __device__ __forceinline__ void join(double other) { total += other; }
+    __device__ __forceinline__ double norm() const { return sqrt(total); }
+};
+
+// |x| as a whole number orders the finite numbers, the infinities above them and NaN above all.
+struct SumInf {
+    double total = 0.0;  // of magnitudes that are FP32 numbers: exact
+    template<int n> __device__ __forceinline__ void add(const float (&x)[n]) {
+        std::uint32_t largest = 0;
+#pragma unroll
+        for (int i = 0; i < n; ++i) { largest = max(largest, __float_as_uint(x[i]) & 0x7FFFFFFFU); }
+        join(static_cast<double>(__uint_as_float(largest)));
+    }
+    __device__ __forceinline__ void join(double other) { total = other > total || other != other ? other : total; }
+    __device__ __forceinline__ double norm() const { return total; }
+};
+
+template<typename T, int n> struct alignas(sizeof(T) * n) Pack {
+    T at[n];
+};
+
+// Elements [begin, end) of a row for all threads of the CTA, `begin` and `end` the same in all: body(index, count-n pack).
+// Whole 16-byte vectors where the address allows it, the ends one by one.
+template<typename T, typename Sum> __device__ __forceinline__ void sumRow(const T* row, std::uint32_t count, Sum& sum) {
+    constexpr std::uint32_t kVector = 16 / sizeof(T);
+    constexpr int kVectors          = kChunk / kVector / kThreads;
+    const std::uint32_t head        = min(count, static_cast<std::uint32_t>((16 - (reinterpret_cast<std::uintptr_t>(row) & 15)) & 15) / static_cast<std::uint32_t>(sizeof(T)));
+    const std::uint32_t vectors     = (count - head) / kVector;
+    const auto* body                = reinterpret_cast<const Pack<T, kVector>*>(row + head);
+    Pack<T, kVector> packs[kVectors];
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+        const std::uint32_t at = threadIdx.x + i * kThreads;
+        if (at < vectors) {
+            packs[i] = body[at];
+        } else {
+#pragma unroll
+            for (std::uint32_t j = 0; j < kVector; ++j) { packs[i].at[j] = Element<T>::narrow(0.0F); }
+        }
+    }
+    // The ends: fewer than kVector elements on either side.
+    const std::uint32_t rest = head + vectors * kVector;
+    const std::uint32_t ends = head + (count - rest);
+    if (threadIdx.x < ends) {
+        const std::uint32_t at = threadIdx.x < head ? threadIdx.x : rest + (threadIdx.x - head);
+        const float x[1]       = {Element<T>::widen(row[at])};
+        sum.add(x);
+    }
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+        float x[kVector];
+#pragma unroll
+        for (std::uint32_t j = 0; j < kVector; ++j) { x[j] = Element<T>::widen(packs[i].at[j]); }
+        if (threadIdx.x + i * kThreads < vectors) { sum.add(x); }
+    }
+}
+
+// n neighbouring elements, 16 bytes at a time on either side.
+template<typename T, int n> __device__ __forceinline__ void loadVector(const T* from, T (&x)[n]) {
+    constexpr int kEach = 16 / sizeof(T) < n ? 16 / sizeof(T) : n;
+#pragma unroll
+    for (int i = 0; i < n; i += kEach) { *reinterpret_cast<Pack<T, kEach>*>(x + i) = *reinterpret_cast<const Pack<T, kEach>*>(from + i); }
+}
+template<typename T, typename U, int n> __device__ __forceinline__ void storeScaled(U* to, const T (&x)[n], float factor) {
+    constexpr int kEach = 16 / sizeof(U) < n ? 16 / sizeof(U) : n;
+#pragma unroll
+    for (int i = 0; i < n; i += kEach) {
+        Pack<U, kEach> o;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) { o.at[j] = Element<U>::narrow(Element<T>::widen(x[i + j]) * factor); }
+        *reinterpret_cast<Pack<U, kEach>*>(to + i) = o;
+    }
+}
+
+template<typename T, typename U>
+__device__ __forceinline__ void scaleRow(const T* row, U* out, std::uint32_t count, float factor) {
+    constexpr std::uint32_t kVector = 16 / (sizeof(T) < sizeof(U) ? sizeof(T) : sizeof(U));
+    constexpr int kVectors          = kChunk / kVector / kThreads;
+    const std::uint32_t head        = min(count, static_cast<std::uint32_t>((16 - (reinterpret_cast<std::uintptr_t>(row) & 15)) & 15) / static_cast<std::uint32_t>(sizeof(T)));
+    // Vectors where both sides are aligned at the same element; then all of a warp's 16-byte pieces are neighbours on both sides.
+    if ((reinterpret_cast<std::uintptr_t>(out + head) & 15) == 0) {
+        const T* const from         = row + head;
+        U* const to                 = out + head;
+        const std::uint32_t vectors = (count - head) / kVector;
+        if (vectors == kVectors * kThreads) {
+            // A whole chunk: everything is asked for before anything is written.
+            alignas(16) T x[kVectors][kVector];
+#pragma unroll
+            for (int i = 0; i < kVectors; ++i) { loadVector(from + (threadIdx.x + i * kThreads) * kVector, x[i]); }
+#pragma unroll
+            for (int i = 0; i < kVectors; ++i) { storeScaled(to + (threadIdx.x + i * kThreads) * kVector, x[i], factor); }
+        } else {
+#pragma unroll 1
+            for (std::uint32_t at = threadIdx.x; at < vectors; at += kThreads) {
+                alignas(16) T x[kVector];
+                loadVector(from + at * kVector, x);
+                storeScaled(to + at * kVector, x, factor);
+            }
+        }
+        const std::uint32_t rest = head + vectors * kVector;
+        const std::uint32_t ends = head + (count - rest);
+        if (threadIdx.x < ends) {
+            const std::uint32_t at = threadIdx.x < head ? threadIdx.x : rest + (threadIdx.x - head);
+            out[at]                = Element<U>::narrow(Element<T>::widen(row[at]) * factor);
+        }
+        return;
+    }
+    if (count == kChunk) {
+        T x[kChunk / kThreads];
+#pragma unroll
+        for (std::uint32_t i = 0; i < kChunk / kThreads; ++i) { x[i] = row[threadIdx.x + i * kThreads]; }
+#pragma unroll
+        for (std::uint32_t i = 0; i < kChunk / kThreads; ++i) { out[threadIdx.x + i * kThreads] = Element<U>::narrow(Element<T>::widen(x[i]) * factor); }
+    } else {
+#pragma unroll 4
+        for (std::uint32_t at = threadIdx.x; at < count; at += kThreads) { out[at] = Element<U>::narrow(Element<T>::widen(row[at]) * factor); }
+    }
+}
+
+// The tensor that chunk `chunk` is of.
+template<std::uint32_t kCapacity>
+__device__ __forceinline__ std::uint32_t findEntry(const Table<kCapacity>& table, std::uint64_t chunk) {
+    std::uint32_t low = 0, high = table.count;  // entries[low].first <= chunk < entries[high].first
+    while (high - low > 1) {
+        const std::uint32_t middle = (low + high) / 2;
+        if (table.entries[middle].first <= chunk) {
+            low = middle;
+        } else {
+            high = middle;
+        }
+    }
+    return low;
+}
+
+struct Piece {
+    std::uint64_t row, col;
+    std::uint32_t count;
+};
+
+__device__ __forceinline__ Piece pieceOf(const Entry& entry, std::uint64_t chunk) {
+    const std::uint64_t local = chunk - entry.first;
+    Piece piece;
+    if (entry.rows == 1) {
+        piece.row = 0;
+        piece.col = local * kChunk;
+    } else {
+        const std::uint64_t per_row = (entry.cols + kChunk - 1) / kChunk;
+        piece.row                   = local / per_row;
+        piece.col                   = (local - piece.row * per_row) * kChunk;
+    }
+    piece.count = static_cast<std::uint32_t>(min(static_cast<std::uint64_t>(kChunk), entry.cols - piece.col));
+    return piece;
+}
+
+// Joined over the CTA, the same order in every call; the result in thread 0.
+template<typename Sum> __device__ __forceinline__ void joinBlock(Sum& sum, double* shared) {
+#pragma unroll
+    for (int offset = 16; offset > 0; offset /= 2) { sum.join(__shfl_down_sync(0xFFFFFFFFU, sum.total, offset)); }
+    if ((threadIdx.x & 31) == 0) { shared[threadIdx.x >> 5] = sum.total; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int warp = 1; warp < kThreads / 32; ++warp) { sum.join(shared[warp]); }
+    }
+}
+
+template<typename Sum, std::uint32_t kCapacity>
+__global__ void __launch_bounds__(kThreads, kSumCtasPerSm) gradientSums(const __grid_constant__ Table<kCapacity> table, double* partials) {
+    __shared__ double shared[kThreads / 32];
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const std::uint64_t begin = table.chunks * blockIdx.x / gridDim.x, end = table.chunks * (blockIdx.x + 1) / gridDim.x;
+    Sum sum;
+    if (begin < end) {
+        std::uint32_t index = findEntry(table, begin);
+#pragma unroll 1
+        for (std::uint64_t chunk = begin; chunk < end; ++chunk) {
+            while (index + 1 < table.count && table.entries[index + 1].first <= chunk) { ++index; }
+            const Entry& entry          = table.entries[index];
+            const Piece piece           = pieceOf(entry, chunk);
+            const std::int64_t offset   = static_cast<std::int64_t>(piece.row) * entry.row_stride + static_cast<std::int64_t>(piece.col);
+            switch (entry.element) {
+                case FTCUDA_ELEMENT_FP32: sumRow(static_cast<const float*>(entry.data) + offset, piece.count, sum); break;
+                case FTCUDA_ELEMENT_FP16: sumRow(static_cast<const __half*>(entry.data) + offset, piece.count, sum); break;
+                default: sumRow(static_cast<const __nv_bfloat16*>(entry.data) + offset, piece.count, sum); break;
+            }
+        }
+    }
+    joinBlock(sum, shared);
+    if (threadIdx.x == 0) { partials[blockIdx.x] = sum.total; }
+}
+
+// All partial sums joined; every CTA and every launch comes to the same number.
+template<typename Sum> __device__ __forceinline__ double joinPartials(const double* partials, std::uint32_t count, double* shared) {
+    Sum sum;
+    for (std::uint32_t at = threadIdx.x; at < count; at += kThreads) { sum.join(__ldcg(partials + at)); }
+    joinBlock(sum, shared);
+    return sum.norm();
+}
+
+template<typename Sum> __global__ void __launch_bounds__(kThreads) gradientNorm(const double* partials, std::uint32_t count, float* norm) {
+    __shared__ double shared[kThreads / 32];
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const double total = joinPartials<Sum>(partials, count, shared);
+    if (threadIdx.x == 0) { *norm = static_cast<float>(total); }
+}
+
+template<typename T> __device__ __forceinline__ void scalePiece(const Entry& entry, const Piece& piece, float factor) {
+    const T* const row          = static_cast<const T*>(entry.data) + static_cast<std::int64_t>(piece.row) * entry.row_stride + static_cast<std::int64_t>(piece.col);
+    const std::int64_t offset   = static_cast<std::int64_t>(piece.row) * entry.out_row_stride + static_cast<std::int64_t>(piece.col);
+    switch (entry.out_element) {
+        case FTCUDA_ELEMENT_FP32: scaleRow(row, static_cast<float*>(entry.out) + offset, piece.count, factor); break;
+        case FTCUDA_ELEMENT_FP16: scaleRow(row, static_cast<__half*>(entry.out) + offset, piece.count, factor); break;
+        default: scaleRow(row, static_cast<__nv_bfloat16*>(entry.out) + offset, piece.count, factor); break;
+    }
+}
+
+template<typename Sum, std::uint32_t kCapacity>
+__global__ void __launch_bounds__(kThreads, kScaleCtasPerSm) gradientScale(const __grid_constant__ Table<kCapacity> table, const double* partials, std::uint32_t count,
+                                                          double max_norm, float* norm) {
+    __shared__ double shared[kThreads / 32];
+    __shared__ float shared_factor;
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const double total = joinPartials<Sum>(partials, count, shared);
+    if (threadIdx.x == 0) {
+        const double ratio = max_norm / (total + 1e-6);
+        shared_factor      = ratio >= 1.0 ? 1.0F : static_cast<float>(ratio);  // a ratio that is not a number stays one
+        if (norm != nullptr && blockIdx.x == 0) { *norm = static_cast<float>(total); }
+    }
+    __syncthreads();
+    const float factor        = shared_factor;
+    const std::uint64_t begin = table.chunks * blockIdx.x / gridDim.x, end = table.chunks * (blockIdx.x + 1) / gridDim.x;
+    if (begin == end) { return; }
+    std::uint32_t index = findEntry(table, end - 1);
+#pragma unroll 1
+    for (std::uint64_t chunk = end; chunk-- > begin;) {
+        while (table.entries[index].first > chunk) { --index; }
+        const Entry& entry = table.entries[index];
+        if (factor == 1.0F && entry.out == entry.data) { continue; }
+        const Piece piece = pieceOf(entry, chunk);
+        switch (entry.element) {
+            case FTCUDA_ELEMENT_FP32: scalePiece<float>(entry, piece, factor); break;
+            case FTCUDA_ELEMENT_FP16: scalePiece<__half>(entry, piece, factor); break;
+            default: scalePiece<__nv_bfloat16>(entry, piece, factor); break;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+std::uint64_t launchesFor(std::uint64_t count) { return count <= kFew ? 1 : ceilDiv(count, kTensors); }
+
+// nullptr, or what is wrong with a gradient (`out` looked at for a clip alone).
+const char* checkGradient(const FtcudaGradient& g, bool clip) {
+    if (g.rows == 0 || g.cols == 0) { return nullptr; }
+    const std::uint64_t bytes = training::elementBytes(g.element);
+    if (bytes == 0) { return "the element type is none of FP32, FP16 and BF16"; }
+    if (g.data == nullptr) { return "no address"; }
+    if (!training::aligned(g.data, bytes)) { return "the address is not a multiple of the element's size"; }
+    if (g.rows >= (1ULL << 40) || g.cols >= (1ULL << 40)) { return "an extent is too large"; }
+    if (g.rows > 1 && (g.row_stride < static_cast<std::int64_t>(g.cols) || g.row_stride >= (1LL << 40))) { return "rows overlap, or lie too far apart"; }
+    if (g.rows > (1ULL << 44) / (g.rows > 1 ? static_cast<std::uint64_t>(g.row_stride) : g.cols)) { return "too many elements, or too far apart"; }
+    if (!clip) { return nullptr; }
+    const std::uint64_t out_bytes = training::elementBytes(g.out_element);
+    if (out_bytes == 0) { return "the output's element type is none of FP32, FP16 and BF16"; }
+    if (g.out == nullptr) { return "no address for the output"; }
+    if (!training::aligned(g.out, out_bytes)) { return "the output's address is not a multiple of its element's size"; }
+    if (g.rows > 1 && (g.out_row_stride < static_cast<std::int64_t>(g.cols) || g.out_row_stride >= (1LL << 40))) { return "the output's rows overlap, or lie too far apart"; }
+    if (g.rows > 1 && g.rows > (1ULL << 44) / static_cast<std::uint64_t>(g.out_row_stride)) { return "the output's rows lie too far apart"; }
+    return nullptr;
+}
+
+// Memory of one operand: `rows` windows of `width` bytes, `stride` bytes apart.
+struct Range {
+    std::uint64_t begin, end, width, stride;
+    std::uint64_t owner;
+    bool written;
+};
+
+Range rangeOf(const void* address, std::uint64_t rows, std::uint64_t cols, std::int64_t row_stride, std::uint64_t bytes, std::uint64_t owner, bool written) {
+    Range r;
+    r.begin   = reinterpret_cast<std::uintptr_t>(address);
+    r.width   = cols * bytes;
+    r.stride  = rows > 1 ? static_cast<std::uint64_t>(row_stride) * bytes : 0;
+    r.end     = r.begin + (rows - 1) * r.stride + r.width;
+    r.owner   = owner;
+    r.written = written;
+    return r;
+}
+
+// Whether two ranges whose hulls meet share no byte as far as their strides show: windows of one matrix, side by side.
+bool sideBySide(const Range& a, const Range& b) {
+    const std::uint64_t stride = a.stride != 0 ? a.stride : b.stride;
+    if (stride == 0 || (a.stride != 0 && b.stride != 0 && a.stride != b.stride) || a.width > stride || b.width > stride) { return false; }
+    const std::uint64_t offset = (b.begin - a.begin) % stride;  // b.begin >= a.begin
+    return offset >= a.width && offset + b.width <= stride;
+}
+
+// nullptr, or why the gradients cannot be clipped at once.
+const char* checkOverlap(const FtcudaGradient* gradients, std::uint64_t count) {
+    std::vector<Range> ranges;
+    ranges.reserve(2 * count);
+    for (std::uint64_t i = 0; i < count; ++i) {
+        const FtcudaGradient& g = gradients[i];
+        if (g.rows == 0 || g.cols == 0) { continue; }
+        const Range in  = rangeOf(g.data, g.rows, g.cols, g.row_stride, training::elementBytes(g.element), i, false);
+        const Range out = rangeOf(g.out, g.rows, g.cols, g.out_row_stride, training::elementBytes(g.out_element), i, true);
+        ranges.push_back(out);
+        if (g.data != g.out) {
+            ranges.push_back(in);
+        } else if (g.element != g.out_element || in.stride != out.stride) {
+            return "a gradient that is its own output has another type or stride there";
+        }
+    }
+    const auto before = [](const Range& a, const Range& b) { return a.begin < b.begin; };
+    if (!std::is_sorted(ranges.begin(), ranges.end(), before)) { std::sort(ranges.begin(), ranges.end(), before); }
+    for (std::size_t i = 0; i < ranges.size(); ++i) {
+        for (std::size_t j = i + 1; j < ranges.size() && ranges[j].begin < ranges[i].end; ++j) {
+            if ((ranges[i].written || ranges[j].written) && !sideBySide(ranges[i], ranges[j])) {
+                return "an output overlaps another gradient or output";
+            }
+        }
+    }
+    return nullptr;
+}
+
+template<std::uint32_t kCapacity>
+void fillTable(Table<kCapacity>& table, const FtcudaGradient* gradients, std::uint64_t count, bool clip) {
+    table.count  = 0;
+    table.chunks = 0;
+    for (std::uint64_t i = 0; i < count; ++i) {
+        const FtcudaGradient& g = gradients[i];
+        if (g.rows == 0 || g.cols == 0) { continue; }
+        Entry& entry         = table.entries[table.count++];
+        entry.data           = g.data;
+        entry.out            = clip ? g.out : nullptr;
+        entry.rows           = g.rows;
+        entry.cols           = g.cols;
+        entry.row_stride     = g.row_stride;
+        entry.out_row_stride = g.out_row_stride;
+        entry.element        = g.element;
+        entry.out_element    = g.out_element;
+        if (g.rows > 1 && g.row_stride == static_cast<std::int64_t>(g.cols) && (!clip || g.out_row_stride == g.row_stride)) {
+            entry.cols = g.rows * g.cols;  // dense after all
+            entry.rows = 1;
+        }
+        entry.first = table.chunks;
+        table.chunks += entry.rows * ceilDiv(entry.cols, kChunk);
+    }
+}
+
+// CTAs for that many chunks: the SMs filled once, or a chunk each.
+std::uint32_t gridFor(std::uint64_t chunks, int sms, int per_sm) {
+    const std::uint64_t most = std::min<std::uint64_t>(kMaxGrid, static_cast<std::uint64_t>(sms) * static_cast<std::uint64_t>(per_sm));
+    return static_cast<std::uint32_t>(std::max<std::uint64_t>(1, std::min(chunks, most)));
+}
+
+struct Call {
+    const FtcudaGradient* gradients;
+    std::uint64_t count;
+    bool clip;
+    double max_norm;
+    float* norm;
+    double* partials;
+    int sms;
+    cudaStream_t stream;
+};
+
+template<typename Sum, std::uint32_t kCapacity> cudaError_t enqueue(const Call& call) {
+    const std::uint64_t launches = launchesFor(call.count);
+    const std::uint64_t each     = launches == 1 ? call.count : kTensors;
+    Table<kCapacity> table;
+    std::uint32_t partials = 0;
+    for (std::uint64_t l = 0; l < launches; ++l) {
+        fillTable(table, call.gradients + l * each, std::min(each, call.count - l * each), call.clip);
+        const std::uint32_t grid = gridFor(table.chunks, call.sms, kSumCtasPerSm);
+        // The first launch of a call is an ordinary one: it starts when what came before in the stream is done.
+        if (l == 0) {
+            gradientSums<Sum, kCapacity><<<grid, kThreads, 0, call.stream>>>(table, call.partials);
+            const cudaError_t error = cudaGetLastError();
+            if (error != cudaSuccess) { return error; }
+            countLaunches(1);
+        } else {
+            const cudaError_t error = training::launchOverlapped(gradientSums<Sum, kCapacity>, dim3(grid), dim3(kThreads), 0, call.stream, table, call.partials + partials);
+            if (error != cudaSuccess) { return error; }
+        }
+        partials += grid;
+    }
+    if (!call.clip) {
+        return training::launchOverlapped(gradientNorm<Sum>, dim3(1), dim3(kThreads), 0, call.stream,
+                                          static_cast<const double*>(call.partials), partials, call.norm);
+    }
+    for (std::uint64_t l = launches; l-- > 0;) {
+        if (launches > 1) { fillTable(table, call.gradients + l * each, std::min(each, call.count - l * each), call.clip); }
+        const cudaError_t error = training::launchOverlapped(gradientScale<Sum, kCapacity>, dim3(gridFor(table.chunks, call.sms, kScaleCtasPerSm)), dim3(kThreads), 0,
+                                                             call.stream, table, static_cast<const double*>(call.partials), partials, call.max_norm, l == 0 ? call.norm : static_cast<float*>(nullptr));
+        if (error != cudaSuccess) { return error; }
+    }
+    return cudaSuccess;
+}
+
+int runCall(const FtcudaGradient* gradients, std::uint64_t count, int norm_kind, bool clip, double max_norm, float* norm, std::int32_t device, void* workspace,
+            std::uint64_t workspace_bytes, void* stream, char* message, std::size_t capacity) {
+    if (gradients == nullptr && count != 0) { return fail(message, capacity, 1, "null gradients"); }
+    if (norm == nullptr || !training::aligned(norm, 4)) { return fail(message, capacity, 1, "the norm has no address, or one that is not a multiple of four"); }
+    if (norm_kind != FTCUDA_NORM_2 && norm_kind != FTCUDA_NORM_INF) { return fail(message, capacity, 1, "unknown kind of norm %d", norm_kind); }
+    if (clip && !(max_norm >= 0.0)) { return fail(message, capacity, 1, "max_norm must not be negative"); }
+    if (count >= (1ULL << 24)) { return fail(message, capacity, 1, "too many gradients"); }
+    for (std::uint64_t i = 0; i < count; ++i) {
+        if (const char* reason = checkGradient(gradients[i], clip)) {
+            return fail(message, capacity, 1, "gradient %llu: %s", static_cast<unsigned long long>(i), reason);
+        }
+    }
+    const std::uint64_t needed = ftcuda_gradient_norm_workspace_bytes(count);
+    if (workspace == nullptr || workspace_bytes < needed || !training::aligned(workspace, 8)) {
+        return fail(message, capacity, 1, "workspace of %llu bytes needed, at a multiple of eight", static_cast<unsigned long long>(needed));
+    }
+    if (clip) {
+        try {
+            if (const char* reason = checkOverlap(gradients, count)) { return fail(message, capacity, 1, "%s", reason); }
+        } catch (const std::bad_alloc&) { return fail(message, capacity, 1, "out of host memory"); }
+    }
+    int sms = 0;
+    if (!training::deviceIsCurrent(device, message, capacity) || !deviceSmCount(device, &sms, message, capacity)) { return 1; }
+    const Call call{gradients, count, clip, max_norm, norm, static_cast<double*>(workspace), sms, static_cast<cudaStream_t>(stream)};
+    cudaError_t error = cudaSuccess;
+    if (norm_kind == FTCUDA_NORM_2) {
+        error = count <= kFew ? enqueue<Sum2, kFew>(call) : enqueue<Sum2, kTensors>(call);
+    } else {
+        error = count <= kFew ? enqueue<SumInf, kFew>(call) : enqueue<SumInf, kTensors>(call);
+    }
+    if (error != cudaSuccess) { return fail(message, capacity, 1, "%s", cudaGetErrorString(error)); }
+    return 0;
+}
+
+}  // namespace
+}  // namespace ftcuda
+
+extern "C" uint64_t ftcuda_gradient_norm_workspace_bytes(uint64_t count) {
+    return ftcuda::launchesFor(count == 0 ? 1 : count) * ftcuda::kMaxGrid * sizeof(double);
+}
+
+extern "C" int ftcuda_gradient_norm(const FtcudaGradient* gradients, uint64_t count, int norm_kind, float* norm, int32_t device, void* workspace,
+                                    uint64_t workspace_bytes, void* stream, char* message, size_t message_capacity) {
+    return ftcuda::runCall(gradients, count, norm_kind, false, 0.0, norm, device, workspace, workspace_bytes, stream, message, message_capacity);
+}
+
+extern "C" int ftcuda_gradient_clip(const FtcudaGradient* gradients, uint64_t count, int norm_kind, double max_norm, float* norm, int32_t device,
+                                    void* workspace, uint64_t workspace_bytes, void* stream, char* message, size_t message_capacity) {
+    return ftcuda::runCall(gradients, count, norm_kind, true, max_norm, norm, device, workspace, workspace_bytes, stream, message, message_capacity);
+}

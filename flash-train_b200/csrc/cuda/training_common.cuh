@@ -1,0 +1,78 @@
+// Shared by the operators of ftcuda/training.h: element types on the device, argument checks on the host.
+#ifndef FTCUDA_TRAINING_COMMON_CUH_
+#define FTCUDA_TRAINING_COMMON_CUH_
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "ftcuda/training.h"
+#include "gemm_kernels.hpp"
+
+namespace ftcuda {
+namespace training {
+
+template<typename T> struct Element;
+template<> struct Element<float> {
+    static constexpr int kCode = FTCUDA_ELEMENT_FP32;
+    static __device__ __forceinline__ float widen(float x) { return x; }
+    static __device__ __forceinline__ float narrow(float x) { return x; }
+};
+template<> struct Element<__half> {
+    static constexpr int kCode = FTCUDA_ELEMENT_FP16;
+    static __device__ __forceinline__ float widen(__half x) { return __half2float(x); }
+    static __device__ __forceinline__ __half narrow(float x) { return __float2half_rn(x); }
+};
+template<> struct Element<__nv_bfloat16> {
+    static constexpr int kCode = FTCUDA_ELEMENT_BF16;
+    static __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+    static __device__ __forceinline__ __nv_bfloat16 narrow(float x) { return __float2bfloat16_rn(x); }
+};
+
+// Bytes of an element, 0 for a type that the operators do not take.
+inline std::uint64_t elementBytes(std::int32_t element) {
+    return element == FTCUDA_ELEMENT_FP32 ? 4 : element == FTCUDA_ELEMENT_FP16 || element == FTCUDA_ELEMENT_BF16 ? 2 : 0;
+}
+
+inline bool aligned(const void* pointer, std::uint64_t bytes) { return reinterpret_cast<std::uintptr_t>(pointer) % bytes == 0; }
+
+// The device exists and is the calling thread's current one.
+inline bool deviceIsCurrent(std::int32_t device, char* message, std::size_t capacity) {
+    int current             = -1;
+    const cudaError_t error = cudaGetDevice(&current);
+    if (error != cudaSuccess) {
+        fail(message, capacity, 1, "%s", cudaGetErrorString(error));
+        return false;
+    }
+    if (current != device) {
+        fail(message, capacity, 1, "device %d must be current, device %d is", device, current);
+        return false;
+    }
+    return true;
+}
+
+// A kernel launch that may start while the stream's preceding kernel ends (which the kernel waits for by gridDependencyWait).
+template<typename... Parameters, typename... Arguments>
+cudaError_t launchOverlapped(void (*kernel)(Parameters...), dim3 grid, dim3 block, std::size_t shared, cudaStream_t stream,
+                             const Arguments&... arguments) {
+    cudaLaunchConfig_t config{};
+    config.gridDim          = grid;
+    config.blockDim         = block;
+    config.dynamicSmemBytes = shared;
+    config.stream           = stream;
+    cudaLaunchAttribute attribute{};
+    attribute.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs                                         = &attribute;
+    config.numAttrs                                      = 1;
+    const cudaError_t error = cudaLaunchKernelEx(&config, kernel, arguments...);
+    if (error == cudaSuccess) { countLaunches(1); }
+    return error;
+}
+
+}  // namespace training
+}  // namespace ftcuda
+
+#endif

@@ -53,7 +53,8 @@ PLATFORM_SYMBOLS = (
     "ftcuda_trace_mark ftcuda_gemm_splitk_static ftcuda_gemm_splitk_static_capacity ftcuda_gemm_launch_scatter "
     "ftcuda_device_status ftcuda_device_status_reset ftcuda_selftest_bounded_wait ftcuda_measure_ffma_tflops "
     "ftcuda_grouped_gemm_supports ftcuda_grouped_gemm_configure ftcuda_grouped_gemm_workspace_bytes "
-    "ftcuda_grouped_gemm_launch ftcuda_grouped_gemm_destroy"
+    "ftcuda_grouped_gemm_launch ftcuda_grouped_gemm_destroy ftcuda_gradient_norm_workspace_bytes ftcuda_gradient_norm "
+    "ftcuda_gradient_clip"
 ).split()
 
 
@@ -611,3 +612,60 @@ def measure_ffma_tflops(device: int = 0) -> float:
     if lib.ftcuda_measure_ffma_tflops(device, byref(value), buffer, 256) != 0:
         raise FTrainError(STATUS_INTERNAL_ERROR, buffer.value.decode())
     return float(value.value)
+
+
+# ---- a training step's operators (include/ftcuda/training.h) ----
+
+ELEMENT_FP32 = 4
+ELEMENT_FP16 = 7
+ELEMENT_BF16 = 8
+NORM_2 = 0
+NORM_INF = 1
+
+
+class Gradient(Structure):
+    """FtcudaGradient."""
+
+    _fields_ = [
+        ("data", c_void_p), ("out", c_void_p), ("rows", c_uint64), ("cols", c_uint64),
+        ("row_stride", c_int64), ("out_row_stride", c_int64), ("element", ctypes.c_int32), ("out_element", ctypes.c_int32),
+    ]
+
+
+def _declare_training(lib) -> None:
+    message = [ctypes.c_char_p, ctypes.c_size_t]
+    lib.ftcuda_gradient_norm_workspace_bytes.argtypes = [c_uint64]
+    lib.ftcuda_gradient_norm_workspace_bytes.restype = c_uint64
+    work = [c_void_p, c_uint64, c_void_p] + message
+    lib.ftcuda_gradient_norm.argtypes = [POINTER(Gradient), c_uint64, ctypes.c_int, c_void_p, ctypes.c_int32] + work
+    lib.ftcuda_gradient_clip.argtypes = [POINTER(Gradient), c_uint64, ctypes.c_int, ctypes.c_double, c_void_p, ctypes.c_int32] + work
+    for name in ("ftcuda_gradient_norm", "ftcuda_gradient_clip"):
+        getattr(lib, name).restype = ctypes.c_int
+
+
+_declare_training(lib)
+
+
+def _run_training(function, *arguments) -> None:
+    buffer = ctypes.create_string_buffer(256)
+    if function(*arguments, buffer, 256) != 0:
+        raise FTrainError(STATUS_INVALID_ARGUMENT, buffer.value.decode())
+
+
+def gradient_norm_workspace_bytes(count: int) -> int:
+    return int(lib.ftcuda_gradient_norm_workspace_bytes(count))
+
+
+def gradient_norm(gradients, norm: int, workspace: int, workspace_bytes: int, norm_kind: int = NORM_2, device: int = 0, stream: int = 0) -> None:
+    """ftcuda_gradient_norm over a list of Gradient; `norm` and `workspace` are device addresses."""
+    array = (Gradient * max(len(gradients), 1))(*gradients)
+    _run_training(lib.ftcuda_gradient_norm, array, len(gradients), norm_kind, c_void_p(norm), device, c_void_p(workspace), workspace_bytes,
+                  c_void_p(stream))
+
+
+def gradient_clip(gradients, max_norm: float, norm: int, workspace: int, workspace_bytes: int, norm_kind: int = NORM_2, device: int = 0,
+                  stream: int = 0) -> None:
+    """ftcuda_gradient_clip; every Gradient's `out` is written."""
+    array = (Gradient * max(len(gradients), 1))(*gradients)
+    _run_training(lib.ftcuda_gradient_clip, array, len(gradients), norm_kind, max_norm, c_void_p(norm), device, c_void_p(workspace),
+                  workspace_bytes, c_void_p(stream))

@@ -34,6 +34,8 @@
 #include <flash_train/env.h>
 #include <flash_train/flash_train.h>
 
+#include "training.hpp"
+
 namespace {
 
 void checkMatrix(const at::Tensor& tensor, const char* name) {
@@ -287,5 +289,6 @@ PYBIND11_MODULE(_flash_train_torch, m) {
     m.doc() = "flash-train PyTorch bindings";
     m.def("gemm", &gemm, "d = alpha * (a @ b) + beta * c on the current stream", py::arg("a"), py::arg("b"),
           py::arg("c") = std::nullopt, py::arg("alpha") = 1.0, py::arg("beta") = 0.0);
+    flash_train_torch::registerGradientNorm(m);
     m.def("last_message", &lastMessage, "diagnostic message of the calling thread's last failed library call");
 }

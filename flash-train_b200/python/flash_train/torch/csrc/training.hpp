@@ -1,0 +1,25 @@
+// The operators around a training step's products, registered beside gemm.
+#ifndef FLASH_TRAIN_TORCH_TRAINING_HPP_
+#define FLASH_TRAIN_TORCH_TRAINING_HPP_
+
+#include <torch/extension.h>
+
+namespace flash_train_torch {
+
+void registerGradientNorm(pybind11::module_& module);
+
+// Room for a reason from the library.
+struct Message {
+    char text[256] = "";
+};
+
+// A block of torch's caching allocator on `like`'s device. The allocator keeps it reserved for the current stream until the work enqueued so
+// far is done, so it may go out of scope behind the call that got it.
+at::Tensor workspaceFor(std::uint64_t bytes, const at::Tensor& like);
+
+// FTCUDA_ELEMENT_* of a floating type that the operators take, 0 for any other.
+std::int32_t elementOf(const at::Tensor& tensor);
+
+}  // namespace flash_train_torch
+
+#endif
