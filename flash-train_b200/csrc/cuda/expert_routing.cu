@@ -1,0 +1,489 @@
+// The experts' router (ftcuda/training.h): softmax, top-k, counts and balance loss in one pass over the logits, and its gradient
+// in another.
+//
+//   p = softmax(x_t),  S_t = the k largest x,  w_i = p_{e_i} (over their sum),  c_e = #{(t, i): e_i = e},  P_e = mean_t p_te
+//   L = E sum_e f_e P_e,  f_e = c_e / (N k)
+//   dL/dx_j = g p_j (s_j - sum_e s_e p_e) with s_e = E f_e / N, and the weights' part: w_i (g_i - sum_i g_i w_i) at the chosen when they are
+//   normalised, else p_j (a_j - sum a p) with a = g_i at the chosen
+//
+// A warp takes a token, lane l the experts l, l + 32, ...: the row stays in registers for all that is done with it. A round of top-k is
+// a maximum over the warp of keys that order as the logits do. Sums over tokens: each lane keeps its experts' p over all of its
+// warp's tokens, a CTA joins its warps and leaves one row of partial sums, and a cluster of eight CTAs adds the rows up; the counts are whole
+// numbers in shared memory. One CTA alone (few tokens) finishes by itself, without the second launch.
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "ptx.cuh"
+#include "training_common.cuh"
+
+namespace ftcuda {
+namespace {
+
+namespace cg = cooperative_groups;
+using training::Element;
+
+constexpr int kWarps              = 16;  // of the forward kernel's CTA
+constexpr int kBackwardWarps      = 8;
+constexpr int kCtasPerSm          = 2;
+constexpr std::uint32_t kMaxExperts = 1024;
+constexpr std::uint32_t kMaxTopK    = 32;
+constexpr std::uint32_t kMaxRows    = 512;  // CTAs of the forward kernel at most
+constexpr int kFinishCtas         = 8;
+constexpr int kFinishThreads      = 512;
+constexpr unsigned kAll           = 0xFFFFFFFFU;
+
+// Whole numbers that order as the numbers do: NaN above all, -0 equal to 0. kDead is that of -inf; 0 is below every number.
+__device__ __forceinline__ std::uint32_t orderOf(float x) {
+    const std::uint32_t bits = __float_as_uint(x + 0.0F);
+    const std::uint32_t key  = (bits & 0x80000000U) != 0 ? ~bits : bits | 0x80000000U;
+    return x != x ? 0xFFFFFFFFU : key;
+}
+__device__ __forceinline__ float valueOf(std::uint32_t key) {
+    return __uint_as_float((key & 0x80000000U) != 0 ? key & 0x7FFFFFFFU : ~key);  // 0xFFFFFFFF: a NaN again
+}
+constexpr std::uint32_t kDead = 0x007FFFFFU;
+
+struct RouteParams {
+    const void* logits;
+    const std::uint8_t* mask;
+    std::uint64_t tokens;
+    std::int64_t row_stride;
+    std::uint32_t experts, top_k;
+    std::int32_t normalize;
+    float* weights;
+    std::int32_t* chosen;
+    std::int32_t* counts;
+    std::int32_t* routed;
+    float* loss;
+    float* sums;             // [CTA][experts]
+    std::int32_t* hits;      // [CTA][experts]
+    std::int32_t* live;      // [CTA]
+};
+
+__device__ __forceinline__ float warpSum(float x) {
+#pragma unroll
+    for (int offset = 16; offset > 0; offset /= 2) { x += __shfl_xor_sync(kAll, x, offset); }
+    return x;
+}
+
+// E sum_e f_e P_e from the sums over all tokens; thread 0's is the result. `shared` has room for a number for each warp.
+__device__ __forceinline__ double balance(double part, double* shared) {
+#pragma unroll
+    for (int offset = 16; offset > 0; offset /= 2) { part += __shfl_xor_sync(kAll, part, offset); }
+    if ((threadIdx.x & 31) == 0) { shared[threadIdx.x >> 5] = part; }
+    __syncthreads();
+    double total = 0.0;
+    if (threadIdx.x == 0) {
+        for (std::uint32_t w = 0; w < blockDim.x / 32; ++w) { total += shared[w]; }
+    }
+    return total;
+}
+
+__device__ __forceinline__ void writeLoss(const RouteParams& p, double total, std::int32_t live) {
+    const double n = static_cast<double>(live);
+    *p.routed      = live;
+    *p.loss        = live == 0 ? 0.0F : static_cast<float>(total * p.experts / (n * p.top_k * n));
+}
+
+template<typename T, int kItems> __global__ void __launch_bounds__(kWarps * 32) routeTokens(const RouteParams p) {
+    extern __shared__ unsigned char memory[];
+    auto* const hits = reinterpret_cast<std::int32_t*>(memory);  // [experts]
+    auto* const rows = reinterpret_cast<float*>(hits + p.experts);  // [kWarps / 2][experts]
+    __shared__ std::int32_t live_total;
+    __shared__ double shared[kWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (std::uint32_t e = threadIdx.x; e < p.experts; e += kWarps * 32) { hits[e] = 0; }
+    if (threadIdx.x == 0) { live_total = 0; }
+    __syncthreads();
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+
+    float sums[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) { sums[i] = 0.0F; }
+    std::int32_t live = 0;
+    for (std::uint64_t token = static_cast<std::uint64_t>(blockIdx.x) * kWarps + warp; token < p.tokens; token += static_cast<std::uint64_t>(gridDim.x) * kWarps) {
+        const T* const row = static_cast<const T*>(p.logits) + static_cast<std::int64_t>(token) * p.row_stride;
+        const bool on      = p.mask == nullptr || p.mask[token] != 0;
+        std::int32_t mine  = -1;
+        float value        = 0.0F, weight = 0.0F;
+        if (on) {
+            float x[kItems];
+            std::uint32_t keys[kItems];
+#pragma unroll
+            for (int i = 0; i < kItems; ++i) {
+                const std::uint32_t e = lane + 32 * i;
+                x[i]                  = e < p.experts ? Element<T>::widen(row[e]) : -INFINITY;
+                keys[i]               = e < p.experts ? orderOf(x[i]) : 0;
+            }
+            float largest = -INFINITY;
+            for (std::uint32_t round = 0; round < p.top_k; ++round) {
+                std::uint32_t best = keys[0];
+#pragma unroll
+                for (int i = 1; i < kItems; ++i) { best = max(best, keys[i]); }
+                best = __reduce_max_sync(kAll, best);
+                if (best <= kDead) { break; }
+                std::uint32_t at = 0xFFFFFFFFU;
+#pragma unroll
+                for (int i = kItems - 1; i >= 0; --i) { at = keys[i] == best ? lane + 32 * i : at; }
+                at = __reduce_min_sync(kAll, at);
+#pragma unroll
+                for (int i = 0; i < kItems; ++i) { keys[i] = at == lane + 32 * i ? 0 : keys[i]; }
+                if (round == 0) { largest = valueOf(best); }
+                if (lane == static_cast<int>(round)) {
+                    mine  = static_cast<std::int32_t>(at);
+                    value = valueOf(best);
+                }
+            }
+            if (largest != -INFINITY) {  // (not a number included)
+                float total = 0.0F;
+#pragma unroll
+                for (int i = 0; i < kItems; ++i) {
+                    x[i] = expf(x[i] - largest);
+                    total += x[i];
+                }
+                total               = warpSum(total);
+                const float inverse = 1.0F / total;
+#pragma unroll
+                for (int i = 0; i < kItems; ++i) { sums[i] += x[i] * inverse; }
+                weight = mine >= 0 ? expf(value - largest) : 0.0F;
+                weight /= p.normalize != 0 ? warpSum(weight) : total;
+                ++live;
+            }
+        }
+        if (lane < static_cast<int>(p.top_k)) {
+            p.weights[token * p.top_k + lane] = weight;
+            p.chosen[token * p.top_k + lane]  = mine;
+            if (mine >= 0) { atomicAdd(hits + mine, 1); }
+        }
+    }
+    if (lane == 0 && live != 0) { atomicAdd(&live_total, live); }
+    // The warps' sums, half of them onto the other half at a time.
+#pragma unroll
+    for (int half = kWarps / 2; half > 0; half /= 2) {
+        if (warp >= half && warp < 2 * half) {
+#pragma unroll
+            for (int i = 0; i < kItems; ++i) {
+                if (lane + 32 * i < static_cast<int>(p.experts)) { rows[(warp - half) * p.experts + lane + 32 * i] = sums[i]; }
+            }
+        }
+        __syncthreads();
+        if (warp < half) {
+#pragma unroll
+            for (int i = 0; i < kItems; ++i) {
+                if (lane + 32 * i < static_cast<int>(p.experts)) { sums[i] += rows[warp * p.experts + lane + 32 * i]; }
+            }
+        }
+        __syncthreads();
+    }
+    if (gridDim.x > 1) {
+        const std::uint64_t at = static_cast<std::uint64_t>(blockIdx.x) * p.experts;
+        if (warp == 0) {
+#pragma unroll
+            for (int i = 0; i < kItems; ++i) {
+                if (lane + 32 * i < static_cast<int>(p.experts)) { p.sums[at + lane + 32 * i] = sums[i]; }
+            }
+        }
+        for (std::uint32_t e = threadIdx.x; e < p.experts; e += kWarps * 32) { p.hits[at + e] = hits[e]; }
+        if (threadIdx.x == 0) { p.live[blockIdx.x] = live_total; }
+        return;
+    }
+    // The only CTA.
+    double part = 0.0;
+    if (warp == 0) {
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const std::uint32_t e = lane + 32 * i;
+            if (e < p.experts) { part += static_cast<double>(sums[i]) * hits[e]; }
+        }
+    }
+    for (std::uint32_t e = threadIdx.x; e < p.experts; e += kWarps * 32) { p.counts[e] = hits[e]; }
+    const double total = balance(part, shared);
+    if (threadIdx.x == 0) { writeLoss(p, total, live_total); }
+}
+
+// The rows of partial sums added up: each CTA of the cluster an eighth of them, the first CTA what they come to.
+__global__ void __cluster_dims__(kFinishCtas, 1, 1) __launch_bounds__(kFinishThreads) finishRouting(const RouteParams p, std::uint32_t rows) {
+    extern __shared__ unsigned char memory[];
+    auto* const sums = reinterpret_cast<double*>(memory);                   // [experts]
+    auto* const hits = reinterpret_cast<std::int32_t*>(sums + p.experts);   // [experts], then the number of live tokens
+    __shared__ double shared[kFinishThreads / 32];
+    cg::cluster_group cluster = cg::this_cluster();
+    const std::uint32_t rank  = cluster.block_rank();
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const std::uint32_t first = rows * rank / kFinishCtas, last = rows * (rank + 1) / kFinishCtas;
+    // A warp's lanes take neighbouring experts, and the threads beyond the experts other rows; joined in shared memory below.
+    for (std::uint32_t e = threadIdx.x; e < p.experts; e += kFinishThreads) {
+        double sum         = 0.0;
+        std::int32_t count = 0;
+#pragma unroll 8
+        for (std::uint32_t row = first; row < last; ++row) {
+            sum += static_cast<double>(__ldcg(p.sums + static_cast<std::uint64_t>(row) * p.experts + e));
+            count += __ldcg(p.hits + static_cast<std::uint64_t>(row) * p.experts + e);
+        }
+        sums[e] = sum;
+        hits[e] = count;
+    }
+    if (threadIdx.x < 32) {
+        std::int32_t live = 0;
+        for (std::uint32_t row = first + threadIdx.x; row < last; row += 32) { live += __ldcg(p.live + row); }
+        live = __reduce_add_sync(kAll, live);
+        if (threadIdx.x == 0) { hits[p.experts] = live; }
+    }
+    cluster.sync();
+    if (rank == 0) {
+        double part       = 0.0;
+        std::int32_t live = 0;
+        for (std::uint32_t e = threadIdx.x; e < p.experts; e += kFinishThreads) {
+            double sum         = 0.0;
+            std::int32_t count = 0;
+#pragma unroll
+            for (int r = 0; r < kFinishCtas; ++r) {
+                sum += cluster.map_shared_rank(sums, r)[e];
+                count += cluster.map_shared_rank(hits, r)[e];
+            }
+            p.counts[e] = count;
+            part += sum * count;
+        }
+        const double total = balance(part, shared);
+        if (threadIdx.x == 0) {
+            for (int r = 0; r < kFinishCtas; ++r) { live += cluster.map_shared_rank(hits, r)[p.experts]; }
+            writeLoss(p, total, live);
+        }
+    }
+    cluster.sync();  // nobody leaves while its shared memory is read
+}
+
+struct RouteGradient {
+    const void* logits;
+    std::uint64_t tokens;
+    std::int64_t row_stride, grad_row_stride;
+    std::uint32_t experts, top_k;
+    std::int32_t normalize;
+    const float* weights;
+    const std::int32_t* chosen;
+    const std::int32_t* counts;
+    const std::int32_t* routed;
+    const float* grad_weights;
+    const float* grad_loss;
+    void* grad_logits;
+};
+
+template<typename T, int kItems> __global__ void __launch_bounds__(kBackwardWarps * 32) routeGradient(const RouteGradient p) {
+    extern __shared__ unsigned char memory[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto* const extra = reinterpret_cast<float*>(memory) + warp * p.experts;  // what the weights add at the chosen experts
+    for (std::uint32_t e = lane; e < p.experts; e += 32) { extra[e] = 0.0F; }
+    __syncwarp();
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const std::int32_t routed = *p.routed;
+    const float gradient      = p.grad_loss != nullptr && routed != 0 ? *p.grad_loss : 0.0F;
+    const float unit          = routed != 0 ? static_cast<float>(static_cast<double>(p.experts) / (static_cast<double>(routed) * p.top_k * routed)) : 0.0F;
+    float slope[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const std::uint32_t e = lane + 32 * i;
+        slope[i]              = e < p.experts ? gradient * (unit * static_cast<float>(p.counts[e])) : 0.0F;
+    }
+    for (std::uint64_t token = static_cast<std::uint64_t>(blockIdx.x) * kBackwardWarps + warp; token < p.tokens;
+         token += static_cast<std::uint64_t>(gridDim.x) * kBackwardWarps) {
+        const T* const row = static_cast<const T*>(p.logits) + static_cast<std::int64_t>(token) * p.row_stride;
+        T* const out       = static_cast<T*>(p.grad_logits) + static_cast<std::int64_t>(token) * p.grad_row_stride;
+        std::int32_t mine  = -1;
+        float weight = 0.0F, upstream = 0.0F;
+        if (lane < static_cast<int>(p.top_k)) {
+            mine = p.chosen[token * p.top_k + lane];
+            if (mine >= 0) {
+                weight   = p.weights[token * p.top_k + lane];
+                upstream = p.grad_weights != nullptr ? p.grad_weights[token * p.top_k + lane] : 0.0F;
+            }
+        }
+        if (__shfl_sync(kAll, mine, 0) < 0) {  // took no part
+#pragma unroll
+            for (int i = 0; i < kItems; ++i) {
+                if (lane + 32 * i < static_cast<int>(p.experts)) { out[lane + 32 * i] = Element<T>::narrow(0.0F); }
+            }
+            continue;
+        }
+        float x[kItems];
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const std::uint32_t e = lane + 32 * i;
+            x[i]                  = e < p.experts ? Element<T>::widen(row[e]) : -INFINITY;
+        }
+        float largest = x[0];
+#pragma unroll
+        for (int i = 1; i < kItems; ++i) { largest = fmaxf(largest, x[i]); }
+#pragma unroll
+        for (int offset = 16; offset > 0; offset /= 2) { largest = fmaxf(largest, __shfl_xor_sync(kAll, largest, offset)); }
+        float total = 0.0F, mean = 0.0F;
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            x[i] = expf(x[i] - largest);
+            total += x[i];
+            mean += x[i] * slope[i];
+        }
+        total               = warpSum(total);
+        const float inverse = 1.0F / total;
+        const float inner   = warpSum(weight * upstream);
+        // Normalised, the weights are a softmax of their own; otherwise they are the whole softmax's, and shift its mean.
+        mean                = warpSum(mean) * inverse + (p.normalize != 0 ? 0.0F : inner);
+        const float added   = weight * (upstream - (p.normalize != 0 ? inner : 0.0F));
+        if (mine >= 0) { extra[mine] = added; }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const std::uint32_t e = lane + 32 * i;
+            if (e < p.experts) { out[e] = Element<T>::narrow(fmaf(x[i] * inverse, slope[i] - mean, extra[e])); }
+        }
+        __syncwarp();
+        if (mine >= 0) { extra[mine] = 0.0F; }
+        __syncwarp();
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+const char* check(const FtcudaRouting& r) {
+    if (training::elementBytes(r.element) == 0) { return "the logits must be FP32, FP16 or BF16"; }
+    if (r.experts == 0 || r.experts > kMaxExperts) { return "1 to 1024 experts"; }
+    if (r.top_k == 0 || r.top_k > r.experts || r.top_k > kMaxTopK) { return "top_k must be from 1 to the number of experts, and at most 32"; }
+    if (r.tokens >= (1ULL << 31)) { return "too many tokens"; }
+    if (r.tokens == 0) { return nullptr; }
+    if (r.logits == nullptr || !training::aligned(r.logits, training::elementBytes(r.element))) { return "the logits have no address, or one that is not a multiple of their element's size"; }
+    if (r.tokens > 1 && (r.row_stride < static_cast<std::int64_t>(r.experts) || r.row_stride >= (1LL << 31))) { return "the logits' rows overlap, or lie too far apart"; }
+    return nullptr;
+}
+
+bool wordAligned(const void* pointer) { return pointer != nullptr && training::aligned(pointer, 4); }
+
+// CTAs of the forward kernel: a warp's worth of tokens at least, the SMs filled at most. 32 tokens and fewer stay in one.
+std::uint32_t forwardRows(std::uint64_t tokens, std::uint32_t sms) {
+    if (tokens <= 2 * kWarps) { return 1; }
+    return static_cast<std::uint32_t>(std::min<std::uint64_t>(ceilDiv(tokens, kWarps), std::min(kMaxRows, sms * kCtasPerSm)));
+}
+
+// One of the kernels' instantiations by type and experts for each lane.
+template<template<typename, int> class Pick, typename Kernel> Kernel choose(std::int32_t element, std::uint32_t experts) {
+    const auto typed = [&](auto sample) -> Kernel {
+        using T = decltype(sample);
+        if (experts <= 32) { return Pick<T, 1>::kernel; }
+        if (experts <= 64) { return Pick<T, 2>::kernel; }
+        if (experts <= 128) { return Pick<T, 4>::kernel; }
+        if (experts <= 256) { return Pick<T, 8>::kernel; }
+        if (experts <= 512) { return Pick<T, 16>::kernel; }
+        return Pick<T, 32>::kernel;
+    };
+    switch (element) {
+        case FTCUDA_ELEMENT_FP32: return typed(float{});
+        case FTCUDA_ELEMENT_FP16: return typed(__half{});
+        default: return typed(__nv_bfloat16{});
+    }
+}
+template<typename T, int kItems> struct Forward { static constexpr auto kernel = &routeTokens<T, kItems>; };
+template<typename T, int kItems> struct Backward { static constexpr auto kernel = &routeGradient<T, kItems>; };
+
+}  // namespace
+}  // namespace ftcuda
+
+extern "C" uint64_t ftcuda_expert_routing_workspace_bytes(const FtcudaRouting* routing) {
+    if (routing == nullptr) { return 0; }
+    const std::uint64_t rows = std::min<std::uint64_t>(ftcuda::kMaxRows, ftcuda::ceilDiv(routing->tokens, ftcuda::kWarps) + 1);
+    return rows * (8ULL * std::min(routing->experts, ftcuda::kMaxExperts) + 4);
+}
+
+extern "C" int ftcuda_expert_routing(const FtcudaRouting* routing, float* weights, int32_t* experts, int32_t* counts, int32_t* routed, float* balance_loss,
+                                     void* workspace, uint64_t workspace_bytes, void* stream, char* message, size_t message_capacity) {
+    using namespace ftcuda;
+    if (routing == nullptr) { return fail(message, message_capacity, 1, "null routing"); }
+    const FtcudaRouting& r = *routing;
+    if (const char* reason = check(r)) { return fail(message, message_capacity, 1, "%s", reason); }
+    if (!wordAligned(counts) || !wordAligned(routed) || !wordAligned(balance_loss) || (r.tokens != 0 && (!wordAligned(weights) || !wordAligned(experts)))) {
+        return fail(message, message_capacity, 1, "an output has no address, or one that is not a multiple of four");
+    }
+    const std::uint64_t needed = ftcuda_expert_routing_workspace_bytes(routing);
+    if (!wordAligned(workspace) || workspace_bytes < needed) {
+        return fail(message, message_capacity, 1, "workspace of %llu bytes needed, at a multiple of four", static_cast<unsigned long long>(needed));
+    }
+    int sms = 0;
+    if (!training::deviceIsCurrent(r.device, message, message_capacity) || !deviceSmCount(r.device, &sms, message, message_capacity)) { return 1; }
+    const std::uint32_t rows = forwardRows(r.tokens, static_cast<std::uint32_t>(sms));
+    RouteParams p{};
+    p.logits     = r.logits;
+    p.mask       = r.mask;
+    p.tokens     = r.tokens;
+    p.row_stride = r.row_stride;
+    p.experts    = r.experts;
+    p.top_k      = r.top_k;
+    p.normalize  = r.normalize;
+    p.weights    = weights;
+    p.chosen     = experts;
+    p.counts     = counts;
+    p.routed     = routed;
+    p.loss       = balance_loss;
+    p.sums       = static_cast<float*>(workspace);
+    p.hits       = reinterpret_cast<std::int32_t*>(p.sums + static_cast<std::uint64_t>(rows) * r.experts);
+    p.live       = p.hits + static_cast<std::uint64_t>(rows) * r.experts;
+    const auto kernel              = choose<Forward, void (*)(RouteParams)>(r.element, r.experts);
+    const std::size_t shared_bytes = r.experts * 4ULL * (1 + kWarps / 2);
+    kernel<<<rows, kWarps * 32, shared_bytes, static_cast<cudaStream_t>(stream)>>>(p);
+    cudaError_t error = cudaGetLastError();
+    if (error == cudaSuccess) {
+        countLaunches(1);
+        if (rows > 1) {
+            error = training::launchOverlapped(finishRouting, dim3(kFinishCtas), dim3(kFinishThreads), r.experts * 12ULL + 4, static_cast<cudaStream_t>(stream), p, rows);
+        }
+    }
+    if (error != cudaSuccess) { return fail(message, message_capacity, 1, "%s", cudaGetErrorString(error)); }
+    return 0;
+}
+
+extern "C" int ftcuda_expert_routing_backward(const FtcudaRouting* routing, const float* weights, const int32_t* experts, const int32_t* counts,
+                                              const int32_t* routed, const float* grad_weights, const float* grad_loss, void* grad_logits,
+                                              int64_t grad_row_stride, void* stream, char* message, size_t message_capacity) {
+    using namespace ftcuda;
+    if (routing == nullptr) { return fail(message, message_capacity, 1, "null routing"); }
+    const FtcudaRouting& r = *routing;
+    if (const char* reason = check(r)) { return fail(message, message_capacity, 1, "%s", reason); }
+    if (r.tokens == 0) { return 0; }
+    if (!wordAligned(weights) || !wordAligned(experts) || !wordAligned(counts) || !wordAligned(routed) || (grad_weights != nullptr && !wordAligned(grad_weights)) ||
+        (grad_loss != nullptr && !wordAligned(grad_loss))) {
+        return fail(message, message_capacity, 1, "an input has no address, or one that is not a multiple of four");
+    }
+    if (grad_logits == nullptr || !training::aligned(grad_logits, training::elementBytes(r.element))) {
+        return fail(message, message_capacity, 1, "the gradient has no address, or one that is not a multiple of its element's size");
+    }
+    if (r.tokens > 1 && (grad_row_stride < static_cast<std::int64_t>(r.experts) || grad_row_stride >= (1LL << 31))) {
+        return fail(message, message_capacity, 1, "the gradient's rows overlap, or lie too far apart");
+    }
+    int sms = 0;
+    if (!training::deviceIsCurrent(r.device, message, message_capacity) || !deviceSmCount(r.device, &sms, message, message_capacity)) { return 1; }
+    RouteGradient p{};
+    p.logits          = r.logits;
+    p.tokens          = r.tokens;
+    p.row_stride      = r.row_stride;
+    p.grad_row_stride = grad_row_stride;
+    p.experts         = r.experts;
+    p.top_k           = r.top_k;
+    p.normalize       = r.normalize;
+    p.weights         = weights;
+    p.chosen          = experts;
+    p.counts          = counts;
+    p.routed          = routed;
+    p.grad_weights    = grad_weights;
+    p.grad_loss       = grad_loss;
+    p.grad_logits     = grad_logits;
+    const auto kernel              = choose<Backward, void (*)(RouteGradient)>(r.element, r.experts);
+    const std::uint32_t grid       = static_cast<std::uint32_t>(std::min<std::uint64_t>(ceilDiv(r.tokens, kBackwardWarps), static_cast<std::uint64_t>(sms) * 4));
+    const std::size_t shared_bytes = r.experts * 4ULL * kBackwardWarps;
+    kernel<<<grid, kBackwardWarps * 32, shared_bytes, static_cast<cudaStream_t>(stream)>>>(p);
+    const cudaError_t error = cudaGetLastError();
+    if (error != cudaSuccess) { return fail(message, message_capacity, 1, "%s", cudaGetErrorString(error)); }
+    countLaunches(1);
+    return 0;
+}

@@ -54,7 +54,7 @@ PLATFORM_SYMBOLS = (
     "ftcuda_device_status ftcuda_device_status_reset ftcuda_selftest_bounded_wait ftcuda_measure_ffma_tflops "
     "ftcuda_grouped_gemm_supports ftcuda_grouped_gemm_configure ftcuda_grouped_gemm_workspace_bytes "
     "ftcuda_grouped_gemm_launch ftcuda_grouped_gemm_destroy ftcuda_gradient_norm_workspace_bytes ftcuda_gradient_norm "
-    "ftcuda_gradient_clip"
+    "ftcuda_gradient_clip ftcuda_expert_routing_workspace_bytes ftcuda_expert_routing ftcuda_expert_routing_backward"
 ).split()
 
 
@@ -632,6 +632,15 @@ class Gradient(Structure):
     ]
 
 
+class Routing(Structure):
+    """FtcudaRouting."""
+
+    _fields_ = [
+        ("logits", c_void_p), ("mask", c_void_p), ("tokens", c_uint64), ("row_stride", c_int64),
+        ("experts", c_uint32), ("top_k", c_uint32), ("normalize", ctypes.c_int32), ("element", ctypes.c_int32), ("device", ctypes.c_int32),
+    ]
+
+
 def _declare_training(lib) -> None:
     message = [ctypes.c_char_p, ctypes.c_size_t]
     lib.ftcuda_gradient_norm_workspace_bytes.argtypes = [c_uint64]
@@ -639,7 +648,11 @@ def _declare_training(lib) -> None:
     work = [c_void_p, c_uint64, c_void_p] + message
     lib.ftcuda_gradient_norm.argtypes = [POINTER(Gradient), c_uint64, ctypes.c_int, c_void_p, ctypes.c_int32] + work
     lib.ftcuda_gradient_clip.argtypes = [POINTER(Gradient), c_uint64, ctypes.c_int, ctypes.c_double, c_void_p, ctypes.c_int32] + work
-    for name in ("ftcuda_gradient_norm", "ftcuda_gradient_clip"):
+    lib.ftcuda_expert_routing_workspace_bytes.argtypes = [POINTER(Routing)]
+    lib.ftcuda_expert_routing_workspace_bytes.restype = c_uint64
+    lib.ftcuda_expert_routing.argtypes = [POINTER(Routing)] + [c_void_p] * 5 + work
+    lib.ftcuda_expert_routing_backward.argtypes = [POINTER(Routing)] + [c_void_p] * 7 + [c_int64, c_void_p] + message
+    for name in ("ftcuda_gradient_norm", "ftcuda_gradient_clip", "ftcuda_expert_routing", "ftcuda_expert_routing_backward"):
         getattr(lib, name).restype = ctypes.c_int
 
 
@@ -669,3 +682,20 @@ def gradient_clip(gradients, max_norm: float, norm: int, workspace: int, workspa
     array = (Gradient * max(len(gradients), 1))(*gradients)
     _run_training(lib.ftcuda_gradient_clip, array, len(gradients), norm_kind, max_norm, c_void_p(norm), device, c_void_p(workspace),
                   workspace_bytes, c_void_p(stream))
+
+
+def expert_routing_workspace_bytes(routing: Routing) -> int:
+    return int(lib.ftcuda_expert_routing_workspace_bytes(byref(routing)))
+
+
+def expert_routing(routing: Routing, weights: int, experts: int, counts: int, routed: int, balance_loss: int, workspace: int,
+                   workspace_bytes: int, stream: int = 0) -> None:
+    """ftcuda_expert_routing; everything but `routing` and the size is a device address."""
+    _run_training(lib.ftcuda_expert_routing, byref(routing), weights, experts, counts, routed, balance_loss, workspace, workspace_bytes, stream)
+
+
+def expert_routing_backward(routing: Routing, weights: int, experts: int, counts: int, routed: int, grad_weights: int, grad_loss: int,
+                            grad_logits: int, grad_row_stride: int, stream: int = 0) -> None:
+    """ftcuda_expert_routing_backward; 0 for grad_weights or grad_loss means that it is zero."""
+    _run_training(lib.ftcuda_expert_routing_backward, byref(routing), weights, experts, counts, routed, grad_weights, grad_loss, grad_logits,
+                  grad_row_stride, stream)

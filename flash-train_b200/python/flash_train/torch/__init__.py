@@ -1,6 +1,6 @@
 """PyTorch binding: `gemm(a, b, c=None, alpha=1.0, beta=0.0) -> Tensor`, plus
 `HostGemm` / `gemm_host` for operands in pinned host memory (host_pipeline.py), and what a
-training step does around its products: `grad_norm`, `clip_grads` and `clip_grad_norm_`.
+training step does around its products: `expert_routing`, `grad_norm`, `clip_grads` and `clip_grad_norm_`.
 
 Signature, defaults, checks and error type (RuntimeError) are those of the
 reference binding (python/flash_train/torch/csrc/flash_train_torch.cpp:34-75
@@ -34,5 +34,7 @@ except ModuleNotFoundError as exc:
 
 from .clipping import clip_grad_norm_  # noqa: E402
 from .host_pipeline import HostGemm, band_ranges, gemm_host  # noqa: E402
+from .routing import ExpertRouting, expert_routing  # noqa: E402
 
-__all__ = ["gemm", "last_message", "HostGemm", "gemm_host", "band_ranges", "grad_norm", "clip_grads", "clip_grad_norm_"]
+__all__ = ["gemm", "last_message", "HostGemm", "gemm_host", "band_ranges", "grad_norm", "clip_grads", "clip_grad_norm_",
+           "expert_routing", "ExpertRouting"]

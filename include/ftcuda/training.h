@@ -1,5 +1,6 @@
 /*
- * ftcuda/training.h -- what a training step does around its products: the gradients' norm.
+ * ftcuda/training.h -- what a training step does around its products: the experts' router,
+ * the gradients' norm.
  *
  * Same manner as ftcuda/ftcuda.h: plain pointers, integers and fixed-size structs; no C++ types, no
  * exceptions; 0 = success, nonzero = failure with a NUL-terminated reason in the caller's message
@@ -67,6 +68,51 @@ FTCUDA_API int ftcuda_gradient_norm(const FtcudaGradient* gradients, uint64_t co
 FTCUDA_API int ftcuda_gradient_clip(const FtcudaGradient* gradients, uint64_t count, int norm_kind, double max_norm, float* norm,
                                     int32_t device, void* workspace, uint64_t workspace_bytes, void* stream, char* message,
                                     size_t message_capacity);
+
+/* ---- the experts' router ---- */
+
+/*
+ * Each token's softmax over its experts' logits p = softmax(logits[t]), its top_k experts, and what they add up to:
+ *   experts[t][i]  the i-th largest logit's index; among equal ones (-0 equals 0) the lowest index comes first. Not a number
+ *                  counts as larger than anything. Logits of -inf are never chosen: the slots they would take say -1.
+ *   weights[t][i]  p of that expert, 0 in a slot of -1; with `normalize` divided by the sum over the token's slots
+ *   counts[e]      how many slots say e: the sizes of the grouped products' groups
+ *   *routed        how many tokens took part: those that the mask does not take out and that have a logit above -inf. The others
+ *                  have -1 and 0 in all slots, and no part in anything below.
+ *   *balance_loss  experts * sum_e f_e P_e with f_e = counts[e] / (routed * top_k) and P_e the mean of p[e] over the routed
+ *                  tokens; 0 where none is. For a gradient f_e is a constant.
+ * logits: [tokens][experts], unit stride along the experts, row_stride elements between tokens; 1 to 1024 experts, top_k at most 32
+ * and at most `experts`. mask: one byte for each token, nonzero = takes part; NULL = all do. Everything is computed in FP32
+ * whatever the logits' type, sums over tokens in an order that depends on the sizes alone.
+ */
+typedef struct {
+    const void* logits;
+    const uint8_t* mask;
+    uint64_t tokens;
+    int64_t row_stride;
+    uint32_t experts;
+    uint32_t top_k;
+    int32_t normalize;
+    int32_t element;
+    int32_t device;
+} FtcudaRouting;
+
+/* Bytes of workspace that ftcuda_expert_routing needs; at most about 5 MB. */
+FTCUDA_API uint64_t ftcuda_expert_routing_workspace_bytes(const FtcudaRouting* routing);
+
+/* weights: FP32 [tokens][top_k]; experts: INT32 [tokens][top_k]; counts: INT32 [experts]; all dense, on the device, none may be NULL. */
+FTCUDA_API int ftcuda_expert_routing(const FtcudaRouting* routing, float* weights, int32_t* experts, int32_t* counts, int32_t* routed,
+                                     float* balance_loss, void* workspace, uint64_t workspace_bytes, void* stream, char* message,
+                                     size_t message_capacity);
+
+/*
+ * grad_logits (of the logits' type, grad_row_stride elements between tokens) from grad_weights (FP32 [tokens][top_k], dense) and *grad_loss (one FP32 on the
+ * device), either of which may be NULL, meaning zero; the other arguments as the forward call took and left them. Needs no workspace.
+ */
+FTCUDA_API int ftcuda_expert_routing_backward(const FtcudaRouting* routing, const float* weights, const int32_t* experts, const int32_t* counts,
+                                              const int32_t* routed, const float* grad_weights, const float* grad_loss,
+                                              void* grad_logits, int64_t grad_row_stride, void* stream, char* message,
+                                              size_t message_capacity);
 
 #ifdef __cplusplus
 }
