@@ -3,7 +3,7 @@
 // The reference ships only a placeholder that names nothing
 // (src/include/flash_train/family/gemm/finder.hpp:21-25), which makes its engine
 // fall back to registration order. B200Heuristic is the real policy of this
-// build: it ranks the CUDA Primitives by problem regime (see finder.cpp).
+// build: it ranks the CUDA Primitives by problem regime (see cuda/gemm_choice.hpp).
 #ifndef FTRAIN_FAMILY_GEMM_FINDER_HPP_
 #define FTRAIN_FAMILY_GEMM_FINDER_HPP_
 
