@@ -121,14 +121,19 @@ bool deviceStatusWord(int device, int** device_pointer, volatile int** host_poin
         // Mapped pinned memory: the kernels can write it, the host can read it
         // without synchronising any stream. Allocated once per device; the
         // device that is current when a Plan is configured is `device`.
+        // Another thread, or this one, may be capturing a graph; the allocation is no part of it.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
         void* host        = nullptr;
         info.status_error = cudaHostAlloc(&host, 64, cudaHostAllocMapped | cudaHostAllocPortable);
-        if (info.status_error != cudaSuccess) { return; }
-        info.status_host    = static_cast<int*>(host);
-        info.status_host[0] = 0;
-        void* device_side   = nullptr;
-        info.status_error   = cudaHostGetDevicePointer(&device_side, host, 0);
-        info.status_device  = static_cast<int*>(device_side);
+        if (info.status_error == cudaSuccess) {
+            info.status_host    = static_cast<int*>(host);
+            info.status_host[0] = 0;
+            void* device_side   = nullptr;
+            info.status_error   = cudaHostGetDevicePointer(&device_side, host, 0);
+            info.status_device  = static_cast<int*>(device_side);
+        }
+        cudaThreadExchangeStreamCaptureMode(&mode);
     });
     if (info.status_error != cudaSuccess) {
         fail(message, capacity, 1, "allocating the device status word failed: %s",
@@ -170,6 +175,27 @@ bool encodeTensorMap2d(CUtensorMap* map, const void* base, std::uint64_t inner, 
         swizzle == kSwizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B
                                : swizzle == kSwizzle128Atom32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_NONE,
         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (result != CUDA_SUCCESS) {
+        fail(message, capacity, 1, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(result));
+        return false;
+    }
+    return true;
+}
+
+bool encodeMap16(CUtensorMap* map, bool bf16, const void* base, std::uint64_t inner, std::uint64_t outer, std::uint64_t row_pitch_bytes,
+                 std::uint32_t box_outer, char* message, std::size_t capacity) {
+    const PFN_cuTensorMapEncodeTiled_v12000 encode = tensorMapEncoder();
+    if (encode == nullptr) {
+        fail(message, capacity, 1, "the CUDA driver does not provide cuTensorMapEncodeTiled");
+        return false;
+    }
+    const cuuint64_t dims[2]     = {inner, outer};
+    const cuuint64_t strides[1]  = {row_pitch_bytes};
+    const cuuint32_t box[2]      = {64, box_outer};
+    const cuuint32_t elements[2] = {1, 1};
+    const CUresult result = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
+                                   strides, box, elements, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (result != CUDA_SUCCESS) {
         fail(message, capacity, 1, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(result));
         return false;

@@ -1,0 +1,770 @@
+// The cross entropy of a product with a large vocabulary (ftcuda/training.h).
+//
+//   z_tv = h_t . w_v,   lse_t = log sum_v exp z_tv,   l_t = lse_t - z_{t, y_t}
+//   dz_tv = g_t (exp(z_tv - lse_t) - [v = y_t]),   dH = dZ W,   dW = dZ^T H
+//
+// The forward call is one pass over the vocabulary, 2 T V D operations; the backward call goes through the vocabulary piece by
+// piece and computes Z of a piece again: dZ of it, then dH += dZ W and dW = dZ^T H, 6 T V D. A piece is as wide as kPieceBytes of dZ allow, so that
+// the passes over dH (one for each piece) and the launches weigh little.
+//
+// Tokens without a target are left out first: the others' hidden states are gathered into the workspace, which costs one pass over H,
+// makes what the padding holds irrelevant (a NaN there would reach dW through 0 * NaN), spares the products those rows, and gives
+// the tensor cores an aligned operand whatever H's strides. How many there are only the GPU knows; the kernels read it there.
+//
+// BF16 and FP16 operands go through loss_products.cu; FP32 ones through the library's own FP32 products, chosen by the same rules as the
+// host pipeline's (gemm_choice.hpp), with Z of a piece in the workspace and a pass over it for the statistics or dZ.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <cstdint>
+
+#include "gemm_choice.hpp"
+#include "loss_products.hpp"
+#include "ptx.cuh"
+#include "training_common.cuh"
+
+namespace ftcuda {
+namespace {
+
+using loss::LiveRows;
+using training::Element;
+
+constexpr int kListThreads             = 1024;
+constexpr int kGatherThreads           = 256;
+constexpr int kJoinRows                = 32;   // rows of a CTA that joins statistics, a warp for each eighth of the pieces
+constexpr int kRowThreads              = 256;  // FP32: threads that go over a row of logits
+constexpr std::uint64_t kPieceBytes    = 512ULL << 20;  // of dZ (FP32: of Z), unless ...
+constexpr std::uint64_t kLeastColumns  = 8192;          // ... that is fewer columns than these
+constexpr std::uint64_t kAlign         = 256;
+
+// ---------------------------------------------------------------- kernels
+
+struct ListParams {
+    const std::int64_t* target;
+    std::int64_t ignore_index, vocabulary;
+    std::uint32_t tokens;
+    std::int32_t reduction;
+    LiveRows rows;
+    std::int32_t* slot;        // [tokens]: a token's row, -1 for none
+    // forward
+    float* loss;
+    float* lse;
+    // backward
+    const float* saved_lse;
+    const float* grad_loss;
+    std::int32_t scale_bits;   // log2 of what the largest |scale| is brought near to; INT_MIN: the scales stay as they are
+};
+
+// One CTA: the list of live tokens, and (backward) their scales.
+template<bool kBackward> __global__ void __launch_bounds__(kListThreads) listTokens(const ListParams p) {
+    __shared__ std::uint32_t warp_counts[kListThreads / 32];
+    __shared__ std::uint32_t largest_bits;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) { largest_bits = 0; }
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    std::uint32_t count = 0, largest = 0;
+    for (std::uint32_t base = 0; base < p.tokens; base += kListThreads) {
+        const std::uint32_t t = base + threadIdx.x;
+        std::int64_t y        = 0;
+        bool on               = false;
+        if (t < p.tokens) {
+            y  = p.target[t];
+            on = y != p.ignore_index;
+        }
+        const unsigned ballot = __ballot_sync(0xFFFFFFFFU, on);
+        if (lane == 0) { warp_counts[warp] = __popc(ballot); }
+        __syncthreads();
+        const std::uint32_t mine   = warp_counts[lane];
+        const std::uint32_t before = __reduce_add_sync(0xFFFFFFFFU, lane < warp ? mine : 0);
+        const std::uint32_t all    = __reduce_add_sync(0xFFFFFFFFU, mine);
+        __syncthreads();
+        if (t < p.tokens) {
+            const std::uint32_t at = count + before + __popc(ballot & ((1U << lane) - 1));
+            p.slot[t]              = on ? static_cast<std::int32_t>(at) : -1;
+            if (on) {
+                p.rows.token[at]  = static_cast<std::int32_t>(t);
+                p.rows.target[at] = y >= 0 && y < p.vocabulary ? static_cast<std::int32_t>(y) : loss::kBadTarget;
+                if (kBackward && p.reduction == FTCUDA_REDUCTION_NONE) { largest = max(largest, __float_as_uint(p.grad_loss[t]) & 0x7FFFFFFFU); }
+            } else if (!kBackward) {
+                p.lse[t] = 0.0F;
+                if (p.reduction == FTCUDA_REDUCTION_NONE) { p.loss[t] = 0.0F; }
+            }
+        }
+        count += all;
+    }
+    const std::uint32_t padded = (max(count, 1U) + loss::kTileRows - 1) / loss::kTileRows * loss::kTileRows;
+    if (kBackward) {
+        float common = 0.0F;
+        if (p.reduction != FTCUDA_REDUCTION_NONE) {
+            common  = p.reduction == FTCUDA_REDUCTION_MEAN ? *p.grad_loss / static_cast<float>(max(count, 1U)) : *p.grad_loss;
+            largest = __float_as_uint(common) & 0x7FFFFFFFU;
+        }
+        atomicMax(&largest_bits, largest);
+        __syncthreads();
+        // The largest |scale| becomes a number in [1, 2) 2^scale_bits; not beyond 2^100 times larger, and not where it is 0 or not a number.
+        const float top    = __uint_as_float(largest_bits);
+        std::int32_t shift = 0;
+        if (p.scale_bits != INT32_MIN) { shift = p.scale_bits - (top > 0.0F && top <= FLT_MAX ? max(-100, ilogbf(top)) : 0); }
+        for (std::uint32_t i = threadIdx.x; i < padded; i += kListThreads) {
+            float scale = 0.0F, lse2 = 0.0F;
+            if (i < count) {
+                const std::int32_t t = p.rows.token[i];
+                scale                = ldexpf(p.reduction == FTCUDA_REDUCTION_NONE ? p.grad_loss[t] : common, shift);
+                lse2                 = p.saved_lse[t] * loss::kLog2E;
+                if (p.rows.target[i] == loss::kBadTarget) { scale = __uint_as_float(0x7FFFFFFFU); }
+            }
+            p.rows.scale[i] = scale;
+            p.rows.lse2[i]  = lse2;
+        }
+        if (threadIdx.x == 0) { *p.rows.unit = ldexpf(1.0F, -shift); }
+    }
+    for (std::uint32_t i = count + threadIdx.x; i < padded; i += kListThreads) {
+        p.rows.token[i]  = -1;
+        p.rows.target[i] = -1;
+    }
+    if (threadIdx.x == 0) { *p.rows.count = count; }
+}
+
+// Row i of the copy = hidden state of the i-th live token; zeros behind the last one. Words of `W` where both sides are aligned for it.
+template<typename W>
+__global__ void __launch_bounds__(kGatherThreads) gatherHidden(const LiveRows rows, std::uint32_t zero_to, const W* hidden, std::int64_t stride, W* copy,
+                                                               std::uint64_t pitch, std::uint32_t words) {
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const std::uint32_t live   = *rows.count;
+    const std::uint32_t padded = max(zero_to, (max(live, 1U) + loss::kTileRows - 1) / loss::kTileRows * loss::kTileRows);
+    const std::uint32_t row    = blockIdx.x;
+    if (row >= padded) { return; }
+    W* const to = copy + row * pitch;
+    if (row < live) {
+        const W* const from = hidden + static_cast<std::int64_t>(rows.token[row]) * stride;
+#pragma unroll 4
+        for (std::uint32_t i = threadIdx.x; i < words; i += kGatherThreads) { to[i] = from[i]; }
+    } else {
+        for (std::uint32_t i = threadIdx.x; i < words; i += kGatherThreads) { to[i] = W{}; }
+    }
+}
+
+// A 16-bit weight that TMA cannot describe, copied with rows at multiples of 16 bytes.
+__global__ void __launch_bounds__(kGatherThreads) copyRows16(const std::uint16_t* from, std::int64_t stride, std::uint16_t* to, std::uint64_t pitch,
+                                                             std::uint32_t depth) {
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    from += static_cast<std::int64_t>(blockIdx.x) * stride;
+    to += blockIdx.x * pitch;
+#pragma unroll 4
+    for (std::uint32_t i = threadIdx.x; i < depth; i += kGatherThreads) { to[i] = from[i]; }
+}
+
+// Two partial results of a row: sums of 2^(x - base), with the bases.
+__device__ __forceinline__ float2 joinPartials(float2 a, float2 b) {
+    const float base = fmaxf(a.x, b.x);
+    // (A base of -inf belongs to a sum of nothing, or of NaN: taken as it is.)
+    const float left  = a.x == -INFINITY ? a.y : a.y * exp2f(a.x - base);
+    const float right = b.x == -INFINITY ? b.y : b.y * exp2f(b.x - base);
+    return make_float2(base, left + right);
+}
+
+struct JoinParams {
+    LiveRows rows;
+    const float2* partials;  // [piece][capacity]
+    std::uint32_t pieces, capacity;
+    float* row_loss;         // [capacity]
+    float* loss;             // [tokens], or NULL
+    float* lse;              // [tokens]
+};
+
+__global__ void __launch_bounds__(256) joinStatistics(const JoinParams p) {
+    __shared__ float2 shared[8][kJoinRows];
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const std::uint32_t live = *p.rows.count;
+    const std::uint32_t row  = blockIdx.x * kJoinRows + (threadIdx.x & 31);
+    if (blockIdx.x * kJoinRows >= live) { return; }
+    const int warp = threadIdx.x >> 5;
+    float2 sum     = make_float2(-INFINITY, 0.0F);
+    // (Rows up to the next multiple of kTileRows have statistics too.)
+#pragma unroll 4
+    for (std::uint32_t piece = warp; piece < p.pieces; piece += 8) { sum = joinPartials(sum, __ldcg(p.partials + static_cast<std::uint64_t>(piece) * p.capacity + row)); }
+    shared[warp][threadIdx.x & 31] = sum;
+    __syncthreads();
+    if (warp == 0 && row < live) {
+        for (int w = 1; w < 8; ++w) { sum = joinPartials(sum, shared[w][threadIdx.x]); }
+        const float lse          = loss::kLn2 * (sum.x + log2f(sum.y));
+        const bool bad           = p.rows.target[row] == loss::kBadTarget;
+        const float value        = bad ? __uint_as_float(0x7FFFFFFFU) : lse - p.rows.picked[row];
+        const std::int32_t token = p.rows.token[row];
+        p.lse[token]             = lse;
+        p.row_loss[row]          = value;
+        if (p.loss != nullptr) { p.loss[token] = value; }
+    }
+}
+
+// One CTA: the live rows' losses added up in 64 bits.
+__global__ void __launch_bounds__(kListThreads) sumLosses(const LiveRows rows, const float* row_loss, bool mean, float* loss) {
+    __shared__ double shared[kListThreads / 32];
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const std::uint32_t live = *rows.count;
+    double sum               = 0.0;
+#pragma unroll 4
+    for (std::uint32_t i = threadIdx.x; i < live; i += kListThreads) { sum += static_cast<double>(row_loss[i]); }
+#pragma unroll
+    for (int offset = 16; offset > 0; offset /= 2) { sum += __shfl_xor_sync(0xFFFFFFFFU, sum, offset); }
+    if ((threadIdx.x & 31) == 0) { shared[threadIdx.x >> 5] = sum; }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        sum = shared[threadIdx.x];
+#pragma unroll
+        for (int offset = 16; offset > 0; offset /= 2) { sum += __shfl_xor_sync(0xFFFFFFFFU, sum, offset); }
+        if (threadIdx.x == 0) { *loss = static_cast<float>(mean ? sum / static_cast<double>(max(live, 1U)) : sum); }
+    }
+}
+
+struct RowParams {
+    LiveRows rows;
+    float* logits;           // of a piece: [rows][pitch]
+    std::uint64_t pitch;
+    std::uint32_t first, columns;
+    float2* partials;        // this piece's: [capacity]
+};
+
+// FP32: the statistics of a row's piece, one CTA for each row.
+__global__ void __launch_bounds__(kRowThreads) rowStatistics(const RowParams p) {
+    __shared__ float2 shared[kRowThreads / 32];
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const std::uint32_t row = blockIdx.x;
+    if (row >= *p.rows.count) { return; }
+    const float* const z = p.logits + row * p.pitch;  // 16-byte aligned, as the pitch is a multiple of four
+    float largest = -INFINITY, base = 0.0F, sum = 0.0F;
+    const auto add = [&](const float (&x)[4]) {
+        const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        if (top > largest) {  // a new reference for the sum
+            const float next = top * loss::kLog2E;
+            sum              = largest == -INFINITY ? sum : sum * exp2f(base - next);
+            largest          = top;
+            base             = next;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { sum += exp2Fast(fmaf(x[i], loss::kLog2E, -base)); }
+    };
+#pragma unroll 2
+    for (std::uint32_t at = 4 * threadIdx.x; at < p.columns; at += 4 * kRowThreads) {
+        float x[4];
+        if (at + 4 <= p.columns) {
+            const float4 four = *reinterpret_cast<const float4*>(z + at);
+            x[0] = four.x, x[1] = four.y, x[2] = four.z, x[3] = four.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { x[i] = at + i < p.columns ? z[at + i] : -INFINITY; }
+        }
+        add(x);
+    }
+    float2 mine = make_float2(largest == -INFINITY ? -INFINITY : base, sum);
+#pragma unroll
+    for (int offset = 16; offset > 0; offset /= 2) {
+        mine = joinPartials(mine, make_float2(__shfl_xor_sync(0xFFFFFFFFU, mine.x, offset), __shfl_xor_sync(0xFFFFFFFFU, mine.y, offset)));
+    }
+    if ((threadIdx.x & 31) == 0) { shared[threadIdx.x >> 5] = mine; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kRowThreads / 32; ++w) { mine = joinPartials(mine, shared[w]); }
+        p.partials[row]       = mine;
+        const std::int32_t at = p.rows.target[row] - static_cast<std::int32_t>(p.first);
+        if (at >= 0 && at < static_cast<std::int32_t>(p.columns)) { p.rows.picked[row] = z[at]; }
+    }
+}
+
+// FP32: Z of a piece becomes dZ, in place; zeros in the rows behind the live ones.
+__global__ void __launch_bounds__(kRowThreads) rowSlopes(const RowParams p) {
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const std::uint32_t row = blockIdx.x;
+    float* const z          = p.logits + row * p.pitch;
+    const bool on           = row < *p.rows.count;
+    const float scale       = on ? p.rows.scale[row] : 0.0F;
+    const float lse2        = on ? p.rows.lse2[row] : 0.0F;
+    const std::uint32_t hit = on ? static_cast<std::uint32_t>(p.rows.target[row]) - p.first : 0xFFFFFFFFU;  // wraps where there is none
+    const auto slope        = [&](float x, std::uint32_t column) {
+        return on ? scale * (exp2Fast(fmaf(x, loss::kLog2E, -lse2)) - (column == hit ? 1.0F : 0.0F)) : 0.0F;
+    };
+#pragma unroll 2
+    for (std::uint32_t at = 4 * threadIdx.x; at < p.columns; at += 4 * kRowThreads) {
+        // (The pitch has room for a whole quad behind the last column.)
+        const float4 x                        = *reinterpret_cast<const float4*>(z + at);
+        *reinterpret_cast<float4*>(z + at) = make_float4(slope(x.x, at), slope(x.y, at + 1), slope(x.z, at + 2), slope(x.w, at + 3));
+    }
+}
+
+// grad_hidden[t] = unit * (the sums' parts added up), 0 for a token that takes no part.
+template<typename T>
+__global__ void __launch_bounds__(kGatherThreads) spreadHidden(const LiveRows rows, const std::int32_t* slot, const float* sums, std::uint64_t part, std::uint64_t pitch,
+                                                               std::uint32_t splits, std::uint32_t depth, T* out, std::int64_t stride) {
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const std::int32_t row = slot[blockIdx.x];
+    const float unit       = *rows.unit;
+    T* const to            = out + static_cast<std::int64_t>(blockIdx.x) * stride;
+    const float* const from = sums + static_cast<std::uint64_t>(max(row, 0)) * pitch;
+#pragma unroll 2
+    for (std::uint32_t i = threadIdx.x; i < depth; i += kGatherThreads) {
+        float sum = 0.0F;
+        if (row >= 0) {
+            for (std::uint32_t s = 0; s < splits; ++s) { sum += from[s * part + i]; }
+        }
+        to[i] = Element<T>::narrow(unit * sum);
+    }
+}
+
+// ---------------------------------------------------------------- host: layout of the workspace
+
+struct Layout {
+    std::uint64_t capacity;       // rows, a multiple of kTileRows
+    std::uint64_t copy_pitch;     // of the hidden states' copy, elements
+    std::uint64_t weight_pitch;   // of the weight's copy, 0: none
+    std::uint64_t columns;        // of a piece
+    std::uint64_t piece_pitch;    // of Z or dZ, elements
+    std::uint64_t pieces;         // partial statistics of a row
+    std::uint32_t splits;         // of the sums for dH
+    std::uint64_t sums_pitch;
+    std::uint64_t count, unit, token, target, scale, lse2, picked, row_loss, slot, hidden, weight, partials, piece, sums, product, product_bytes;
+    std::uint64_t total;
+};
+
+std::uint64_t roundUp(std::uint64_t x, std::uint64_t unit) { return (x + unit - 1) / unit * unit; }
+
+bool isFp32(const FtcudaLinearCrossEntropy& q) { return q.element == FTCUDA_ELEMENT_FP32; }
+
+// Whether TMA can fetch the weight as it is.
+bool weightFits(const FtcudaLinearCrossEntropy& q) { return training::aligned(q.weight, 16) && (q.vocabulary == 1 || q.weight_row_stride % 8 == 0); }
+
+std::uint64_t weightStride(const FtcudaLinearCrossEntropy& q) {
+    return q.vocabulary == 1 ? roundUp(q.depth, 8) : static_cast<std::uint64_t>(q.weight_row_stride);
+}
+
+// One FP32 product by the first family that takes it, in its prepared form where that is faster.
+struct Product {
+    FtcudaGemmLaunch launch;
+    std::uint64_t bytes;
+};
+int configureProduct(const FtcudaGemmDesc& desc, bool b_along_k, int sms, std::uint64_t bytes_left, Product& product, char* message, std::size_t capacity) {
+    const GemmCandidates candidates = gemmCandidates(desc.m, desc.n, desc.k, b_along_k && desc.n > 1, static_cast<std::uint64_t>(sms));
+    for (int i = 0; i < candidates.count; ++i) {
+        const int kernel = candidates.kernels[i];
+        if (ftcuda_gemm_supports(kernel, &desc, nullptr, 0) != 0) { continue; }
+        if (const int status = ftcuda_gemm_configure(kernel, &desc, &product.launch, message, capacity)) { return status; }
+        product.bytes = ftcuda_gemm_workspace_bytes(&product.launch);
+        if (product.bytes > bytes_left) { continue; }
+        if ((kernel == FTCUDA_GEMM_TF32X3 || kernel == FTCUDA_GEMM_TF32X3_SPLITK) && preparedFormPays(desc.m, desc.n, desc.k)) {
+            Product prepared;
+            if (ftcuda_gemm_prepare(&product.launch, &desc, &prepared.launch, nullptr, 0) == 0) {
+                prepared.bytes = ftcuda_gemm_workspace_bytes(&prepared.launch);
+                if (prepared.bytes <= bytes_left) { product = prepared; }
+            }
+        }
+        return 0;
+    }
+    return fail(message, capacity, 1, "no FP32 product takes the problem");
+}
+
+// The three FP32 products of a piece of `columns` columns from `first` on.
+FtcudaGemmDesc describeLogits(const FtcudaLinearCrossEntropy& q, const Layout& l, unsigned char* base, std::uint64_t first, std::uint64_t columns) {
+    FtcudaGemmDesc d{};
+    d.a            = reinterpret_cast<const float*>(base + l.hidden);
+    d.b            = static_cast<const float*>(q.weight) + static_cast<std::int64_t>(first) * q.weight_row_stride;
+    d.d            = reinterpret_cast<float*>(base + l.piece);
+    d.alpha        = 1.0F;
+    d.m            = q.tokens;
+    d.n            = columns;
+    d.k            = q.depth;
+    d.a_row_stride = static_cast<std::int64_t>(l.copy_pitch);
+    d.a_col_stride = 1;
+    d.b_row_stride = 1;
+    d.b_col_stride = q.vocabulary == 1 ? static_cast<std::int64_t>(q.depth) : q.weight_row_stride;
+    d.d_row_stride = static_cast<std::int64_t>(l.piece_pitch);
+    d.d_col_stride = 1;
+    d.device       = q.device;
+    return d;
+}
+FtcudaGemmDesc describeHidden(const FtcudaLinearCrossEntropy& q, const Layout& l, unsigned char* base, std::uint64_t first, std::uint64_t columns) {
+    FtcudaGemmDesc d = describeLogits(q, l, base, first, columns);
+    d.a              = d.d;
+    d.d              = reinterpret_cast<float*>(base + l.sums);
+    d.n              = q.depth;
+    d.k              = columns;
+    d.a_row_stride   = static_cast<std::int64_t>(l.piece_pitch);
+    d.b_row_stride   = d.b_col_stride;
+    d.b_col_stride   = 1;
+    d.d_row_stride   = static_cast<std::int64_t>(l.sums_pitch);
+    if (first != 0) {
+        d.beta         = 1.0F;
+        d.c            = d.d;
+        d.c_row_stride = d.d_row_stride;
+        d.c_col_stride = 1;
+    }
+    return d;
+}
+FtcudaGemmDesc describeWeight(const FtcudaLinearCrossEntropy& q, const Layout& l, unsigned char* base, std::uint64_t first, std::uint64_t columns, void* grad_weight,
+                              std::int64_t stride) {
+    FtcudaGemmDesc d = describeLogits(q, l, base, first, columns);
+    d.b              = d.a;
+    d.a              = d.d;
+    d.d              = static_cast<float*>(grad_weight) + static_cast<std::int64_t>(first) * stride;
+    d.m              = columns;
+    d.n              = q.depth;
+    d.k              = q.tokens;
+    d.a_row_stride   = 1;
+    d.a_col_stride   = static_cast<std::int64_t>(l.piece_pitch);
+    d.b_row_stride   = static_cast<std::int64_t>(l.copy_pitch);
+    d.b_col_stride   = 1;
+    d.d_row_stride   = stride;
+    return d;
+}
+
+int layOut(const FtcudaLinearCrossEntropy& q, bool backward, int sms, Layout& l, char* message, std::size_t capacity) {
+    const std::uint64_t bytes = training::elementBytes(q.element);
+    const bool fp32           = isFp32(q);
+    l                         = Layout{};
+    l.capacity                = roundUp(std::max<std::uint64_t>(q.tokens, 1), loss::kTileRows);
+    l.copy_pitch              = roundUp(q.depth, 16 / bytes);
+    l.weight_pitch            = !fp32 && !weightFits(q) ? roundUp(q.depth, 8) : 0;
+    const std::uint64_t fill  = roundUp(q.vocabulary, 256);
+    l.columns                 = std::min(fill, std::max(kLeastColumns, kPieceBytes / (l.capacity * bytes) / 256 * 256));
+    l.columns                 = roundUp(ceilDiv(fill, ceilDiv(fill, l.columns)), 256);  // pieces of about one size
+    l.piece_pitch             = l.columns;
+    l.pieces                  = fp32 ? ceilDiv(q.vocabulary, l.columns) : loss::statisticsPieces(static_cast<std::uint32_t>(q.vocabulary));
+    l.sums_pitch              = roundUp(q.depth, 8);
+    l.splits                  = fp32 ? 1 : loss::hiddenSplits(static_cast<std::uint32_t>(l.capacity), static_cast<std::uint32_t>(q.depth),
+                                                              static_cast<std::uint32_t>(std::min(l.columns, q.vocabulary)), sms);
+    std::uint64_t at = 0;
+    const auto take  = [&](std::uint64_t size) {
+        const std::uint64_t here = at;
+        at += roundUp(size, kAlign);
+        return here;
+    };
+    l.count  = take(4);
+    l.unit   = take(4);
+    l.token  = take(4 * l.capacity);
+    l.target = take(4 * l.capacity);
+    l.slot   = take(4 * l.capacity);
+    l.hidden = take(bytes * l.capacity * l.copy_pitch);
+    if (l.weight_pitch != 0) { l.weight = take(2 * q.vocabulary * l.weight_pitch); }
+    if (backward) {
+        l.scale = take(4 * l.capacity);
+        l.lse2  = take(4 * l.capacity);
+        l.sums  = take(4 * l.capacity * l.sums_pitch * l.splits);
+    } else {
+        l.picked   = take(4 * l.capacity);
+        l.row_loss = take(4 * l.capacity);
+        l.partials = take(8 * l.capacity * l.pieces);
+    }
+    if (backward || fp32) { l.piece = take(bytes * l.capacity * l.piece_pitch); }
+    if (fp32 && q.tokens != 0) {
+        // The most that any product of any piece wants. (The addresses are not known yet, but how they are aligned is.)
+        l.product            = at;
+        auto* const stand_in = reinterpret_cast<unsigned char*>(std::uintptr_t{1} << 40);
+        for (std::uint64_t first = 0; first < q.vocabulary; first += l.columns) {
+            const std::uint64_t columns = std::min(l.columns, q.vocabulary - first);
+            if (first != 0 && columns == l.columns && first != l.columns) { continue; }  // like the piece before
+            Product product;
+            if (configureProduct(describeLogits(q, l, stand_in, first, columns), true, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
+            l.product_bytes = std::max(l.product_bytes, product.bytes);
+            if (!backward) { continue; }
+            if (configureProduct(describeHidden(q, l, stand_in, first, columns), false, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
+            l.product_bytes = std::max(l.product_bytes, product.bytes);
+            if (configureProduct(describeWeight(q, l, stand_in, first, columns, stand_in, static_cast<std::int64_t>(q.depth)), false, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
+            l.product_bytes = std::max(l.product_bytes, product.bytes);
+        }
+        take(l.product_bytes);
+    }
+    l.total = at;
+    return 0;
+}
+
+const char* check(const FtcudaLinearCrossEntropy& q) {
+    const std::uint64_t bytes = training::elementBytes(q.element);
+    if (bytes == 0) { return "the operands must be FP32, FP16 or BF16"; }
+    if (q.reduction < FTCUDA_REDUCTION_NONE || q.reduction > FTCUDA_REDUCTION_SUM) { return "unknown reduction"; }
+    if (q.vocabulary == 0 || q.vocabulary >= (1ULL << 24)) { return "1 to 2^24 - 1 columns of the vocabulary"; }
+    if (q.depth == 0 || q.depth >= (1ULL << 20)) { return "a depth of 1 to 2^20 - 1"; }
+    if (q.tokens >= (1ULL << 24)) { return "at most 2^24 - 1 tokens"; }
+    if (q.weight == nullptr || !training::aligned(q.weight, bytes)) { return "the weight has no address, or one that is not a multiple of its element's size"; }
+    if (q.vocabulary > 1 && (q.weight_row_stride < static_cast<std::int64_t>(q.depth) || q.weight_row_stride >= (1LL << 31))) { return "the weight's rows overlap, or lie too far apart"; }
+    if (q.tokens == 0) { return nullptr; }
+    if (q.hidden == nullptr || !training::aligned(q.hidden, bytes)) { return "the hidden states have no address, or one that is not a multiple of their element's size"; }
+    if (q.tokens > 1 && (q.hidden_row_stride < static_cast<std::int64_t>(q.depth) || q.hidden_row_stride >= (1LL << 31))) { return "the hidden states' rows overlap, or lie too far apart"; }
+    if (q.target == nullptr || !training::aligned(q.target, 8)) { return "the targets have no address, or one that is not a multiple of eight"; }
+    return nullptr;
+}
+
+// ---------------------------------------------------------------- host: the calls
+
+class Call final {
+  public:
+    Call(const FtcudaLinearCrossEntropy& problem, char* message, std::size_t capacity) : q_(problem), message_(message), capacity_(capacity) {}
+
+    // Everything that is the same in both directions; 0 or a failure that has its message.
+    int begin(bool backward, void* workspace, std::uint64_t workspace_bytes, void* stream) {
+        if (!training::deviceIsCurrent(q_.device, message_, capacity_) || !deviceSmCount(q_.device, &sms_, message_, capacity_)) { return 1; }
+        if (layOut(q_, backward, sms_, l_, message_, capacity_) != 0) { return 1; }
+        if (workspace == nullptr || workspace_bytes < l_.total || !training::aligned(workspace, kAlign)) {
+            return fail(message_, capacity_, 1, "workspace of %llu bytes needed, at a multiple of 256", static_cast<unsigned long long>(l_.total));
+        }
+        int* status              = nullptr;
+        volatile int* host       = nullptr;
+        if (!deviceStatusWord(q_.device, &status, &host, message_, capacity_)) { return 1; }
+        if (const int code = takeDeviceStatus(host)) {
+            return fail(message_, capacity_, 1, "an earlier kernel reported a timed-out wait (code %d)", code);
+        }
+        base_        = static_cast<unsigned char*>(workspace);
+        stream_      = static_cast<cudaStream_t>(stream);
+        rows_.count  = at<std::uint32_t>(l_.count);
+        rows_.unit   = at<float>(l_.unit);
+        rows_.token  = at<std::int32_t>(l_.token);
+        rows_.target = at<std::int32_t>(l_.target);
+        rows_.scale  = at<float>(l_.scale);
+        rows_.lse2   = at<float>(l_.lse2);
+        rows_.picked = at<float>(l_.picked);
+        products_    = loss::ProductCall{q_.element == FTCUDA_ELEMENT_BF16, static_cast<std::uint32_t>(l_.capacity), static_cast<std::uint32_t>(q_.depth), rows_,
+                                      {base_ + l_.hidden, l_.copy_pitch}, status, sms_, stream_, message_, capacity_};
+        if (message_ != nullptr && capacity_ != 0) { message_[0] = '\0'; }
+        return 0;
+    }
+
+    cudaError_t forward(float* loss, float* lse) {
+        ListParams list = listParams();
+        list.loss       = loss;
+        list.lse        = lse;
+        // (The first kernel of a call is an ordinary launch: it starts when what came before in the stream is done.)
+        listTokens<false><<<1, kListThreads, 0, stream_>>>(list);
+        cudaError_t error = started();
+        if (error == cudaSuccess) { error = gather(); }
+        float2* const partials = at<float2>(l_.partials);
+        if (!isFp32(q_)) {
+            if (error == cudaSuccess) { error = loss::launchStatistics(products_, weight(0), static_cast<std::uint32_t>(q_.vocabulary), partials); }
+        } else {
+            std::uint64_t piece = 0;
+            for (std::uint64_t first = 0; first < q_.vocabulary && error == cudaSuccess; first += l_.columns, ++piece) {
+                const std::uint64_t columns = std::min(l_.columns, q_.vocabulary - first);
+                error                       = multiply(describeLogits(q_, l_, base_, first, columns), true);
+                if (error == cudaSuccess) {
+                    error = training::launchOverlapped(rowStatistics, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(first, columns, partials + piece * l_.capacity));
+                }
+            }
+        }
+        if (error != cudaSuccess) { return error; }
+        JoinParams join{};
+        join.rows     = rows_;
+        join.partials = partials;
+        join.pieces   = static_cast<std::uint32_t>(l_.pieces);
+        join.capacity = static_cast<std::uint32_t>(l_.capacity);
+        join.row_loss = at<float>(l_.row_loss);
+        join.loss     = q_.reduction == FTCUDA_REDUCTION_NONE ? loss : nullptr;
+        join.lse      = lse;
+        error = training::launchOverlapped(joinStatistics, dim3(static_cast<unsigned>(l_.capacity / kJoinRows)), dim3(256), 0, stream_, join);
+        if (error == cudaSuccess && q_.reduction != FTCUDA_REDUCTION_NONE) {
+            error = training::launchOverlapped(sumLosses, dim3(1), dim3(kListThreads), 0, stream_, rows_, static_cast<const float*>(at<float>(l_.row_loss)),
+                                               q_.reduction == FTCUDA_REDUCTION_MEAN, loss);
+        }
+        return error;
+    }
+
+    cudaError_t backward(const float* lse, const float* grad_loss, void* grad_hidden, std::int64_t hidden_stride, void* grad_weight, std::int64_t weight_stride) {
+        ListParams list = listParams();
+        list.saved_lse  = lse;
+        list.grad_loss  = grad_loss;
+        list.scale_bits = isFp32(q_) ? INT32_MIN : q_.element == FTCUDA_ELEMENT_FP16 ? 13 : 0;
+        listTokens<true><<<1, kListThreads, 0, stream_>>>(list);
+        cudaError_t error = started();
+        if (error == cudaSuccess) { error = gather(); }
+        for (std::uint64_t first = 0; first < q_.vocabulary && error == cudaSuccess; first += l_.columns) {
+            error = piece(first, std::min(l_.columns, q_.vocabulary - first), grad_hidden != nullptr, grad_weight, weight_stride);
+        }
+        if (error != cudaSuccess || grad_hidden == nullptr) { return error; }
+        switch (q_.element) {
+            case FTCUDA_ELEMENT_FP32: return spread(static_cast<float*>(grad_hidden), hidden_stride);
+            case FTCUDA_ELEMENT_FP16: return spread(static_cast<__half*>(grad_hidden), hidden_stride);
+            default: return spread(static_cast<__nv_bfloat16*>(grad_hidden), hidden_stride);
+        }
+    }
+
+  private:
+    template<typename T> T* at(std::uint64_t offset) const { return reinterpret_cast<T*>(base_ + offset); }
+
+    static cudaError_t started() {
+        const cudaError_t error = cudaGetLastError();
+        if (error == cudaSuccess) { countLaunches(1); }
+        return error;
+    }
+
+    ListParams listParams() const {
+        ListParams list{};
+        list.target       = q_.target;
+        list.ignore_index = q_.ignore_index;
+        list.vocabulary   = static_cast<std::int64_t>(q_.vocabulary);
+        list.tokens       = static_cast<std::uint32_t>(q_.tokens);
+        list.reduction    = q_.reduction;
+        list.rows         = rows_;
+        list.slot         = at<std::int32_t>(l_.slot);
+        return list;
+    }
+
+    RowParams rowParams(std::uint64_t first, std::uint64_t columns, float2* partials) const {
+        return RowParams{rows_, at<float>(l_.piece), l_.piece_pitch, static_cast<std::uint32_t>(first), static_cast<std::uint32_t>(columns), partials};
+    }
+
+    // The live hidden states, and the weight where TMA cannot fetch it as it is.
+    cudaError_t gather() const {
+        const std::uint64_t bytes = training::elementBytes(q_.element);
+        // The FP32 products go over all rows, the others over whole tiles of live ones.
+        const std::uint32_t zero_to = isFp32(q_) ? static_cast<std::uint32_t>(q_.tokens) : 0;
+        const auto run = [&](auto word) {
+            using W                   = decltype(word);
+            const std::uint64_t ratio = sizeof(W) / bytes;
+            return training::launchOverlapped(gatherHidden<W>, dim3(static_cast<unsigned>(l_.capacity)), dim3(kGatherThreads), 0, stream_, rows_, zero_to,
+                                              static_cast<const W*>(q_.hidden), static_cast<std::int64_t>(q_.hidden_row_stride / static_cast<std::int64_t>(ratio)), at<W>(l_.hidden),
+                                              l_.copy_pitch / ratio, static_cast<std::uint32_t>(q_.depth / ratio));
+        };
+        const std::uint64_t row  = q_.depth * bytes;
+        const bool wide          = row % 16 == 0 && training::aligned(q_.hidden, 16) && (q_.tokens <= 1 || static_cast<std::uint64_t>(q_.hidden_row_stride) * bytes % 16 == 0);
+        cudaError_t error        = wide ? run(uint4{}) : bytes == 4 ? run(std::uint32_t{}) : run(std::uint16_t{});
+        if (error == cudaSuccess && l_.weight_pitch != 0) {
+            error = training::launchOverlapped(copyRows16, dim3(static_cast<unsigned>(q_.vocabulary)), dim3(kGatherThreads), 0, stream_, static_cast<const std::uint16_t*>(q_.weight),
+                                               q_.weight_row_stride, at<std::uint16_t>(l_.weight), l_.weight_pitch, static_cast<std::uint32_t>(q_.depth));
+        }
+        return error;
+    }
+
+    // The weight from row `first` on, as the 16-bit products fetch it.
+    loss::Matrix16 weight(std::uint64_t first) const {
+        const bool copied         = l_.weight_pitch != 0;
+        const std::uint64_t pitch = copied ? l_.weight_pitch : weightStride(q_);
+        const void* const from    = copied ? base_ + l_.weight : q_.weight;
+        return loss::Matrix16{static_cast<const unsigned char*>(from) + 2 * first * pitch, pitch};
+    }
+
+    // One FP32 product.
+    cudaError_t multiply(const FtcudaGemmDesc& desc, bool b_along_k) const {
+        Product product;
+        if (configureProduct(desc, b_along_k, sms_, l_.product_bytes, product, message_, capacity_) != 0 ||
+            ftcuda_gemm_launch(&product.launch, base_ + l_.product, l_.product_bytes, stream_, message_, capacity_) != 0) {
+            return cudaErrorUnknown;  // the message says which
+        }
+        return cudaSuccess;
+    }
+
+    cudaError_t piece(std::uint64_t first, std::uint64_t columns, bool hidden, void* grad_weight, std::int64_t weight_stride) const {
+        const std::uint32_t first32 = static_cast<std::uint32_t>(first), columns32 = static_cast<std::uint32_t>(columns);
+        if (!isFp32(q_)) {
+            cudaError_t error = loss::launchSlopes(products_, weight(first), first32, columns32, base_ + l_.piece, l_.piece_pitch);
+            if (error != cudaSuccess) { return error; }
+            loss::Gradients gradients{};
+            gradients.sums                  = hidden ? at<float>(l_.sums) : nullptr;
+            gradients.sums_pitch            = l_.sums_pitch;
+            gradients.splits                = l_.splits;
+            gradients.accumulate            = first != 0;
+            gradients.weight_gradient       = grad_weight == nullptr ? nullptr : static_cast<unsigned char*>(grad_weight) + 2 * static_cast<std::int64_t>(first) * weight_stride;
+            gradients.weight_gradient_pitch = weight_stride;
+            return loss::launchGradients(products_, weight(first), columns32, base_ + l_.piece, l_.piece_pitch, gradients);
+        }
+        cudaError_t error = multiply(describeLogits(q_, l_, base_, first, columns), true);
+        if (error == cudaSuccess) {
+            error = training::launchOverlapped(rowSlopes, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(first, columns, nullptr));
+        }
+        if (error == cudaSuccess && hidden) { error = multiply(describeHidden(q_, l_, base_, first, columns), false); }
+        if (error == cudaSuccess && grad_weight != nullptr) { error = multiply(describeWeight(q_, l_, base_, first, columns, grad_weight, weight_stride), false); }
+        return error;
+    }
+
+    template<typename T> cudaError_t spread(T* out, std::int64_t stride) const {
+        return training::launchOverlapped(spreadHidden<T>, dim3(static_cast<unsigned>(q_.tokens)), dim3(kGatherThreads), 0, stream_, rows_,
+                                          static_cast<const std::int32_t*>(at<std::int32_t>(l_.slot)), static_cast<const float*>(at<float>(l_.sums)), l_.capacity * l_.sums_pitch,
+                                          l_.sums_pitch, l_.splits, static_cast<std::uint32_t>(q_.depth), out, stride);
+    }
+
+    const FtcudaLinearCrossEntropy& q_;
+    char* message_;
+    std::size_t capacity_;
+    int sms_ = 0;
+    Layout l_{};
+    unsigned char* base_ = nullptr;
+    cudaStream_t stream_ = nullptr;
+    LiveRows rows_{};
+    loss::ProductCall products_{};
+};
+
+// What a call came to. A failure below may have left its own message.
+int finish(cudaError_t error, char* message, std::size_t capacity) {
+    if (error == cudaSuccess) { return 0; }
+    if (message != nullptr && capacity != 0 && message[0] != '\0') { return 1; }
+    return fail(message, capacity, 1, "%s", cudaGetErrorString(error));
+}
+
+bool wordAligned(const void* pointer) { return pointer != nullptr && training::aligned(pointer, 4); }
+
+}  // namespace
+}  // namespace ftcuda
+
+extern "C" int ftcuda_linear_cross_entropy_workspace_bytes(const FtcudaLinearCrossEntropy* problem, int backward, uint64_t* workspace_bytes, char* message,
+                                                           size_t message_capacity) {
+    using namespace ftcuda;
+    if (problem == nullptr || workspace_bytes == nullptr) { return fail(message, message_capacity, 1, "null argument"); }
+    if (const char* reason = check(*problem)) { return fail(message, message_capacity, 1, "%s", reason); }
+    int sms = 0;
+    Layout layout;
+    if (!deviceSmCount(problem->device, &sms, message, message_capacity) || layOut(*problem, backward != 0, sms, layout, message, message_capacity) != 0) { return 1; }
+    *workspace_bytes = layout.total;
+    return 0;
+}
+
+extern "C" int ftcuda_linear_cross_entropy(const FtcudaLinearCrossEntropy* problem, float* loss, float* lse, void* workspace, uint64_t workspace_bytes, void* stream,
+                                           char* message, size_t message_capacity) {
+    using namespace ftcuda;
+    if (problem == nullptr) { return fail(message, message_capacity, 1, "null problem"); }
+    if (const char* reason = check(*problem)) { return fail(message, message_capacity, 1, "%s", reason); }
+    const bool empty = problem->tokens == 0;
+    if (!(empty && problem->reduction == FTCUDA_REDUCTION_NONE) && !wordAligned(loss)) { return fail(message, message_capacity, 1, "the loss has no address, or one that is not a multiple of four"); }
+    if (!empty && !wordAligned(lse)) { return fail(message, message_capacity, 1, "lse has no address, or one that is not a multiple of four"); }
+    Call call(*problem, message, message_capacity);
+    if (const int status = call.begin(false, workspace, workspace_bytes, stream)) { return status; }
+    if (empty) {
+        return finish(problem->reduction == FTCUDA_REDUCTION_NONE ? cudaSuccess : cudaMemsetAsync(loss, 0, sizeof(float), static_cast<cudaStream_t>(stream)), message,
+                      message_capacity);
+    }
+    return finish(call.forward(loss, lse), message, message_capacity);
+}
+
+extern "C" int ftcuda_linear_cross_entropy_backward(const FtcudaLinearCrossEntropy* problem, const float* lse, const float* grad_loss, void* grad_hidden,
+                                                    int64_t grad_hidden_row_stride, void* grad_weight, int64_t grad_weight_row_stride, void* workspace,
+                                                    uint64_t workspace_bytes, void* stream, char* message, size_t message_capacity) {
+    using namespace ftcuda;
+    if (problem == nullptr) { return fail(message, message_capacity, 1, "null problem"); }
+    if (const char* reason = check(*problem)) { return fail(message, message_capacity, 1, "%s", reason); }
+    const std::uint64_t bytes = training::elementBytes(problem->element);
+    const std::int64_t depth  = static_cast<std::int64_t>(problem->depth);
+    const bool empty          = problem->tokens == 0;
+    if (!empty && (!wordAligned(lse) || !wordAligned(grad_loss))) { return fail(message, message_capacity, 1, "lse or the loss's gradient has no address, or one that is not a multiple of four"); }
+    if ((grad_hidden != nullptr && !training::aligned(grad_hidden, bytes)) || (grad_weight != nullptr && !training::aligned(grad_weight, bytes))) {
+        return fail(message, message_capacity, 1, "a gradient's address is not a multiple of its element's size");
+    }
+    if (grad_hidden != nullptr && problem->tokens > 1 && (grad_hidden_row_stride < depth || grad_hidden_row_stride >= (1LL << 31))) {
+        return fail(message, message_capacity, 1, "the rows of the hidden states' gradient overlap, or lie too far apart");
+    }
+    if (grad_weight != nullptr && problem->vocabulary > 1 && (grad_weight_row_stride < depth || grad_weight_row_stride >= (1LL << 31))) {
+        return fail(message, message_capacity, 1, "the rows of the weight's gradient overlap, or lie too far apart");
+    }
+    if (problem->vocabulary == 1) { grad_weight_row_stride = depth; }
+    Call call(*problem, message, message_capacity);
+    if (const int status = call.begin(true, workspace, workspace_bytes, stream)) { return status; }
+    if (empty) {
+        if (grad_weight == nullptr) { return 0; }
+        return finish(cudaMemset2DAsync(grad_weight, static_cast<std::size_t>(grad_weight_row_stride) * bytes, 0, problem->depth * bytes, problem->vocabulary,
+                                        static_cast<cudaStream_t>(stream)), message, message_capacity);
+    }
+    if (grad_hidden == nullptr && grad_weight == nullptr) { return 0; }
+    return finish(call.backward(lse, grad_loss, grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride), message, message_capacity);
+}

@@ -1,0 +1,621 @@
+// The products of the linear cross entropy on BF16 or FP16 operands, each with its epilogue (linear_cross_entropy.cu has the whole).
+//
+//   statistics   Z = H W^T; of a tile of Z nothing is kept but the rows' maxima and sums of exponentials
+//   slopes       Z once more; dZ = scale (exp(Z - lse) - onehot), rounded to the operands' type, goes to memory for a piece of the vocabulary
+//   gradients    dH (+)= dZ W and dW = dZ^T H of that piece, in one launch
+//
+// dZ is rounded to 16 bits because the tensor cores take it as an operand of the type that W and H have; half a step (2^-9, 2^-12
+// of each value) is what the gradients' own rounding comes to as well. Its scale brings the largest possible value near 1 (BF16) or 2^14 (FP16, whose
+// exponents would not hold the small probabilities otherwise).
+//
+// One kernel does all three. A pair of CTAs (tcgen05 cta_group::2, a cluster of two) takes tiles of 256 rows and up to 256 columns, K in
+// blocks of 64; a CTA brings its 128 rows of A and its half of B, each as the matrix lies in memory: an operand whose
+// neighbours run along K is a K-major operand, one whose neighbours run along its rows an MN-major one, so nothing is ever transposed.
+//
+//   warp 0       TMA producer (one thread, in both CTAs; the bytes of both count on the first CTA's barrier)
+//   warp 1       MMA issuer (one thread, in the first CTA, for both CTAs' tensor cores)
+//   warps 4-11   epilogue, 32 rows x half of the columns each
+//
+// Tensor memory holds two accumulators of 256 columns: one is filled while the other is read. What the epilogue reads goes to registers at once
+// and the accumulator back to the issuer; a thread has one row, so maxima, sums and the target's column need no
+// exchange between threads, and its output is 256 neighbouring bytes, written 32 at a time.
+//
+// Every wait is bounded, as in the other kernels (ptx.cuh).
+#include "loss_products.hpp"
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "gemm_kernels.hpp"
+#include "ptx.cuh"
+#include "training_common.cuh"
+
+namespace ftcuda {
+namespace loss {
+namespace {
+
+constexpr std::uint32_t kBlockK = 64;  // 128 bytes, one swizzle row
+constexpr std::uint32_t kTileN  = 256;
+constexpr int kStages           = 7;
+constexpr int kThreads          = 384;
+constexpr int kOperandBytes     = 128 * 128;  // a CTA's share of A, and of a B of 256 columns
+constexpr int kStageBytes       = 2 * kOperandBytes;
+constexpr int kBarrierOffset    = kStages * kStageBytes;
+constexpr int kSmemBytes        = kBarrierOffset + 256 + 1024;
+static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
+constexpr std::uint32_t kBoxBytes = 64 * 128;  // 64 rows of 128 bytes: one box of an MN-major operand
+
+constexpr int kRegsLight = 72;   // producer, issuer (warpgroup 0)
+constexpr int kRegsDrain = 216;  // epilogue (warpgroups 1, 2)
+static_assert(128 * kRegsLight + 256 * kRegsDrain <= 168 * kThreads, "the CTA's register pool is what it was launched with");
+constexpr int kProducerWarp  = 0;
+constexpr int kIssuerWarp    = 1;
+constexpr int kFirstEpilogue = 4;
+constexpr std::uint32_t kTmemColumns = 512;
+
+enum Mode : int { kStatistics, kSlopes, kGradients };
+
+struct Barriers {
+    std::uint64_t full[kStages];  // used in the pair's first CTA
+    std::uint64_t empty[kStages];
+    std::uint64_t sum_full[2];
+    std::uint64_t sum_empty[2];   // used in the pair's first CTA
+    std::uint64_t flush;
+    std::uint32_t tmem_base;
+    int abort_flag;
+};
+static_assert(sizeof(Barriers) <= 256, "barrier block");
+
+struct Problem {
+    std::uint32_t rows;          // 0: the live rows
+    std::uint32_t blocks;        // K blocks; 0: those of the live rows
+    std::uint32_t columns, tile_n, tiles_n;
+    std::uint32_t splits, blocks_per_split;
+    std::uint32_t a_along_rows, b_along_rows;  // MN-major
+};
+
+struct ProductParams {
+    Problem problem[2];
+    std::uint32_t problems, band;
+    std::uint32_t instruction;  // the operands' type
+    std::uint32_t bf16, capacity;
+    std::uint32_t first;        // column of the vocabulary that column 0 is
+    LiveRows rows;
+    float2* partials;
+    void* slopes;
+    std::uint64_t slopes_pitch;
+    float* sums;
+    std::uint64_t sums_pitch;
+    std::uint32_t accumulate;
+    std::uint32_t weight_problem;  // which of the problems is the weight's gradient
+    void* weight_gradient;
+    std::int64_t weight_gradient_pitch;
+    std::uint32_t weight_vector;   // elements of it that one aligned store takes: 16, 8, or 1
+    int* status;
+};
+
+struct ProductMaps {
+    CUtensorMap a[2], b[2];
+};
+
+struct Item {
+    std::uint32_t problem, row, col, split, first_block, blocks;
+};
+
+// The launch's tiles, from the number of live rows.
+struct Work {
+    std::uint32_t tiles_m[2], blocks[2], items[2];
+    std::uint32_t total;
+};
+
+__device__ __forceinline__ Work workOf(const ProductParams& p, std::uint32_t live) {
+    live = max(live, 1U);
+    Work w;
+    w.items[1] = 0;
+#pragma unroll
+    for (std::uint32_t i = 0; i < 2; ++i) {
+        if (i < p.problems) {
+            const Problem& problem = p.problem[i];
+            w.tiles_m[i]           = ((problem.rows != 0 ? problem.rows : live) + kTileRows - 1) / kTileRows;
+            w.blocks[i]            = problem.blocks != 0 ? problem.blocks : (live + kBlockK - 1) / kBlockK;
+            w.items[i]             = w.tiles_m[i] * problem.tiles_n * problem.splits;
+        }
+    }
+    w.total = w.items[0] + w.items[1];
+    return w;
+}
+
+__device__ __forceinline__ Item decode(const ProductParams& p, const Work& work, std::uint32_t item) {
+    Item w;
+    w.problem              = item < work.items[0] ? 0 : 1;
+    const Problem& problem = p.problem[w.problem];
+    if (w.problem != 0) { item -= work.items[0]; }
+    const std::uint32_t tiles_m = w.problem != 0 ? work.tiles_m[1] : work.tiles_m[0];
+    const std::uint32_t blocks  = w.problem != 0 ? work.blocks[1] : work.blocks[0];
+    const std::uint32_t tiles   = tiles_m * problem.tiles_n;
+    w.split                     = item / tiles;
+    const std::uint32_t tile    = item - w.split * tiles;
+    const std::uint32_t band    = tile / (p.band * problem.tiles_n);
+    const std::uint32_t first   = band * p.band;
+    const std::uint32_t rows    = min(p.band, tiles_m - first);
+    const std::uint32_t rest    = tile - band * p.band * problem.tiles_n;
+    w.row                       = (first + rest % rows) * kTileRows;
+    w.col                       = rest / rows * problem.tile_n;
+    w.first_block               = w.split * problem.blocks_per_split;
+    w.blocks                    = problem.splits == 1 ? blocks : min(blocks - w.first_block, problem.blocks_per_split);
+    return w;
+}
+
+struct Ring {
+    std::uint32_t slot = 0, round = 0;
+    __device__ __forceinline__ void next() {
+        if (++slot == kStages) {
+            slot = 0;
+            ++round;
+        }
+    }
+};
+
+__device__ __forceinline__ std::uint32_t pack16(float low, float high, bool bf16) {
+    if (bf16) {
+        const __nv_bfloat162 pair = __floats2bfloat162_rn(low, high);
+        return *reinterpret_cast<const std::uint32_t*>(&pair);
+    }
+    const __half2 pair = __floats2half2_rn(low, high);
+    return *reinterpret_cast<const std::uint32_t*>(&pair);
+}
+
+// What a warp does with 32 rows (`row`: this thread's) and 32 * pieces columns from `col` on, held in v.
+__device__ __forceinline__ void finishStatistics(const ProductParams& p, const Item& w, std::uint32_t row, std::uint32_t col, std::uint32_t pieces,
+                                                 std::uint32_t half, std::uint32_t live, float (&v)[128]) {
+    const std::uint32_t columns = p.problem[0].columns;
+    const std::int32_t at       = row < live ? p.rows.target[row] - static_cast<std::int32_t>(col) : -1;
+    const bool here             = at >= 0 && at < static_cast<std::int32_t>(32 * pieces);
+    // Rarely: a target lies among these columns.
+    if (__any_sync(0xFFFFFFFFU, here)) {
+        float picked = 0.0F;
+#pragma unroll
+        for (int j = 0; j < 128; ++j) { picked = j == at ? v[j] : picked; }
+        if (here) { p.rows.picked[row] = picked; }
+    }
+    if (col + 32 * pieces > columns) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j) { v[j] = col + j < columns ? v[j] : -INFINITY; }
+    }
+    float largest = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 128; ++j) {
+        if (j < 64 || pieces == 4) { largest = fmaxf(largest, v[j]); }
+    }
+    const bool none  = largest == -INFINITY;  // and no reference to subtract; sums of nothing (or of NaN) come out
+    const float base = none ? 0.0F : largest * kLog2E;
+    float sum[4] = {0.0F, 0.0F, 0.0F, 0.0F};
+#pragma unroll
+    for (int j = 0; j < 128; ++j) {
+        if (j < 64 || pieces == 4) { sum[j % 4] += exp2Fast(fmaf(v[j], kLog2E, -base)); }
+    }
+    const std::uint32_t piece = 2 * (w.col / p.problem[0].tile_n) + half;
+    p.partials[static_cast<std::uint64_t>(piece) * p.capacity + row] = make_float2(none ? -INFINITY : base, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+}
+
+__device__ __forceinline__ void finishSlopes(const ProductParams& p, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, std::uint32_t live,
+                                             float (&v)[128]) {
+    const bool on            = row < live;
+    const float scale        = on ? p.rows.scale[row] : 0.0F;
+    const float lse2         = on ? p.rows.lse2[row] : 0.0F;
+    const std::int32_t at    = on ? p.rows.target[row] - static_cast<std::int32_t>(p.first + col) : -1;
+    const bool here          = at >= 0 && at < static_cast<std::int32_t>(32 * pieces);
+#pragma unroll
+    for (int j = 0; j < 128; ++j) { v[j] = exp2Fast(fmaf(v[j], kLog2E, -lse2)); }
+    if (__any_sync(0xFFFFFFFFU, here)) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j) { v[j] = j == at ? v[j] - 1.0F : v[j]; }
+    }
+    // The buffer has room for whole tiles; what lies beyond the columns is never fetched.
+    unsigned char* const out = static_cast<unsigned char*>(p.slopes) + (static_cast<std::uint64_t>(row) * p.slopes_pitch + col) * 2;
+#pragma unroll
+    for (int j = 0; j < 128; j += 16) {
+        if (j < 64 || pieces == 4) {
+            std::uint32_t packed[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { packed[i] = on ? pack16(scale * v[j + 2 * i], scale * v[j + 2 * i + 1], p.bf16 != 0) : 0; }
+            storeGlobal8(out + 2 * j, packed);
+        }
+    }
+}
+
+__device__ __forceinline__ void finishSums(const ProductParams& p, const Item& w, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, float (&v)[128]) {
+    float* const at = p.sums + (static_cast<std::uint64_t>(w.split) * p.capacity + row) * p.sums_pitch + col;
+#pragma unroll
+    for (int j = 0; j < 128; j += 8) {
+        if ((j < 64 || pieces == 4) && col + j < p.sums_pitch) {
+            float o[8];
+            if (p.accumulate != 0) {
+                loadGlobal8(at + j, o);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { o[i] += v[j + i]; }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { o[i] = v[j + i]; }
+            }
+            storeGlobal8(at + j, o);
+        }
+    }
+}
+
+__device__ __forceinline__ void finishWeight(const ProductParams& p, const Problem& problem, std::uint32_t row, std::uint32_t col, std::uint32_t pieces,
+                                             float unit, float (&v)[128]) {
+    if (row >= problem.rows) { return; }
+    unsigned char* const at = static_cast<unsigned char*>(p.weight_gradient) + (static_cast<std::int64_t>(row) * p.weight_gradient_pitch + col) * 2;
+#pragma unroll
+    for (int j = 0; j < 128; j += 16) {
+        if (j < 64 || pieces == 4) {
+            std::uint32_t packed[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { packed[i] = pack16(unit * v[j + 2 * i], unit * v[j + 2 * i + 1], p.bf16 != 0); }
+            if (p.weight_vector == 16) {
+                if (col + j < problem.columns) { storeGlobal8(at + 2 * j, packed); }
+            } else if (p.weight_vector == 8) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (col + j + 8 * i < problem.columns) {
+                        *reinterpret_cast<uint4*>(at + 2 * j + 16 * i) = make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (col + j + i < problem.columns) {
+                        *reinterpret_cast<std::uint16_t*>(at + 2 * (j + i)) = static_cast<std::uint16_t>(packed[i / 2] >> (16 * (i % 2)));
+                    }
+                }
+            }
+        }
+    }
+}
+
+template<int kMode>
+__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
+lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ ProductParams p) {
+    extern __shared__ unsigned char smem_raw[];
+    const std::uint32_t align_offset = (1024 - (smemAddress(smem_raw) & 1023)) & 1023;
+    unsigned char* smem              = smem_raw + align_offset;
+    Barriers* bars                   = reinterpret_cast<Barriers*>(smem + kBarrierOffset);
+    volatile int* abort_flag         = &bars->abort_flag;
+    const int warp                   = threadIdx.x >> 5;
+    const int lane                   = threadIdx.x & 31;
+    const std::uint32_t rank         = clusterCtaRank();
+    const std::uint32_t pair         = blockIdx.x >> 1;
+    const std::uint32_t pairs        = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbarrierInit(&bars->full[s], 1);
+            mbarrierInit(&bars->empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbarrierInit(&bars->sum_full[s], 1);
+            mbarrierInit(&bars->sum_empty[s], 16);
+        }
+        mbarrierInit(&bars->flush, 1);
+        bars->abort_flag = 0;
+        fenceBarrierInit();
+        for (std::uint32_t i = 0; i < p.problems; ++i) {
+            prefetchTensorMap(&maps.a[i]);
+            prefetchTensorMap(&maps.b[i]);
+        }
+    }
+    if (warp == kIssuerWarp) { tmemAllocatePair(&bars->tmem_base, kTmemColumns); }
+    tcgen05FenceBeforeSync();
+    __syncthreads();
+    clusterBarrierArrive();
+    clusterBarrierWait();
+    tcgen05FenceAfterSync();
+    const std::uint32_t tmem_base = bars->tmem_base;
+
+    // Launched with programmatic stream serialization: what is above overlaps the predecessor's tail.
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const std::uint32_t live = *p.rows.count;
+    const Work work          = workOf(p, live);
+
+    if (warp >= kFirstEpilogue) {
+        registersGrow<kRegsDrain>();
+        const int e                   = warp - kFirstEpilogue;                    // 0..7
+        const std::uint32_t half      = static_cast<std::uint32_t>(e >> 2);
+        const std::uint32_t in_tile   = static_cast<std::uint32_t>(32 * (warp & 3));  // the tensor-memory lanes a warp can read
+        const std::uint32_t tmem_row  = tmem_base + (in_tile << 16);
+        const std::uint32_t sum_empty[2] = {mapToRank(&bars->sum_empty[0], 0), mapToRank(&bars->sum_empty[1], 0)};
+        const float unit              = kMode == kGradients ? *p.rows.unit : 1.0F;
+        std::uint32_t sums = 0;
+        bool ok = true;
+        for (std::uint32_t item = pair; item < work.total && ok; item += pairs, ++sums) {
+            const Item w                 = decode(p, work, item);
+            const Problem& problem       = p.problem[w.problem];
+            const std::uint32_t pieces   = problem.tile_n / 64;  // of 32 columns, for this warp
+            const std::uint32_t which    = sums & 1;
+            const std::uint32_t row      = w.row + rank * 128 + in_tile + lane;
+            const std::uint32_t col      = w.col + half * 32 * pieces;
+            ok = mbarrierWait(&bars->sum_full[which], (sums >> 1) & 1, abort_flag);
+            if (!ok) { break; }
+            tcgen05FenceAfterSync();
+            float v[128];
+#pragma unroll
+            for (std::uint32_t q = 0; q < 4; ++q) {
+                if (q < pieces) {
+                    float part[32];
+                    tmemLoad32(tmem_row + which * kTileN + half * 32 * pieces + q * 32, part);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) { v[q * 32 + j] = part[j]; }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) { v[q * 32 + j] = 0.0F; }
+                }
+            }
+            tcgen05FenceBeforeSync();
+            __syncwarp();
+            if (lane == 0) { mbarrierArriveCluster(sum_empty[which]); }
+            if (kMode == kStatistics) {
+                finishStatistics(p, w, row, col, pieces, half, live, v);
+            } else if (kMode == kSlopes) {
+                finishSlopes(p, row, col, pieces, live, v);
+            } else if (w.problem == p.weight_problem) {
+                finishWeight(p, problem, row, col, pieces, unit, v);
+            } else {
+                finishSums(p, w, row, col, pieces, v);
+            }
+        }
+        if (!ok) { *abort_flag = 1; }
+    } else {
+        registersShrink<kRegsLight>();
+        if (warp == kProducerWarp) {
+            bool ok = true;
+            if (lane == 0) {
+                Ring ring;
+                std::uint32_t filled = 0;
+                for (std::uint32_t item = pair; item < work.total && ok; item += pairs) {
+                    const Item w                    = decode(p, work, item);
+                    const Problem& problem          = p.problem[w.problem];
+                    const CUtensorMap* const map_a  = &maps.a[w.problem];
+                    const CUtensorMap* const map_b  = &maps.b[w.problem];
+                    const std::int32_t row_a        = static_cast<std::int32_t>(w.row + rank * 128);
+                    const std::int32_t row_b        = static_cast<std::int32_t>(w.col + rank * (problem.tile_n / 2));
+                    const std::uint32_t bytes       = kOperandBytes + problem.tile_n / 2 * 128;
+                    for (std::uint32_t kb = 0; kb < w.blocks; ++kb, ++filled, ring.next()) {
+                        ok = mbarrierWait(&bars->empty[ring.slot], (ring.round & 1) ^ 1, abort_flag);
+                        if (!ok) { break; }
+                        // The bytes of both CTAs count on the first CTA's barrier, which that CTA arms. (The other's
+                        // may land first: the phase cannot complete before it has been armed.)
+                        if (rank == 0) { mbarrierArriveExpectTx(&bars->full[ring.slot], 2 * bytes); }
+                        const std::uint32_t full  = mapToRank(&bars->full[ring.slot], 0);
+                        unsigned char* const slot = smem + ring.slot * kStageBytes;
+                        const std::int32_t k      = static_cast<std::int32_t>((w.first_block + kb) * kBlockK);
+                        if (problem.a_along_rows != 0) {
+                            tmaLoad2dPair(slot, map_a, full, row_a, k);
+                            tmaLoad2dPair(slot + kBoxBytes, map_a, full, row_a + 64, k);
+                        } else {
+                            tmaLoad2dPair(slot, map_a, full, k, row_a);
+                        }
+                        if (problem.b_along_rows != 0) {
+                            tmaLoad2dPair(slot + kOperandBytes, map_b, full, row_b, k);
+                            if (problem.tile_n == kTileN) { tmaLoad2dPair(slot + kOperandBytes + kBoxBytes, map_b, full, row_b + 64, k); }
+                        } else {
+                            tmaLoad2dPair(slot + kOperandBytes, map_b, full, k, row_b);
+                        }
+                    }
+                }
+                // Neither CTA leaves before the last commits have arrived on its barriers.
+                for (std::uint32_t i = 0; i < kStages && i < filled && ok; ++i) {
+                    const std::uint32_t use = filled - 1 - i;
+                    ok = mbarrierWait(&bars->empty[use % kStages], (use / kStages) & 1, abort_flag);
+                }
+                if (!ok) { *abort_flag = 1; }
+            }
+            __syncwarp();
+        } else if (warp == kIssuerWarp && rank == 0) {
+            if (lane == 0) {
+                const std::uint64_t stage_step = kStageBytes >> 4;
+                const std::uint32_t base       = smemAddress(smem);
+                Ring ring;
+                std::uint32_t sums = 0;
+                bool ok            = true;
+                for (std::uint32_t item = pair; item < work.total && ok; item += pairs, ++sums) {
+                    const Item w           = decode(p, work, item);
+                    const Problem& problem = p.problem[w.problem];
+                    const bool a_mn = problem.a_along_rows != 0, b_mn = problem.b_along_rows != 0;
+                    // Sixteen of K are 32 bytes of a K-major tile's rows, or sixteen rows of an MN-major one.
+                    const std::uint64_t a0 = a_mn ? umaDescriptorMn128(base, kBoxBytes) : umaDescriptorK128(base);
+                    const std::uint64_t b0 = b_mn ? umaDescriptorMn128(base + kOperandBytes, kBoxBytes) : umaDescriptorK128(base + kOperandBytes);
+                    const std::uint64_t a_step = a_mn ? 16 * 128 >> 4 : 2, b_step = b_mn ? 16 * 128 >> 4 : 2;
+                    const std::uint32_t instruction =
+                        p.instruction | umaInstructionF16(kTileRows, problem.tile_n) | (a_mn ? kUmaAMnMajor : 0) | (b_mn ? kUmaBMnMajor : 0);
+                    const std::uint32_t which = sums & 1;
+                    const std::uint32_t d     = tmem_base + which * kTileN;
+                    ok = mbarrierWait(&bars->sum_empty[which], ((sums >> 1) & 1) ^ 1, abort_flag);
+                    if (!ok) { break; }
+                    tcgen05FenceAfterSync();
+                    for (std::uint32_t kb = 0; kb < w.blocks; ++kb, ring.next()) {
+                        ok = mbarrierWait(&bars->full[ring.slot], ring.round & 1, abort_flag);
+                        if (!ok) { break; }
+                        tcgen05FenceAfterSync();
+                        const std::uint64_t a = a0 + ring.slot * stage_step, b = b0 + ring.slot * stage_step;
+#pragma unroll
+                        for (std::uint32_t step = 0; step < kBlockK / 16; ++step) {
+                            umaF16Pair(d, a + step * a_step, b + step * b_step, instruction, kb != 0 || step != 0 ? 1U : 0U);
+                        }
+                        umaCommitPair(&bars->empty[ring.slot]);
+                    }
+                    if (!ok) { break; }
+                    umaCommitPair(&bars->sum_full[which]);
+                }
+                if (!ok) {
+                    *abort_flag = 1;
+                    // Let MMAs already issued finish before tensor memory is freed.
+                    umaCommitPair(&bars->flush);
+                    int never = 0;
+                    mbarrierWait(&bars->flush, 0, &never);
+                }
+            }
+            __syncwarp();
+        }
+    }
+
+    __syncthreads();
+    if (*abort_flag != 0) {
+        if (threadIdx.x == 0) {
+            if (p.status != nullptr) { *p.status = 2; }
+            // Copies that were armed but never consumed may still be landing (their bytes count on the
+            // first CTA's barriers; the second waits for the first below).
+            int never = 0;
+            for (int s = 0; s < kStages && rank == 0; ++s) {
+                mbarrierWait(&bars->full[s], 0, &never);
+                mbarrierWait(&bars->full[s], 1, &never);
+            }
+        }
+        __syncthreads();
+    }
+    tcgen05FenceBeforeSync();
+    clusterBarrierArrive();
+    clusterBarrierWait();
+    if (warp == kIssuerWarp) {
+        tcgen05FenceAfterSync();
+        tmemFreePair(tmem_base, kTmemColumns);
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+std::uint32_t divideUp(std::uint32_t x, std::uint32_t y) { return (x + y - 1) / y; }
+
+// 128 columns where that is all there are: B's tile is half as wide then.
+std::uint32_t tileColumns(std::uint32_t columns) { return columns <= 128 ? 128 : kTileN; }
+
+// An operand whose rows (of the product) are `rows` and whose depth is `k`: neighbours along K, or along the rows.
+bool encodeOperand(CUtensorMap* map, const ProductCall& call, Matrix16 matrix, bool along_rows, std::uint32_t rows, std::uint32_t k, std::uint32_t tile_rows) {
+    return along_rows ? encodeMap16(map, call.bf16, matrix.at, rows, k, matrix.pitch * 2, 64, call.message, call.message_capacity)
+                      : encodeMap16(map, call.bf16, matrix.at, k, rows, matrix.pitch * 2, tile_rows, call.message, call.message_capacity);
+}
+
+template<int kMode> cudaError_t launch(const ProductCall& call, const ProductMaps& maps, const ProductParams& p, std::uint64_t items) {
+    cudaError_t error = cudaFuncSetAttribute(lossProduct<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (error != cudaSuccess) { return error; }
+    const std::uint64_t pairs = std::max<std::uint64_t>(1, std::min<std::uint64_t>(static_cast<std::uint64_t>(call.sms) / 2, items));
+    return training::launchOverlapped(lossProduct<kMode>, dim3(static_cast<unsigned>(2 * pairs)), dim3(kThreads), kSmemBytes, call.stream, maps, p);
+}
+
+ProductParams paramsFor(const ProductCall& call) {
+    ProductParams p{};
+    p.problems       = 1;
+    p.band           = 8;
+    p.instruction    = call.bf16 ? kUmaBf16 : 0;
+    p.bf16           = call.bf16 ? 1 : 0;
+    p.capacity       = call.capacity;
+    p.rows           = call.rows;
+    p.status         = call.status;
+    p.weight_problem = 2;
+    return p;
+}
+
+// Z = H W^T over `columns` rows of the weight.
+bool describeLogits(const ProductCall& call, Matrix16 weight, std::uint32_t columns, ProductMaps& maps, ProductParams& p) {
+    Problem& problem          = p.problem[0];
+    problem.columns           = columns;
+    problem.tile_n            = tileColumns(columns);
+    problem.tiles_n           = divideUp(columns, problem.tile_n);
+    problem.blocks            = divideUp(call.depth, kBlockK);
+    problem.splits            = 1;
+    problem.blocks_per_split  = problem.blocks;
+    return encodeOperand(&maps.a[0], call, call.hidden, false, call.capacity, call.depth, 128) &&
+           encodeOperand(&maps.b[0], call, weight, false, columns, call.depth, problem.tile_n / 2);
+}
+
+}  // namespace
+
+std::uint32_t statisticsPieces(std::uint32_t columns) { return 2 * divideUp(columns, tileColumns(columns)); }
+
+cudaError_t launchStatistics(const ProductCall& call, Matrix16 weight, std::uint32_t vocabulary, float2* partials) {
+    ProductMaps maps;
+    ProductParams p = paramsFor(call);
+    p.partials      = partials;
+    if (!describeLogits(call, weight, vocabulary, maps, p)) { return cudaErrorInvalidValue; }
+    return launch<kStatistics>(call, maps, p, static_cast<std::uint64_t>(call.capacity / kTileRows) * p.problem[0].tiles_n);
+}
+
+cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, std::uint64_t slopes_pitch) {
+    ProductMaps maps;
+    ProductParams p = paramsFor(call);
+    p.first         = first;
+    p.slopes        = slopes;
+    p.slopes_pitch  = slopes_pitch;
+    if (!describeLogits(call, weight, columns, maps, p)) { return cudaErrorInvalidValue; }
+    return launch<kSlopes>(call, maps, p, static_cast<std::uint64_t>(call.capacity / kTileRows) * p.problem[0].tiles_n);
+}
+
+// With few tiles the sum over the columns is cut until there are about two items for each pair of SMs, eight K blocks each at least.
+std::uint32_t hiddenSplits(std::uint32_t capacity, std::uint32_t depth, std::uint32_t columns, int sms) {
+    const std::uint32_t tiles = capacity / kTileRows * divideUp(depth, tileColumns(depth));
+    const std::uint32_t pairs = static_cast<std::uint32_t>(std::max(1, sms / 2));
+    const std::uint32_t blocks = divideUp(columns, kBlockK);
+    const std::uint32_t wanted = std::min({std::max(1U, blocks / 8), 16U, std::max(1U, 2 * pairs / tiles)});
+    return divideUp(blocks, divideUp(blocks, wanted));  // none of them empty
+}
+
+cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint32_t columns, const void* slopes, std::uint64_t slopes_pitch,
+                            const Gradients& gradients) {
+    ProductMaps maps;
+    ProductParams p = paramsFor(call);
+    p.problems      = 0;
+    const Matrix16 slope_matrix{slopes, slopes_pitch};
+    std::uint64_t items        = 0;
+    const std::uint32_t tile_n = tileColumns(call.depth), tiles_n = divideUp(call.depth, tile_n);
+    bool encoded = true;
+    if (gradients.sums != nullptr) {
+        Problem& problem          = p.problem[p.problems];
+        problem.columns           = call.depth;
+        problem.tile_n            = tile_n;
+        problem.tiles_n           = tiles_n;
+        problem.blocks            = divideUp(columns, kBlockK);
+        problem.blocks_per_split  = divideUp(problem.blocks, gradients.splits);
+        problem.splits            = divideUp(problem.blocks, problem.blocks_per_split);
+        problem.b_along_rows      = 1;
+        p.sums                    = gradients.sums;
+        p.sums_pitch              = gradients.sums_pitch;
+        p.accumulate              = gradients.accumulate ? 1 : 0;
+        encoded = encodeOperand(&maps.a[p.problems], call, slope_matrix, false, call.capacity, columns, 128) &&
+                  encodeOperand(&maps.b[p.problems], call, weight, true, call.depth, columns, 64);
+        items += static_cast<std::uint64_t>(call.capacity / kTileRows) * tiles_n * problem.splits;
+        ++p.problems;
+    }
+    if (encoded && gradients.weight_gradient != nullptr) {
+        Problem& problem          = p.problem[p.problems];
+        problem.rows              = columns;
+        problem.columns           = call.depth;
+        problem.tile_n            = tile_n;
+        problem.tiles_n           = tiles_n;
+        problem.splits            = 1;
+        problem.a_along_rows      = 1;
+        problem.b_along_rows      = 1;
+        p.weight_problem          = p.problems;
+        p.weight_gradient         = gradients.weight_gradient;
+        p.weight_gradient_pitch   = gradients.weight_gradient_pitch;
+        const auto fits = [&](std::uint32_t n) {
+            return call.depth % n == 0 && gradients.weight_gradient_pitch % n == 0 && training::aligned(gradients.weight_gradient, 2 * n);
+        };
+        p.weight_vector = fits(16) ? 16 : fits(8) ? 8 : 1;
+        encoded = encodeOperand(&maps.a[p.problems], call, slope_matrix, true, columns, call.capacity, 128) &&
+                  encodeOperand(&maps.b[p.problems], call, call.hidden, true, call.depth, call.capacity, 64);
+        items += static_cast<std::uint64_t>(divideUp(columns, kTileRows)) * tiles_n;
+        ++p.problems;
+    }
+    if (!encoded) { return cudaErrorInvalidValue; }
+    if (p.problems == 0) { return cudaSuccess; }
+    return launch<kGradients>(call, maps, p, items);
+}
+
+}  // namespace loss
+}  // namespace ftcuda

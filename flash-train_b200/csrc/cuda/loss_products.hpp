@@ -1,0 +1,80 @@
+// The products of the linear cross entropy on 16-bit operands (loss_products.cu), as linear_cross_entropy.cu calls them.
+#ifndef FTCUDA_LOSS_PRODUCTS_HPP_
+#define FTCUDA_LOSS_PRODUCTS_HPP_
+
+#include <cuda_runtime_api.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace ftcuda {
+namespace loss {
+
+constexpr std::uint32_t kTileRows = 256;  // rows of a CTA pair's tile; the live tokens' arrays are filled up to a multiple of it
+constexpr float kLog2E            = 1.4426950408889634F;
+constexpr float kLn2              = 0.6931471805599453F;
+
+// The tokens that have a target, in their order. Behind the last one, up to a multiple of kTileRows (one at least), stand
+// neutral rows: hidden state 0, target -1, scale 0.
+struct LiveRows {
+    std::uint32_t* count;
+    float* unit;            // what a sum of products of slopes is multiplied by in the end: a power of two
+    std::int32_t* token;    // the token a row is of
+    std::int32_t* target;   // its column, -1 for none, kBadTarget for one outside of the vocabulary
+    float* scale;           // upstream gradient of the row's loss over `unit`
+    float* lse2;            // log2 of the row's sum of exponentials
+    float* picked;          // the logit of the target
+};
+constexpr std::int32_t kBadTarget = -2;
+
+// A matrix of 16-bit elements in memory, rows of neighbours.
+struct Matrix16 {
+    const void* at;
+    std::uint64_t pitch;  // elements between rows
+};
+
+struct ProductCall {
+    bool bf16;
+    std::uint32_t capacity;   // rows that the live arrays have room for, a multiple of kTileRows
+    std::uint32_t depth;      // elements of a hidden state
+    LiveRows rows;
+    Matrix16 hidden;          // [capacity][depth]: the live rows' hidden states
+    int* status;
+    int sms;
+    cudaStream_t stream;
+    char* message;
+    std::size_t message_capacity;
+};
+
+// Columns of the vocabulary that one partial result of the statistics covers, and how many of those there are.
+std::uint32_t statisticsPieces(std::uint32_t columns);
+
+// For every live row and piece of columns: {largest logit times log2 e, sum of 2^(logit log2 e - that)} to
+// partials[piece][capacity]; and the target's logit to rows.picked.
+cudaError_t launchStatistics(const ProductCall& call, Matrix16 weight, std::uint32_t vocabulary, float2* partials);
+
+// slopes[row][column - first] = scale (2^(logit log2 e - lse2) - [column is the target]) for `columns` columns from `first` on;
+// `weight` starts at row `first`. The pitch is a multiple of 256.
+cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, std::uint64_t slopes_pitch);
+
+// How many parts the sum over `columns` columns is cut into for the gradient of the hidden states. (Over fewer columns
+// launchGradients may fill fewer of them, never more.)
+std::uint32_t hiddenSplits(std::uint32_t capacity, std::uint32_t depth, std::uint32_t columns, int sms);
+
+struct Gradients {
+    // hidden: sums[split][capacity][pitch] (+)= slopes times weight; NULL when not wanted.
+    float* sums;
+    std::uint64_t sums_pitch;  // a multiple of 8
+    std::uint32_t splits;
+    bool accumulate;
+    // weight: rows of the piece = unit * slopes^T times hidden; NULL when not wanted.
+    void* weight_gradient;
+    std::int64_t weight_gradient_pitch;
+};
+cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint32_t columns, const void* slopes, std::uint64_t slopes_pitch,
+                            const Gradients& gradients);
+
+}  // namespace loss
+}  // namespace ftcuda
+
+#endif

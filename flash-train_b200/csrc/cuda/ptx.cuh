@@ -398,6 +398,19 @@ __device__ __forceinline__ void storeGlobal8(float* to, const float (&in)[8]) {
                  : "memory");
 }
 
+__device__ __forceinline__ void storeGlobal8(void* to, const std::uint32_t (&in)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(in[0]), "r"(in[1]), "r"(in[2]), "r"(in[3]), "r"(in[4]),
+                 "r"(in[5]), "r"(in[6]), "r"(in[7])
+                 : "memory");
+}
+
+// 2^x, within two units of the last place; results under 2^-126 are 0.
+__device__ __forceinline__ float exp2Fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // ---------------------------------------------------------------- CTA pairs (tcgen05 cta_group::2)
 // Two CTAs of a cluster of two, on neighbouring SMs, share one MMA: 256 rows of D, 128 in each CTA's tensor
 // memory, A's rows and half of B's rows from each CTA's shared memory at the same offsets.
@@ -435,6 +448,27 @@ __device__ __forceinline__ void tmaLoad3dPair(void* smem_destination, const void
         "l"(reinterpret_cast<std::uint64_t>(tensor_map)), "r"(barrier), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
+
+// The same for a 2-D tile; x * the element's size must be a multiple of 16 bytes.
+__device__ __forceinline__ void tmaLoad2dPair(void* smem_destination, const void* tensor_map, std::uint32_t barrier, std::int32_t x, std::int32_t y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(smemAddress(smem_destination)),
+        "l"(reinterpret_cast<std::uint64_t>(tensor_map)), "r"(barrier), "r"(x), "r"(y)
+        : "memory");
+}
+
+// Shared-memory operand descriptor for an MN-major tile of 16-bit elements with the 128-byte swizzle: rows of 128 bytes hold 64
+// consecutive MN elements at one k; eight consecutive k form a swizzle atom of 1024 bytes (what a TMA load of a box of 64 (MN) x 8j (K)
+// leaves, j atoms one after another). `mn_atom_bytes` is the distance to the next 64 MN elements ("leading" offset, bits
+// [16,30)); the next eight k lie 1024 bytes on ("stride" offset, bits [32,46)). Layout code 2 in bits [61,64).
+__device__ __forceinline__ std::uint64_t umaDescriptorMn128(std::uint32_t smem_address, std::uint32_t mn_atom_bytes) {
+    return umaDescriptorK128(smem_address) | static_cast<std::uint64_t>((mn_atom_bytes >> 4) & 0x3FFF) << 16;
+}
+
+// Bits of the instruction descriptor: both operands BF16 instead of FP16; the A operand MN-major.
+constexpr std::uint32_t kUmaBf16     = (1u << 7) | (1u << 10);
+constexpr std::uint32_t kUmaAMnMajor = 1u << 15;
 
 // Instruction descriptor for kind::f16 with FP16 operands (format 0), FP32 accumulation, both operands K-major.
 __host__ __device__ constexpr std::uint32_t umaInstructionF16(std::uint32_t m, std::uint32_t n) {

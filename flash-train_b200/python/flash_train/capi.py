@@ -54,7 +54,8 @@ PLATFORM_SYMBOLS = (
     "ftcuda_device_status ftcuda_device_status_reset ftcuda_selftest_bounded_wait ftcuda_measure_ffma_tflops "
     "ftcuda_grouped_gemm_supports ftcuda_grouped_gemm_configure ftcuda_grouped_gemm_workspace_bytes "
     "ftcuda_grouped_gemm_launch ftcuda_grouped_gemm_destroy ftcuda_gradient_norm_workspace_bytes ftcuda_gradient_norm "
-    "ftcuda_gradient_clip ftcuda_expert_routing_workspace_bytes ftcuda_expert_routing ftcuda_expert_routing_backward"
+    "ftcuda_gradient_clip ftcuda_expert_routing_workspace_bytes ftcuda_expert_routing ftcuda_expert_routing_backward "
+    "ftcuda_linear_cross_entropy_workspace_bytes ftcuda_linear_cross_entropy ftcuda_linear_cross_entropy_backward"
 ).split()
 
 
@@ -621,6 +622,9 @@ ELEMENT_FP16 = 7
 ELEMENT_BF16 = 8
 NORM_2 = 0
 NORM_INF = 1
+REDUCTION_NONE = 0
+REDUCTION_MEAN = 1
+REDUCTION_SUM = 2
 
 
 class Gradient(Structure):
@@ -629,6 +633,16 @@ class Gradient(Structure):
     _fields_ = [
         ("data", c_void_p), ("out", c_void_p), ("rows", c_uint64), ("cols", c_uint64),
         ("row_stride", c_int64), ("out_row_stride", c_int64), ("element", ctypes.c_int32), ("out_element", ctypes.c_int32),
+    ]
+
+
+class LinearCrossEntropy(Structure):
+    """FtcudaLinearCrossEntropy."""
+
+    _fields_ = [
+        ("hidden", c_void_p), ("weight", c_void_p), ("target", c_void_p), ("tokens", c_uint64), ("vocabulary", c_uint64), ("depth", c_uint64),
+        ("hidden_row_stride", c_int64), ("weight_row_stride", c_int64), ("ignore_index", c_int64),
+        ("element", ctypes.c_int32), ("reduction", ctypes.c_int32), ("device", ctypes.c_int32),
     ]
 
 
@@ -652,7 +666,12 @@ def _declare_training(lib) -> None:
     lib.ftcuda_expert_routing_workspace_bytes.restype = c_uint64
     lib.ftcuda_expert_routing.argtypes = [POINTER(Routing)] + [c_void_p] * 5 + work
     lib.ftcuda_expert_routing_backward.argtypes = [POINTER(Routing)] + [c_void_p] * 7 + [c_int64, c_void_p] + message
-    for name in ("ftcuda_gradient_norm", "ftcuda_gradient_clip", "ftcuda_expert_routing", "ftcuda_expert_routing_backward"):
+    problem = [POINTER(LinearCrossEntropy)]
+    lib.ftcuda_linear_cross_entropy_workspace_bytes.argtypes = problem + [ctypes.c_int, POINTER(c_uint64)] + message
+    lib.ftcuda_linear_cross_entropy.argtypes = problem + [c_void_p] * 2 + work
+    lib.ftcuda_linear_cross_entropy_backward.argtypes = problem + [c_void_p] * 3 + [c_int64, c_void_p, c_int64] + work
+    for name in ("ftcuda_gradient_norm", "ftcuda_gradient_clip", "ftcuda_expert_routing", "ftcuda_expert_routing_backward",
+                 "ftcuda_linear_cross_entropy_workspace_bytes", "ftcuda_linear_cross_entropy", "ftcuda_linear_cross_entropy_backward"):
         getattr(lib, name).restype = ctypes.c_int
 
 
@@ -699,3 +718,21 @@ def expert_routing_backward(routing: Routing, weights: int, experts: int, counts
     """ftcuda_expert_routing_backward; 0 for grad_weights or grad_loss means that it is zero."""
     _run_training(lib.ftcuda_expert_routing_backward, byref(routing), weights, experts, counts, routed, grad_weights, grad_loss, grad_logits,
                   grad_row_stride, stream)
+
+
+def linear_cross_entropy_workspace_bytes(problem: LinearCrossEntropy, backward: bool) -> int:
+    size = c_uint64()
+    _run_training(lib.ftcuda_linear_cross_entropy_workspace_bytes, byref(problem), int(backward), byref(size))
+    return int(size.value)
+
+
+def linear_cross_entropy(problem: LinearCrossEntropy, loss: int, lse: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    """ftcuda_linear_cross_entropy; everything but `problem` and the size is a device address."""
+    _run_training(lib.ftcuda_linear_cross_entropy, byref(problem), loss, lse, workspace, workspace_bytes, stream)
+
+
+def linear_cross_entropy_backward(problem: LinearCrossEntropy, lse: int, grad_loss: int, grad_hidden: int, grad_hidden_row_stride: int, grad_weight: int,
+                                  grad_weight_row_stride: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    """ftcuda_linear_cross_entropy_backward; 0 for a gradient that is not wanted."""
+    _run_training(lib.ftcuda_linear_cross_entropy_backward, byref(problem), lse, grad_loss, grad_hidden, grad_hidden_row_stride, grad_weight,
+                  grad_weight_row_stride, workspace, workspace_bytes, stream)

@@ -1,6 +1,7 @@
 """PyTorch binding: `gemm(a, b, c=None, alpha=1.0, beta=0.0) -> Tensor`, plus
 `HostGemm` / `gemm_host` for operands in pinned host memory (host_pipeline.py), and what a
-training step does around its products: `expert_routing`, `grad_norm`, `clip_grads` and `clip_grad_norm_`.
+training step does around its products:
+`linear_cross_entropy`, `expert_routing`, `grad_norm`, `clip_grads` and `clip_grad_norm_`.
 
 Signature, defaults, checks and error type (RuntimeError) are those of the
 reference binding (python/flash_train/torch/csrc/flash_train_torch.cpp:34-75
@@ -24,7 +25,7 @@ if not os.path.exists(_native_library):
 ctypes.CDLL(_native_library, mode=ctypes.RTLD_GLOBAL)
 
 try:
-    from ._flash_train_torch import clip_grads, gemm, grad_norm, last_message
+    from ._flash_train_torch import clip_grads, gemm, grad_norm, last_message, linear_cross_entropy
 except ModuleNotFoundError as exc:
     if exc.name != "flash_train.torch._flash_train_torch":
         raise
@@ -37,4 +38,4 @@ from .host_pipeline import HostGemm, band_ranges, gemm_host  # noqa: E402
 from .routing import ExpertRouting, expert_routing  # noqa: E402
 
 __all__ = ["gemm", "last_message", "HostGemm", "gemm_host", "band_ranges", "grad_norm", "clip_grads", "clip_grad_norm_",
-           "expert_routing", "ExpertRouting"]
+           "expert_routing", "ExpertRouting", "linear_cross_entropy"]

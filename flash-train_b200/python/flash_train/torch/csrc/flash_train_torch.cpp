@@ -289,6 +289,7 @@ PYBIND11_MODULE(_flash_train_torch, m) {
     m.doc() = "flash-train PyTorch bindings";
     m.def("gemm", &gemm, "d = alpha * (a @ b) + beta * c on the current stream", py::arg("a"), py::arg("b"),
           py::arg("c") = std::nullopt, py::arg("alpha") = 1.0, py::arg("beta") = 0.0);
+    flash_train_torch::registerLinearCrossEntropy(m);
     flash_train_torch::registerGradientNorm(m);
     flash_train_torch::registerExpertRouting(m);
     m.def("last_message", &lastMessage, "diagnostic message of the calling thread's last failed library call");

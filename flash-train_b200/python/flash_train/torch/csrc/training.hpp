@@ -8,6 +8,7 @@ namespace flash_train_torch {
 
 void registerGradientNorm(pybind11::module_& module);
 void registerExpertRouting(pybind11::module_& module);
+void registerLinearCrossEntropy(pybind11::module_& module);
 
 // Room for a reason from the library.
 struct Message {

@@ -1,6 +1,6 @@
 /*
- * ftcuda/training.h -- what a training step does around its products: the experts' router,
- * the gradients' norm.
+ * ftcuda/training.h -- what a training step does around its products: the loss over a large
+ * vocabulary, the experts' router, the gradients' norm.
  *
  * Same manner as ftcuda/ftcuda.h: plain pointers, integers and fixed-size structs; no C++ types, no
  * exceptions; 0 = success, nonzero = failure with a NUL-terminated reason in the caller's message
@@ -24,6 +24,57 @@ enum {
     FTCUDA_ELEMENT_FP16 = 7,
     FTCUDA_ELEMENT_BF16 = 8,
 };
+
+/* ---- the cross entropy of a product with a large vocabulary ---- */
+
+enum {
+    FTCUDA_REDUCTION_NONE = 0, /* a loss for each token */
+    FTCUDA_REDUCTION_MEAN = 1, /* their sum over the number of tokens that have a target; 0 where none has */
+    FTCUDA_REDUCTION_SUM  = 2,
+};
+
+/*
+ * logits[t][v] = hidden[t] . weight[v],  loss[t] = log(sum_v exp(logits[t][v])) - logits[t][target[t]].
+ * The logits are never in memory, but for a piece of the vocabulary at a time in the backward call (and, for FP32 operands, the forward
+ * call).
+ *   - hidden [tokens][depth], weight [vocabulary][depth]: unit stride along the depth, the others any that keep rows apart; both
+ *     of one type. BF16 and FP16 are multiplied by the tensor cores with FP32 sums; FP32 by the library's FP32 products.
+ *   - target [tokens]: INT64. A token whose target is ignore_index takes no part: its loss and gradient are 0, whatever its hidden
+ *     state holds, and (BF16, FP16) nothing is computed for it. Any other target outside of [0, vocabulary) makes the token's loss NaN, and
+ *     the gradients too.
+ *   - a gradient's rounding: with BF16 and FP16 operands the logits' gradients are rounded to that type before they are
+ *     multiplied, at a scale that keeps FP16's range, and the products' sums once at the end.
+ * Sums are in an order that depends on the sizes and on which tokens take part alone: equal calls give equal bits.
+ */
+typedef struct {
+    const void* hidden;
+    const void* weight;
+    const int64_t* target;
+    uint64_t tokens, vocabulary, depth;
+    int64_t hidden_row_stride, weight_row_stride;
+    int64_t ignore_index;
+    int32_t element;
+    int32_t reduction;
+    int32_t device;
+} FtcudaLinearCrossEntropy;
+
+/* Bytes of workspace that the forward (backward = 0) or the backward call needs. */
+FTCUDA_API int ftcuda_linear_cross_entropy_workspace_bytes(const FtcudaLinearCrossEntropy* problem, int backward, uint64_t* workspace_bytes, char* message,
+                                                           size_t message_capacity);
+
+/* loss: FP32, one number, or [tokens] without reduction; lse: FP32 [tokens], the logarithm of each token's sum (0 for a token that takes no
+ * part), which the backward call wants back. The workspace starts at a multiple of 256. */
+FTCUDA_API int ftcuda_linear_cross_entropy(const FtcudaLinearCrossEntropy* problem, float* loss, float* lse, void* workspace, uint64_t workspace_bytes,
+                                           void* stream, char* message, size_t message_capacity);
+
+/*
+ * The gradients of hidden and weight, each of the operands' type and dense along the depth; either may be NULL (not wanted).
+ * grad_loss: FP32 on the device, in the loss's shape. They are written, not added to.
+ */
+FTCUDA_API int ftcuda_linear_cross_entropy_backward(const FtcudaLinearCrossEntropy* problem, const float* lse, const float* grad_loss, void* grad_hidden,
+                                                    int64_t grad_hidden_row_stride, void* grad_weight, int64_t grad_weight_row_stride,
+                                                    void* workspace, uint64_t workspace_bytes, void* stream, char* message,
+                                                    size_t message_capacity);
 
 /* ---- the norm over many tensors, and clipping ---- */
 

@@ -1,0 +1,361 @@
+"""linear_cross_entropy and its gradients against the definition in 64 bits."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+
+STEP = 2.0 ** -24  # half a step of FP32
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def ft(native_library):
+    if not torch.cuda.is_available():
+        pytest.fail("the GPU tests need a CUDA device")
+    from conftest import load_build_module
+
+    load_build_module().build_torch_binding(verbose=False)
+    import flash_train.torch
+
+    return flash_train.torch
+
+
+def make(tokens, depth, vocabulary, dtype, seed=0, spread=2.0):
+    generator = torch.Generator(device="cuda").manual_seed(seed)
+    hidden = torch.randn(tokens, depth, device="cuda", generator=generator).to(dtype)
+    weight = (torch.randn(vocabulary, depth, device="cuda", generator=generator) * spread * depth ** -0.5).to(dtype)
+    target = torch.randint(0, vocabulary, (tokens,), device="cuda", generator=generator)
+    return hidden, weight, target
+
+
+class Oracle:
+    """The definition in 64 bits, and how far FP32 sums and the stated roundings can be from it.
+
+    A logit is a sum of `depth` products: with n terms added one after another (the tensor cores add 8 or 16 at a time, and cut off
+    instead of rounding: two half steps each) it is off by at most (n / 8 + 8) 2^-23 of the sum of the products' magnitudes. That
+    allows as well for the products of split FP32 operands. An exponential is off by its argument's error, by two steps of its
+    own and by the argument's rounding, whose size is that of the logits (in powers of two)."""
+
+    def __init__(self, hidden, weight, target, ignore_index=-100):
+        self.live = target != ignore_index
+        self.h = torch.where(self.live[:, None], hidden.double(), 0.0)
+        self.w = weight.double()
+        self.target = torch.where(self.live, target, 0)
+        z = self.h @ self.w.T
+        self.lse = torch.logsumexp(z, 1)
+        self.loss = torch.where(self.live, self.lse - z.gather(1, self.target[:, None])[:, 0], 0.0)
+        depth = hidden.shape[1]
+        z_error = (depth / 8 + 8) * 2 * STEP * (self.h.abs() @ self.w.abs().T).amax(1)
+        size = z.abs().amax(1) + self.lse.abs()
+        self.relative = 2 * z_error + (32 + 4 * size) * 2 * STEP  # of an exponential against the sum
+        self.loss_error = torch.where(self.live, self.relative + 4 * size * STEP, 0.0)
+        self.z = z
+
+    def gradients(self, grad, dtype):
+        """For upstream gradients `grad` of each token: (dH, its bound, dW, its bound), the roundings of the results to `dtype` among them."""
+        grad = torch.where(self.live, grad.double(), 0.0)
+        slope = torch.exp(self.z - self.lse[:, None])
+        error = slope * self.relative[:, None]
+        slope.scatter_add_(1, self.target[:, None], torch.full_like(self.lse, -1.0)[:, None])
+        half_step = torch.finfo(dtype).eps / 2
+        # The slopes' rounding; and the smallest that FP16 holds at its scale of 2^13 for the largest gradient.
+        error += (half_step + 4 * STEP) * slope.abs()
+        slope *= grad[:, None]
+        error *= grad.abs()[:, None]
+        # Below 2^-126, FP32's smallest normal number, exponentials come out as 0, and so may operands of the products: with p < 2^-126 the
+        # slope g p is off by |g p| < 2^-126 |g|, with |g p| < 2^-126 by less than that.
+        error += (grad.abs()[:, None] + 1.0) * 2.0 ** -126
+        if dtype == torch.float16:
+            error += grad.abs().max() * 2.0 ** -38
+        vocabulary, tokens = self.w.shape[0], self.h.shape[0]
+        finfo = torch.finfo(dtype)
+        out = []
+        for a, e, b, terms in ((slope, error, self.w, vocabulary), (slope.T, error.T, self.h, tokens)):
+            value = a @ b
+            bound = (e + (terms / 8 + 24) * 2 * STEP * a.abs()) @ b.abs() + half_step * value.abs() * 1.01 + finfo.smallest_normal * finfo.eps
+            out += [value, bound]
+        return out
+
+
+def check(got, value, bound, what):
+    error = (got.double() - value).abs() - bound
+    assert torch.isfinite(got).all() and (error <= 0).all(), f"{what}: {error.max().item():.3g} beyond a bound of {bound.max().item():.3g}"
+
+
+def run(ft, hidden, weight, target, reduction="mean", upstream=None, **options):
+    h, w = hidden.detach().requires_grad_(), weight.detach().requires_grad_()
+    loss = ft.linear_cross_entropy(h, w, target, reduction=reduction, **options)
+    upstream = torch.ones_like(loss) if upstream is None else upstream
+    return loss.detach(), *torch.autograd.grad(loss, (h, w), upstream)
+
+
+def run_and_check(ft, hidden, weight, target, reduction="mean", scale=1.0, ignore_index=-100):
+    tokens = hidden.shape[0]
+    oracle = Oracle(hidden, weight, target, ignore_index)
+    count = max(1, int(oracle.live.sum()))
+    if reduction == "none":
+        upstream = torch.randn(tokens, device="cuda", generator=torch.Generator(device="cuda").manual_seed(9)) * scale
+        each = upstream
+    else:
+        upstream = torch.tensor(scale, device="cuda")
+        each = torch.full((tokens,), scale / (count if reduction == "mean" else 1), device="cuda", dtype=torch.float64)
+    loss, grad_hidden, grad_weight = run(ft, hidden, weight, target, reduction, upstream, ignore_index=ignore_index)
+    assert loss.dtype == torch.float32 and grad_hidden.dtype == hidden.dtype and grad_weight.dtype == weight.dtype
+    if reduction == "none":
+        check(loss, oracle.loss, oracle.loss_error, "loss")
+    else:
+        divisor = count if reduction == "mean" else 1
+        total = oracle.loss.sum() / divisor
+        check(loss, total, oracle.loss_error.sum() / divisor + 2 * STEP * total.abs(), "loss")
+    dh, dh_bound, dw, dw_bound = oracle.gradients(each, hidden.dtype)
+    check(grad_hidden, dh, dh_bound, "hidden's gradient")
+    check(grad_weight, dw, dw_bound, "weight's gradient")
+    assert not grad_hidden[~oracle.live].any()
+    return loss, grad_hidden, grad_weight
+
+
+SIZES = [(1, 64, 128), (1, 1, 1), (2, 8, 1), (5, 16, 2), (1, 4096, 300), (3, 100, 17), (33, 65, 131), (64, 128, 129), (255, 72, 257), (256, 64, 256), (257, 200, 1000),
+         (300, 512, 2049), (513, 33, 700), (1000, 1024, 3000), (90, 130, 20011)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens, depth, vocabulary", SIZES)
+def test_against_the_definition(ft, tokens, depth, vocabulary, dtype):
+    hidden, weight, target = make(tokens, depth, vocabulary, dtype)
+    run_and_check(ft, hidden, weight, target, scale=64.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_reductions(ft, dtype, reduction):
+    hidden, weight, target = make(170, 96, 450, dtype, seed=2)
+    target[::3] = -100
+    target[5:20] = 7
+    run_and_check(ft, hidden, weight, target, reduction)
+    target[target == 7] = -1
+    run_and_check(ft, hidden, weight, target.clamp(min=-1), reduction, ignore_index=-1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_upstream_gradients_of_any_size(ft, dtype):
+    """The slopes' scale follows the largest upstream gradient; small ones beside it, and zeros, keep their own precision in BF16 and FP32."""
+    hidden, weight, target = make(100, 64, 300, dtype, seed=3)
+    for scale in ((1e-30, 1e-3, 1.0, 1e4) if dtype != torch.float16 else (1e-3, 1.0, 50.0)):
+        run_and_check(ft, hidden, weight, target, "none", scale)
+    zero = torch.zeros(100, device="cuda")
+    _, grad_hidden, grad_weight = run(ft, hidden, weight, target, "none", zero)
+    assert not grad_hidden.any() and not grad_weight.any()
+    bad = zero.clone()
+    bad[3] = math.inf
+    _, grad_hidden, _ = run(ft, hidden, weight, target, "none", bad)
+    assert not torch.isfinite(grad_hidden[3]).any() and not grad_hidden[4].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_what_padding_holds_does_not_matter(ft, dtype):
+    hidden, weight, target = make(600, 80, 333, dtype, seed=4)
+    target[100:400] = -100
+    target[599] = -100
+    expected = run_and_check(ft, hidden, weight, target)
+    hidden[target == -100] = math.nan
+    hidden[150] = math.inf
+    got = run(ft, hidden, weight, target)
+    assert all(torch.equal(a, b) for a, b in zip(got[:1] + got[2:], expected[:1] + expected[2:])) and torch.equal(got[1], expected[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [0, 1, 300])
+def test_no_target_at_all(ft, dtype, tokens):
+    hidden, weight, target = make(tokens, 72, 200, dtype, seed=5)
+    hidden.fill_(math.nan)
+    target.fill_(-100)
+    for reduction in ("mean", "sum", "none"):
+        loss, grad_hidden, grad_weight = run(ft, hidden, weight, target, reduction)
+        assert not loss.any() and loss.shape == (target.shape if reduction == "none" else ()) and not grad_hidden.any() and not grad_weight.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_target_outside_of_the_vocabulary_shows(ft, dtype):
+    hidden, weight, target = make(40, 64, 100, dtype, seed=6)
+    for bad in (100, -1, -101, 1 << 40, -(1 << 63)):
+        wrong = target.clone()
+        wrong[11] = bad
+        loss, grad_hidden, grad_weight = run(ft, hidden, weight, wrong, "none")
+        assert torch.isnan(loss[11]) and torch.isfinite(loss).sum() == 39
+        assert torch.isnan(grad_hidden[11]).all() and torch.isfinite(grad_hidden[12]).all() and torch.isnan(grad_weight).all()
+        assert torch.isnan(ft.linear_cross_entropy(hidden, weight, wrong))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_logits(ft, dtype):
+    """Only differences to the largest logit are exponentials' arguments."""
+    hidden, weight, target = make(70, 64, 500, dtype, seed=7, spread=200.0)
+    run_and_check(ft, hidden, weight, target)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_infinities_and_nan_show(ft, dtype):
+    hidden, weight, target = make(50, 64, 300, dtype, seed=8)
+    hidden[3, 5] = math.nan
+    loss = ft.linear_cross_entropy(hidden, weight, target, reduction="none")
+    assert torch.isnan(loss[3]) and torch.isfinite(loss).sum() == 49
+    # A logit of -inf is a column of probability zero; all of them leave nothing.
+    hidden = hidden.abs().nan_to_num(1.0) + 0.01
+    weight[7] = -math.inf
+    target[target == 7] = 8
+    target[0] = 7
+    loss = ft.linear_cross_entropy(hidden.to(dtype), weight, target, reduction="none")
+    keep = torch.arange(300, device="cuda") != 7
+    rest = target - (target > 7).long()
+    without = ft.linear_cross_entropy(hidden.to(dtype), weight[keep], rest, reduction="none")
+    assert loss[0].item() == math.inf and torch.allclose(loss[1:], without[1:], rtol=0, atol=1e-4)
+
+
+@pytest.mark.parametrize("dtype, tokens, vocabulary", [(torch.bfloat16, 4096, 140001), (torch.float16, 4500, 131072), (torch.float32, 4096, 70001)])
+def test_several_pieces_of_the_vocabulary(ft, dtype, tokens, vocabulary):
+    hidden, weight, target = make(tokens, 40, vocabulary, dtype, seed=10)
+    target[::7] = -100
+    target[1], target[2] = 0, vocabulary - 1
+    loss, grad_hidden, grad_weight = run(ft, hidden, weight, target, "sum", torch.tensor(2.0, device="cuda"))
+    # In 64 bits, some rows at a time; each result's 2-norm against that of its error: the slopes' rounding and the results' own.
+    total, dw, worst = 0.0, torch.zeros(vocabulary, 40, device="cuda", dtype=torch.float64), 0.0
+    w = weight.double()
+    tolerance = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2e-6}[dtype] * 1.5
+    for part in torch.arange(tokens, device="cuda").split(500):
+        h, y = hidden[part].double(), target[part]
+        live = y != -100
+        log_p = torch.log_softmax(h @ w.T, 1)
+        total -= log_p.gather(1, y.clamp(min=0)[:, None])[live].sum().item()
+        slope = log_p.exp_()
+        slope[torch.arange(len(part), device="cuda"), y.clamp(min=0)] -= 1.0
+        slope *= 2.0 * live[:, None]
+        dh = slope @ w
+        assert (grad_hidden[part].double() - dh).norm() <= tolerance * dh.norm()
+        dw += slope.T @ h
+    assert abs(loss.item() - total) <= 2e-6 * total
+    assert (grad_weight.double() - dw).norm() <= tolerance * dw.norm()
+    edges = [0, 255, 256, vocabulary - 1]
+    assert (grad_weight[edges].double() - dw[edges]).norm() <= 2 * tolerance * dw[edges].norm()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_and_alignment(ft, dtype):
+    hidden, weight, target = make(130, 80, 300, dtype, seed=11)
+    wide_h = torch.zeros(260, 101, device="cuda", dtype=dtype)
+    wide_w = torch.zeros(301, 97, device="cuda", dtype=dtype)
+    odd_h, odd_w = wide_h[::2, 3:83], wide_w[1:, 1:81]
+    odd_h.copy_(hidden)
+    odd_w.copy_(weight)
+    padded_w = torch.zeros(300, 96, device="cuda", dtype=dtype)[:, :80]
+    padded_w.copy_(weight)
+    expected = run_and_check(ft, hidden, weight, target)
+    run_and_check(ft, odd_h, odd_w, target)
+    for h, w in ((odd_h, weight), (hidden, padded_w)):
+        got = run(ft, h, w, target)
+        assert all(torch.allclose(a.float(), b.float(), rtol=1e-6, atol=0) or torch.equal(a, b) for a, b in zip(got, expected))
+
+
+def test_leading_dimensions(ft):
+    hidden, weight, target = make(60, 64, 200, torch.bfloat16, seed=12)
+    flat = run(ft, hidden, weight, target, "none", torch.arange(60, device="cuda").float())
+    cube = run(ft, hidden.view(3, 20, 64), weight, target.view(3, 20), "none", torch.arange(60, device="cuda").float().view(3, 20))
+    assert cube[0].shape == (3, 20) and cube[1].shape == (3, 20, 64)
+    assert torch.equal(cube[0].view(-1), flat[0]) and torch.equal(cube[1].view(60, 64), flat[1]) and torch.equal(cube[2], flat[2])
+    one = ft.linear_cross_entropy(hidden[0], weight, target[0])
+    assert abs(one.item() - flat[0][0].item()) <= 1e-5
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_either_operand_alone(ft, dtype):
+    hidden, weight, target = make(100, 64, 300, dtype, seed=13)
+    _, both_h, both_w = run(ft, hidden, weight, target)
+    h = hidden.clone().requires_grad_()
+    ft.linear_cross_entropy(h, weight, target).backward()
+    assert torch.equal(h.grad, both_h)
+    w = weight.clone().requires_grad_()
+    ft.linear_cross_entropy(hidden, w, target).backward()
+    assert torch.equal(w.grad, both_w)
+    assert not ft.linear_cross_entropy(hidden, weight, target).requires_grad
+    loss = ft.linear_cross_entropy(h, w, target)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(loss, h, create_graph=True)
+
+
+def test_gradient_against_differences(ft):
+    """Central differences of the FP32 loss, summed. Their own error: a third derivative of at most 6 max|w|^3 (max|h|^3 for each of the tokens)
+    times h^2 / 6, and the loss's rounding over h."""
+    hidden, weight, target = make(3, 8, 11, torch.float32, seed=14, spread=1.0)
+    _, grad_hidden, grad_weight = run(ft, hidden, weight, target, "sum")
+    step = 2.0 ** -5
+
+    def value(h, w):
+        return ft.linear_cross_entropy(h, w, target, reduction="sum").item()
+
+    total = value(hidden, weight)
+    for matrix, gradient, other, copies in ((hidden, grad_hidden, weight, 1), (weight, grad_weight, hidden, 3)):
+        bound = copies * other.abs().max().item() ** 3 * step ** 2 + 32 * STEP * total / step
+        for i in range(matrix.shape[0]):
+            for j in range(matrix.shape[1]):
+                change = torch.zeros_like(matrix)
+                change[i, j] = step
+                up, down = ((value(matrix + change, weight), value(matrix - change, weight)) if matrix is hidden else
+                            (value(hidden, matrix + change), value(hidden, matrix - change)))
+                assert abs((up - down) / (2 * step) - gradient[i, j].item()) <= bound
+
+
+def test_like_torch(ft):
+    hidden, weight, target = make(200, 128, 1000, torch.float32, seed=15)
+    target[::5] = -100
+    h, w = hidden.clone().requires_grad_(), weight.clone().requires_grad_()
+    expected = F.cross_entropy(h @ w.t(), target)
+    expected.backward()
+    loss, grad_hidden, grad_weight = run(ft, hidden, weight, target)
+    assert torch.allclose(loss, expected.detach(), rtol=1e-5) and torch.allclose(grad_hidden, h.grad, rtol=1e-3, atol=1e-6)
+    assert torch.allclose(grad_weight, w.grad, rtol=1e-3, atol=1e-6)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_equal_calls_give_equal_bits(ft, dtype):
+    hidden, weight, target = make(700, 256, 5000, dtype, seed=16)
+    first = run(ft, hidden, weight, target)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(run(ft, hidden, weight, target), first))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_another_stream_and_a_graph(ft, dtype):
+    hidden, weight, target = make(300, 128, 900, dtype, seed=17)
+    expected = run(ft, hidden, weight, target)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = run(ft, hidden, weight, target)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(on_side, expected))
+    held = hidden.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run(ft, held, weight, target)
+    for fraction in (2, 3):  # other hidden states and other numbers of live tokens
+        held.copy_(make(300, 128, 900, dtype, seed=17 + fraction)[0])
+        target[::fraction] = -100
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(captured, run(ft, held, weight, target)))
+
+
+def test_refusals(ft):
+    h, w, y = make(10, 16, 20, torch.float32)
+    for call, reason in [
+        (lambda: ft.linear_cross_entropy(h.cpu(), w, y), "device tensors"), (lambda: ft.linear_cross_entropy(h.double(), w.double(), y), "FP32, FP16 or BF16"),
+        (lambda: ft.linear_cross_entropy(h.half(), w, y), "one type"), (lambda: ft.linear_cross_entropy(h, w[:, :8], y), "columns"),
+        (lambda: ft.linear_cross_entropy(h, w, y.int()), "INT64"), (lambda: ft.linear_cross_entropy(h, w, y[:9]), "each hidden state"),
+        (lambda: ft.linear_cross_entropy(h, w, y, reduction="max"), "reduction"), (lambda: ft.linear_cross_entropy(h, w.t().contiguous().t(), y), "contiguous along"),
+        (lambda: ft.linear_cross_entropy(h[:1].expand(10, 16), w, y), "rows overlap"), (lambda: ft.linear_cross_entropy(h, w.view(20, 4, 4), y), "rank two"),
+        (lambda: ft.linear_cross_entropy(h, w[:0], y), "empty"),
+    ]:
+        with pytest.raises(RuntimeError, match=reason):
+            call()
