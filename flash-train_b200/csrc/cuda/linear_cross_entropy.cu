@@ -98,28 +98,34 @@ template<bool kBackward> __global__ void __launch_bounds__(kListThreads) listTok
     const std::uint32_t padded = (max(count, 1U) + loss::kTileRows - 1) / loss::kTileRows * loss::kTileRows;
     if (kBackward) {
         float common = 0.0F;
-        if (p.reduction != FTCUDA_REDUCTION_NONE) {
-            common  = p.reduction == FTCUDA_REDUCTION_MEAN ? *p.grad_loss / static_cast<float>(max(count, 1U)) : *p.grad_loss;
-            largest = __float_as_uint(common) & 0x7FFFFFFFU;
-        }
+        if (p.reduction != FTCUDA_REDUCTION_NONE) { common = p.reduction == FTCUDA_REDUCTION_MEAN ? *p.grad_loss / static_cast<float>(max(count, 1U)) : *p.grad_loss; }
         atomicMax(&largest_bits, largest);
         __syncthreads();
-        // The largest |scale| becomes a number in [1, 2) 2^scale_bits; not beyond 2^100 times larger, and not where it is 0 or not a number.
+        // With one upstream gradient for all, the scale is the power of two alone, so that -1, the slope of a target that has hardly any
+        // probability, stays exact (BF16's rounding of -1 / N would be off by the same for every token). With one for each, the largest |scale|
+        // becomes a number in [1, 2) 2^scale_bits; not beyond 2^100 times larger, and not where it is 0 or not a number.
+        const bool each    = p.reduction == FTCUDA_REDUCTION_NONE;
+        const bool rounded = p.scale_bits != INT32_MIN;
         const float top    = __uint_as_float(largest_bits);
         std::int32_t shift = 0;
-        if (p.scale_bits != INT32_MIN) { shift = p.scale_bits - (top > 0.0F && top <= FLT_MAX ? max(-100, ilogbf(top)) : 0); }
+        if (rounded) { shift = p.scale_bits - (each && top > 0.0F && top <= FLT_MAX ? max(-100, ilogbf(top)) : 0); }
+        if (rounded && !each) {
+            if (threadIdx.x == 0) { *p.rows.unit = ldexpf(common, -shift); }
+            common = 1.0F;
+        } else if (threadIdx.x == 0) {
+            *p.rows.unit = ldexpf(1.0F, -shift);
+        }
         for (std::uint32_t i = threadIdx.x; i < padded; i += kListThreads) {
             float scale = 0.0F, lse2 = 0.0F;
             if (i < count) {
                 const std::int32_t t = p.rows.token[i];
-                scale                = ldexpf(p.reduction == FTCUDA_REDUCTION_NONE ? p.grad_loss[t] : common, shift);
+                scale                = ldexpf(each ? p.grad_loss[t] : common, shift);
                 lse2                 = p.saved_lse[t] * loss::kLog2E;
                 if (p.rows.target[i] == loss::kBadTarget) { scale = __uint_as_float(0x7FFFFFFFU); }
             }
             p.rows.scale[i] = scale;
             p.rows.lse2[i]  = lse2;
         }
-        if (threadIdx.x == 0) { *p.rows.unit = ldexpf(1.0F, -shift); }
     }
     for (std::uint32_t i = count + threadIdx.x; i < padded; i += kListThreads) {
         p.rows.token[i]  = -1;

@@ -18,7 +18,7 @@ constexpr float kLn2              = 0.6931471805599453F;
 // neutral rows: hidden state 0, target -1, scale 0.
 struct LiveRows {
     std::uint32_t* count;
-    float* unit;            // what a sum of products of slopes is multiplied by in the end: a power of two
+    float* unit;            // what a sum of products of slopes is multiplied by in the end
     std::int32_t* token;    // the token a row is of
     std::int32_t* target;   // its column, -1 for none, kBadTarget for one outside of the vocabulary
     float* scale;           // upstream gradient of the row's loss over `unit`
