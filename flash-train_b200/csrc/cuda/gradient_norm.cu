@@ -28,9 +28,12 @@ namespace {
 using training::Element;
 
 constexpr int kThreads            = 256;
-constexpr int kSumCtasPerSm       = 8;
-constexpr int kScaleCtasPerSm     = 4;  // what a thread holds between its loads and its stores takes twice the registers
-constexpr std::uint32_t kChunk    = 16 * kThreads;  // elements: 16 a thread, 64 bytes of FP32 in flight
+constexpr int kSumCtasPerSm       = 4;
+constexpr int kScaleCtasPerSm     = 4;
+constexpr int kSumBatch           = 4;  // packs of 16 bytes that a thread asks for at a time, twice over
+constexpr int kScaleBatch         = 4;
+constexpr int kScaleSingles       = 8;  // ... or single elements, where the two sides' alignment differs
+constexpr std::uint32_t kChunk    = 16 * kThreads;  // elements
 constexpr std::uint32_t kTensors  = 480;            // of one launch: 30 KiB of the nearly 32 that a kernel's parameters may take
 constexpr std::uint32_t kFew      = 64;             // ... of the launch for few tensors, whose parameters are quicker to hand over
 constexpr std::uint64_t kMaxGrid  = 2048;           // CTAs of one launch at most (and room for their sums)
@@ -90,101 +93,104 @@ template<typename T, int n> struct alignas(sizeof(T) * n) Pack {
     T at[n];
 };
 
-// Elements [begin, end) of a row for all threads of the CTA, `begin` and `end` the same in all: body(index, count-n pack).
-// Whole 16-byte vectors where the address allows it, the ends one by one.
-template<typename T, typename Sum> __device__ __forceinline__ void sumRow(const T* row, std::uint32_t count, Sum& sum) {
-    constexpr std::uint32_t kVector = 16 / sizeof(T);
-    constexpr int kVectors          = kChunk / kVector / kThreads;
-    const std::uint32_t head        = min(count, static_cast<std::uint32_t>((16 - (reinterpret_cast<std::uintptr_t>(row) & 15)) & 15) / static_cast<std::uint32_t>(sizeof(T)));
-    const std::uint32_t vectors     = (count - head) / kVector;
-    const auto* body                = reinterpret_cast<const Pack<T, kVector>*>(row + head);
-    Pack<T, kVector> packs[kVectors];
+// Elements up to the first one at a multiple of 16 bytes.
+template<typename T> __device__ __forceinline__ std::uint32_t misaligned(const T* at) {
+    return static_cast<std::uint32_t>((16 - (reinterpret_cast<std::uintptr_t>(at) & 15)) & 15) / static_cast<std::uint32_t>(sizeof(T));
+}
+
+// Goes over `count` packs with all threads of the CTA, from the last one back with kBack, kBatch at a time for each: the next batch is asked
+// for before `use` is called for the packs of the one at hand, so that loads are always on their way.
+template<int kBatch, bool kBack, typename P, typename Use>
+__device__ __forceinline__ void stream(const P* from, std::uint64_t count, const Use& use) {
+    constexpr std::int64_t kStep  = kBack ? -kBatch * kThreads : kBatch * kThreads;
+    constexpr std::int64_t kEach  = kBack ? -kThreads : kThreads;
+    const std::uint64_t batches   = count / (kBatch * kThreads);
+    std::int64_t at               = kBack ? static_cast<std::int64_t>(count) - 1 - threadIdx.x : threadIdx.x;
+    if (batches != 0) {
+        P now[kBatch];
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-        const std::uint32_t at = threadIdx.x + i * kThreads;
-        if (at < vectors) {
-            packs[i] = body[at];
-        } else {
+        for (int i = 0; i < kBatch; ++i) { now[i] = from[at + i * kEach]; }
+#pragma unroll 1
+        for (std::uint64_t batch = 1; batch < batches; ++batch) {
+            P next[kBatch];
 #pragma unroll
-            for (std::uint32_t j = 0; j < kVector; ++j) { packs[i].at[j] = Element<T>::narrow(0.0F); }
+            for (int i = 0; i < kBatch; ++i) { next[i] = from[at + kStep + i * kEach]; }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) { use(at + i * kEach, now[i]); }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) { now[i] = next[i]; }
+            at += kStep;
         }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) { use(at + i * kEach, now[i]); }
+        at += kStep;
     }
-    // The ends: fewer than kVector elements on either side.
-    const std::uint32_t rest = head + vectors * kVector;
-    const std::uint32_t ends = head + (count - rest);
+#pragma unroll 1
+    for (; kBack ? at >= 0 : at < static_cast<std::int64_t>(count); at += kEach) {
+        const P one = from[at];
+        use(at, one);
+    }
+}
+
+// Written once and not read again here: leaves what the first pass read in L2.
+template<typename Q> __device__ __forceinline__ void storeStreaming(Q* to, const Q& value) {
+    if constexpr (sizeof(Q) == 16) {
+        __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(&value));
+    } else if constexpr (sizeof(Q) == 8) {
+        __stcs(reinterpret_cast<uint2*>(to), *reinterpret_cast<const uint2*>(&value));
+    } else if constexpr (sizeof(Q) == 4) {
+        __stcs(reinterpret_cast<unsigned int*>(to), *reinterpret_cast<const unsigned int*>(&value));
+    } else {
+        __stcs(reinterpret_cast<unsigned short*>(to), *reinterpret_cast<const unsigned short*>(&value));
+    }
+}
+
+// `count` neighbouring elements: packs of 16 bytes, and the ends one by one.
+template<typename T, typename Sum> __device__ __forceinline__ void sumRow(const T* row, std::uint64_t count, Sum& sum) {
+    constexpr int kEach         = 16 / sizeof(T);
+    using P                     = Pack<T, kEach>;
+    const std::uint32_t head    = static_cast<std::uint32_t>(min(count, static_cast<std::uint64_t>(misaligned(row))));
+    const std::uint64_t packs   = (count - head) / kEach;
+    const std::uint64_t rest    = head + packs * kEach;
+    const std::uint32_t ends    = head + static_cast<std::uint32_t>(count - rest);
     if (threadIdx.x < ends) {
-        const std::uint32_t at = threadIdx.x < head ? threadIdx.x : rest + (threadIdx.x - head);
-        const float x[1]       = {Element<T>::widen(row[at])};
+        const float x[1] = {Element<T>::widen(row[threadIdx.x < head ? threadIdx.x : rest + (threadIdx.x - head)])};
         sum.add(x);
     }
+    stream<kSumBatch, false>(reinterpret_cast<const P*>(row + head), packs, [&](std::int64_t, const P& pack) {
+        float x[kEach];
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-        float x[kVector];
-#pragma unroll
-        for (std::uint32_t j = 0; j < kVector; ++j) { x[j] = Element<T>::widen(packs[i].at[j]); }
-        if (threadIdx.x + i * kThreads < vectors) { sum.add(x); }
-    }
+        for (int j = 0; j < kEach; ++j) { x[j] = Element<T>::widen(pack.at[j]); }
+        sum.add(x);
+    });
 }
 
-// n neighbouring elements, 16 bytes at a time on either side.
-template<typename T, int n> __device__ __forceinline__ void loadVector(const T* from, T (&x)[n]) {
-    constexpr int kEach = 16 / sizeof(T) < n ? 16 / sizeof(T) : n;
-#pragma unroll
-    for (int i = 0; i < n; i += kEach) { *reinterpret_cast<Pack<T, kEach>*>(x + i) = *reinterpret_cast<const Pack<T, kEach>*>(from + i); }
-}
-template<typename T, typename U, int n> __device__ __forceinline__ void storeScaled(U* to, const T (&x)[n], float factor) {
-    constexpr int kEach = 16 / sizeof(U) < n ? 16 / sizeof(U) : n;
-#pragma unroll
-    for (int i = 0; i < n; i += kEach) {
-        Pack<U, kEach> o;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) { o.at[j] = Element<U>::narrow(Element<T>::widen(x[i + j]) * factor); }
-        *reinterpret_cast<Pack<U, kEach>*>(to + i) = o;
-    }
-}
-
+// out = row * factor. Packs of four elements (eight where both sides have 16 bits) where both sides are aligned for them at the same element: a
+// warp's accesses are neighbours on both sides then. Otherwise one element at a time.
 template<typename T, typename U>
-__device__ __forceinline__ void scaleRow(const T* row, U* out, std::uint32_t count, float factor) {
-    constexpr std::uint32_t kVector = 16 / (sizeof(T) < sizeof(U) ? sizeof(T) : sizeof(U));
-    constexpr int kVectors          = kChunk / kVector / kThreads;
-    const std::uint32_t head        = min(count, static_cast<std::uint32_t>((16 - (reinterpret_cast<std::uintptr_t>(row) & 15)) & 15) / static_cast<std::uint32_t>(sizeof(T)));
-    // Vectors where both sides are aligned at the same element; then all of a warp's 16-byte pieces are neighbours on both sides.
-    if ((reinterpret_cast<std::uintptr_t>(out + head) & 15) == 0) {
-        const T* const from         = row + head;
-        U* const to                 = out + head;
-        const std::uint32_t vectors = (count - head) / kVector;
-        if (vectors == kVectors * kThreads) {
-            // A whole chunk: everything is asked for before anything is written.
-            alignas(16) T x[kVectors][kVector];
-#pragma unroll
-            for (int i = 0; i < kVectors; ++i) { loadVector(from + (threadIdx.x + i * kThreads) * kVector, x[i]); }
-#pragma unroll
-            for (int i = 0; i < kVectors; ++i) { storeScaled(to + (threadIdx.x + i * kThreads) * kVector, x[i], factor); }
-        } else {
-#pragma unroll 1
-            for (std::uint32_t at = threadIdx.x; at < vectors; at += kThreads) {
-                alignas(16) T x[kVector];
-                loadVector(from + at * kVector, x);
-                storeScaled(to + at * kVector, x, factor);
-            }
-        }
-        const std::uint32_t rest = head + vectors * kVector;
-        const std::uint32_t ends = head + (count - rest);
+__device__ __forceinline__ void scaleRow(const T* row, U* out, std::uint64_t count, float factor) {
+    constexpr int kEach      = 16 / (sizeof(T) > sizeof(U) ? sizeof(T) : sizeof(U));
+    using P                  = Pack<T, kEach>;
+    using Q                  = Pack<U, kEach>;
+    const std::uint32_t head = static_cast<std::uint32_t>(min(count, static_cast<std::uint64_t>(sizeof(T) >= sizeof(U) ? misaligned(row) : misaligned(out))));
+    const bool both          = reinterpret_cast<std::uintptr_t>(row + head) % sizeof(P) == 0 && reinterpret_cast<std::uintptr_t>(out + head) % sizeof(Q) == 0;
+    if (both) {
+        const std::uint64_t packs = (count - head) / kEach;
+        const std::uint64_t rest  = head + packs * kEach;
+        const std::uint32_t ends  = head + static_cast<std::uint32_t>(count - rest);
         if (threadIdx.x < ends) {
-            const std::uint32_t at = threadIdx.x < head ? threadIdx.x : rest + (threadIdx.x - head);
+            const std::uint64_t at = threadIdx.x < head ? threadIdx.x : rest + (threadIdx.x - head);
             out[at]                = Element<U>::narrow(Element<T>::widen(row[at]) * factor);
         }
-        return;
-    }
-    if (count == kChunk) {
-        T x[kChunk / kThreads];
+        Q* const to = reinterpret_cast<Q*>(out + head);
+        stream<kScaleBatch, true>(reinterpret_cast<const P*>(row + head), packs, [&](std::int64_t at, const P& pack) {
+            Q o;
 #pragma unroll
-        for (std::uint32_t i = 0; i < kChunk / kThreads; ++i) { x[i] = row[threadIdx.x + i * kThreads]; }
-#pragma unroll
-        for (std::uint32_t i = 0; i < kChunk / kThreads; ++i) { out[threadIdx.x + i * kThreads] = Element<U>::narrow(Element<T>::widen(x[i]) * factor); }
+            for (int j = 0; j < kEach; ++j) { o.at[j] = Element<U>::narrow(Element<T>::widen(pack.at[j]) * factor); }
+            storeStreaming(to + at, o);
+        });
     } else {
-#pragma unroll 4
-        for (std::uint32_t at = threadIdx.x; at < count; at += kThreads) { out[at] = Element<U>::narrow(Element<T>::widen(row[at]) * factor); }
+        stream<kScaleSingles, true>(row, count, [&](std::int64_t at, const T& x) { storeStreaming(out + at, Element<U>::narrow(Element<T>::widen(x) * factor)); });
     }
 }
 
@@ -203,24 +209,26 @@ __device__ __forceinline__ std::uint32_t findEntry(const Table<kCapacity>& table
     return low;
 }
 
-struct Piece {
-    std::uint64_t row, col;
-    std::uint32_t count;
+// Neighbouring elements in the chunks from `begin` up to `end` of one tensor: of a dense one all of them, of a row of others the first chunk's
+// (kBack: the last one's).
+struct Stretch {
+    std::uint64_t row, col, count, chunks;
 };
 
-__device__ __forceinline__ Piece pieceOf(const Entry& entry, std::uint64_t chunk) {
-    const std::uint64_t local = chunk - entry.first;
-    Piece piece;
+template<bool kBack> __device__ __forceinline__ Stretch stretchOf(const Entry& entry, std::uint64_t begin, std::uint64_t end) {
+    Stretch s;
     if (entry.rows == 1) {
-        piece.row = 0;
-        piece.col = local * kChunk;
+        s.row    = 0;
+        s.col    = (begin - entry.first) * kChunk;
+        s.chunks = end - begin;
     } else {
-        const std::uint64_t per_row = (entry.cols + kChunk - 1) / kChunk;
-        piece.row                   = local / per_row;
-        piece.col                   = (local - piece.row * per_row) * kChunk;
+        const std::uint64_t local = (kBack ? end - 1 : begin) - entry.first, per_row = (entry.cols + kChunk - 1) / kChunk;
+        s.row                     = local / per_row;
+        s.col                     = (local - s.row * per_row) * kChunk;
+        s.chunks                  = 1;
     }
-    piece.count = static_cast<std::uint32_t>(min(static_cast<std::uint64_t>(kChunk), entry.cols - piece.col));
-    return piece;
+    s.count = min(s.chunks * kChunk, entry.cols - s.col);
+    return s;
 }
 
 // Joined over the CTA, the same order in every call; the result in thread 0.
@@ -244,16 +252,18 @@ __global__ void __launch_bounds__(kThreads, kSumCtasPerSm) gradientSums(const __
     if (begin < end) {
         std::uint32_t index = findEntry(table, begin);
 #pragma unroll 1
-        for (std::uint64_t chunk = begin; chunk < end; ++chunk) {
+        for (std::uint64_t chunk = begin; chunk < end;) {
             while (index + 1 < table.count && table.entries[index + 1].first <= chunk) { ++index; }
-            const Entry& entry          = table.entries[index];
-            const Piece piece           = pieceOf(entry, chunk);
-            const std::int64_t offset   = static_cast<std::int64_t>(piece.row) * entry.row_stride + static_cast<std::int64_t>(piece.col);
+            const Entry& entry        = table.entries[index];
+            const std::uint64_t last  = index + 1 < table.count ? min(end, table.entries[index + 1].first) : end;
+            const Stretch s           = stretchOf<false>(entry, chunk, last);
+            const std::int64_t offset = static_cast<std::int64_t>(s.row) * entry.row_stride + static_cast<std::int64_t>(s.col);
             switch (entry.element) {
-                case FTCUDA_ELEMENT_FP32: sumRow(static_cast<const float*>(entry.data) + offset, piece.count, sum); break;
-                case FTCUDA_ELEMENT_FP16: sumRow(static_cast<const __half*>(entry.data) + offset, piece.count, sum); break;
-                default: sumRow(static_cast<const __nv_bfloat16*>(entry.data) + offset, piece.count, sum); break;
+                case FTCUDA_ELEMENT_FP32: sumRow(static_cast<const float*>(entry.data) + offset, s.count, sum); break;
+                case FTCUDA_ELEMENT_FP16: sumRow(static_cast<const __half*>(entry.data) + offset, s.count, sum); break;
+                default: sumRow(static_cast<const __nv_bfloat16*>(entry.data) + offset, s.count, sum); break;
             }
+            chunk += s.chunks;
         }
     }
     joinBlock(sum, shared);
@@ -276,13 +286,13 @@ template<typename Sum> __global__ void __launch_bounds__(kThreads) gradientNorm(
     if (threadIdx.x == 0) { *norm = static_cast<float>(total); }
 }
 
-template<typename T> __device__ __forceinline__ void scalePiece(const Entry& entry, const Piece& piece, float factor) {
-    const T* const row          = static_cast<const T*>(entry.data) + static_cast<std::int64_t>(piece.row) * entry.row_stride + static_cast<std::int64_t>(piece.col);
-    const std::int64_t offset   = static_cast<std::int64_t>(piece.row) * entry.out_row_stride + static_cast<std::int64_t>(piece.col);
+template<typename T> __device__ __forceinline__ void scaleStretch(const Entry& entry, const Stretch& s, float factor) {
+    const T* const row        = static_cast<const T*>(entry.data) + static_cast<std::int64_t>(s.row) * entry.row_stride + static_cast<std::int64_t>(s.col);
+    const std::int64_t offset = static_cast<std::int64_t>(s.row) * entry.out_row_stride + static_cast<std::int64_t>(s.col);
     switch (entry.out_element) {
-        case FTCUDA_ELEMENT_FP32: scaleRow(row, static_cast<float*>(entry.out) + offset, piece.count, factor); break;
-        case FTCUDA_ELEMENT_FP16: scaleRow(row, static_cast<__half*>(entry.out) + offset, piece.count, factor); break;
-        default: scaleRow(row, static_cast<__nv_bfloat16*>(entry.out) + offset, piece.count, factor); break;
+        case FTCUDA_ELEMENT_FP32: scaleRow(row, static_cast<float*>(entry.out) + offset, s.count, factor); break;
+        case FTCUDA_ELEMENT_FP16: scaleRow(row, static_cast<__half*>(entry.out) + offset, s.count, factor); break;
+        default: scaleRow(row, static_cast<__nv_bfloat16*>(entry.out) + offset, s.count, factor); break;
     }
 }
 
@@ -305,15 +315,16 @@ __global__ void __launch_bounds__(kThreads, kScaleCtasPerSm) gradientScale(const
     if (begin == end) { return; }
     std::uint32_t index = findEntry(table, end - 1);
 #pragma unroll 1
-    for (std::uint64_t chunk = end; chunk-- > begin;) {
-        while (table.entries[index].first > chunk) { --index; }
+    for (std::uint64_t chunk = end; chunk > begin;) {
+        while (table.entries[index].first >= chunk) { --index; }
         const Entry& entry = table.entries[index];
+        const Stretch s    = stretchOf<true>(entry, max(begin, entry.first), chunk);
+        chunk -= s.chunks;
         if (factor == 1.0F && entry.out == entry.data) { continue; }
-        const Piece piece = pieceOf(entry, chunk);
         switch (entry.element) {
-            case FTCUDA_ELEMENT_FP32: scalePiece<float>(entry, piece, factor); break;
-            case FTCUDA_ELEMENT_FP16: scalePiece<__half>(entry, piece, factor); break;
-            default: scalePiece<__nv_bfloat16>(entry, piece, factor); break;
+            case FTCUDA_ELEMENT_FP32: scaleStretch<float>(entry, s, factor); break;
+            case FTCUDA_ELEMENT_FP16: scaleStretch<__half>(entry, s, factor); break;
+            default: scaleStretch<__nv_bfloat16>(entry, s, factor); break;
         }
     }
 }
