@@ -45,6 +45,7 @@ struct SplitOperand {
     std::uint32_t grouped;    // kColumnGroup rows share a scale, and `inverse` has one entry for each group
     std::uint32_t along_k;    // the source runs faster along K than along its rows
     std::uint32_t vector;     // 16-byte loads in that direction are aligned
+    std::uint32_t absolute;   // gray elements are well enough within 2^-50 of the largest that shares their scale
     std::uint32_t blocks;     // CTAs
     unsigned char* split;
     float* inverse;           // [slab][pitch]: 1 / (scale of the row or group in the slab), a power of two

@@ -81,6 +81,15 @@ PFN_cuTensorMapEncodeTiled_v12000 tensorMapEncoder() {
     return encoder;
 }
 
+// The encoder wants a current context, which a thread that has only ever inherited its device (an autograd engine's, for
+// one) need not have yet: the runtime binds it with the first call that needs it, and this is a driver's call.
+template<typename Encode> CUresult encodeInContext(const Encode& encode) {
+    const CUresult result = encode();
+    int device            = 0;
+    if (result != CUDA_ERROR_INVALID_CONTEXT || cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) { return result; }
+    return encode();
+}
+
 }  // namespace
 
 int fail(char* message, std::size_t capacity, int code, const char* format, ...) {
@@ -169,12 +178,12 @@ bool encodeTensorMap2d(CUtensorMap* map, const void* base, std::uint64_t inner, 
     const cuuint64_t strides[1]  = {row_pitch_bytes};
     const cuuint32_t box[2]      = {box_inner, box_outer};
     const cuuint32_t elements[2] = {1, 1};
-    const CUresult result        = encode(
-        map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(base), dims, strides, box, elements,
-        CU_TENSOR_MAP_INTERLEAVE_NONE,
-        swizzle == kSwizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                               : swizzle == kSwizzle128Atom32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_NONE,
-        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult result        = encodeInContext([&] {
+        return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(base), dims, strides, box, elements, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      swizzle == kSwizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                             : swizzle == kSwizzle128Atom32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
     if (result != CUDA_SUCCESS) {
         fail(message, capacity, 1, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(result));
         return false;
@@ -193,9 +202,10 @@ bool encodeMap16(CUtensorMap* map, bool bf16, const void* base, std::uint64_t in
     const cuuint64_t strides[1]  = {row_pitch_bytes};
     const cuuint32_t box[2]      = {64, box_outer};
     const cuuint32_t elements[2] = {1, 1};
-    const CUresult result = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
-                                   strides, box, elements, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult result = encodeInContext([&] {
+        return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, elements,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
     if (result != CUDA_SUCCESS) {
         fail(message, capacity, 1, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(result));
         return false;
@@ -215,9 +225,10 @@ bool encodeSplitMap(CUtensorMap* map, const void* base, std::uint64_t rows, std:
     const cuuint64_t strides[2]  = {blocks * 256, 128};
     const cuuint32_t box[3]      = {64, box_rows, 2};
     const cuuint32_t elements[3] = {1, 1, 1};
-    const CUresult result = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, elements,
-                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult result = encodeInContext([&] {
+        return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, elements, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
     if (result != CUDA_SUCCESS) {
         fail(message, capacity, 1, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(result));
         return false;

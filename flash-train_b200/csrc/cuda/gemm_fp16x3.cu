@@ -624,6 +624,7 @@ cudaError_t launchPrepared(const LaunchState& state, void* workspace, cudaStream
         o.split                 = base + prepared.split_at[i];
         o.inverse               = reinterpret_cast<float*>(base + prepared.inverse_at[i]);
         o.pitch                 = prepared.inverse_pitch[i];
+        o.absolute              = i == 0 ? prepared.absolute_a : 0;
         fp16x3::planSplit(o, split.slabs);
         o.verdicts = verdicts + (i == 0 ? 0 : split.operand[0].blocks);
     }

@@ -21,6 +21,8 @@
 // NaN, the launch is left to the TF32 kernel, which splits without scaling. Every CTA leaves a verdict; the
 // multiplying kernel decides slab by slab and then for the whole launch.
 //
+// An operand whose caller is content with 2^-50 of the largest (SplitOperand::absolute) has no gray elements in this sense.
+//
 // The scales belong to slabs, and not to whole rows, so that one pass is enough: a CTA holds a slab of
 // some rows, takes their largest magnitudes, and converts. HBM-bound: 4 bytes read and 4 written an element.
 // At 4096 x 4096 for each operand (134 MB read, as many written; 41 us at the copy rate) 49 us with both sources along K,
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 2) splitOperands(const SplitParams p
                     *reinterpret_cast<uint2*>(target + i * 2 * kBlockBytes + 2 * kBlockK) = lo;
                 }
             }
-            if (__any_sync(0xFFFFFFFFU, splitter.sawGray())) {
+            if (o.absolute == 0 && __any_sync(0xFFFFFFFFU, splitter.sawGray())) {
                 std::uint32_t gray = 0;
 #pragma unroll
                 for (std::uint32_t i = 0; i < kSlabK / 128; ++i) {
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 2) splitOperands(const SplitParams p
                 *reinterpret_cast<uint4*>(at + 2 * kBlockK) = lo;
             }
         }
-        if (splitter.sawGray()) {
+        if (o.absolute == 0 && splitter.sawGray()) {
             std::uint32_t gray = 0;
             from               = tile + (first * kBlockK + lane % 8 * 8) * kTilePitch + at_row;
 #pragma unroll 1

@@ -46,6 +46,7 @@ struct PreparedState {
     std::int32_t fallback_kernel;  // 0 is never a fallback: nonzero marks a prepared launch
     std::uint32_t tile_n, splits, blocks_per_split, chunk_blocks;
     std::uint32_t grid;
+    std::uint32_t absolute_a;      // SplitOperand::absolute of A: set behind configurePrepared by a caller that knows what A is
     std::uint64_t verdicts_at, inverse_at[2], inverse_pitch[2], split_at[2], partials_at;  // byte offsets; pitch in elements
 };
 

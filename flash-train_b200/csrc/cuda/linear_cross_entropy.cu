@@ -33,7 +33,8 @@ using training::Element;
 
 constexpr int kListThreads             = 1024;
 constexpr int kGatherThreads           = 256;
-constexpr int kJoinRows                = 32;   // rows of a CTA that joins statistics, a warp for each eighth of the pieces
+constexpr int kJoinRows                = 32;   // rows of a CTA that joins statistics ...
+constexpr int kJoinWarps               = 32;   // ... each of its warps some of the pieces
 constexpr int kRowThreads              = 256;  // FP32: threads that go over a row of logits
 constexpr std::uint64_t kPieceBytes    = 512ULL << 20;  // of dZ (FP32: of Z), unless ...
 constexpr std::uint64_t kLeastColumns  = 8192;          // ... that is fewer columns than these
@@ -183,8 +184,8 @@ struct JoinParams {
     float* lse;              // [tokens]
 };
 
-__global__ void __launch_bounds__(256) joinStatistics(const JoinParams p) {
-    __shared__ float2 shared[8][kJoinRows];
+__global__ void __launch_bounds__(kJoinWarps * 32) joinStatistics(const JoinParams p) {
+    __shared__ float2 shared[kJoinWarps][kJoinRows];
     gridDependencyWait();
     gridDependencyLaunchDependents();
     const std::uint32_t live = *p.rows.count;
@@ -192,13 +193,26 @@ __global__ void __launch_bounds__(256) joinStatistics(const JoinParams p) {
     if (blockIdx.x * kJoinRows >= live) { return; }
     const int warp = threadIdx.x >> 5;
     float2 sum     = make_float2(-INFINITY, 0.0F);
-    // (Rows up to the next multiple of kTileRows have statistics too.)
-#pragma unroll 4
-    for (std::uint32_t piece = warp; piece < p.pieces; piece += 8) { sum = joinPartials(sum, __ldcg(p.partials + static_cast<std::uint64_t>(piece) * p.capacity + row)); }
+    // Eight pieces at a time: one reference for them and what came before. (Rows up to the next multiple of kTileRows have statistics too.)
+    for (std::uint32_t piece = warp; piece < p.pieces; piece += 8 * kJoinWarps) {
+        float2 part[8];
+        float base = sum.x;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const std::uint32_t at = piece + i * kJoinWarps;
+            part[i] = at < p.pieces ? __ldcg(p.partials + static_cast<std::uint64_t>(at) * p.capacity + row) : make_float2(-INFINITY, 0.0F);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { base = fmaxf(base, part[i].x); }
+        float total = sum.x == -INFINITY ? sum.y : sum.y * exp2f(sum.x - base);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { total += part[i].x == -INFINITY ? part[i].y : part[i].y * exp2f(part[i].x - base); }
+        sum = make_float2(base, total);
+    }
     shared[warp][threadIdx.x & 31] = sum;
     __syncthreads();
     if (warp == 0 && row < live) {
-        for (int w = 1; w < 8; ++w) { sum = joinPartials(sum, shared[w][threadIdx.x]); }
+        for (int w = 1; w < kJoinWarps; ++w) { sum = joinPartials(sum, shared[w][threadIdx.x]); }
         const float lse          = loss::kLn2 * (sum.x + log2f(sum.y));
         const bool bad           = p.rows.target[row] == loss::kBadTarget;
         const float value        = bad ? __uint_as_float(0x7FFFFFFFU) : lse - p.rows.picked[row];
@@ -352,13 +366,16 @@ std::uint64_t weightStride(const FtcudaLinearCrossEntropy& q) {
     return q.vocabulary == 1 ? roundUp(q.depth, 8) : static_cast<std::uint64_t>(q.weight_row_stride);
 }
 
-// One FP32 product by the first family that takes it, in its prepared form where that is faster.
+// One FP32 product by the first family that takes it, in its prepared form where that is faster. `slopes`: A is dZ. What a slope is off by already,
+// as its logit is a rounded sum, is over 2^-24 of it; next to the largest of 768 slopes that share a scale, one of under
+// 2^-26 of that may be rounded at 2^-50 of it (the other operand's elements have to be within 2^26 of one another all the same). Without
+// that, the small probabilities of every vocabulary would send these products to the form that is half as fast.
 struct Product {
     FtcudaGemmLaunch launch;
     std::uint64_t bytes;
 };
-int configureProduct(const FtcudaGemmDesc& desc, bool b_along_k, int sms, std::uint64_t bytes_left, Product& product, char* message, std::size_t capacity) {
-    const GemmCandidates candidates = gemmCandidates(desc.m, desc.n, desc.k, b_along_k && desc.n > 1, static_cast<std::uint64_t>(sms));
+int configureProduct(const FtcudaGemmDesc& desc, bool slopes, int sms, std::uint64_t bytes_left, Product& product, char* message, std::size_t capacity) {
+    const GemmCandidates candidates = gemmCandidates(desc.m, desc.n, desc.k, desc.b_row_stride == 1 && desc.n > 1, static_cast<std::uint64_t>(sms));
     for (int i = 0; i < candidates.count; ++i) {
         const int kernel = candidates.kernels[i];
         if (ftcuda_gemm_supports(kernel, &desc, nullptr, 0) != 0) { continue; }
@@ -369,6 +386,7 @@ int configureProduct(const FtcudaGemmDesc& desc, bool b_along_k, int sms, std::u
             Product prepared;
             if (ftcuda_gemm_prepare(&product.launch, &desc, &prepared.launch, nullptr, 0) == 0) {
                 prepared.bytes = ftcuda_gemm_workspace_bytes(&prepared.launch);
+                reinterpret_cast<LaunchState*>(&prepared.launch)->prepared.absolute_a = slopes ? 1 : 0;
                 if (prepared.bytes <= bytes_left) { product = prepared; }
             }
         }
@@ -477,12 +495,12 @@ int layOut(const FtcudaLinearCrossEntropy& q, bool backward, int sms, Layout& l,
             const std::uint64_t columns = std::min(l.columns, q.vocabulary - first);
             if (first != 0 && columns == l.columns && first != l.columns) { continue; }  // like the piece before
             Product product;
-            if (configureProduct(describeLogits(q, l, stand_in, first, columns), true, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
+            if (configureProduct(describeLogits(q, l, stand_in, first, columns), false, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
             l.product_bytes = std::max(l.product_bytes, product.bytes);
             if (!backward) { continue; }
-            if (configureProduct(describeHidden(q, l, stand_in, first, columns), false, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
+            if (configureProduct(describeHidden(q, l, stand_in, first, columns), true, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
             l.product_bytes = std::max(l.product_bytes, product.bytes);
-            if (configureProduct(describeWeight(q, l, stand_in, first, columns, stand_in, static_cast<std::int64_t>(q.depth)), false, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
+            if (configureProduct(describeWeight(q, l, stand_in, first, columns, stand_in, static_cast<std::int64_t>(q.depth)), true, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
             l.product_bytes = std::max(l.product_bytes, product.bytes);
         }
         take(l.product_bytes);
@@ -556,7 +574,7 @@ class Call final {
             std::uint64_t piece = 0;
             for (std::uint64_t first = 0; first < q_.vocabulary && error == cudaSuccess; first += l_.columns, ++piece) {
                 const std::uint64_t columns = std::min(l_.columns, q_.vocabulary - first);
-                error                       = multiply(describeLogits(q_, l_, base_, first, columns), true);
+                error                       = multiply(describeLogits(q_, l_, base_, first, columns), false);
                 if (error == cudaSuccess) {
                     error = training::launchOverlapped(rowStatistics, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(first, columns, partials + piece * l_.capacity));
                 }
@@ -571,7 +589,7 @@ class Call final {
         join.row_loss = at<float>(l_.row_loss);
         join.loss     = q_.reduction == FTCUDA_REDUCTION_NONE ? loss : nullptr;
         join.lse      = lse;
-        error = training::launchOverlapped(joinStatistics, dim3(static_cast<unsigned>(l_.capacity / kJoinRows)), dim3(256), 0, stream_, join);
+        error = training::launchOverlapped(joinStatistics, dim3(static_cast<unsigned>(l_.capacity / kJoinRows)), dim3(kJoinWarps * 32), 0, stream_, join);
         if (error == cudaSuccess && q_.reduction != FTCUDA_REDUCTION_NONE) {
             error = training::launchOverlapped(sumLosses, dim3(1), dim3(kListThreads), 0, stream_, rows_, static_cast<const float*>(at<float>(l_.row_loss)),
                                                q_.reduction == FTCUDA_REDUCTION_MEAN, loss);
@@ -654,9 +672,9 @@ class Call final {
     }
 
     // One FP32 product.
-    cudaError_t multiply(const FtcudaGemmDesc& desc, bool b_along_k) const {
+    cudaError_t multiply(const FtcudaGemmDesc& desc, bool slopes) const {
         Product product;
-        if (configureProduct(desc, b_along_k, sms_, l_.product_bytes, product, message_, capacity_) != 0 ||
+        if (configureProduct(desc, slopes, sms_, l_.product_bytes, product, message_, capacity_) != 0 ||
             ftcuda_gemm_launch(&product.launch, base_ + l_.product, l_.product_bytes, stream_, message_, capacity_) != 0) {
             return cudaErrorUnknown;  // the message says which
         }
@@ -677,12 +695,12 @@ class Call final {
             gradients.weight_gradient_pitch = weight_stride;
             return loss::launchGradients(products_, weight(first), columns32, base_ + l_.piece, l_.piece_pitch, gradients);
         }
-        cudaError_t error = multiply(describeLogits(q_, l_, base_, first, columns), true);
+        cudaError_t error = multiply(describeLogits(q_, l_, base_, first, columns), false);
         if (error == cudaSuccess) {
             error = training::launchOverlapped(rowSlopes, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(first, columns, nullptr));
         }
-        if (error == cudaSuccess && hidden) { error = multiply(describeHidden(q_, l_, base_, first, columns), false); }
-        if (error == cudaSuccess && grad_weight != nullptr) { error = multiply(describeWeight(q_, l_, base_, first, columns, grad_weight, weight_stride), false); }
+        if (error == cudaSuccess && hidden) { error = multiply(describeHidden(q_, l_, base_, first, columns), true); }
+        if (error == cudaSuccess && grad_weight != nullptr) { error = multiply(describeWeight(q_, l_, base_, first, columns, grad_weight, weight_stride), true); }
         return error;
     }
 

@@ -41,6 +41,7 @@ namespace {
 
 constexpr std::uint32_t kBlockK = 64;  // 128 bytes, one swizzle row
 constexpr std::uint32_t kTileN  = 256;
+constexpr std::uint32_t kItemBlocks = 12;
 constexpr int kStages           = 7;
 constexpr int kThreads          = 384;
 constexpr int kOperandBytes     = 128 * 128;  // a CTA's share of A, and of a B of 256 columns
@@ -110,10 +111,12 @@ struct Item {
 // The launch's tiles, from the number of live rows.
 struct Work {
     std::uint32_t tiles_m[2], blocks[2], items[2];
-    std::uint32_t total;
+    // Every pair takes its share of the first problem's items and then of the second's. Where the first ones do not come out even, the
+    // pairs from `late` on, which have one less of them, take `early` items of the second problem each meanwhile.
+    std::uint32_t late, early;
 };
 
-__device__ __forceinline__ Work workOf(const ProductParams& p, std::uint32_t live) {
+__device__ __forceinline__ Work workOf(const ProductParams& p, std::uint32_t live, std::uint32_t pairs) {
     live = max(live, 1U);
     Work w;
     w.items[1] = 0;
@@ -126,8 +129,25 @@ __device__ __forceinline__ Work workOf(const ProductParams& p, std::uint32_t liv
             w.items[i]             = w.tiles_m[i] * problem.tiles_n * problem.splits;
         }
     }
-    w.total = w.items[0] + w.items[1];
+    w.late  = w.items[0] % pairs;
+    // (An item costs about kItemBlocks blocks' time beside its own.)
+    const std::uint32_t first = p.problem[0].splits == 1 ? w.blocks[0] : p.problem[0].blocks_per_split;
+    w.early                   = w.items[1] != 0 && w.late != 0 ? (first + kItemBlocks) / (w.blocks[1] + kItemBlocks) : 0;
     return w;
+}
+
+// The number of a pair's n-th item, or kNoItem.
+constexpr std::uint32_t kNoItem = 0xFFFFFFFFU;
+__device__ __forceinline__ std::uint32_t itemOf(const Work& work, std::uint32_t pair, std::uint32_t pairs, std::uint32_t n) {
+    const std::uint32_t own = work.items[0] / pairs + (pair < work.late ? 1 : 0);
+    if (n < own) { return pair + n * pairs; }
+    n -= own;
+    const std::uint32_t others = work.early * (pairs - work.late);  // taken early
+    std::uint32_t item         = others + pair + n * pairs;
+    if (pair >= work.late) {
+        item = n < work.early ? pair - work.late + n * (pairs - work.late) : others + pair + (n - work.early) * pairs;
+    }
+    return item < work.items[1] ? work.items[0] + item : kNoItem;
 }
 
 __device__ __forceinline__ Item decode(const ProductParams& p, const Work& work, std::uint32_t item) {
@@ -322,7 +342,7 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
     gridDependencyWait();
     gridDependencyLaunchDependents();
     const std::uint32_t live = *p.rows.count;
-    const Work work          = workOf(p, live);
+    const Work work          = workOf(p, live, pairs);
 
     if (warp >= kFirstEpilogue) {
         registersGrow<kRegsDrain>();
@@ -334,7 +354,7 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
         const float unit              = kMode == kGradients ? *p.rows.unit : 1.0F;
         std::uint32_t sums = 0;
         bool ok = true;
-        for (std::uint32_t item = pair; item < work.total && ok; item += pairs, ++sums) {
+        for (std::uint32_t item; ok && (item = itemOf(work, pair, pairs, sums)) != kNoItem; ++sums) {
             const Item w                 = decode(p, work, item);
             const Problem& problem       = p.problem[w.problem];
             const std::uint32_t pieces   = problem.tile_n / 64;  // of 32 columns, for this warp
@@ -378,7 +398,7 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
             if (lane == 0) {
                 Ring ring;
                 std::uint32_t filled = 0;
-                for (std::uint32_t item = pair; item < work.total && ok; item += pairs) {
+                for (std::uint32_t n = 0, item; ok && (item = itemOf(work, pair, pairs, n)) != kNoItem; ++n) {
                     const Item w                    = decode(p, work, item);
                     const Problem& problem          = p.problem[w.problem];
                     const CUtensorMap* const map_a  = &maps.a[w.problem];
@@ -424,7 +444,7 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
                 Ring ring;
                 std::uint32_t sums = 0;
                 bool ok            = true;
-                for (std::uint32_t item = pair; item < work.total && ok; item += pairs, ++sums) {
+                for (std::uint32_t item; ok && (item = itemOf(work, pair, pairs, sums)) != kNoItem; ++sums) {
                     const Item w           = decode(p, work, item);
                     const Problem& problem = p.problem[w.problem];
                     const bool a_mn = problem.a_along_rows != 0, b_mn = problem.b_along_rows != 0;
