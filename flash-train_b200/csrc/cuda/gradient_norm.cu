@@ -296,21 +296,8 @@ template<typename T> __device__ __forceinline__ void scaleStretch(const Entry& e
     }
 }
 
-template<typename Sum, std::uint32_t kCapacity>
-__global__ void __launch_bounds__(kThreads, kScaleCtasPerSm) gradientScale(const __grid_constant__ Table<kCapacity> table, const double* partials, std::uint32_t count,
-                                                          double max_norm, float* norm) {
-    __shared__ double shared[kThreads / 32];
-    __shared__ float shared_factor;
-    gridDependencyWait();
-    gridDependencyLaunchDependents();
-    const double total = joinPartials<Sum>(partials, count, shared);
-    if (threadIdx.x == 0) {
-        const double ratio = max_norm / (total + 1e-6);
-        shared_factor      = ratio >= 1.0 ? 1.0F : static_cast<float>(ratio);  // a ratio that is not a number stays one
-        if (norm != nullptr && blockIdx.x == 0) { *norm = static_cast<float>(total); }
-    }
-    __syncthreads();
-    const float factor        = shared_factor;
+// The CTA's run of chunks, from the last one back.
+template<std::uint32_t kCapacity> __device__ __forceinline__ void scaleRun(const Table<kCapacity>& table, float factor) {
     const std::uint64_t begin = table.chunks * blockIdx.x / gridDim.x, end = table.chunks * (blockIdx.x + 1) / gridDim.x;
     if (begin == end) { return; }
     std::uint32_t index = findEntry(table, end - 1);
@@ -327,6 +314,31 @@ __global__ void __launch_bounds__(kThreads, kScaleCtasPerSm) gradientScale(const
             default: scaleStretch<__nv_bfloat16>(entry, s, factor); break;
         }
     }
+}
+
+template<typename Sum, std::uint32_t kCapacity>
+__global__ void __launch_bounds__(kThreads, kScaleCtasPerSm) gradientScale(const __grid_constant__ Table<kCapacity> table, const double* partials, std::uint32_t count,
+                                                          double max_norm, float* norm) {
+    __shared__ double shared[kThreads / 32];
+    __shared__ float shared_factor;
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const double total = joinPartials<Sum>(partials, count, shared);
+    if (threadIdx.x == 0) {
+        const double ratio = max_norm / (total + 1e-6);
+        shared_factor      = ratio >= 1.0 ? 1.0F : static_cast<float>(ratio);  // a ratio that is not a number stays one
+        if (norm != nullptr && blockIdx.x == 0) { *norm = static_cast<float>(total); }
+    }
+    __syncthreads();
+    scaleRun(table, shared_factor);
+}
+
+// The factor as the caller gives it.
+template<std::uint32_t kCapacity>
+__global__ void __launch_bounds__(kThreads, kScaleCtasPerSm) gradientMultiply(const __grid_constant__ Table<kCapacity> table, const float* factor) {
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    scaleRun(table, *factor);
 }
 
 // ---------------------------------------------------------------- host
@@ -482,27 +494,51 @@ template<typename Sum, std::uint32_t kCapacity> cudaError_t enqueue(const Call& 
     return cudaSuccess;
 }
 
-int runCall(const FtcudaGradient* gradients, std::uint64_t count, int norm_kind, bool clip, double max_norm, float* norm, std::int32_t device, void* workspace,
-            std::uint64_t workspace_bytes, void* stream, char* message, std::size_t capacity) {
+template<std::uint32_t kCapacity> cudaError_t enqueueMultiply(const FtcudaGradient* gradients, std::uint64_t count, const float* factor, int sms, cudaStream_t stream) {
+    const std::uint64_t launches = launchesFor(count), each = launches == 1 ? count : kTensors;
+    Table<kCapacity> table;
+    for (std::uint64_t l = 0; l < launches; ++l) {
+        fillTable(table, gradients + l * each, std::min(each, count - l * each), true);
+        const std::uint32_t grid = gridFor(table.chunks, sms, kScaleCtasPerSm);
+        if (l == 0) {  // an ordinary launch: it starts when what came before in the stream is done
+            gradientMultiply<kCapacity><<<grid, kThreads, 0, stream>>>(table, factor);
+            const cudaError_t error = cudaGetLastError();
+            if (error != cudaSuccess) { return error; }
+            countLaunches(1);
+        } else {
+            const cudaError_t error = training::launchOverlapped(gradientMultiply<kCapacity>, dim3(grid), dim3(kThreads), 0, stream, table, factor);
+            if (error != cudaSuccess) { return error; }
+        }
+    }
+    return cudaSuccess;
+}
+
+// What every call minds about its gradients; 0, or a failure with its message.
+int checkGradients(const FtcudaGradient* gradients, std::uint64_t count, bool written, char* message, std::size_t capacity) {
     if (gradients == nullptr && count != 0) { return fail(message, capacity, 1, "null gradients"); }
-    if (norm == nullptr || !training::aligned(norm, 4)) { return fail(message, capacity, 1, "the norm has no address, or one that is not a multiple of four"); }
-    if (norm_kind != FTCUDA_NORM_2 && norm_kind != FTCUDA_NORM_INF) { return fail(message, capacity, 1, "unknown kind of norm %d", norm_kind); }
-    if (clip && !(max_norm >= 0.0)) { return fail(message, capacity, 1, "max_norm must not be negative"); }
     if (count >= (1ULL << 24)) { return fail(message, capacity, 1, "too many gradients"); }
     for (std::uint64_t i = 0; i < count; ++i) {
-        if (const char* reason = checkGradient(gradients[i], clip)) {
+        if (const char* reason = checkGradient(gradients[i], written)) {
             return fail(message, capacity, 1, "gradient %llu: %s", static_cast<unsigned long long>(i), reason);
         }
     }
+    if (!written) { return 0; }
+    try {
+        if (const char* reason = checkOverlap(gradients, count)) { return fail(message, capacity, 1, "%s", reason); }
+    } catch (const std::bad_alloc&) { return fail(message, capacity, 1, "out of host memory"); }
+    return 0;
+}
+
+int runCall(const FtcudaGradient* gradients, std::uint64_t count, int norm_kind, bool clip, double max_norm, float* norm, std::int32_t device, void* workspace,
+            std::uint64_t workspace_bytes, void* stream, char* message, std::size_t capacity) {
+    if (norm == nullptr || !training::aligned(norm, 4)) { return fail(message, capacity, 1, "the norm has no address, or one that is not a multiple of four"); }
+    if (norm_kind != FTCUDA_NORM_2 && norm_kind != FTCUDA_NORM_INF) { return fail(message, capacity, 1, "unknown kind of norm %d", norm_kind); }
+    if (clip && !(max_norm >= 0.0)) { return fail(message, capacity, 1, "max_norm must not be negative"); }
     const std::uint64_t needed = ftcuda_gradient_norm_workspace_bytes(count);
     if (workspace == nullptr || workspace_bytes < needed || !training::aligned(workspace, 8)) {
         return fail(message, capacity, 1, "workspace of %llu bytes needed, at a multiple of eight", static_cast<unsigned long long>(needed));
     }
-    if (clip) {
-        try {
-            if (const char* reason = checkOverlap(gradients, count)) { return fail(message, capacity, 1, "%s", reason); }
-        } catch (const std::bad_alloc&) { return fail(message, capacity, 1, "out of host memory"); }
-    }
+    if (const int status = checkGradients(gradients, count, clip, message, capacity)) { return status; }
     int sms = 0;
     if (!training::deviceIsCurrent(device, message, capacity) || !deviceSmCount(device, &sms, message, capacity)) { return 1; }
     const Call call{gradients, count, clip, max_norm, norm, static_cast<double*>(workspace), sms, static_cast<cudaStream_t>(stream)};
@@ -531,4 +567,17 @@ extern "C" int ftcuda_gradient_norm(const FtcudaGradient* gradients, uint64_t co
 extern "C" int ftcuda_gradient_clip(const FtcudaGradient* gradients, uint64_t count, int norm_kind, double max_norm, float* norm, int32_t device,
                                     void* workspace, uint64_t workspace_bytes, void* stream, char* message, size_t message_capacity) {
     return ftcuda::runCall(gradients, count, norm_kind, true, max_norm, norm, device, workspace, workspace_bytes, stream, message, message_capacity);
+}
+
+extern "C" int ftcuda_gradient_scale(const FtcudaGradient* gradients, uint64_t count, const float* factor, int32_t device, void* stream, char* message,
+                                     size_t message_capacity) {
+    using namespace ftcuda;
+    if (factor == nullptr || !training::aligned(factor, 4)) { return fail(message, message_capacity, 1, "the factor has no address, or one that is not a multiple of four"); }
+    if (const int status = checkGradients(gradients, count, true, message, message_capacity)) { return status; }
+    int sms = 0;
+    if (!training::deviceIsCurrent(device, message, message_capacity) || !deviceSmCount(device, &sms, message, message_capacity)) { return 1; }
+    const cudaError_t error = count <= kFew ? enqueueMultiply<kFew>(gradients, count, factor, sms, static_cast<cudaStream_t>(stream))
+                                            : enqueueMultiply<kTensors>(gradients, count, factor, sms, static_cast<cudaStream_t>(stream));
+    if (error != cudaSuccess) { return fail(message, message_capacity, 1, "%s", cudaGetErrorString(error)); }
+    return 0;
 }

@@ -5,7 +5,9 @@
 //
 // The forward call is one pass over the vocabulary, 2 T V D operations; the backward call goes through the vocabulary piece by
 // piece and computes Z of a piece again: dZ of it, then dH += dZ W and dW = dZ^T H, 6 T V D. A piece is as wide as kPieceBytes of dZ allow, so that
-// the passes over dH (one for each piece) and the launches weigh little.
+// the passes over dH (one for each piece) and the launches weigh little. The step call does both for an upstream gradient of 1 without
+// computing Z twice, 6 T V D in all, where kStepBytes have room for all of Z's exponentials, 16 bits each (FP32: for Z), during the call:
+// a pass over them, two bytes read and two written for each, makes them dZ.
 //
 // Tokens without a target are left out first: the others' hidden states are gathered into the workspace, which costs one pass over H,
 // makes what the padding holds irrelevant (a NaN there would reach dW through 0 * NaN), spares the products those rows, and gives
@@ -38,7 +40,10 @@ constexpr int kJoinWarps               = 32;   // ... each of its warps some of 
 constexpr int kRowThreads              = 256;  // FP32: threads that go over a row of logits
 constexpr std::uint64_t kPieceBytes    = 512ULL << 20;  // of dZ (FP32: of Z), unless ...
 constexpr std::uint64_t kLeastColumns  = 8192;          // ... that is fewer columns than these
+constexpr std::uint64_t kStepBytes     = 2ULL << 30;    // that the step call's exponentials may take at most
 constexpr std::uint64_t kAlign         = 256;
+constexpr int kKeptRows                = 32;            // rows of a CTA that turns exponentials into slopes ...
+constexpr int kKeptPieces              = 4;             // ... and pieces of the statistics
 
 // ---------------------------------------------------------------- kernels
 
@@ -49,17 +54,17 @@ struct ListParams {
     std::int32_t reduction;
     LiveRows rows;
     std::int32_t* slot;        // [tokens]: a token's row, -1 for none
-    // forward
-    float* loss;
+    // where a loss is wanted: written for the tokens that take no part
+    float* loss;               // NULL with a reduction
     float* lse;
-    // backward
-    const float* saved_lse;
-    const float* grad_loss;
+    // where gradients are
+    const float* saved_lse;    // NULL in the step call, which has none yet
+    const float* grad_loss;    // NULL: 1
     std::int32_t scale_bits;   // log2 of what the largest |scale| is brought near to; INT_MIN: the scales stay as they are
 };
 
-// One CTA: the list of live tokens, and (backward) their scales.
-template<bool kBackward> __global__ void __launch_bounds__(kListThreads) listTokens(const ListParams p) {
+// One CTA: the list of live tokens, and (where gradients are wanted) their scales.
+template<bool kScales> __global__ void __launch_bounds__(kListThreads) listTokens(const ListParams p) {
     __shared__ std::uint32_t warp_counts[kListThreads / 32];
     __shared__ std::uint32_t largest_bits;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -88,18 +93,21 @@ template<bool kBackward> __global__ void __launch_bounds__(kListThreads) listTok
             if (on) {
                 p.rows.token[at]  = static_cast<std::int32_t>(t);
                 p.rows.target[at] = y >= 0 && y < p.vocabulary ? static_cast<std::int32_t>(y) : loss::kBadTarget;
-                if (kBackward && p.reduction == FTCUDA_REDUCTION_NONE) { largest = max(largest, __float_as_uint(p.grad_loss[t]) & 0x7FFFFFFFU); }
-            } else if (!kBackward) {
-                p.lse[t] = 0.0F;
-                if (p.reduction == FTCUDA_REDUCTION_NONE) { p.loss[t] = 0.0F; }
+                if (kScales && p.reduction == FTCUDA_REDUCTION_NONE) { largest = max(largest, __float_as_uint(p.grad_loss[t]) & 0x7FFFFFFFU); }
+            } else {
+                if (p.lse != nullptr) { p.lse[t] = 0.0F; }
+                if (p.loss != nullptr) { p.loss[t] = 0.0F; }
             }
         }
         count += all;
     }
     const std::uint32_t padded = (max(count, 1U) + loss::kTileRows - 1) / loss::kTileRows * loss::kTileRows;
-    if (kBackward) {
+    if (kScales) {
         float common = 0.0F;
-        if (p.reduction != FTCUDA_REDUCTION_NONE) { common = p.reduction == FTCUDA_REDUCTION_MEAN ? *p.grad_loss / static_cast<float>(max(count, 1U)) : *p.grad_loss; }
+        if (p.reduction != FTCUDA_REDUCTION_NONE) {
+            common = p.grad_loss != nullptr ? *p.grad_loss : 1.0F;
+            if (p.reduction == FTCUDA_REDUCTION_MEAN) { common /= static_cast<float>(max(count, 1U)); }
+        }
         atomicMax(&largest_bits, largest);
         __syncthreads();
         // With one upstream gradient for all, the scale is the power of two alone, so that -1, the slope of a target that has hardly any
@@ -121,7 +129,7 @@ template<bool kBackward> __global__ void __launch_bounds__(kListThreads) listTok
             if (i < count) {
                 const std::int32_t t = p.rows.token[i];
                 scale                = ldexpf(each ? p.grad_loss[t] : common, shift);
-                lse2                 = p.saved_lse[t] * loss::kLog2E;
+                lse2                 = p.saved_lse != nullptr ? p.saved_lse[t] * loss::kLog2E : 0.0F;
                 if (p.rows.target[i] == loss::kBadTarget) { scale = __uint_as_float(0x7FFFFFFFU); }
             }
             p.rows.scale[i] = scale;
@@ -181,7 +189,8 @@ struct JoinParams {
     std::uint32_t pieces, capacity;
     float* row_loss;         // [capacity]
     float* loss;             // [tokens], or NULL
-    float* lse;              // [tokens]
+    float* lse;              // [tokens], or NULL
+    bool keep;               // rows.lse2 is wanted
 };
 
 __global__ void __launch_bounds__(kJoinWarps * 32) joinStatistics(const JoinParams p) {
@@ -213,12 +222,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) joinStatistics(const JoinPara
     __syncthreads();
     if (warp == 0 && row < live) {
         for (int w = 1; w < kJoinWarps; ++w) { sum = joinPartials(sum, shared[w][threadIdx.x]); }
-        const float lse          = loss::kLn2 * (sum.x + log2f(sum.y));
+        const float lse2         = sum.x + log2f(sum.y);
+        const float lse          = loss::kLn2 * lse2;
         const bool bad           = p.rows.target[row] == loss::kBadTarget;
         const float value        = bad ? __uint_as_float(0x7FFFFFFFU) : lse - p.rows.picked[row];
         const std::int32_t token = p.rows.token[row];
-        p.lse[token]             = lse;
         p.row_loss[row]          = value;
+        if (p.lse != nullptr) { p.lse[token] = lse; }
+        if (p.keep) { p.rows.lse2[row] = lse2; }
         if (p.loss != nullptr) { p.loss[token] = value; }
     }
 }
@@ -317,6 +328,59 @@ __global__ void __launch_bounds__(kRowThreads) rowSlopes(const RowParams p) {
         // (The pitch has room for a whole quad behind the last column.)
         const float4 x                        = *reinterpret_cast<const float4*>(z + at);
         *reinterpret_cast<float4*>(z + at) = make_float4(slope(x.x, at), slope(x.y, at + 1), slope(x.z, at + 2), slope(x.w, at + 3));
+    }
+}
+
+struct KeptParams {
+    LiveRows rows;
+    const float2* partials;  // [piece][capacity]
+    std::uint32_t pieces, width, capacity;
+    std::uint64_t pitch;
+};
+
+// What the product kept becomes dZ, in place: 2^(logit - piece's largest) 2^(that - lse), less the target's one; zeros in the neutral rows. A thread
+// takes eight columns of a row at a time, neighbouring threads neighbouring ones.
+template<typename T> __global__ void __launch_bounds__(256) keptSlopes(const KeptParams p, __half* kept) {
+    __shared__ float factors[kKeptPieces][kKeptRows];
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const std::uint32_t live   = *p.rows.count;
+    const std::uint32_t row0   = blockIdx.y * kKeptRows, piece0 = blockIdx.x * kKeptPieces;
+    const std::uint32_t padded = (max(live, 1U) + loss::kTileRows - 1) / loss::kTileRows * loss::kTileRows;
+    if (row0 >= padded) { return; }
+    const std::uint32_t pieces = min(p.pieces - piece0, static_cast<std::uint32_t>(kKeptPieces));
+    if (threadIdx.x < kKeptPieces * kKeptRows) {
+        const std::uint32_t piece = threadIdx.x / kKeptRows, row = row0 + threadIdx.x % kKeptRows;
+        if (piece < pieces && row < live) {
+            const float base = p.partials[static_cast<std::uint64_t>(piece0 + piece) * p.capacity + row].x;
+            // (A piece of -inf alone kept zeros; against a sum of nothing, or of NaN, NaN comes out.)
+            const float lse2 = p.rows.lse2[row];
+            factors[piece][threadIdx.x % kKeptRows] = p.rows.scale[row] * (1.0F / loss::kKeptScale) * (base == -INFINITY && lse2 > -INFINITY ? 0.0F : exp2f(base - lse2));
+        }
+    }
+    __syncthreads();
+    const std::uint32_t each  = p.width / 8;  // packs of a piece's row
+    const std::uint32_t packs = pieces * each;
+    for (std::uint32_t i = threadIdx.x; i < packs * kKeptRows; i += 256) {
+        const std::uint32_t in_row = i / packs, pack = i - in_row * packs;
+        const std::uint32_t row    = row0 + in_row, col = piece0 * p.width + pack * 8;
+        uint4* const at            = reinterpret_cast<uint4*>(kept + row * p.pitch + col);
+        if (row >= live) {
+            *at = make_uint4(0, 0, 0, 0);
+            continue;
+        }
+        const float factor        = factors[pack / each][in_row];
+        const std::int32_t hit    = p.rows.target[row] - static_cast<std::int32_t>(col);
+        alignas(16) __half from[8];
+        alignas(16) T to[8];
+        *reinterpret_cast<uint4*>(from) = *at;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float slope = factor * __half2float(from[j]);
+            if (j == hit) { slope -= p.rows.scale[row]; }
+            to[j] = Element<T>::narrow(slope);
+        }
+        *at = *reinterpret_cast<const uint4*>(to);
     }
 }
 
@@ -449,7 +513,16 @@ FtcudaGemmDesc describeWeight(const FtcudaLinearCrossEntropy& q, const Layout& l
     return d;
 }
 
-int layOut(const FtcudaLinearCrossEntropy& q, bool backward, int sms, Layout& l, char* message, std::size_t capacity) {
+// What a call computes: the loss, the gradients from a loss that is known, or both at once.
+enum class Form { kLoss, kGradients, kStep };
+
+// What the step call holds of all logits at once, in bytes.
+std::uint64_t stepBytes(const FtcudaLinearCrossEntropy& q) {
+    return roundUp(std::max<std::uint64_t>(q.tokens, 1), loss::kTileRows) * roundUp(q.vocabulary, 256) * training::elementBytes(q.element);
+}
+
+int layOut(const FtcudaLinearCrossEntropy& q, Form form, int sms, Layout& l, char* message, std::size_t capacity) {
+    const bool gradients      = form != Form::kLoss;
     const std::uint64_t bytes = training::elementBytes(q.element);
     const bool fp32           = isFp32(q);
     l                         = Layout{};
@@ -457,7 +530,7 @@ int layOut(const FtcudaLinearCrossEntropy& q, bool backward, int sms, Layout& l,
     l.copy_pitch              = roundUp(q.depth, 16 / bytes);
     l.weight_pitch            = !fp32 && !weightFits(q) ? roundUp(q.depth, 8) : 0;
     const std::uint64_t fill  = roundUp(q.vocabulary, 256);
-    l.columns                 = std::min(fill, std::max(kLeastColumns, kPieceBytes / (l.capacity * bytes) / 256 * 256));
+    l.columns                 = form == Form::kStep ? fill : std::min(fill, std::max(kLeastColumns, kPieceBytes / (l.capacity * bytes) / 256 * 256));
     l.columns                 = roundUp(ceilDiv(fill, ceilDiv(fill, l.columns)), 256);  // pieces of about one size
     l.piece_pitch             = l.columns;
     l.pieces                  = fp32 ? ceilDiv(q.vocabulary, l.columns) : loss::statisticsPieces(static_cast<std::uint32_t>(q.vocabulary));
@@ -477,16 +550,17 @@ int layOut(const FtcudaLinearCrossEntropy& q, bool backward, int sms, Layout& l,
     l.slot   = take(4 * l.capacity);
     l.hidden = take(bytes * l.capacity * l.copy_pitch);
     if (l.weight_pitch != 0) { l.weight = take(2 * q.vocabulary * l.weight_pitch); }
-    if (backward) {
+    if (gradients) {
         l.scale = take(4 * l.capacity);
         l.lse2  = take(4 * l.capacity);
         l.sums  = take(4 * l.capacity * l.sums_pitch * l.splits);
-    } else {
+    }
+    if (form != Form::kGradients) {
         l.picked   = take(4 * l.capacity);
         l.row_loss = take(4 * l.capacity);
         l.partials = take(8 * l.capacity * l.pieces);
     }
-    if (backward || fp32) { l.piece = take(bytes * l.capacity * l.piece_pitch); }
+    if (gradients || fp32) { l.piece = take(bytes * l.capacity * l.piece_pitch); }
     if (fp32 && q.tokens != 0) {
         // The most that any product of any piece wants. (The addresses are not known yet, but how they are aligned is.)
         l.product            = at;
@@ -497,7 +571,7 @@ int layOut(const FtcudaLinearCrossEntropy& q, bool backward, int sms, Layout& l,
             Product product;
             if (configureProduct(describeLogits(q, l, stand_in, first, columns), false, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
             l.product_bytes = std::max(l.product_bytes, product.bytes);
-            if (!backward) { continue; }
+            if (!gradients) { continue; }
             if (configureProduct(describeHidden(q, l, stand_in, first, columns), true, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
             l.product_bytes = std::max(l.product_bytes, product.bytes);
             if (configureProduct(describeWeight(q, l, stand_in, first, columns, stand_in, static_cast<std::int64_t>(q.depth)), true, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
@@ -532,9 +606,9 @@ class Call final {
     Call(const FtcudaLinearCrossEntropy& problem, char* message, std::size_t capacity) : q_(problem), message_(message), capacity_(capacity) {}
 
     // Everything that is the same in both directions; 0 or a failure that has its message.
-    int begin(bool backward, void* workspace, std::uint64_t workspace_bytes, void* stream) {
+    int begin(Form form, void* workspace, std::uint64_t workspace_bytes, void* stream) {
         if (!training::deviceIsCurrent(q_.device, message_, capacity_) || !deviceSmCount(q_.device, &sms_, message_, capacity_)) { return 1; }
-        if (layOut(q_, backward, sms_, l_, message_, capacity_) != 0) { return 1; }
+        if (layOut(q_, form, sms_, l_, message_, capacity_) != 0) { return 1; }
         if (workspace == nullptr || workspace_bytes < l_.total || !training::aligned(workspace, kAlign)) {
             return fail(message_, capacity_, 1, "workspace of %llu bytes needed, at a multiple of 256", static_cast<unsigned long long>(l_.total));
         }
@@ -561,7 +635,7 @@ class Call final {
 
     cudaError_t forward(float* loss, float* lse) {
         ListParams list = listParams();
-        list.loss       = loss;
+        list.loss       = q_.reduction == FTCUDA_REDUCTION_NONE ? loss : nullptr;
         list.lse        = lse;
         // (The first kernel of a call is an ordinary launch: it starts when what came before in the stream is done.)
         listTokens<false><<<1, kListThreads, 0, stream_>>>(list);
@@ -580,40 +654,52 @@ class Call final {
                 }
             }
         }
-        if (error != cudaSuccess) { return error; }
-        JoinParams join{};
-        join.rows     = rows_;
-        join.partials = partials;
-        join.pieces   = static_cast<std::uint32_t>(l_.pieces);
-        join.capacity = static_cast<std::uint32_t>(l_.capacity);
-        join.row_loss = at<float>(l_.row_loss);
-        join.loss     = q_.reduction == FTCUDA_REDUCTION_NONE ? loss : nullptr;
-        join.lse      = lse;
-        error = training::launchOverlapped(joinStatistics, dim3(static_cast<unsigned>(l_.capacity / kJoinRows)), dim3(kJoinWarps * 32), 0, stream_, join);
-        if (error == cudaSuccess && q_.reduction != FTCUDA_REDUCTION_NONE) {
-            error = training::launchOverlapped(sumLosses, dim3(1), dim3(kListThreads), 0, stream_, rows_, static_cast<const float*>(at<float>(l_.row_loss)),
-                                               q_.reduction == FTCUDA_REDUCTION_MEAN, loss);
+        return error == cudaSuccess ? join(loss, lse, false) : error;
+    }
+
+    // The loss, and the gradients for an upstream gradient of 1, with the logits computed once.
+    cudaError_t step(float* loss, void* grad_hidden, std::int64_t hidden_stride, void* grad_weight, std::int64_t weight_stride, std::int32_t grad_element) {
+        ListParams list = listParams();
+        list.scale_bits = scaleBits();
+        listTokens<true><<<1, kListThreads, 0, stream_>>>(list);
+        cudaError_t error = started();
+        if (error == cudaSuccess) { error = gather(); }
+        float2* const partials        = at<float2>(l_.partials);
+        const std::uint32_t columns   = static_cast<std::uint32_t>(q_.vocabulary);
+        if (error == cudaSuccess && !isFp32(q_)) { error = loss::launchKept(products_, weight(0), columns, partials, base_ + l_.piece, l_.piece_pitch); }
+        if (isFp32(q_)) {
+            if (error == cudaSuccess) { error = multiply(describeLogits(q_, l_, base_, 0, columns), false); }
+            if (error == cudaSuccess) { error = training::launchOverlapped(rowStatistics, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(0, columns, partials)); }
         }
-        return error;
+        if (error == cudaSuccess) { error = join(loss, nullptr, true); }
+        if (error != cudaSuccess) { return error; }
+        if (isFp32(q_)) {
+            error = training::launchOverlapped(rowSlopes, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(0, columns, nullptr));
+        } else {
+            const KeptParams kept{rows_, partials, static_cast<std::uint32_t>(l_.pieces), loss::statisticsWidth(columns), static_cast<std::uint32_t>(l_.capacity),
+                                  l_.piece_pitch};
+            const dim3 grid(static_cast<unsigned>(ceilDiv(l_.pieces, kKeptPieces)), static_cast<unsigned>(l_.capacity / kKeptRows));
+            error = training::launchOverlapped(q_.element == FTCUDA_ELEMENT_FP16 ? keptSlopes<__half> : keptSlopes<__nv_bfloat16>, grid, dim3(256), 0, stream_, kept,
+                                               at<__half>(l_.piece));
+        }
+        if (error == cudaSuccess) { error = multiplySlopes(0, columns, grad_hidden != nullptr, grad_weight, weight_stride, grad_element); }
+        return error == cudaSuccess && grad_hidden != nullptr ? spreadTyped(grad_hidden, hidden_stride, grad_element) : error;
     }
 
     cudaError_t backward(const float* lse, const float* grad_loss, void* grad_hidden, std::int64_t hidden_stride, void* grad_weight, std::int64_t weight_stride) {
         ListParams list = listParams();
         list.saved_lse  = lse;
         list.grad_loss  = grad_loss;
-        list.scale_bits = isFp32(q_) ? INT32_MIN : q_.element == FTCUDA_ELEMENT_FP16 ? 13 : 0;
+        list.scale_bits = scaleBits();
         listTokens<true><<<1, kListThreads, 0, stream_>>>(list);
         cudaError_t error = started();
         if (error == cudaSuccess) { error = gather(); }
         for (std::uint64_t first = 0; first < q_.vocabulary && error == cudaSuccess; first += l_.columns) {
-            error = piece(first, std::min(l_.columns, q_.vocabulary - first), grad_hidden != nullptr, grad_weight, weight_stride);
+            const std::uint64_t columns = std::min(l_.columns, q_.vocabulary - first);
+            error                       = slopes(first, columns);
+            if (error == cudaSuccess) { error = multiplySlopes(first, columns, grad_hidden != nullptr, grad_weight, weight_stride, q_.element); }
         }
-        if (error != cudaSuccess || grad_hidden == nullptr) { return error; }
-        switch (q_.element) {
-            case FTCUDA_ELEMENT_FP32: return spread(static_cast<float*>(grad_hidden), hidden_stride);
-            case FTCUDA_ELEMENT_FP16: return spread(static_cast<__half*>(grad_hidden), hidden_stride);
-            default: return spread(static_cast<__nv_bfloat16*>(grad_hidden), hidden_stride);
-        }
+        return error == cudaSuccess && grad_hidden != nullptr ? spreadTyped(grad_hidden, hidden_stride, q_.element) : error;
     }
 
   private:
@@ -624,6 +710,9 @@ class Call final {
         if (error == cudaSuccess) { countLaunches(1); }
         return error;
     }
+
+    // FP16's exponents do not hold small probabilities unless the largest slope is near 2^13.
+    std::int32_t scaleBits() const { return isFp32(q_) ? INT32_MIN : q_.element == FTCUDA_ELEMENT_FP16 ? 13 : 0; }
 
     ListParams listParams() const {
         ListParams list{};
@@ -681,27 +770,60 @@ class Call final {
         return cudaSuccess;
     }
 
-    cudaError_t piece(std::uint64_t first, std::uint64_t columns, bool hidden, void* grad_weight, std::int64_t weight_stride) const {
+    // The statistics of all rows joined: the loss, and (keep) rows_.lse2.
+    cudaError_t join(float* loss, float* lse, bool keep) const {
+        JoinParams join{};
+        join.rows     = rows_;
+        join.partials = at<float2>(l_.partials);
+        join.pieces   = static_cast<std::uint32_t>(l_.pieces);
+        join.capacity = static_cast<std::uint32_t>(l_.capacity);
+        join.row_loss = at<float>(l_.row_loss);
+        join.loss     = q_.reduction == FTCUDA_REDUCTION_NONE ? loss : nullptr;
+        join.lse      = lse;
+        join.keep     = keep;
+        const cudaError_t error = training::launchOverlapped(joinStatistics, dim3(static_cast<unsigned>(l_.capacity / kJoinRows)), dim3(kJoinWarps * 32), 0, stream_, join);
+        if (error != cudaSuccess || q_.reduction == FTCUDA_REDUCTION_NONE) { return error; }
+        return training::launchOverlapped(sumLosses, dim3(1), dim3(kListThreads), 0, stream_, rows_, static_cast<const float*>(at<float>(l_.row_loss)),
+                                          q_.reduction == FTCUDA_REDUCTION_MEAN, loss);
+    }
+
+    // dZ of a piece of the vocabulary, to the workspace.
+    cudaError_t slopes(std::uint64_t first, std::uint64_t columns) const {
         const std::uint32_t first32 = static_cast<std::uint32_t>(first), columns32 = static_cast<std::uint32_t>(columns);
+        if (!isFp32(q_)) { return loss::launchSlopes(products_, weight(first), first32, columns32, base_ + l_.piece, l_.piece_pitch); }
+        const cudaError_t error = multiply(describeLogits(q_, l_, base_, first, columns), false);
+        if (error != cudaSuccess) { return error; }
+        return training::launchOverlapped(rowSlopes, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(first, columns, nullptr));
+    }
+
+    // What dZ of a piece is multiplied with.
+    cudaError_t multiplySlopes(std::uint64_t first, std::uint64_t columns, bool hidden, void* grad_weight, std::int64_t weight_stride, std::int32_t grad_element) const {
         if (!isFp32(q_)) {
-            cudaError_t error = loss::launchSlopes(products_, weight(first), first32, columns32, base_ + l_.piece, l_.piece_pitch);
-            if (error != cudaSuccess) { return error; }
             loss::Gradients gradients{};
             gradients.sums                  = hidden ? at<float>(l_.sums) : nullptr;
             gradients.sums_pitch            = l_.sums_pitch;
             gradients.splits                = l_.splits;
             gradients.accumulate            = first != 0;
-            gradients.weight_gradient       = grad_weight == nullptr ? nullptr : static_cast<unsigned char*>(grad_weight) + 2 * static_cast<std::int64_t>(first) * weight_stride;
+            gradients.weight_gradient_fp32  = grad_element == FTCUDA_ELEMENT_FP32;
             gradients.weight_gradient_pitch = weight_stride;
-            return loss::launchGradients(products_, weight(first), columns32, base_ + l_.piece, l_.piece_pitch, gradients);
+            if (grad_weight != nullptr) {
+                gradients.weight_gradient =
+                    static_cast<unsigned char*>(grad_weight) + static_cast<std::int64_t>(training::elementBytes(grad_element) * first) * weight_stride;
+            }
+            return loss::launchGradients(products_, weight(first), static_cast<std::uint32_t>(columns), base_ + l_.piece, l_.piece_pitch, gradients);
         }
-        cudaError_t error = multiply(describeLogits(q_, l_, base_, first, columns), false);
-        if (error == cudaSuccess) {
-            error = training::launchOverlapped(rowSlopes, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(first, columns, nullptr));
-        }
-        if (error == cudaSuccess && hidden) { error = multiply(describeHidden(q_, l_, base_, first, columns), true); }
+        cudaError_t error = cudaSuccess;
+        if (hidden) { error = multiply(describeHidden(q_, l_, base_, first, columns), true); }
         if (error == cudaSuccess && grad_weight != nullptr) { error = multiply(describeWeight(q_, l_, base_, first, columns, grad_weight, weight_stride), true); }
         return error;
+    }
+
+    cudaError_t spreadTyped(void* out, std::int64_t stride, std::int32_t element) const {
+        switch (element) {
+            case FTCUDA_ELEMENT_FP32: return spread(static_cast<float*>(out), stride);
+            case FTCUDA_ELEMENT_FP16: return spread(static_cast<__half*>(out), stride);
+            default: return spread(static_cast<__nv_bfloat16*>(out), stride);
+        }
     }
 
     template<typename T> cudaError_t spread(T* out, std::int64_t stride) const {
@@ -730,19 +852,69 @@ int finish(cudaError_t error, char* message, std::size_t capacity) {
 
 bool wordAligned(const void* pointer) { return pointer != nullptr && training::aligned(pointer, 4); }
 
+// nullptr, or why the step call does not take the problem.
+const char* checkStep(const FtcudaLinearCrossEntropy& q) {
+    if (q.reduction == FTCUDA_REDUCTION_NONE) { return "without reduction the upstream gradients differ from token to token"; }
+    if (q.tokens == 0) { return "there are no tokens"; }
+    if (stepBytes(q) > kStepBytes) { return "the exponentials of all logits take more than 2 GiB"; }
+    return nullptr;
+}
+
+// nullptr, or what is wrong with where the gradients go. The weight's stride comes out as one that rows can have.
+const char* checkGradients(const FtcudaLinearCrossEntropy& q, std::uint64_t bytes, const void* grad_hidden, std::int64_t hidden_stride, const void* grad_weight,
+                           std::int64_t& weight_stride) {
+    const std::int64_t depth = static_cast<std::int64_t>(q.depth);
+    if ((grad_hidden != nullptr && !training::aligned(grad_hidden, bytes)) || (grad_weight != nullptr && !training::aligned(grad_weight, bytes))) {
+        return "a gradient's address is not a multiple of its element's size";
+    }
+    if (grad_hidden != nullptr && q.tokens > 1 && (hidden_stride < depth || hidden_stride >= (1LL << 31))) {
+        return "the rows of the hidden states' gradient overlap, or lie too far apart";
+    }
+    if (grad_weight != nullptr && q.vocabulary > 1 && (weight_stride < depth || weight_stride >= (1LL << 31))) {
+        return "the rows of the weight's gradient overlap, or lie too far apart";
+    }
+    if (q.vocabulary == 1) { weight_stride = depth; }
+    return nullptr;
+}
+
+int workspaceBytes(const FtcudaLinearCrossEntropy* problem, Form form, std::uint64_t* bytes, char* message, std::size_t capacity) {
+    if (problem == nullptr || bytes == nullptr) { return fail(message, capacity, 1, "null argument"); }
+    const char* reason = check(*problem);
+    if (reason == nullptr && form == Form::kStep) { reason = checkStep(*problem); }
+    if (reason != nullptr) { return fail(message, capacity, 1, "%s", reason); }
+    int sms = 0;
+    Layout layout;
+    if (!deviceSmCount(problem->device, &sms, message, capacity) || layOut(*problem, form, sms, layout, message, capacity) != 0) { return 1; }
+    *bytes = layout.total;
+    return 0;
+}
+
 }  // namespace
 }  // namespace ftcuda
 
 extern "C" int ftcuda_linear_cross_entropy_workspace_bytes(const FtcudaLinearCrossEntropy* problem, int backward, uint64_t* workspace_bytes, char* message,
                                                            size_t message_capacity) {
+    return ftcuda::workspaceBytes(problem, backward != 0 ? ftcuda::Form::kGradients : ftcuda::Form::kLoss, workspace_bytes, message, message_capacity);
+}
+
+extern "C" int ftcuda_linear_cross_entropy_step_workspace_bytes(const FtcudaLinearCrossEntropy* problem, uint64_t* workspace_bytes, char* message, size_t message_capacity) {
+    return ftcuda::workspaceBytes(problem, ftcuda::Form::kStep, workspace_bytes, message, message_capacity);
+}
+
+extern "C" int ftcuda_linear_cross_entropy_step(const FtcudaLinearCrossEntropy* problem, float* loss, int32_t grad_element, void* grad_hidden, int64_t grad_hidden_row_stride,
+                                                void* grad_weight, int64_t grad_weight_row_stride, void* workspace, uint64_t workspace_bytes, void* stream,
+                                                char* message, size_t message_capacity) {
     using namespace ftcuda;
-    if (problem == nullptr || workspace_bytes == nullptr) { return fail(message, message_capacity, 1, "null argument"); }
-    if (const char* reason = check(*problem)) { return fail(message, message_capacity, 1, "%s", reason); }
-    int sms = 0;
-    Layout layout;
-    if (!deviceSmCount(problem->device, &sms, message, message_capacity) || layOut(*problem, backward != 0, sms, layout, message, message_capacity) != 0) { return 1; }
-    *workspace_bytes = layout.total;
-    return 0;
+    if (problem == nullptr) { return fail(message, message_capacity, 1, "null problem"); }
+    const char* reason = check(*problem);
+    if (reason == nullptr) { reason = checkStep(*problem); }
+    if (reason == nullptr && grad_element != problem->element && grad_element != FTCUDA_ELEMENT_FP32) { reason = "the gradients are of the operands' type, or FP32"; }
+    if (reason == nullptr && !wordAligned(loss)) { reason = "the loss has no address, or one that is not a multiple of four"; }
+    if (reason == nullptr) { reason = checkGradients(*problem, training::elementBytes(grad_element), grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride); }
+    if (reason != nullptr) { return fail(message, message_capacity, 1, "%s", reason); }
+    Call call(*problem, message, message_capacity);
+    if (const int status = call.begin(Form::kStep, workspace, workspace_bytes, stream)) { return status; }
+    return finish(call.step(loss, grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride, grad_element), message, message_capacity);
 }
 
 extern "C" int ftcuda_linear_cross_entropy(const FtcudaLinearCrossEntropy* problem, float* loss, float* lse, void* workspace, uint64_t workspace_bytes, void* stream,
@@ -754,7 +926,7 @@ extern "C" int ftcuda_linear_cross_entropy(const FtcudaLinearCrossEntropy* probl
     if (!(empty && problem->reduction == FTCUDA_REDUCTION_NONE) && !wordAligned(loss)) { return fail(message, message_capacity, 1, "the loss has no address, or one that is not a multiple of four"); }
     if (!empty && !wordAligned(lse)) { return fail(message, message_capacity, 1, "lse has no address, or one that is not a multiple of four"); }
     Call call(*problem, message, message_capacity);
-    if (const int status = call.begin(false, workspace, workspace_bytes, stream)) { return status; }
+    if (const int status = call.begin(Form::kLoss, workspace, workspace_bytes, stream)) { return status; }
     if (empty) {
         return finish(problem->reduction == FTCUDA_REDUCTION_NONE ? cudaSuccess : cudaMemsetAsync(loss, 0, sizeof(float), static_cast<cudaStream_t>(stream)), message,
                       message_capacity);
@@ -769,21 +941,13 @@ extern "C" int ftcuda_linear_cross_entropy_backward(const FtcudaLinearCrossEntro
     if (problem == nullptr) { return fail(message, message_capacity, 1, "null problem"); }
     if (const char* reason = check(*problem)) { return fail(message, message_capacity, 1, "%s", reason); }
     const std::uint64_t bytes = training::elementBytes(problem->element);
-    const std::int64_t depth  = static_cast<std::int64_t>(problem->depth);
     const bool empty          = problem->tokens == 0;
     if (!empty && (!wordAligned(lse) || !wordAligned(grad_loss))) { return fail(message, message_capacity, 1, "lse or the loss's gradient has no address, or one that is not a multiple of four"); }
-    if ((grad_hidden != nullptr && !training::aligned(grad_hidden, bytes)) || (grad_weight != nullptr && !training::aligned(grad_weight, bytes))) {
-        return fail(message, message_capacity, 1, "a gradient's address is not a multiple of its element's size");
+    if (const char* reason = checkGradients(*problem, bytes, grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride)) {
+        return fail(message, message_capacity, 1, "%s", reason);
     }
-    if (grad_hidden != nullptr && problem->tokens > 1 && (grad_hidden_row_stride < depth || grad_hidden_row_stride >= (1LL << 31))) {
-        return fail(message, message_capacity, 1, "the rows of the hidden states' gradient overlap, or lie too far apart");
-    }
-    if (grad_weight != nullptr && problem->vocabulary > 1 && (grad_weight_row_stride < depth || grad_weight_row_stride >= (1LL << 31))) {
-        return fail(message, message_capacity, 1, "the rows of the weight's gradient overlap, or lie too far apart");
-    }
-    if (problem->vocabulary == 1) { grad_weight_row_stride = depth; }
     Call call(*problem, message, message_capacity);
-    if (const int status = call.begin(true, workspace, workspace_bytes, stream)) { return status; }
+    if (const int status = call.begin(Form::kGradients, workspace, workspace_bytes, stream)) { return status; }
     if (empty) {
         if (grad_weight == nullptr) { return 0; }
         return finish(cudaMemset2DAsync(grad_weight, static_cast<std::size_t>(grad_weight_row_stride) * bytes, 0, problem->depth * bytes, problem->vocabulary,

@@ -1,6 +1,7 @@
 // The products of the linear cross entropy on BF16 or FP16 operands, each with its epilogue (linear_cross_entropy.cu has the whole).
 //
 //   statistics   Z = H W^T; of a tile of Z nothing is kept but the rows' maxima and sums of exponentials
+//   kept         the same, and the exponentials go to memory in FP16, each against its row's maximum in 128 columns
 //   slopes       Z once more; dZ = scale (exp(Z - lse) - onehot), rounded to the operands' type, goes to memory for a piece of the vocabulary
 //   gradients    dH (+)= dZ W and dW = dZ^T H of that piece, in one launch
 //
@@ -8,7 +9,7 @@
 // of each value) is what the gradients' own rounding comes to as well. Its scale brings the largest possible value near 1 (BF16) or 2^14 (FP16, whose
 // exponents would not hold the small probabilities otherwise).
 //
-// One kernel does all three. A pair of CTAs (tcgen05 cta_group::2, a cluster of two) takes tiles of 256 rows and up to 256 columns, K in
+// One kernel does all four. A pair of CTAs (tcgen05 cta_group::2, a cluster of two) takes tiles of 256 rows and up to 256 columns, K in
 // blocks of 64; a CTA brings its 128 rows of A and its half of B, each as the matrix lies in memory: an operand whose
 // neighbours run along K is a K-major operand, one whose neighbours run along its rows an MN-major one, so nothing is ever transposed.
 //
@@ -59,7 +60,7 @@ constexpr int kIssuerWarp    = 1;
 constexpr int kFirstEpilogue = 4;
 constexpr std::uint32_t kTmemColumns = 512;
 
-enum Mode : int { kStatistics, kSlopes, kGradients };
+enum Mode : int { kStatistics, kKept, kSlopes, kGradients };
 
 struct Barriers {
     std::uint64_t full[kStages];  // used in the pair's first CTA
@@ -88,7 +89,7 @@ struct ProductParams {
     std::uint32_t first;        // column of the vocabulary that column 0 is
     LiveRows rows;
     float2* partials;
-    void* slopes;
+    void* slopes;               // or what is kept
     std::uint64_t slopes_pitch;
     float* sums;
     std::uint64_t sums_pitch;
@@ -96,6 +97,7 @@ struct ProductParams {
     std::uint32_t weight_problem;  // which of the problems is the weight's gradient
     void* weight_gradient;
     std::int64_t weight_gradient_pitch;
+    std::uint32_t weight_fp32;
     std::uint32_t weight_vector;   // elements of it that one aligned store takes: 16, 8, or 1
     int* status;
 };
@@ -190,7 +192,23 @@ __device__ __forceinline__ std::uint32_t pack16(float low, float high, bool bf16
     return *reinterpret_cast<const std::uint32_t*>(&pair);
 }
 
+// This thread's row of a 16-bit matrix that has room for whole tiles; what lies beyond the columns is never fetched.
+__device__ __forceinline__ void storeRow(const ProductParams& p, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, float scale, bool on, bool bf16,
+                                         const float (&v)[128]) {
+    unsigned char* const out = static_cast<unsigned char*>(p.slopes) + (static_cast<std::uint64_t>(row) * p.slopes_pitch + col) * 2;
+#pragma unroll
+    for (int j = 0; j < 128; j += 16) {
+        if (j < 64 || pieces == 4) {
+            std::uint32_t packed[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { packed[i] = on ? pack16(scale * v[j + 2 * i], scale * v[j + 2 * i + 1], bf16) : 0; }
+            storeGlobal8(out + 2 * j, packed);
+        }
+    }
+}
+
 // What a warp does with 32 rows (`row`: this thread's) and 32 * pieces columns from `col` on, held in v.
+template<bool kKeep>
 __device__ __forceinline__ void finishStatistics(const ProductParams& p, const Item& w, std::uint32_t row, std::uint32_t col, std::uint32_t pieces,
                                                  std::uint32_t half, std::uint32_t live, float (&v)[128]) {
     const std::uint32_t columns = p.problem[0].columns;
@@ -217,10 +235,15 @@ __device__ __forceinline__ void finishStatistics(const ProductParams& p, const I
     float sum[4] = {0.0F, 0.0F, 0.0F, 0.0F};
 #pragma unroll
     for (int j = 0; j < 128; ++j) {
-        if (j < 64 || pieces == 4) { sum[j % 4] += exp2Fast(fmaf(v[j], kLog2E, -base)); }
+        if (j < 64 || pieces == 4) {
+            const float e = exp2Fast(fmaf(v[j], kLog2E, -base));
+            sum[j % 4] += e;
+            if (kKeep) { v[j] = e; }
+        }
     }
     const std::uint32_t piece = 2 * (w.col / p.problem[0].tile_n) + half;
     p.partials[static_cast<std::uint64_t>(piece) * p.capacity + row] = make_float2(none ? -INFINITY : base, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+    if (kKeep) { storeRow(p, row, col, pieces, kKeptScale, true, false, v); }
 }
 
 __device__ __forceinline__ void finishSlopes(const ProductParams& p, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, std::uint32_t live,
@@ -236,17 +259,7 @@ __device__ __forceinline__ void finishSlopes(const ProductParams& p, std::uint32
 #pragma unroll
         for (int j = 0; j < 128; ++j) { v[j] = j == at ? v[j] - 1.0F : v[j]; }
     }
-    // The buffer has room for whole tiles; what lies beyond the columns is never fetched.
-    unsigned char* const out = static_cast<unsigned char*>(p.slopes) + (static_cast<std::uint64_t>(row) * p.slopes_pitch + col) * 2;
-#pragma unroll
-    for (int j = 0; j < 128; j += 16) {
-        if (j < 64 || pieces == 4) {
-            std::uint32_t packed[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { packed[i] = on ? pack16(scale * v[j + 2 * i], scale * v[j + 2 * i + 1], p.bf16 != 0) : 0; }
-            storeGlobal8(out + 2 * j, packed);
-        }
-    }
+    storeRow(p, row, col, pieces, scale, on, p.bf16 != 0, v);
 }
 
 __device__ __forceinline__ void finishSums(const ProductParams& p, const Item& w, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, float (&v)[128]) {
@@ -271,6 +284,26 @@ __device__ __forceinline__ void finishSums(const ProductParams& p, const Item& w
 __device__ __forceinline__ void finishWeight(const ProductParams& p, const Problem& problem, std::uint32_t row, std::uint32_t col, std::uint32_t pieces,
                                              float unit, float (&v)[128]) {
     if (row >= problem.rows) { return; }
+    if (p.weight_fp32 != 0) {
+        float* const at = static_cast<float*>(p.weight_gradient) + static_cast<std::int64_t>(row) * p.weight_gradient_pitch + col;
+#pragma unroll
+        for (int j = 0; j < 128; j += 8) {
+            if (j < 64 || pieces == 4) {
+                float o[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { o[i] = unit * v[j + i]; }
+                if (p.weight_vector == 8) {
+                    if (col + j < problem.columns) { storeGlobal8(at + j, o); }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (col + j + i < problem.columns) { at[j + i] = o[i]; }
+                    }
+                }
+            }
+        }
+        return;
+    }
     unsigned char* const at = static_cast<unsigned char*>(p.weight_gradient) + (static_cast<std::int64_t>(row) * p.weight_gradient_pitch + col) * 2;
 #pragma unroll
     for (int j = 0; j < 128; j += 16) {
@@ -381,7 +414,9 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
             __syncwarp();
             if (lane == 0) { mbarrierArriveCluster(sum_empty[which]); }
             if (kMode == kStatistics) {
-                finishStatistics(p, w, row, col, pieces, half, live, v);
+                finishStatistics<false>(p, w, row, col, pieces, half, live, v);
+            } else if (kMode == kKept) {
+                finishStatistics<true>(p, w, row, col, pieces, half, live, v);
             } else if (kMode == kSlopes) {
                 finishSlopes(p, row, col, pieces, live, v);
             } else if (w.problem == p.weight_problem) {
@@ -556,6 +591,7 @@ bool describeLogits(const ProductCall& call, Matrix16 weight, std::uint32_t colu
 
 }  // namespace
 
+std::uint32_t statisticsWidth(std::uint32_t columns) { return tileColumns(columns) / 2; }
 std::uint32_t statisticsPieces(std::uint32_t columns) { return 2 * divideUp(columns, tileColumns(columns)); }
 
 cudaError_t launchStatistics(const ProductCall& call, Matrix16 weight, std::uint32_t vocabulary, float2* partials) {
@@ -564,6 +600,16 @@ cudaError_t launchStatistics(const ProductCall& call, Matrix16 weight, std::uint
     p.partials      = partials;
     if (!describeLogits(call, weight, vocabulary, maps, p)) { return cudaErrorInvalidValue; }
     return launch<kStatistics>(call, maps, p, static_cast<std::uint64_t>(call.capacity / kTileRows) * p.problem[0].tiles_n);
+}
+
+cudaError_t launchKept(const ProductCall& call, Matrix16 weight, std::uint32_t vocabulary, float2* partials, void* kept, std::uint64_t kept_pitch) {
+    ProductMaps maps;
+    ProductParams p = paramsFor(call);
+    p.partials      = partials;
+    p.slopes        = kept;
+    p.slopes_pitch  = kept_pitch;
+    if (!describeLogits(call, weight, vocabulary, maps, p)) { return cudaErrorInvalidValue; }
+    return launch<kKept>(call, maps, p, static_cast<std::uint64_t>(call.capacity / kTileRows) * p.problem[0].tiles_n);
 }
 
 cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, std::uint64_t slopes_pitch) {
@@ -623,10 +669,12 @@ cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint3
         p.weight_problem          = p.problems;
         p.weight_gradient         = gradients.weight_gradient;
         p.weight_gradient_pitch   = gradients.weight_gradient_pitch;
+        p.weight_fp32             = gradients.weight_gradient_fp32 ? 1 : 0;
+        const std::uint32_t bytes = gradients.weight_gradient_fp32 ? 4 : 2;
         const auto fits = [&](std::uint32_t n) {
-            return call.depth % n == 0 && gradients.weight_gradient_pitch % n == 0 && training::aligned(gradients.weight_gradient, 2 * n);
+            return call.depth % n == 0 && gradients.weight_gradient_pitch % n == 0 && training::aligned(gradients.weight_gradient, bytes * n);
         };
-        p.weight_vector = fits(16) ? 16 : fits(8) ? 8 : 1;
+        p.weight_vector = !gradients.weight_gradient_fp32 && fits(16) ? 16 : fits(8) ? 8 : 1;
         encoded = encodeOperand(&maps.a[p.problems], call, slope_matrix, true, columns, call.capacity, 128) &&
                   encodeOperand(&maps.b[p.problems], call, call.hidden, true, call.depth, call.capacity, 64);
         items += static_cast<std::uint64_t>(divideUp(columns, kTileRows)) * tiles_n;

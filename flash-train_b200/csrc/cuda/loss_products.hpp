@@ -47,6 +47,7 @@ struct ProductCall {
 };
 
 // Columns of the vocabulary that one partial result of the statistics covers, and how many of those there are.
+std::uint32_t statisticsWidth(std::uint32_t columns);
 std::uint32_t statisticsPieces(std::uint32_t columns);
 
 // For every live row and piece of columns: {largest logit times log2 e, sum of 2^(logit log2 e - that)} to
@@ -56,6 +57,11 @@ cudaError_t launchStatistics(const ProductCall& call, Matrix16 weight, std::uint
 // slopes[row][column - first] = scale (2^(logit log2 e - lse2) - [column is the target]) for `columns` columns from `first` on;
 // `weight` starts at row `first`. The pitch is a multiple of 256.
 cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, std::uint64_t slopes_pitch);
+
+// The same, and kept[row][column] = 2^(logit log2 e - its piece's largest), times kKeptScale, in FP16 whatever the operands' type: against the
+// largest of its piece a number needs no more range, and BF16 would round 2^3 times as much. The pitch is a multiple of 256.
+constexpr float kKeptScale = 8192.0F;
+cudaError_t launchKept(const ProductCall& call, Matrix16 weight, std::uint32_t vocabulary, float2* partials, void* kept, std::uint64_t kept_pitch);
 
 // How many parts the sum over `columns` columns is cut into for the gradient of the hidden states. (Over fewer columns
 // launchGradients may fill fewer of them, never more.)
@@ -70,6 +76,7 @@ struct Gradients {
     // weight: rows of the piece = unit * slopes^T times hidden; NULL when not wanted.
     void* weight_gradient;
     std::int64_t weight_gradient_pitch;
+    bool weight_gradient_fp32;  // or of the operands' type
 };
 cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint32_t columns, const void* slopes, std::uint64_t slopes_pitch,
                             const Gradients& gradients);

@@ -55,7 +55,8 @@ PLATFORM_SYMBOLS = (
     "ftcuda_grouped_gemm_supports ftcuda_grouped_gemm_configure ftcuda_grouped_gemm_workspace_bytes "
     "ftcuda_grouped_gemm_launch ftcuda_grouped_gemm_destroy ftcuda_gradient_norm_workspace_bytes ftcuda_gradient_norm "
     "ftcuda_gradient_clip ftcuda_expert_routing_workspace_bytes ftcuda_expert_routing ftcuda_expert_routing_backward "
-    "ftcuda_linear_cross_entropy_workspace_bytes ftcuda_linear_cross_entropy ftcuda_linear_cross_entropy_backward"
+    "ftcuda_linear_cross_entropy_workspace_bytes ftcuda_linear_cross_entropy ftcuda_linear_cross_entropy_backward "
+    "ftcuda_linear_cross_entropy_step_workspace_bytes ftcuda_linear_cross_entropy_step ftcuda_gradient_scale"
 ).split()
 
 
@@ -669,9 +670,13 @@ def _declare_training(lib) -> None:
     problem = [POINTER(LinearCrossEntropy)]
     lib.ftcuda_linear_cross_entropy_workspace_bytes.argtypes = problem + [ctypes.c_int, POINTER(c_uint64)] + message
     lib.ftcuda_linear_cross_entropy.argtypes = problem + [c_void_p] * 2 + work
+    lib.ftcuda_linear_cross_entropy_step_workspace_bytes.argtypes = problem + [POINTER(c_uint64)] + message
+    lib.ftcuda_linear_cross_entropy_step.argtypes = problem + [c_void_p, ctypes.c_int32, c_void_p, c_int64, c_void_p, c_int64] + work
+    lib.ftcuda_gradient_scale.argtypes = [POINTER(Gradient), c_uint64, c_void_p, ctypes.c_int32, c_void_p] + message
     lib.ftcuda_linear_cross_entropy_backward.argtypes = problem + [c_void_p] * 3 + [c_int64, c_void_p, c_int64] + work
     for name in ("ftcuda_gradient_norm", "ftcuda_gradient_clip", "ftcuda_expert_routing", "ftcuda_expert_routing_backward",
-                 "ftcuda_linear_cross_entropy_workspace_bytes", "ftcuda_linear_cross_entropy", "ftcuda_linear_cross_entropy_backward"):
+                 "ftcuda_linear_cross_entropy_workspace_bytes", "ftcuda_linear_cross_entropy", "ftcuda_linear_cross_entropy_backward",
+                 "ftcuda_linear_cross_entropy_step_workspace_bytes", "ftcuda_linear_cross_entropy_step", "ftcuda_gradient_scale"):
         getattr(lib, name).restype = ctypes.c_int
 
 
@@ -736,3 +741,22 @@ def linear_cross_entropy_backward(problem: LinearCrossEntropy, lse: int, grad_lo
     """ftcuda_linear_cross_entropy_backward; 0 for a gradient that is not wanted."""
     _run_training(lib.ftcuda_linear_cross_entropy_backward, byref(problem), lse, grad_loss, grad_hidden, grad_hidden_row_stride, grad_weight,
                   grad_weight_row_stride, workspace, workspace_bytes, stream)
+
+
+def linear_cross_entropy_step_workspace_bytes(problem: LinearCrossEntropy) -> int:
+    size = c_uint64()
+    _run_training(lib.ftcuda_linear_cross_entropy_step_workspace_bytes, byref(problem), byref(size))
+    return int(size.value)
+
+
+def linear_cross_entropy_step(problem: LinearCrossEntropy, loss: int, grad_element: int, grad_hidden: int, grad_hidden_row_stride: int, grad_weight: int,
+                              grad_weight_row_stride: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    """ftcuda_linear_cross_entropy_step: the loss, and the gradients for an upstream gradient of 1; 0 for one that is not wanted."""
+    _run_training(lib.ftcuda_linear_cross_entropy_step, byref(problem), loss, grad_element, grad_hidden, grad_hidden_row_stride, grad_weight,
+                  grad_weight_row_stride, workspace, workspace_bytes, stream)
+
+
+def gradient_scale(gradients, factor: int, device: int = 0, stream: int = 0) -> None:
+    """ftcuda_gradient_scale: out = data times the FP32 number at the device address `factor`."""
+    array = (Gradient * max(len(gradients), 1))(*gradients)
+    _run_training(lib.ftcuda_gradient_scale, array, len(gradients), c_void_p(factor), device, c_void_p(stream))

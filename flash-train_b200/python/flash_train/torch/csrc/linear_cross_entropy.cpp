@@ -3,8 +3,11 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/engine.h>
+#include <torch/csrc/autograd/graph_task.h>
 
 #include <string>
+#include <vector>
 
 #include <ftcuda/training.h>
 
@@ -40,6 +43,11 @@ at::Tensor workspaceOf(const FtcudaLinearCrossEntropy& q, bool backward, const a
     return workspaceFor(bytes, like);
 }
 
+cudaStream_t streamOf(const FtcudaLinearCrossEntropy& q) { return c10::cuda::getCurrentCUDAStream(q.device).stream(); }
+
+void* addressOf(const at::Tensor& tensor) { return tensor.defined() ? tensor.data_ptr() : nullptr; }
+
+// The loss now, the gradients when they are asked for: the logits are computed twice.
 class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> {
   public:
     static at::Tensor forward(AutogradContext* context, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, std::int64_t ignore_index,
@@ -52,8 +60,8 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
         std::uint64_t bytes              = 0;
         const at::Tensor workspace       = workspaceOf(q, false, hidden, bytes);
         Message message;
-        const int status = ftcuda_linear_cross_entropy(&q, loss.data_ptr<float>(), lse.data_ptr<float>(), workspace.data_ptr(), bytes,
-                                                       c10::cuda::getCurrentCUDAStream(q.device).stream(), message.text, sizeof message.text);
+        const int status = ftcuda_linear_cross_entropy(&q, loss.data_ptr<float>(), lse.data_ptr<float>(), workspace.data_ptr(), bytes, streamOf(q), message.text,
+                                                       sizeof message.text);
         TORCH_CHECK(status == 0, "flash_train linear_cross_entropy failed: ", message.text);
         context->save_for_backward({hidden, weight, target, lse});
         context->saved_data["ignore_index"] = ignore_index;
@@ -75,12 +83,67 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
         std::uint64_t bytes        = 0;
         const at::Tensor workspace = workspaceOf(q, true, hidden, bytes);
         Message message;
-        const int status = ftcuda_linear_cross_entropy_backward(
-            &q, lse.data_ptr<float>(), grad_loss.data_ptr<float>(), grad_hidden.defined() ? grad_hidden.data_ptr() : nullptr, hidden.size(1),
-            grad_weight.defined() ? grad_weight.data_ptr() : nullptr, hidden.size(1), workspace.data_ptr(), bytes,
-            c10::cuda::getCurrentCUDAStream(q.device).stream(), message.text, sizeof message.text);
+        const int status = ftcuda_linear_cross_entropy_backward(&q, lse.data_ptr<float>(), grad_loss.data_ptr<float>(), addressOf(grad_hidden), hidden.size(1),
+                                                                addressOf(grad_weight), hidden.size(1), workspace.data_ptr(), bytes, streamOf(q), message.text,
+                                                                sizeof message.text);
         TORCH_CHECK(status == 0, "flash_train linear_cross_entropy's gradient failed: ", message.text);
         return {grad_hidden, grad_weight, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+// Both at once, for an upstream gradient of 1; the backward pass only multiplies by the one that comes. FP16 operands' gradients
+// wait in FP32: without the loss's scale, which comes then, many of them are too small for FP16.
+class LinearCrossEntropyStep : public torch::autograd::Function<LinearCrossEntropyStep> {
+  public:
+    static at::Tensor forward(AutogradContext* context, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, std::int64_t ignore_index,
+                              std::int64_t reduction, std::int64_t workspace_bytes) {
+        const c10::cuda::CUDAGuard guard(hidden.device());
+        const FtcudaLinearCrossEntropy q = describe(hidden, weight, target, ignore_index, reduction);
+        const auto floats                = hidden.options().dtype(at::kFloat).requires_grad(false);
+        const auto kept                  = hidden.scalar_type() == at::kHalf ? floats : hidden.options().requires_grad(false);
+        at::Tensor loss                  = at::empty({}, floats);
+        at::Tensor grad_hidden, grad_weight;
+        if (hidden.requires_grad()) { grad_hidden = at::empty(hidden.sizes(), kept); }
+        if (weight.requires_grad()) { grad_weight = at::empty(weight.sizes(), kept); }
+        const at::Tensor workspace = workspaceFor(static_cast<std::uint64_t>(workspace_bytes), hidden);
+        Message message;
+        const int status = ftcuda_linear_cross_entropy_step(&q, loss.data_ptr<float>(), elementOf(grad_hidden.defined() ? grad_hidden : grad_weight), addressOf(grad_hidden),
+                                                            hidden.size(1), addressOf(grad_weight), hidden.size(1), workspace.data_ptr(),
+                                                            static_cast<std::uint64_t>(workspace_bytes), streamOf(q), message.text, sizeof message.text);
+        TORCH_CHECK(status == 0, "flash_train linear_cross_entropy failed: ", message.text);
+        context->save_for_backward({grad_hidden, grad_weight});
+        context->saved_data["type"] = hidden.scalar_type();
+        return loss;
+    }
+
+    static variable_list backward(AutogradContext* context, const variable_list& gradients) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "linear_cross_entropy has no second derivative (create_graph=True)");
+        const variable_list saved  = context->get_saved_variables();
+        const at::ScalarType type  = context->saved_data["type"].toScalarType();
+        const at::Tensor grad_loss = gradients[0].to(at::kFloat).contiguous();
+        const c10::cuda::CUDAGuard guard(grad_loss.device());
+        // Without another backward pass to come, what waited is the result's memory as well.
+        const bool last = !torch::autograd::get_current_graph_task_keep_graph();
+        variable_list out(6);
+        std::vector<FtcudaGradient> described;
+        for (std::size_t i = 0; i < 2; ++i) {
+            const at::Tensor& from = saved[i];
+            if (!from.defined() || !context->needs_input_grad(i)) { continue; }
+            out[i] = last && from.scalar_type() == type ? from : at::empty(from.sizes(), from.options().dtype(type));
+            FtcudaGradient g{};
+            g.data        = from.data_ptr();
+            g.out         = out[i].data_ptr();
+            g.rows        = 1;
+            g.cols        = static_cast<std::uint64_t>(from.numel());
+            g.element     = elementOf(from);
+            g.out_element = elementOf(out[i]);
+            described.push_back(g);
+        }
+        Message message;
+        const int status = ftcuda_gradient_scale(described.data(), described.size(), grad_loss.data_ptr<float>(), grad_loss.device().index(),
+                                                 c10::cuda::getCurrentCUDAStream(grad_loss.device().index()).stream(), message.text, sizeof message.text);
+        TORCH_CHECK(status == 0, "flash_train linear_cross_entropy's gradient failed: ", message.text);
+        return out;
     }
 };
 
@@ -101,7 +164,15 @@ at::Tensor linearCrossEntropy(const at::Tensor& hidden, const at::Tensor& weight
     TORCH_CHECK(kind != FTCUDA_REDUCTION_SUM || reduction == "sum", "reduction must be 'none', 'mean' or 'sum'");
     const at::Tensor flat = hidden.dim() == 2 ? hidden : hidden.reshape({hidden.numel() / depth, depth});
     TORCH_CHECK((flat.stride(1) == 1 && weight.stride(1) == 1) || depth == 1, "hidden and weight must be contiguous along their last dimension");
-    const at::Tensor loss = LinearCrossEntropy::apply(flat, weight, target.reshape({-1}).contiguous(), ignore_index, kind);
+    const at::Tensor indices = target.reshape({-1}).contiguous();
+    if (at::GradMode::is_enabled() && (flat.requires_grad() || weight.requires_grad())) {
+        const FtcudaLinearCrossEntropy q = describe(flat, weight, indices, ignore_index, kind);
+        std::uint64_t bytes              = 0;
+        if (ftcuda_linear_cross_entropy_step_workspace_bytes(&q, &bytes, nullptr, 0) == 0) {
+            return LinearCrossEntropyStep::apply(flat, weight, indices, ignore_index, kind, static_cast<std::int64_t>(bytes));
+        }
+    }
+    const at::Tensor loss = LinearCrossEntropy::apply(flat, weight, indices, ignore_index, kind);
     return kind == FTCUDA_REDUCTION_NONE ? loss.view(target.sizes()) : loss;
 }
 

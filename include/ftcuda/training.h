@@ -36,7 +36,7 @@ enum {
 /*
  * logits[t][v] = hidden[t] . weight[v],  loss[t] = log(sum_v exp(logits[t][v])) - logits[t][target[t]].
  * The logits are never in memory, but for a piece of the vocabulary at a time in the backward call (and, for FP32 operands, the forward
- * call).
+ * call), or, in 16 bits and at most 2 GiB of them, for the time of a step call.
  *   - hidden [tokens][depth], weight [vocabulary][depth]: unit stride along the depth, the others any that keep rows apart; both
  *     of one type. BF16 and FP16 are multiplied by the tensor cores with FP32 sums; FP32 by the library's FP32 products.
  *   - target [tokens]: INT64. A token whose target is ignore_index takes no part: its loss and gradient are 0, whatever its hidden
@@ -119,6 +119,27 @@ FTCUDA_API int ftcuda_gradient_norm(const FtcudaGradient* gradients, uint64_t co
 FTCUDA_API int ftcuda_gradient_clip(const FtcudaGradient* gradients, uint64_t count, int norm_kind, double max_norm, float* norm,
                                     int32_t device, void* workspace, uint64_t workspace_bytes, void* stream, char* message,
                                     size_t message_capacity);
+
+/*
+ * out = data * *factor (one FP32 on the device), rounded once. Where the factor is 1, gradients that are their own `out` are left alone, without
+ * being written. Needs no workspace; the rest as for ftcuda_gradient_clip.
+ */
+FTCUDA_API int ftcuda_gradient_scale(const FtcudaGradient* gradients, uint64_t count, const float* factor, int32_t device, void* stream,
+                                     char* message, size_t message_capacity);
+
+/*
+ * The loss, and the gradients for an upstream gradient of 1, in one call that computes the logits once: three quarters of the work of the
+ * two calls above. Their exponentials (FP32: the logits) are in the workspace meanwhile. With a reduction only, and only where they take at most
+ * 2 GiB; ftcuda_linear_cross_entropy_step_workspace_bytes answers with a failure where that is not so.
+ * grad_element: the operands' type, or FP32, for a caller that multiplies by an upstream gradient afterwards and wants nothing rounded (or, with
+ * FP16, lost) before. Either gradient may be NULL.
+ */
+FTCUDA_API int ftcuda_linear_cross_entropy_step_workspace_bytes(const FtcudaLinearCrossEntropy* problem, uint64_t* workspace_bytes, char* message,
+                                                                size_t message_capacity);
+FTCUDA_API int ftcuda_linear_cross_entropy_step(const FtcudaLinearCrossEntropy* problem, float* loss, int32_t grad_element, void* grad_hidden,
+                                                int64_t grad_hidden_row_stride, void* grad_weight, int64_t grad_weight_row_stride,
+                                                void* workspace, uint64_t workspace_bytes, void* stream, char* message,
+                                                size_t message_capacity);
 
 /* ---- the experts' router ---- */
 

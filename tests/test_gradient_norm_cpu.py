@@ -87,3 +87,12 @@ def test_what_is_sound_reaches_the_device_check(capi):
 def test_the_workspace_grows_with_the_launches(capi):
     sizes = [capi.gradient_norm_workspace_bytes(n) for n in (0, 1, 64, 65, 480, 481, 5000)]
     assert sizes == sorted(sizes) and sizes[0] == sizes[1] > 0 and sizes[-1] <= MIB
+
+
+def test_scaling_refuses_the_same(capi):
+    good = gradient(capi)
+    for gradients, factor, reason in (([good], 0, "the factor"), ([good], 0x2002, "the factor"), ([gradient(capi, element=2)], 0x2000, "element type"),
+                                      ([good, good], 0x2000, "overlaps"), ([gradient(capi, out=0)], 0x2000, "no address for the output")):
+        with pytest.raises(capi.FTrainError) as info:
+            capi.gradient_scale(gradients, factor)
+        assert reason in info.value.message

@@ -260,3 +260,15 @@ def test_refusals(ft):
     ]:
         with pytest.raises(RuntimeError, match=reason):
             call()
+
+
+@pytest.mark.parametrize("count", [1, 70, 600])
+def test_scale_by_a_number_on_the_device(ft, capi, count):
+    elements = {torch.float32: capi.ELEMENT_FP32, torch.bfloat16: capi.ELEMENT_BF16, torch.float16: capi.ELEMENT_FP16}
+    gradients = [make([(1 + 53 * i % 777,)], TYPES[i % 3], seed=i)[0] for i in range(count)]
+    outs = [torch.empty_like(g, dtype=TYPES[(i // 3) % 3]) for i, g in enumerate(gradients)]
+    described = [capi.Gradient(g.data_ptr(), o.data_ptr(), 1, g.numel(), 0, 0, elements[g.dtype], elements[o.dtype]) for g, o in zip(gradients, outs)]
+    factor = torch.tensor(0.7, device="cuda")
+    capi.gradient_scale(described, factor.data_ptr(), 0, torch.cuda.current_stream().cuda_stream)
+    for g, o in zip(gradients, outs):
+        assert torch.equal(o, (g.float() * factor).to(o.dtype))

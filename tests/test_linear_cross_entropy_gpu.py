@@ -54,11 +54,15 @@ class Oracle:
         self.loss_error = torch.where(self.live, self.relative + 4 * size * STEP, 0.0)
         self.z = z
 
-    def gradients(self, grad, dtype):
+    def gradients(self, grad, dtype, step=True):
         """For upstream gradients `grad` of each token: (dH, its bound, dW, its bound), the roundings of the results to `dtype` among them."""
         grad = torch.where(self.live, grad.double(), 0.0)
         slope = torch.exp(self.z - self.lse[:, None])
         error = slope * self.relative[:, None]
+        if step and dtype != torch.float32:
+            # In the step call an exponential is in FP16 for a while, at 2^13 for the largest of its piece of the vocabulary: one more rounding, of half
+            # a step (2^-11 relative, or 2^-25 of what is at most 2^13 where it is subnormal).
+            error += 2.0 ** -11 * slope + 2.0 ** -38
         slope.scatter_add_(1, self.target[:, None], torch.full_like(self.lse, -1.0)[:, None])
         half_step = torch.finfo(dtype).eps / 2
         # The slopes' rounding; and the smallest that FP16 holds at its scale of 2^13 for the largest gradient.
@@ -376,3 +380,108 @@ def test_refusals(ft):
     ]:
         with pytest.raises(RuntimeError, match=reason):
             call()
+
+
+# ---- the step in one call: what torch runs wherever there is a reduction and room for the exponentials
+
+def split_in_two(capi, hidden, weight, target, upstream, reduction=1):
+    """The loss and the gradients through the two calls of the C interface, the logits computed in each."""
+    tokens, depth = hidden.shape
+    element = {torch.float32: capi.ELEMENT_FP32, torch.float16: capi.ELEMENT_FP16, torch.bfloat16: capi.ELEMENT_BF16}[hidden.dtype]
+    q = capi.LinearCrossEntropy(hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), tokens, weight.shape[0], depth, depth, depth, -100, element, reduction, 0)
+    size = max(capi.linear_cross_entropy_workspace_bytes(q, False), capi.linear_cross_entropy_workspace_bytes(q, True))
+    workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+    loss, lse = torch.empty((), device="cuda"), torch.empty(tokens, device="cuda")
+    grad_hidden, grad_weight = torch.full_like(hidden, math.nan), torch.full_like(weight, math.nan)
+    stream = torch.cuda.current_stream().cuda_stream
+    capi.linear_cross_entropy(q, loss.data_ptr(), lse.data_ptr(), workspace.data_ptr(), size, stream)
+    capi.linear_cross_entropy_backward(q, lse.data_ptr(), upstream.data_ptr(), grad_hidden.data_ptr(), depth, grad_weight.data_ptr(), depth, workspace.data_ptr(),
+                                       size, stream)
+    torch.cuda.synchronize()
+    return loss, grad_hidden, grad_weight
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens, depth, vocabulary", SIZES)
+def test_the_two_calls_against_the_definition(ft, capi, tokens, depth, vocabulary, dtype):
+    hidden, weight, target = make(tokens, depth, vocabulary, dtype)
+    target[1::4] = -100
+    oracle = Oracle(hidden, weight, target)
+    count = max(1, int(oracle.live.sum()))
+    upstream = torch.tensor(48.0, device="cuda")
+    loss, grad_hidden, grad_weight = split_in_two(capi, hidden, weight, target, upstream)
+    total = oracle.loss.sum() / count
+    check(loss, total, oracle.loss_error.sum() / count + 2 * STEP * total.abs(), "loss")
+    dh, dh_bound, dw, dw_bound = oracle.gradients(torch.full((tokens,), 48.0 / count, device="cuda", dtype=torch.float64), dtype, step=False)
+    check(grad_hidden, dh, dh_bound, "hidden's gradient")
+    check(grad_weight, dw, dw_bound, "weight's gradient")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("factor", [1.0, 2.0 ** -3, 0.3, 1e-20, 0.0])
+def test_any_upstream_gradient_of_the_step(ft, dtype, factor):
+    """BF16 gradients wait rounded, and are rounded again where the factor is no power of two; the others are rounded once."""
+    hidden, weight, target = make(200, 96, 700, dtype, seed=20)
+    one = run(ft, hidden, weight, target)
+    got = run(ft, hidden, weight, target, upstream=torch.tensor(factor, device="cuda"))
+    oracle = Oracle(hidden, weight, target)
+    dh, dh_bound, dw, dw_bound = oracle.gradients(torch.full((200,), factor / 200, device="cuda", dtype=torch.float64), dtype)
+    again = torch.finfo(dtype).eps / 2
+    for g, value, bound in ((got[1], dh, dh_bound), (got[2], dw, dw_bound)):
+        check(g, value, bound + again * value.abs() * 1.01, "gradient")
+    if dtype != torch.float16 and math.log2(factor or 1.0) % 1.0 == 0.0 and factor:
+        assert torch.equal(got[1], one[1] * factor) and torch.equal(got[2], one[2] * factor)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_backward_passes(ft, dtype):
+    """The gradients that wait in the graph are given away only where no other pass can come."""
+    hidden, weight, target = make(90, 64, 300, dtype, seed=21)
+    h, w = hidden.clone().requires_grad_(), weight.clone().requires_grad_()
+    loss = ft.linear_cross_entropy(h, w, target)
+    first = torch.autograd.grad(loss, (h, w), torch.tensor(4.0, device="cuda"), retain_graph=True)
+    kept = [g.clone() for g in first]
+    for g in first:
+        g.fill_(math.nan)
+    second = torch.autograd.grad(loss, (h, w), torch.tensor(8.0, device="cuda"), retain_graph=True)
+    only = torch.autograd.grad(loss, w, torch.tensor(4.0, device="cuda"), retain_graph=True)[0]
+    third = torch.autograd.grad(loss, (h, w), torch.tensor(4.0, device="cuda"))
+    # (Below FP16's smallest normal number each rounding is half of 2^-24, the first of them doubled here.)
+    tiny = 1.5 * 2.0 ** -24 if dtype == torch.float16 else 0.0
+    assert all(((a.float() * 2 - b.float()).abs() <= tiny).all() and torch.equal(a, c) for a, b, c in zip(kept, second, third)) and torch.equal(only, kept[1])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, (h, w))
+    # The loss in two places of one graph, and accumulation into what is there.
+    loss = ft.linear_cross_entropy(h, w, target)
+    (loss + 3 * loss).backward()
+    assert torch.equal(h.grad, kept[0]) and torch.equal(w.grad, kept[1])
+    ft.linear_cross_entropy(h, w, target).mul(4).backward()
+    assert torch.equal(w.grad, kept[1] + kept[1])
+
+
+def test_a_loss_scale_keeps_small_fp16_gradients(ft):
+    hidden, weight, target = make(500, 64, 4000, torch.float16, seed=22)
+    _, _, grad_weight = run(ft, hidden * 2.0 ** -6, weight, target, upstream=torch.tensor(2.0 ** 16, device="cuda"))
+    oracle = Oracle(hidden * 2.0 ** -6, weight, target)
+    _, _, dw, dw_bound = oracle.gradients(torch.full((500,), 2.0 ** 16 / 500, device="cuda", dtype=torch.float64), torch.float16)
+    check(grad_weight, dw, dw_bound, "weight's gradient")
+    assert (dw.abs().median() / 2 ** 16) < torch.finfo(torch.float16).smallest_normal  # unscaled, most would have been lost
+
+
+def test_what_the_step_refuses(ft, capi):
+    hidden, weight, target = make(10, 16, 20, torch.bfloat16)
+
+    def problem(**change):
+        fields = dict(hidden=hidden.data_ptr(), weight=weight.data_ptr(), target=target.data_ptr(), tokens=10, vocabulary=20, depth=16, hidden_row_stride=16,
+                      weight_row_stride=16, ignore_index=-100, element=8, reduction=1, device=0)
+        return capi.LinearCrossEntropy(**{**fields, **change})
+
+    for change, reason in (({"reduction": 0}, "without reduction"), ({"tokens": 0}, "no tokens"), ({"tokens": 1 << 20, "vocabulary": 1 << 20}, "2 GiB")):
+        with pytest.raises(capi.FTrainError, match=reason):
+            capi.linear_cross_entropy_step_workspace_bytes(problem(**change))
+    size = capi.linear_cross_entropy_step_workspace_bytes(problem())
+    workspace, out = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.empty(4096, device="cuda")
+    with pytest.raises(capi.FTrainError, match="operands' type"):
+        capi.linear_cross_entropy_step(problem(), out.data_ptr(), 7, 0, 0, 0, 0, workspace.data_ptr(), size)
+    with pytest.raises(capi.FTrainError, match="workspace of"):
+        capi.linear_cross_entropy_step(problem(), out.data_ptr(), 8, 0, 0, 0, 0, workspace.data_ptr(), size - 1)
