@@ -13,13 +13,19 @@
 // blocks of 64; a CTA brings its 128 rows of A and its half of B, each as the matrix lies in memory: an operand whose
 // neighbours run along K is a K-major operand, one whose neighbours run along its rows an MN-major one, so nothing is ever transposed.
 //
-//   warp 0       TMA producer (one thread, in both CTAs; the bytes of both count on the first CTA's barrier)
+//   warps 0, 2   TMA producers of A and of B (one thread each, in both CTAs; the bytes of both count on the first CTA's barrier)
 //   warp 1       MMA issuer (one thread, in the first CTA, for both CTAs' tensor cores)
 //   warps 4-11   epilogue, 32 rows x half of the columns each
 //
 // Tensor memory holds two accumulators of 256 columns: one is filled while the other is read. What the epilogue reads goes to registers at once
 // and the accumulator back to the issuer; a thread has one row, so maxima, sums and the target's column need no
 // exchange between threads, and its output is 256 neighbouring bytes, written 32 at a time.
+//
+// A K block is 512 cycles of MMAs, and the threads that feed them must need less. One producer for both operands, with its parameters read again for
+// every block, took 660; an issuer under `if (lane == 0)` as much, as the compiler moves every descriptor into uniform registers where the
+// branch may diverge. With a producer for each operand and the issuing warp in step (one thread elected for the instructions alone) the
+// tensor pipe is busy for 90 % of the time instead of 73: statistics of 8192 x 4096 x 65536 1237 -> 1347 TFLOP/s in a seconds-long loop (power-limited, at
+// 1233 MHz instead of 1410; the library's product 1358 beside it), 1384 -> 1540 in a burst. 16 row tiles walked together instead of 8 give 3 %.
 //
 // Every wait is bounded, as in the other kernels (ptx.cuh).
 #include "loss_products.hpp"
@@ -43,7 +49,7 @@ namespace {
 constexpr std::uint32_t kBlockK = 64;  // 128 bytes, one swizzle row
 constexpr std::uint32_t kTileN  = 256;
 constexpr std::uint32_t kItemBlocks = 12;
-constexpr int kStages           = 7;
+constexpr int kStages           = 5;  // seven are no faster; what is left is the stores' L1
 constexpr int kThreads          = 384;
 constexpr int kOperandBytes     = 128 * 128;  // a CTA's share of A, and of a B of 256 columns
 constexpr int kStageBytes       = 2 * kOperandBytes;
@@ -55,8 +61,9 @@ constexpr std::uint32_t kBoxBytes = 64 * 128;  // 64 rows of 128 bytes: one box 
 constexpr int kRegsLight = 72;   // producer, issuer (warpgroup 0)
 constexpr int kRegsDrain = 216;  // epilogue (warpgroups 1, 2)
 static_assert(128 * kRegsLight + 256 * kRegsDrain <= 168 * kThreads, "the CTA's register pool is what it was launched with");
-constexpr int kProducerWarp  = 0;
+constexpr int kProducerA     = 0;
 constexpr int kIssuerWarp    = 1;
+constexpr int kProducerB     = 2;
 constexpr int kFirstEpilogue = 4;
 constexpr std::uint32_t kTmemColumns = 512;
 
@@ -340,7 +347,7 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
     unsigned char* smem              = smem_raw + align_offset;
     Barriers* bars                   = reinterpret_cast<Barriers*>(smem + kBarrierOffset);
     volatile int* abort_flag         = &bars->abort_flag;
-    const int warp                   = threadIdx.x >> 5;
+    const int warp                   = __shfl_sync(0xFFFFFFFFU, static_cast<int>(threadIdx.x >> 5), 0);  // known to be the warp's
     const int lane                   = threadIdx.x & 31;
     const std::uint32_t rank         = clusterCtaRank();
     const std::uint32_t pair         = blockIdx.x >> 1;
@@ -428,40 +435,38 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
         if (!ok) { *abort_flag = 1; }
     } else {
         registersShrink<kRegsLight>();
-        if (warp == kProducerWarp) {
+        if (warp == kProducerA || warp == kProducerB) {
             bool ok = true;
             if (lane == 0) {
+                const bool second        = warp == kProducerB;
+                const bool arms          = !second && rank == 0;
+                unsigned char* const to  = smem + (second ? kOperandBytes : 0);
+                const std::uint32_t full = mapToRank(&bars->full[0], 0);
                 Ring ring;
                 std::uint32_t filled = 0;
                 for (std::uint32_t n = 0, item; ok && (item = itemOf(work, pair, pairs, n)) != kNoItem; ++n) {
-                    const Item w                    = decode(p, work, item);
-                    const Problem& problem          = p.problem[w.problem];
-                    const CUtensorMap* const map_a  = &maps.a[w.problem];
-                    const CUtensorMap* const map_b  = &maps.b[w.problem];
-                    const std::int32_t row_a        = static_cast<std::int32_t>(w.row + rank * 128);
-                    const std::int32_t row_b        = static_cast<std::int32_t>(w.col + rank * (problem.tile_n / 2));
-                    const std::uint32_t bytes       = kOperandBytes + problem.tile_n / 2 * 128;
+                    // What does not change within an item is in registers before its K blocks: this loop has 512 cycles a block.
+                    const Item w                 = decode(p, work, item);
+                    const Problem& problem       = p.problem[w.problem];
+                    const CUtensorMap* const map = second ? &maps.b[w.problem] : &maps.a[w.problem];
+                    const std::uint32_t rows     = second ? problem.tile_n / 2 : 128;
+                    const std::int32_t row       = static_cast<std::int32_t>((second ? w.col : w.row) + rank * rows);
+                    const bool along             = (second ? problem.b_along_rows : problem.a_along_rows) != 0;
+                    const bool two               = along && rows == 128;  // boxes: an MN-major one has 64 rows
+                    const std::int32_t first     = static_cast<std::int32_t>(w.first_block * kBlockK);
+                    const std::int32_t step_x = along ? 0 : static_cast<std::int32_t>(kBlockK), step_y = along ? static_cast<std::int32_t>(kBlockK) : 0;
+                    const std::uint32_t bytes    = 2 * (kOperandBytes + problem.tile_n / 2 * 128);
+                    std::int32_t x = along ? row : first, y = along ? first : row;
                     for (std::uint32_t kb = 0; kb < w.blocks; ++kb, ++filled, ring.next()) {
                         ok = mbarrierWait(&bars->empty[ring.slot], (ring.round & 1) ^ 1, abort_flag);
                         if (!ok) { break; }
                         // The bytes of both CTAs count on the first CTA's barrier, which that CTA arms. (The other's
                         // may land first: the phase cannot complete before it has been armed.)
-                        if (rank == 0) { mbarrierArriveExpectTx(&bars->full[ring.slot], 2 * bytes); }
-                        const std::uint32_t full  = mapToRank(&bars->full[ring.slot], 0);
-                        unsigned char* const slot = smem + ring.slot * kStageBytes;
-                        const std::int32_t k      = static_cast<std::int32_t>((w.first_block + kb) * kBlockK);
-                        if (problem.a_along_rows != 0) {
-                            tmaLoad2dPair(slot, map_a, full, row_a, k);
-                            tmaLoad2dPair(slot + kBoxBytes, map_a, full, row_a + 64, k);
-                        } else {
-                            tmaLoad2dPair(slot, map_a, full, k, row_a);
-                        }
-                        if (problem.b_along_rows != 0) {
-                            tmaLoad2dPair(slot + kOperandBytes, map_b, full, row_b, k);
-                            if (problem.tile_n == kTileN) { tmaLoad2dPair(slot + kOperandBytes + kBoxBytes, map_b, full, row_b + 64, k); }
-                        } else {
-                            tmaLoad2dPair(slot + kOperandBytes, map_b, full, k, row_b);
-                        }
+                        if (arms) { mbarrierArriveExpectTx(&bars->full[ring.slot], bytes); }
+                        tmaLoad2dPair(to + ring.slot * kStageBytes, map, full + ring.slot * 8, x, y);
+                        if (two) { tmaLoad2dPair(to + ring.slot * kStageBytes + kBoxBytes, map, full + ring.slot * 8, x + 64, y); }
+                        x += step_x;
+                        y += step_y;
                     }
                 }
                 // Neither CTA leaves before the last commits have arrived on its barriers.
@@ -473,48 +478,52 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
             }
             __syncwarp();
         } else if (warp == kIssuerWarp && rank == 0) {
-            if (lane == 0) {
-                const std::uint64_t stage_step = kStageBytes >> 4;
-                const std::uint32_t base       = smemAddress(smem);
-                Ring ring;
-                std::uint32_t sums = 0;
-                bool ok            = true;
-                for (std::uint32_t item; ok && (item = itemOf(work, pair, pairs, sums)) != kNoItem; ++sums) {
-                    const Item w           = decode(p, work, item);
-                    const Problem& problem = p.problem[w.problem];
-                    const bool a_mn = problem.a_along_rows != 0, b_mn = problem.b_along_rows != 0;
-                    // Sixteen of K are 32 bytes of a K-major tile's rows, or sixteen rows of an MN-major one.
-                    const std::uint64_t a0 = a_mn ? umaDescriptorMn128(base, kBoxBytes) : umaDescriptorK128(base);
-                    const std::uint64_t b0 = b_mn ? umaDescriptorMn128(base + kOperandBytes, kBoxBytes) : umaDescriptorK128(base + kOperandBytes);
-                    const std::uint64_t a_step = a_mn ? 16 * 128 >> 4 : 2, b_step = b_mn ? 16 * 128 >> 4 : 2;
-                    const std::uint32_t instruction =
-                        p.instruction | umaInstructionF16(kTileRows, problem.tile_n) | (a_mn ? kUmaAMnMajor : 0) | (b_mn ? kUmaBMnMajor : 0);
-                    const std::uint32_t which = sums & 1;
-                    const std::uint32_t d     = tmem_base + which * kTileN;
-                    ok = mbarrierWait(&bars->sum_empty[which], ((sums >> 1) & 1) ^ 1, abort_flag);
+            // The whole warp goes through the loop and one thread issues: descriptors that are the warp's stay in uniform registers.
+            const bool leads               = electOne();
+            const std::uint64_t stage_step = kStageBytes >> 4;
+            const std::uint32_t base       = smemAddress(smem);
+            Ring ring;
+            std::uint32_t sums = 0;
+            bool ok            = true;
+            for (std::uint32_t item; ok && (item = itemOf(work, pair, pairs, sums)) != kNoItem; ++sums) {
+                const Item w           = decode(p, work, item);
+                const Problem& problem = p.problem[w.problem];
+                const bool a_mn = problem.a_along_rows != 0, b_mn = problem.b_along_rows != 0;
+                // Sixteen of K are 32 bytes of a K-major tile's rows, or sixteen rows of an MN-major one.
+                const std::uint64_t a0 = a_mn ? umaDescriptorMn128(base, kBoxBytes) : umaDescriptorK128(base);
+                const std::uint64_t b0 = b_mn ? umaDescriptorMn128(base + kOperandBytes, kBoxBytes) : umaDescriptorK128(base + kOperandBytes);
+                const std::uint64_t a_step = a_mn ? 16 * 128 >> 4 : 2, b_step = b_mn ? 16 * 128 >> 4 : 2;
+                const std::uint32_t instruction =
+                    p.instruction | umaInstructionF16(kTileRows, problem.tile_n) | (a_mn ? kUmaAMnMajor : 0) | (b_mn ? kUmaBMnMajor : 0);
+                const std::uint32_t which = sums & 1;
+                const std::uint32_t d     = tmem_base + which * kTileN;
+                ok = mbarrierWait(&bars->sum_empty[which], ((sums >> 1) & 1) ^ 1, abort_flag);
+                if (!ok) { break; }
+                tcgen05FenceAfterSync();
+                for (std::uint32_t kb = 0; kb < w.blocks; ++kb, ring.next()) {
+                    ok = mbarrierWait(&bars->full[ring.slot], ring.round & 1, abort_flag);
                     if (!ok) { break; }
                     tcgen05FenceAfterSync();
-                    for (std::uint32_t kb = 0; kb < w.blocks; ++kb, ring.next()) {
-                        ok = mbarrierWait(&bars->full[ring.slot], ring.round & 1, abort_flag);
-                        if (!ok) { break; }
-                        tcgen05FenceAfterSync();
-                        const std::uint64_t a = a0 + ring.slot * stage_step, b = b0 + ring.slot * stage_step;
+                    const std::uint64_t a = a0 + ring.slot * stage_step, b = b0 + ring.slot * stage_step;
+                    if (leads) {
 #pragma unroll
                         for (std::uint32_t step = 0; step < kBlockK / 16; ++step) {
                             umaF16Pair(d, a + step * a_step, b + step * b_step, instruction, kb != 0 || step != 0 ? 1U : 0U);
                         }
                         umaCommitPair(&bars->empty[ring.slot]);
                     }
-                    if (!ok) { break; }
-                    umaCommitPair(&bars->sum_full[which]);
+                    __syncwarp();
                 }
-                if (!ok) {
-                    *abort_flag = 1;
-                    // Let MMAs already issued finish before tensor memory is freed.
-                    umaCommitPair(&bars->flush);
-                    int never = 0;
-                    mbarrierWait(&bars->flush, 0, &never);
-                }
+                if (!ok) { break; }
+                if (leads) { umaCommitPair(&bars->sum_full[which]); }
+                __syncwarp();
+            }
+            if (!ok && leads) {
+                *abort_flag = 1;
+                // Let MMAs already issued finish before tensor memory is freed.
+                umaCommitPair(&bars->flush);
+                int never = 0;
+                mbarrierWait(&bars->flush, 0, &never);
             }
             __syncwarp();
         }
@@ -566,7 +575,7 @@ template<int kMode> cudaError_t launch(const ProductCall& call, const ProductMap
 ProductParams paramsFor(const ProductCall& call) {
     ProductParams p{};
     p.problems       = 1;
-    p.band           = 8;
+    p.band           = 16;
     p.instruction    = call.bf16 ? kUmaBf16 : 0;
     p.bf16           = call.bf16 ? 1 : 0;
     p.capacity       = call.capacity;

@@ -126,6 +126,19 @@ __device__ __forceinline__ void tcgen05FenceAfterSync() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
+// True in one thread of a converged warp, the same one every time.
+__device__ __forceinline__ bool electOne() {
+    std::uint32_t elected;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "elect.sync _|p, 0xFFFFFFFF;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}"
+        : "=r"(elected));
+    return elected != 0;
+}
+
 // ---------------------------------------------------------------- TMA
 
 // 2-D tiled load global -> shared, completion counted in bytes on `barrier`.
