@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "ptx.cuh"
 #include "training_common.cuh"
@@ -88,6 +89,98 @@ __device__ __forceinline__ void writeLoss(const RouteParams& p, double total, st
     *p.loss        = live == 0 ? 0.0F : static_cast<float>(total * p.experts / (n * p.top_k * n));
 }
 
+// The largest keys of a warp, one after another, the lowest index first among equal ones.
+template<typename T, int kItems> struct TopK;
+
+// FP32: a round is two reductions, for the key and for the index.
+template<int kItems> struct TopK<float, kItems> {
+    std::uint32_t keys[kItems];
+    __device__ __forceinline__ void set(int i, float x, std::uint32_t) { keys[i] = orderOf(x); }
+    __device__ __forceinline__ void none(int i) { keys[i] = 0; }
+    __device__ __forceinline__ void ready() {}
+    // The next one; false when only -inf is left.
+    __device__ __forceinline__ bool next(int lane, std::uint32_t& index, float& value) {
+        std::uint32_t best = keys[0];
+#pragma unroll
+        for (int i = 1; i < kItems; ++i) { best = max(best, keys[i]); }
+        best = __reduce_max_sync(kAll, best);
+        if (best <= kDead) { return false; }
+        std::uint32_t at = 0xFFFFFFFFU;
+#pragma unroll
+        for (int i = kItems - 1; i >= 0; --i) { at = keys[i] == best ? lane + 32 * i : at; }
+        index = __reduce_min_sync(kAll, at);
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) { keys[i] = index == lane + 32 * i ? 0 : keys[i]; }
+        value = valueOf(best);
+        return true;
+    }
+};
+
+// 16 bits: key and index fit one word, the index upside down, and one reduction does a round. No two words are equal. Up to eight words a
+// lane are sorted first, so that a round only looks at each lane's first one, and the lane it belonged to moves its others up; more
+// are gone through in each round.
+template<typename T, int kItems> struct TopK {
+    // That of -inf, in the upper half.
+    static constexpr bool kSorted          = kItems <= 8;
+    static constexpr std::uint32_t kDead16 = std::is_same<T, __half>::value ? 0x03FF0000U : 0x007F0000U;
+    std::uint32_t keys[kItems];
+    __device__ __forceinline__ void set(int i, T x, std::uint32_t index) {
+        std::uint32_t bits = *reinterpret_cast<const unsigned short*>(&x);
+        bits               = bits == 0x8000U ? 0 : bits;
+        std::uint32_t key  = (bits & 0x8000U) != 0 ? 0xFFFFU - bits : bits | 0x8000U;
+        if (__hisnan(x)) { key = 0xFFFFU; }
+        keys[i] = key << 16 | (0xFFFFU - index);
+    }
+    __device__ __forceinline__ void none(int i) { keys[i] = 0; }
+    __device__ __forceinline__ void ready() {
+        if (!kSorted) { return; }
+        // Odd-even merging (Batcher's network).
+#pragma unroll
+        for (int size = 1; size < kItems; size *= 2) {
+#pragma unroll
+            for (int gap = size; gap > 0; gap /= 2) {
+#pragma unroll
+                for (int start = gap % size; start + gap < kItems; start += 2 * gap) {
+#pragma unroll
+                    for (int i = 0; i < gap; ++i) {
+                        if (i + start + gap < kItems && (i + start) / (2 * size) == (i + start + gap) / (2 * size)) {
+                            const std::uint32_t low = keys[i + start], high = keys[i + start + gap];
+                            keys[i + start]       = max(low, high);
+                            keys[i + start + gap] = min(low, high);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ bool next(int, std::uint32_t& index, float& value) {
+        std::uint32_t first = keys[0];
+        if (!kSorted) {
+#pragma unroll
+            for (int i = 1; i < kItems; ++i) { first = max(first, keys[i]); }
+        }
+        const std::uint32_t best = __reduce_max_sync(kAll, first);
+        if (best <= (kDead16 | 0xFFFFU)) { return false; }
+        if (kSorted) {
+            const bool mine = first == best;
+#pragma unroll
+            for (int i = 0; i + 1 < kItems; ++i) { keys[i] = mine ? keys[i + 1] : keys[i]; }
+            keys[kItems - 1] = mine ? 0 : keys[kItems - 1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < kItems; ++i) { keys[i] = keys[i] == best ? 0 : keys[i]; }
+        }
+        index = 0xFFFFU - (best & 0xFFFFU);
+        const std::uint32_t key   = best >> 16;
+        const unsigned short bits = static_cast<unsigned short>((key & 0x8000U) != 0 ? key & 0x7FFFU : 0xFFFFU - key);
+        value                     = Element<T>::widen(*reinterpret_cast<const T*>(&bits));
+        return true;
+    }
+};
+
+// e^x, within a few units of the last place for the arguments that a softmax has (|x| 2^-24 more for large ones).
+__device__ __forceinline__ float expFast(float x) { return exp2Fast(x * 1.4426950408889634F); }
+
 template<typename T, int kItems> __global__ void __launch_bounds__(kWarps * 32) routeTokens(const RouteParams p) {
     extern __shared__ unsigned char memory[];
     auto* const hits = reinterpret_cast<std::int32_t*>(memory);  // [experts]
@@ -112,44 +205,43 @@ template<typename T, int kItems> __global__ void __launch_bounds__(kWarps * 32) 
         float value        = 0.0F, weight = 0.0F;
         if (on) {
             float x[kItems];
-            std::uint32_t keys[kItems];
+            TopK<T, kItems> top;
 #pragma unroll
             for (int i = 0; i < kItems; ++i) {
                 const std::uint32_t e = lane + 32 * i;
-                x[i]                  = e < p.experts ? Element<T>::widen(row[e]) : -INFINITY;
-                keys[i]               = e < p.experts ? orderOf(x[i]) : 0;
+                if (e < p.experts) {
+                    const T raw = row[e];
+                    x[i]        = Element<T>::widen(raw);
+                    top.set(i, raw, e);
+                } else {
+                    x[i] = -INFINITY;
+                    top.none(i);
+                }
             }
+            top.ready();
             float largest = -INFINITY;
             for (std::uint32_t round = 0; round < p.top_k; ++round) {
-                std::uint32_t best = keys[0];
-#pragma unroll
-                for (int i = 1; i < kItems; ++i) { best = max(best, keys[i]); }
-                best = __reduce_max_sync(kAll, best);
-                if (best <= kDead) { break; }
-                std::uint32_t at = 0xFFFFFFFFU;
-#pragma unroll
-                for (int i = kItems - 1; i >= 0; --i) { at = keys[i] == best ? lane + 32 * i : at; }
-                at = __reduce_min_sync(kAll, at);
-#pragma unroll
-                for (int i = 0; i < kItems; ++i) { keys[i] = at == lane + 32 * i ? 0 : keys[i]; }
-                if (round == 0) { largest = valueOf(best); }
+                std::uint32_t index;
+                float best;
+                if (!top.next(lane, index, best)) { break; }
+                if (round == 0) { largest = best; }
                 if (lane == static_cast<int>(round)) {
-                    mine  = static_cast<std::int32_t>(at);
-                    value = valueOf(best);
+                    mine  = static_cast<std::int32_t>(index);
+                    value = best;
                 }
             }
             if (largest != -INFINITY) {  // (not a number included)
                 float total = 0.0F;
 #pragma unroll
                 for (int i = 0; i < kItems; ++i) {
-                    x[i] = expf(x[i] - largest);
+                    x[i] = expFast(x[i] - largest);
                     total += x[i];
                 }
                 total               = warpSum(total);
                 const float inverse = 1.0F / total;
 #pragma unroll
                 for (int i = 0; i < kItems; ++i) { sums[i] += x[i] * inverse; }
-                weight = mine >= 0 ? expf(value - largest) : 0.0F;
+                weight = mine >= 0 ? expFast(value - largest) : 0.0F;
                 weight /= p.normalize != 0 ? warpSum(weight) : total;
                 ++live;
             }
@@ -205,25 +297,48 @@ template<typename T, int kItems> __global__ void __launch_bounds__(kWarps * 32) 
     if (threadIdx.x == 0) { writeLoss(p, total, live_total); }
 }
 
+// Shared memory of the kernel below, in words: the sums (two words each), those of the groups with their counts, the counts, one more.
+__host__ __device__ __forceinline__ std::uint32_t finishWords(std::uint32_t experts) {
+    const std::uint32_t groups = experts < kFinishThreads ? kFinishThreads / experts : 1;
+    return 2 * experts + 3 * groups * experts + experts + 1;
+}
+
 // The rows of partial sums added up: each CTA of the cluster an eighth of them, the first CTA what they come to.
 __global__ void __cluster_dims__(kFinishCtas, 1, 1) __launch_bounds__(kFinishThreads) finishRouting(const RouteParams p, std::uint32_t rows) {
     extern __shared__ unsigned char memory[];
     auto* const sums = reinterpret_cast<double*>(memory);                   // [experts]
-    auto* const hits = reinterpret_cast<std::int32_t*>(sums + p.experts);   // [experts], then the number of live tokens
+    auto* const hits = reinterpret_cast<std::int32_t*>(sums) + finishWords(p.experts) - p.experts - 1;  // [experts], then the number of live tokens
     __shared__ double shared[kFinishThreads / 32];
     cg::cluster_group cluster = cg::this_cluster();
     const std::uint32_t rank  = cluster.block_rank();
     gridDependencyWait();
     gridDependencyLaunchDependents();
     const std::uint32_t first = rows * rank / kFinishCtas, last = rows * (rank + 1) / kFinishCtas;
-    // A warp's lanes take neighbouring experts, and the threads beyond the experts other rows; joined in shared memory below.
+    // Threads beyond the experts take other rows: `groups` of them for each expert, one row in so many each.
+    const std::uint32_t groups = max(1U, kFinishThreads / p.experts);
+    const std::uint32_t group  = threadIdx.x / p.experts;  // (with more experts than threads, a thread takes several)
+    double* const group_sums       = sums + p.experts;
+    std::int32_t* const group_hits = reinterpret_cast<std::int32_t*>(group_sums + groups * p.experts);
+    if (group < groups || groups == 1) {
+        for (std::uint32_t e = threadIdx.x - (groups == 1 ? 0 : group * p.experts); e < p.experts; e += kFinishThreads) {
+            double sum         = 0.0;
+            std::int32_t count = 0;
+#pragma unroll 8
+            for (std::uint32_t row = first + (groups == 1 ? 0 : group); row < last; row += groups) {
+                sum += static_cast<double>(__ldcg(p.sums + static_cast<std::uint64_t>(row) * p.experts + e));
+                count += __ldcg(p.hits + static_cast<std::uint64_t>(row) * p.experts + e);
+            }
+            group_sums[(groups == 1 ? 0 : group) * p.experts + e] = sum;
+            group_hits[(groups == 1 ? 0 : group) * p.experts + e] = count;
+        }
+    }
+    __syncthreads();
     for (std::uint32_t e = threadIdx.x; e < p.experts; e += kFinishThreads) {
         double sum         = 0.0;
         std::int32_t count = 0;
-#pragma unroll 8
-        for (std::uint32_t row = first; row < last; ++row) {
-            sum += static_cast<double>(__ldcg(p.sums + static_cast<std::uint64_t>(row) * p.experts + e));
-            count += __ldcg(p.hits + static_cast<std::uint64_t>(row) * p.experts + e);
+        for (std::uint32_t g = 0; g < groups; ++g) {
+            sum += group_sums[g * p.experts + e];
+            count += group_hits[g * p.experts + e];
         }
         sums[e] = sum;
         hits[e] = count;
@@ -324,7 +439,7 @@ template<typename T, int kItems> __global__ void __launch_bounds__(kBackwardWarp
         float total = 0.0F, mean = 0.0F;
 #pragma unroll
         for (int i = 0; i < kItems; ++i) {
-            x[i] = expf(x[i] - largest);
+            x[i] = expFast(x[i] - largest);
             total += x[i];
             mean += x[i] * slope[i];
         }
@@ -436,7 +551,7 @@ extern "C" int ftcuda_expert_routing(const FtcudaRouting* routing, float* weight
     if (error == cudaSuccess) {
         countLaunches(1);
         if (rows > 1) {
-            error = training::launchOverlapped(finishRouting, dim3(kFinishCtas), dim3(kFinishThreads), r.experts * 12ULL + 4, static_cast<cudaStream_t>(stream), p, rows);
+            error = training::launchOverlapped(finishRouting, dim3(kFinishCtas), dim3(kFinishThreads), finishWords(r.experts) * 4ULL, static_cast<cudaStream_t>(stream), p, rows);
         }
     }
     if (error != cudaSuccess) { return fail(message, message_capacity, 1, "%s", cudaGetErrorString(error)); }
