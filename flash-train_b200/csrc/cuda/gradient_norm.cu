@@ -368,50 +368,63 @@ const char* checkGradient(const FtcudaGradient& g, bool clip) {
 // Memory of one operand: `rows` windows of `width` bytes, `stride` bytes apart.
 struct Range {
     std::uint64_t begin, end, width, stride;
-    std::uint64_t owner;
-    bool written;
 };
 
-Range rangeOf(const void* address, std::uint64_t rows, std::uint64_t cols, std::int64_t row_stride, std::uint64_t bytes, std::uint64_t owner, bool written) {
+Range rangeOf(const void* address, std::uint64_t rows, std::uint64_t cols, std::int64_t row_stride, std::uint64_t bytes) {
     Range r;
-    r.begin   = reinterpret_cast<std::uintptr_t>(address);
-    r.width   = cols * bytes;
-    r.stride  = rows > 1 ? static_cast<std::uint64_t>(row_stride) * bytes : 0;
-    r.end     = r.begin + (rows - 1) * r.stride + r.width;
-    r.owner   = owner;
-    r.written = written;
+    r.begin  = reinterpret_cast<std::uintptr_t>(address);
+    r.width  = cols * bytes;
+    r.stride = rows > 1 ? static_cast<std::uint64_t>(row_stride) * bytes : 0;
+    r.end    = r.begin + (rows - 1) * r.stride + r.width;
     return r;
 }
+Range inputOf(const FtcudaGradient& g) { return rangeOf(g.data, g.rows, g.cols, g.row_stride, training::elementBytes(g.element)); }
+Range outputOf(const FtcudaGradient& g) { return rangeOf(g.out, g.rows, g.cols, g.out_row_stride, training::elementBytes(g.out_element)); }
 
-// Whether two ranges whose hulls meet share no byte as far as their strides show: windows of one matrix, side by side.
+// Whether two ranges whose hulls meet, the second beginning no earlier, share no byte as far as their strides show: windows of one matrix, side by side.
 bool sideBySide(const Range& a, const Range& b) {
     const std::uint64_t stride = a.stride != 0 ? a.stride : b.stride;
     if (stride == 0 || (a.stride != 0 && b.stride != 0 && a.stride != b.stride) || a.width > stride || b.width > stride) { return false; }
-    const std::uint64_t offset = (b.begin - a.begin) % stride;  // b.begin >= a.begin
+    const std::uint64_t offset = (b.begin - a.begin) % stride;
     return offset >= a.width && offset + b.width <= stride;
 }
 
-// nullptr, or why the gradients cannot be clipped at once.
+// An operand by where it begins, and which: gradient 2 i is read, 2 i + 1 written.
+struct Operand {
+    std::uint64_t begin;
+    std::uint64_t which;
+};
+
+// nullptr, or why the gradients cannot be clipped at once: no byte may be written that another operand reads or writes. What is read outside of
+// all that is written is left out before anything is sorted.
 const char* checkOverlap(const FtcudaGradient* gradients, std::uint64_t count) {
-    std::vector<Range> ranges;
-    ranges.reserve(2 * count);
+    std::uint64_t lowest = ~std::uint64_t{0}, highest = 0;
+    for (std::uint64_t i = 0; i < count; ++i) {
+        if (gradients[i].rows == 0 || gradients[i].cols == 0) { continue; }
+        const Range out = outputOf(gradients[i]);
+        lowest          = std::min(lowest, out.begin);
+        highest         = std::max(highest, out.end);
+    }
+    std::vector<Operand> operands;
+    operands.reserve(2 * count);
     for (std::uint64_t i = 0; i < count; ++i) {
         const FtcudaGradient& g = gradients[i];
         if (g.rows == 0 || g.cols == 0) { continue; }
-        const Range in  = rangeOf(g.data, g.rows, g.cols, g.row_stride, training::elementBytes(g.element), i, false);
-        const Range out = rangeOf(g.out, g.rows, g.cols, g.out_row_stride, training::elementBytes(g.out_element), i, true);
-        ranges.push_back(out);
-        if (g.data != g.out) {
-            ranges.push_back(in);
-        } else if (g.element != g.out_element || in.stride != out.stride) {
-            return "a gradient that is its own output has another type or stride there";
+        operands.push_back({reinterpret_cast<std::uintptr_t>(g.out), 2 * i + 1});
+        if (g.data == g.out) {
+            if (g.element != g.out_element || inputOf(g).stride != outputOf(g).stride) { return "a gradient that is its own output has another type or stride there"; }
+            continue;
         }
+        const Range in = inputOf(g);
+        if (in.begin < highest && in.end > lowest) { operands.push_back({in.begin, 2 * i}); }
     }
-    const auto before = [](const Range& a, const Range& b) { return a.begin < b.begin; };
-    if (!std::is_sorted(ranges.begin(), ranges.end(), before)) { std::sort(ranges.begin(), ranges.end(), before); }
-    for (std::size_t i = 0; i < ranges.size(); ++i) {
-        for (std::size_t j = i + 1; j < ranges.size() && ranges[j].begin < ranges[i].end; ++j) {
-            if ((ranges[i].written || ranges[j].written) && !sideBySide(ranges[i], ranges[j])) {
+    const auto before = [](const Operand& a, const Operand& b) { return a.begin < b.begin; };
+    if (!std::is_sorted(operands.begin(), operands.end(), before)) { std::sort(operands.begin(), operands.end(), before); }
+    const auto range = [&](const Operand& o) { return (o.which & 1) != 0 ? outputOf(gradients[o.which / 2]) : inputOf(gradients[o.which / 2]); };
+    for (std::size_t i = 0; i < operands.size(); ++i) {
+        const Range a = range(operands[i]);
+        for (std::size_t j = i + 1; j < operands.size() && operands[j].begin < a.end; ++j) {
+            if (((operands[i].which | operands[j].which) & 1) != 0 && !sideBySide(a, range(operands[j]))) {
                 return "an output overlaps another gradient or output";
             }
         }

@@ -2,11 +2,11 @@
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <cmath>
-#include <optional>
 #include <vector>
 
 #include <ftcuda/training.h>
@@ -45,6 +45,11 @@ FtcudaGradient describe(const at::Tensor& gradient, const at::Tensor& out, std::
     g.element     = elementOf(gradient);
     g.out_element = elementOf(out);
     if (gradient.numel() == 0) { return g; }
+    if (gradient.is_contiguous() && out.is_contiguous()) {
+        g.rows = 1;
+        g.cols = static_cast<std::uint64_t>(gradient.numel());
+        return g;
+    }
     struct Dimension {
         std::int64_t size, stride, out_stride;
     };
@@ -79,24 +84,41 @@ int normKind(double norm_type) {
     return norm_type == 2.0 ? FTCUDA_NORM_2 : FTCUDA_NORM_INF;
 }
 
-at::Tensor normOf(const std::vector<at::Tensor>& gradients, const std::vector<at::Tensor>* outs, double norm_type, double max_norm) {
+// The tensors of a Python sequence, looked at in place: with many small ones, what the host does for each is most of a call.
+class TensorList final {
+  public:
+    TensorList(pybind11::handle sequence, const char* name) : items_(pybind11::reinterpret_steal<pybind11::object>(PySequence_Fast(sequence.ptr(), name))) {
+        if (!items_) { throw pybind11::error_already_set(); }
+        for (std::size_t i = 0; i < size(); ++i) { TORCH_CHECK(THPVariable_Check(item(i)), name, " ", i, " must be a tensor"); }
+    }
+    std::size_t size() const { return static_cast<std::size_t>(PySequence_Fast_GET_SIZE(items_.ptr())); }
+    const at::Tensor& operator[](std::size_t i) const { return THPVariable_Unpack(item(i)); }
+
+  private:
+    PyObject* item(std::size_t i) const { return PySequence_Fast_GET_ITEM(items_.ptr(), static_cast<Py_ssize_t>(i)); }
+    pybind11::object items_;  // a list or a tuple
+};
+
+at::Tensor normOf(const TensorList& gradients, const TensorList* outs, double norm_type, double max_norm) {
     const int kind = normKind(norm_type);
     TORCH_CHECK(outs == nullptr || max_norm >= 0.0, "max_norm must not be negative");
-    if (gradients.empty()) { return at::zeros({}, at::kFloat); }
-    const at::Tensor& first = gradients.front();
+    if (gradients.size() == 0) { return at::zeros({}, at::kFloat); }
+    const at::Tensor& first = gradients[0];
     std::vector<FtcudaGradient> described;
     described.reserve(gradients.size());
+    const bool recording = at::GradMode::is_enabled();
     for (std::size_t i = 0; i < gradients.size(); ++i) {
-        checkGradient(gradients[i], first, "gradient", i);
+        const at::Tensor& gradient = gradients[i];
+        const at::Tensor& out      = outs != nullptr ? (*outs)[i] : gradient;
+        checkGradient(gradient, first, "gradient", i);
         if (outs != nullptr) {
-            const at::Tensor& out = (*outs)[i];
-            if (!out.is_same(gradients[i])) {
+            if (!out.is_same(gradient)) {
                 checkGradient(out, first, "out", i);
-                TORCH_CHECK(out.sizes() == gradients[i].sizes(), "out ", i, " must have its gradient's shape");
+                TORCH_CHECK(out.sizes() == gradient.sizes(), "out ", i, " must have its gradient's shape");
             }
-            TORCH_CHECK(!at::GradMode::is_enabled() || !out.requires_grad(), "out ", i, " must not require a gradient");
+            TORCH_CHECK(!recording || !out.requires_grad(), "out ", i, " must not require a gradient");
         }
-        described.push_back(describe(gradients[i], outs != nullptr ? (*outs)[i] : gradients[i], i));
+        described.push_back(describe(gradient, out, i));
     }
     const c10::cuda::CUDAGuard guard(first.device());
     const auto stream             = c10::cuda::getCurrentCUDAStream(first.device().index()).stream();
@@ -110,19 +132,20 @@ at::Tensor normOf(const std::vector<at::Tensor>& gradients, const std::vector<at
                                        : ftcuda_gradient_clip(described.data(), described.size(), kind, max_norm, norm.data_ptr<float>(), device,
                                                               workspace.data_ptr(), bytes, stream, message.text, sizeof message.text);
     TORCH_CHECK(status == 0, "flash_train ", outs == nullptr ? "grad_norm" : "clip_grads", " failed: ", message.text);
-    if (outs != nullptr) {
-        for (const at::Tensor& out : *outs) {
-            if (!out.is_inference()) { torch::autograd::impl::bump_version(out); }
-        }
+    for (std::size_t i = 0; outs != nullptr && i < outs->size(); ++i) {
+        if (!(*outs)[i].is_inference()) { torch::autograd::impl::bump_version((*outs)[i]); }
     }
     return norm;
 }
 
-at::Tensor gradNorm(const std::vector<at::Tensor>& gradients, double norm_type) { return normOf(gradients, nullptr, norm_type, 0.0); }
+at::Tensor gradNorm(const pybind11::object& gradients, double norm_type) { return normOf(TensorList(gradients, "gradients"), nullptr, norm_type, 0.0); }
 
-at::Tensor clipGrads(const std::vector<at::Tensor>& gradients, double max_norm, double norm_type, const std::optional<std::vector<at::Tensor>>& out) {
-    TORCH_CHECK(!out.has_value() || out->size() == gradients.size(), "out must have one tensor for each gradient");
-    return normOf(gradients, out.has_value() ? &*out : &gradients, norm_type, max_norm);
+at::Tensor clipGrads(const pybind11::object& gradients, double max_norm, double norm_type, const pybind11::object& out) {
+    const TensorList from(gradients, "gradients");
+    if (out.is_none()) { return normOf(from, &from, norm_type, max_norm); }
+    const TensorList to(out, "out");
+    TORCH_CHECK(to.size() == from.size(), "out must have one tensor for each gradient");
+    return normOf(from, &to, norm_type, max_norm);
 }
 
 }  // namespace
@@ -135,7 +158,7 @@ void registerGradientNorm(pybind11::module_& module) {
     module.def("clip_grads", &clipGrads,
                "Multiplies every gradient by min(1, max_norm / (norm + 1e-6)) and returns the norm before that, without waiting for it.\n\n"
                "In place, or into `out`: tensors of the same shapes in any of the three types.",
-               pybind11::arg("gradients"), pybind11::arg("max_norm"), pybind11::arg("norm_type") = 2.0, pybind11::arg("out") = std::nullopt);
+               pybind11::arg("gradients"), pybind11::arg("max_norm"), pybind11::arg("norm_type") = 2.0, pybind11::arg("out") = pybind11::none());
 }
 
 }  // namespace flash_train_torch
