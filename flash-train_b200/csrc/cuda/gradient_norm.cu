@@ -3,7 +3,7 @@
 //   n = (sum of all x^2)^(1/2)  or  max |x|,     out = x * min(1, max_norm / (n + 1e-6))
 //
 // Two passes over the gradients, since the factor depends on every element: the first reads them, the second
-// reads and writes them. Both are bound by HBM. A pass is one launch for up to kTensors tensors, whose
+// reads and writes them. Both are bound by HBM. A pass is one launch for up to kDense tensors, whose
 // table travels in the kernel's parameters (no copy to the device, so that a captured graph holds it). The tensors are cut into
 // chunks of kChunk elements, and every CTA takes a contiguous run of about as many chunks as any other, whatever tensors they are
 // of: one of a thousand small tensors costs what its bytes cost. Runs instead of single chunks spare the search for a chunk's tensor.
@@ -34,8 +34,14 @@ constexpr int kSumBatch           = 4;  // packs of 16 bytes that a thread asks 
 constexpr int kScaleBatch         = 4;
 constexpr int kScaleSingles       = 8;  // ... or single elements, where the two sides' alignment differs
 constexpr std::uint32_t kChunk    = 16 * kThreads;  // elements
-constexpr std::uint32_t kTensors  = 480;            // of one launch: 30 KiB of the nearly 32 that a kernel's parameters may take
-constexpr std::uint32_t kFew      = 64;             // ... of the launch for few tensors, whose parameters are quicker to hand over
+// Tensors of one launch: what nearly fills the 32764 bytes that a kernel's parameters may take; and few of them, whose table is quicker
+// to hand over.
+constexpr std::uint32_t kDense    = 1152;           // dense ones
+constexpr std::uint32_t kRows     = 608;            // with rows apart among them
+constexpr std::uint32_t kFew      = 64;
+constexpr std::uint64_t kMostGradients = 1ULL << 20;
+constexpr std::uint64_t kMostLaunches  = (kMostGradients + kRows - 1) / kRows;
+constexpr std::uint64_t kMostChunks    = 1ULL << 30;  // of all gradients, so that their numbers fit 32 bits: 2^42 elements
 constexpr std::uint64_t kMaxGrid  = 2048;           // CTAs of one launch at most (and room for their sums)
 
 struct Entry {
@@ -47,11 +53,55 @@ struct Entry {
     std::int32_t element, out_element;
 };
 
-template<std::uint32_t kCapacity> struct Table {
-    Entry entries[kCapacity];
-    std::uint64_t chunks;
-    std::uint32_t count;
+// Where rows lie apart.
+template<std::uint32_t kCapacity, bool kWithRows> struct RowTable {
+    std::uint64_t rows[kCapacity];
+    std::int64_t row_stride[kCapacity], out_row_stride[kCapacity];
 };
+template<std::uint32_t kCapacity> struct RowTable<kCapacity, false> {};
+
+template<std::uint32_t kCapacity, bool kWithRows> struct Table : RowTable<kCapacity, kWithRows> {
+    static constexpr std::uint32_t kTensors = kCapacity;
+    const void* data[kCapacity];
+    void* out[kCapacity];
+    std::uint64_t shape[kCapacity];  // cols, the element's type and the output's: 48, 8, 8 bits
+    std::uint32_t first[kCapacity];
+    std::uint32_t chunks, count;
+
+    __host__ __device__ __forceinline__ void set(std::uint32_t i, const Entry& entry) {
+        data[i]  = entry.data;
+        out[i]   = entry.out;
+        shape[i] = entry.cols | static_cast<std::uint64_t>(entry.element) << 48 | static_cast<std::uint64_t>(entry.out_element) << 56;
+        first[i] = static_cast<std::uint32_t>(entry.first);
+        if constexpr (kWithRows) {
+            this->rows[i]           = entry.rows;
+            this->row_stride[i]     = entry.row_stride;
+            this->out_row_stride[i] = entry.out_row_stride;
+        }
+    }
+    __device__ __forceinline__ Entry get(std::uint32_t i) const {
+        Entry entry;
+        entry.data           = data[i];
+        entry.out            = out[i];
+        entry.cols           = shape[i] & 0xFFFFFFFFFFFFULL;
+        entry.element        = static_cast<std::int32_t>(shape[i] >> 48 & 0xFF);
+        entry.out_element    = static_cast<std::int32_t>(shape[i] >> 56);
+        entry.first          = first[i];
+        entry.rows           = 1;
+        entry.row_stride     = 0;
+        entry.out_row_stride = 0;
+        if constexpr (kWithRows) {
+            entry.rows           = this->rows[i];
+            entry.row_stride     = this->row_stride[i];
+            entry.out_row_stride = this->out_row_stride[i];
+        }
+        return entry;
+    }
+};
+using FewTable   = Table<kFew, true>;
+using RowsTable  = Table<kRows, true>;
+using DenseTable = Table<kDense, false>;
+static_assert(sizeof(RowsTable) + 64 <= 32764 && sizeof(DenseTable) + 64 <= 32764, "kernel parameters");
 
 // Largest and smallest sum of squares that FP32 holds as well as 64 bits would: with a sum of up to 16 squares in here, none overflowed, and what
 // underflowed in one (2^-150) is under 2^-60 of the sum.
@@ -195,12 +245,11 @@ __device__ __forceinline__ void scaleRow(const T* row, U* out, std::uint64_t cou
 }
 
 // The tensor that chunk `chunk` is of.
-template<std::uint32_t kCapacity>
-__device__ __forceinline__ std::uint32_t findEntry(const Table<kCapacity>& table, std::uint64_t chunk) {
-    std::uint32_t low = 0, high = table.count;  // entries[low].first <= chunk < entries[high].first
+template<typename TableT> __device__ __forceinline__ std::uint32_t findEntry(const TableT& table, std::uint64_t chunk) {
+    std::uint32_t low = 0, high = table.count;  // first[low] <= chunk < first[high]
     while (high - low > 1) {
         const std::uint32_t middle = (low + high) / 2;
-        if (table.entries[middle].first <= chunk) {
+        if (table.first[middle] <= chunk) {
             low = middle;
         } else {
             high = middle;
@@ -242,20 +291,19 @@ template<typename Sum> __device__ __forceinline__ void joinBlock(Sum& sum, doubl
     }
 }
 
-template<typename Sum, std::uint32_t kCapacity>
-__global__ void __launch_bounds__(kThreads, kSumCtasPerSm) gradientSums(const __grid_constant__ Table<kCapacity> table, double* partials) {
+template<typename Sum, typename TableT> __global__ void __launch_bounds__(kThreads, kSumCtasPerSm) gradientSums(const __grid_constant__ TableT table, double* partials) {
     __shared__ double shared[kThreads / 32];
     gridDependencyWait();
     gridDependencyLaunchDependents();
-    const std::uint64_t begin = table.chunks * blockIdx.x / gridDim.x, end = table.chunks * (blockIdx.x + 1) / gridDim.x;
+    const std::uint64_t all = table.chunks, begin = all * blockIdx.x / gridDim.x, end = all * (blockIdx.x + 1) / gridDim.x;
     Sum sum;
     if (begin < end) {
         std::uint32_t index = findEntry(table, begin);
 #pragma unroll 1
         for (std::uint64_t chunk = begin; chunk < end;) {
-            while (index + 1 < table.count && table.entries[index + 1].first <= chunk) { ++index; }
-            const Entry& entry        = table.entries[index];
-            const std::uint64_t last  = index + 1 < table.count ? min(end, table.entries[index + 1].first) : end;
+            while (index + 1 < table.count && table.first[index + 1] <= chunk) { ++index; }
+            const Entry entry         = table.get(index);
+            const std::uint64_t last  = index + 1 < table.count ? min(end, static_cast<std::uint64_t>(table.first[index + 1])) : end;
             const Stretch s           = stretchOf<false>(entry, chunk, last);
             const std::int64_t offset = static_cast<std::int64_t>(s.row) * entry.row_stride + static_cast<std::int64_t>(s.col);
             switch (entry.element) {
@@ -297,14 +345,14 @@ template<typename T> __device__ __forceinline__ void scaleStretch(const Entry& e
 }
 
 // The CTA's run of chunks, from the last one back.
-template<std::uint32_t kCapacity> __device__ __forceinline__ void scaleRun(const Table<kCapacity>& table, float factor) {
-    const std::uint64_t begin = table.chunks * blockIdx.x / gridDim.x, end = table.chunks * (blockIdx.x + 1) / gridDim.x;
+template<typename TableT> __device__ __forceinline__ void scaleRun(const TableT& table, float factor) {
+    const std::uint64_t all = table.chunks, begin = all * blockIdx.x / gridDim.x, end = all * (blockIdx.x + 1) / gridDim.x;
     if (begin == end) { return; }
     std::uint32_t index = findEntry(table, end - 1);
 #pragma unroll 1
     for (std::uint64_t chunk = end; chunk > begin;) {
-        while (table.entries[index].first >= chunk) { --index; }
-        const Entry& entry = table.entries[index];
+        while (table.first[index] >= chunk) { --index; }
+        const Entry entry  = table.get(index);
         const Stretch s    = stretchOf<true>(entry, max(begin, entry.first), chunk);
         chunk -= s.chunks;
         if (factor == 1.0F && entry.out == entry.data) { continue; }
@@ -316,9 +364,9 @@ template<std::uint32_t kCapacity> __device__ __forceinline__ void scaleRun(const
     }
 }
 
-template<typename Sum, std::uint32_t kCapacity>
-__global__ void __launch_bounds__(kThreads, kScaleCtasPerSm) gradientScale(const __grid_constant__ Table<kCapacity> table, const double* partials, std::uint32_t count,
-                                                          double max_norm, float* norm) {
+template<typename Sum, typename TableT>
+__global__ void __launch_bounds__(kThreads, kScaleCtasPerSm) gradientScale(const __grid_constant__ TableT table, const double* partials, std::uint32_t count,
+                                                                           double max_norm, float* norm) {
     __shared__ double shared[kThreads / 32];
     __shared__ float shared_factor;
     gridDependencyWait();
@@ -334,16 +382,13 @@ __global__ void __launch_bounds__(kThreads, kScaleCtasPerSm) gradientScale(const
 }
 
 // The factor as the caller gives it.
-template<std::uint32_t kCapacity>
-__global__ void __launch_bounds__(kThreads, kScaleCtasPerSm) gradientMultiply(const __grid_constant__ Table<kCapacity> table, const float* factor) {
+template<typename TableT> __global__ void __launch_bounds__(kThreads, kScaleCtasPerSm) gradientMultiply(const __grid_constant__ TableT table, const float* factor) {
     gridDependencyWait();
     gridDependencyLaunchDependents();
     scaleRun(table, *factor);
 }
 
 // ---------------------------------------------------------------- host
-
-std::uint64_t launchesFor(std::uint64_t count) { return count <= kFew ? 1 : ceilDiv(count, kTensors); }
 
 // nullptr, or what is wrong with a gradient (`out` looked at for a clip alone).
 const char* checkGradient(const FtcudaGradient& g, bool clip) {
@@ -432,30 +477,36 @@ const char* checkOverlap(const FtcudaGradient* gradients, std::uint64_t count) {
     return nullptr;
 }
 
-template<std::uint32_t kCapacity>
-void fillTable(Table<kCapacity>& table, const FtcudaGradient* gradients, std::uint64_t count, bool clip) {
-    table.count  = 0;
-    table.chunks = 0;
-    for (std::uint64_t i = 0; i < count; ++i) {
-        const FtcudaGradient& g = gradients[i];
-        if (g.rows == 0 || g.cols == 0) { continue; }
-        Entry& entry         = table.entries[table.count++];
-        entry.data           = g.data;
-        entry.out            = clip ? g.out : nullptr;
-        entry.rows           = g.rows;
-        entry.cols           = g.cols;
-        entry.row_stride     = g.row_stride;
-        entry.out_row_stride = g.out_row_stride;
-        entry.element        = g.element;
-        entry.out_element    = g.out_element;
-        if (g.rows > 1 && g.row_stride == static_cast<std::int64_t>(g.cols) && (!clip || g.out_row_stride == g.row_stride)) {
-            entry.cols = g.rows * g.cols;  // dense after all
-            entry.rows = 1;
-        }
-        entry.first = table.chunks;
-        table.chunks += entry.rows * ceilDiv(entry.cols, kChunk);
+// The gradient as the kernels see it: rows that follow one another are one.
+Entry entryOf(const FtcudaGradient& g, bool clip) {
+    Entry entry{g.data, clip ? g.out : nullptr, g.rows, g.cols, g.row_stride, g.out_row_stride, 0, g.element, g.out_element};
+    if (g.rows == 1 || (g.row_stride == static_cast<std::int64_t>(g.cols) && (!clip || g.out_row_stride == g.row_stride))) {
+        entry.cols = g.rows * g.cols;
+        entry.rows = 1;
     }
+    return entry;
 }
+
+std::uint64_t chunksOf(const Entry& entry) { return entry.rows * ceilDiv(entry.cols, kChunk); }
+
+// As many gradients from `begin` on as one launch takes; returns where the next one begins.
+template<typename TableT> std::uint64_t fillTable(TableT& table, const FtcudaGradient* gradients, std::uint64_t begin, std::uint64_t count, bool clip) {
+    table.count          = 0;
+    std::uint64_t chunks = 0, i = begin;
+    for (; i < count && table.count < TableT::kTensors; ++i) {
+        if (gradients[i].rows == 0 || gradients[i].cols == 0) { continue; }
+        Entry entry                = entryOf(gradients[i], clip);
+        const std::uint64_t wanted = chunksOf(entry);
+        entry.first = chunks;
+        table.set(table.count++, entry);
+        chunks += wanted;
+    }
+    table.chunks = static_cast<std::uint32_t>(chunks);
+    return i;
+}
+
+// Launches that `count` gradients can take.
+std::uint64_t launchesFor(std::uint64_t count) { return count <= kFew ? 1 : ceilDiv(count, kRows); }
 
 // CTAs for that many chunks: the SMs filled once, or a chunk each.
 std::uint32_t gridFor(std::uint64_t chunks, int sms, int per_sm) {
@@ -474,66 +525,81 @@ struct Call {
     cudaStream_t stream;
 };
 
-template<typename Sum, std::uint32_t kCapacity> cudaError_t enqueue(const Call& call) {
-    const std::uint64_t launches = launchesFor(call.count);
-    const std::uint64_t each     = launches == 1 ? call.count : kTensors;
-    Table<kCapacity> table;
-    std::uint32_t partials = 0;
-    for (std::uint64_t l = 0; l < launches; ++l) {
-        fillTable(table, call.gradients + l * each, std::min(each, call.count - l * each), call.clip);
+template<typename Sum, typename TableT> cudaError_t enqueue(const Call& call) {
+    TableT table;
+    std::uint64_t starts[kMostLaunches + 1] = {0};
+    std::uint32_t partials = 0, launches = 0;
+    for (std::uint64_t at = 0; launches == 0 || at < call.count; ++launches) {
+        if (launches == kMostLaunches) { return cudaErrorInvalidValue; }  // (not with the counts and sizes that the checks allow)
+        at                       = fillTable(table, call.gradients, at, call.count, call.clip);
+        starts[launches + 1]     = at;
         const std::uint32_t grid = gridFor(table.chunks, call.sms, kSumCtasPerSm);
         // The first launch of a call is an ordinary one: it starts when what came before in the stream is done.
-        if (l == 0) {
-            gradientSums<Sum, kCapacity><<<grid, kThreads, 0, call.stream>>>(table, call.partials);
+        if (launches == 0) {
+            gradientSums<Sum, TableT><<<grid, kThreads, 0, call.stream>>>(table, call.partials);
             const cudaError_t error = cudaGetLastError();
             if (error != cudaSuccess) { return error; }
             countLaunches(1);
         } else {
-            const cudaError_t error = training::launchOverlapped(gradientSums<Sum, kCapacity>, dim3(grid), dim3(kThreads), 0, call.stream, table, call.partials + partials);
+            const cudaError_t error = training::launchOverlapped(gradientSums<Sum, TableT>, dim3(grid), dim3(kThreads), 0, call.stream, table, call.partials + partials);
             if (error != cudaSuccess) { return error; }
         }
         partials += grid;
     }
     if (!call.clip) {
-        return training::launchOverlapped(gradientNorm<Sum>, dim3(1), dim3(kThreads), 0, call.stream,
-                                          static_cast<const double*>(call.partials), partials, call.norm);
+        return training::launchOverlapped(gradientNorm<Sum>, dim3(1), dim3(kThreads), 0, call.stream, static_cast<const double*>(call.partials), partials, call.norm);
     }
-    for (std::uint64_t l = launches; l-- > 0;) {
-        if (launches > 1) { fillTable(table, call.gradients + l * each, std::min(each, call.count - l * each), call.clip); }
-        const cudaError_t error = training::launchOverlapped(gradientScale<Sum, kCapacity>, dim3(gridFor(table.chunks, call.sms, kScaleCtasPerSm)), dim3(kThreads), 0,
-                                                             call.stream, table, static_cast<const double*>(call.partials), partials, call.max_norm, l == 0 ? call.norm : static_cast<float*>(nullptr));
+    for (std::uint32_t l = launches; l-- > 0;) {
+        if (launches > 1) { fillTable(table, call.gradients, starts[l], starts[l + 1], call.clip); }
+        const cudaError_t error = training::launchOverlapped(gradientScale<Sum, TableT>, dim3(gridFor(table.chunks, call.sms, kScaleCtasPerSm)), dim3(kThreads), 0,
+                                                             call.stream, table, static_cast<const double*>(call.partials), partials, call.max_norm,
+                                                             l == 0 ? call.norm : static_cast<float*>(nullptr));
         if (error != cudaSuccess) { return error; }
     }
     return cudaSuccess;
 }
 
-template<std::uint32_t kCapacity> cudaError_t enqueueMultiply(const FtcudaGradient* gradients, std::uint64_t count, const float* factor, int sms, cudaStream_t stream) {
-    const std::uint64_t launches = launchesFor(count), each = launches == 1 ? count : kTensors;
-    Table<kCapacity> table;
-    for (std::uint64_t l = 0; l < launches; ++l) {
-        fillTable(table, gradients + l * each, std::min(each, count - l * each), true);
+template<typename TableT> cudaError_t enqueueMultiply(const FtcudaGradient* gradients, std::uint64_t count, const float* factor, int sms, cudaStream_t stream) {
+    TableT table;
+    for (std::uint64_t at = 0; at < count;) {
+        const bool first         = at == 0;
+        at                       = fillTable(table, gradients, at, count, true);
         const std::uint32_t grid = gridFor(table.chunks, sms, kScaleCtasPerSm);
-        if (l == 0) {  // an ordinary launch: it starts when what came before in the stream is done
-            gradientMultiply<kCapacity><<<grid, kThreads, 0, stream>>>(table, factor);
+        if (first) {  // an ordinary launch: it starts when what came before in the stream is done
+            gradientMultiply<TableT><<<grid, kThreads, 0, stream>>>(table, factor);
             const cudaError_t error = cudaGetLastError();
             if (error != cudaSuccess) { return error; }
             countLaunches(1);
         } else {
-            const cudaError_t error = training::launchOverlapped(gradientMultiply<kCapacity>, dim3(grid), dim3(kThreads), 0, stream, table, factor);
+            const cudaError_t error = training::launchOverlapped(gradientMultiply<TableT>, dim3(grid), dim3(kThreads), 0, stream, table, factor);
             if (error != cudaSuccess) { return error; }
         }
     }
     return cudaSuccess;
 }
 
+// The table that a list of gradients takes: the small one, the one for many dense tensors, or the one that can have rows apart.
+template<typename Few, typename Dense, typename Rows>
+cudaError_t withTable(const FtcudaGradient* gradients, std::uint64_t count, bool clip, const Few& few, const Dense& dense, const Rows& rows) {
+    if (count <= kFew) { return few(); }
+    for (std::uint64_t i = 0; i < count; ++i) {
+        if (gradients[i].rows != 0 && gradients[i].cols != 0 && entryOf(gradients[i], clip).rows != 1) { return rows(); }
+    }
+    return dense();
+}
+
 // What every call minds about its gradients; 0, or a failure with its message.
 int checkGradients(const FtcudaGradient* gradients, std::uint64_t count, bool written, char* message, std::size_t capacity) {
     if (gradients == nullptr && count != 0) { return fail(message, capacity, 1, "null gradients"); }
-    if (count >= (1ULL << 24)) { return fail(message, capacity, 1, "too many gradients"); }
+    if (count > kMostGradients) { return fail(message, capacity, 1, "too many gradients"); }
+    std::uint64_t chunks = 0;
     for (std::uint64_t i = 0; i < count; ++i) {
-        if (const char* reason = checkGradient(gradients[i], written)) {
-            return fail(message, capacity, 1, "gradient %llu: %s", static_cast<unsigned long long>(i), reason);
+        const char* reason = checkGradient(gradients[i], written);
+        if (reason == nullptr && gradients[i].rows != 0 && gradients[i].cols != 0) {
+            chunks += chunksOf(entryOf(gradients[i], written));  // (at most 2^44 each)
+            if (chunks > kMostChunks) { reason = "too many elements, or rows apart, in all"; }
         }
+        if (reason != nullptr) { return fail(message, capacity, 1, "gradient %llu: %s", static_cast<unsigned long long>(i), reason); }
     }
     if (!written) { return 0; }
     try {
@@ -555,12 +621,12 @@ int runCall(const FtcudaGradient* gradients, std::uint64_t count, int norm_kind,
     int sms = 0;
     if (!training::deviceIsCurrent(device, message, capacity) || !deviceSmCount(device, &sms, message, capacity)) { return 1; }
     const Call call{gradients, count, clip, max_norm, norm, static_cast<double*>(workspace), sms, static_cast<cudaStream_t>(stream)};
-    cudaError_t error = cudaSuccess;
-    if (norm_kind == FTCUDA_NORM_2) {
-        error = count <= kFew ? enqueue<Sum2, kFew>(call) : enqueue<Sum2, kTensors>(call);
-    } else {
-        error = count <= kFew ? enqueue<SumInf, kFew>(call) : enqueue<SumInf, kTensors>(call);
-    }
+    const auto run = [&](auto sum) {
+        using Sum = decltype(sum);
+        return withTable(gradients, count, clip, [&] { return enqueue<Sum, FewTable>(call); }, [&] { return enqueue<Sum, DenseTable>(call); },
+                         [&] { return enqueue<Sum, RowsTable>(call); });
+    };
+    const cudaError_t error = norm_kind == FTCUDA_NORM_2 ? run(Sum2{}) : run(SumInf{});
     if (error != cudaSuccess) { return fail(message, capacity, 1, "%s", cudaGetErrorString(error)); }
     return 0;
 }
@@ -589,8 +655,10 @@ extern "C" int ftcuda_gradient_scale(const FtcudaGradient* gradients, uint64_t c
     if (const int status = checkGradients(gradients, count, true, message, message_capacity)) { return status; }
     int sms = 0;
     if (!training::deviceIsCurrent(device, message, message_capacity) || !deviceSmCount(device, &sms, message, message_capacity)) { return 1; }
-    const cudaError_t error = count <= kFew ? enqueueMultiply<kFew>(gradients, count, factor, sms, static_cast<cudaStream_t>(stream))
-                                            : enqueueMultiply<kTensors>(gradients, count, factor, sms, static_cast<cudaStream_t>(stream));
+    const auto queue        = static_cast<cudaStream_t>(stream);
+    const cudaError_t error = withTable(gradients, count, true, [&] { return enqueueMultiply<FewTable>(gradients, count, factor, sms, queue); },
+                                        [&] { return enqueueMultiply<DenseTable>(gradients, count, factor, sms, queue); },
+                                        [&] { return enqueueMultiply<RowsTable>(gradients, count, factor, sms, queue); });
     if (error != cudaSuccess) { return fail(message, message_capacity, 1, "%s", cudaGetErrorString(error)); }
     return 0;
 }

@@ -272,3 +272,21 @@ def test_scale_by_a_number_on_the_device(ft, capi, count):
     capi.gradient_scale(described, factor.data_ptr(), 0, torch.cuda.current_stream().cuda_stream)
     for g, o in zip(gradients, outs):
         assert torch.equal(o, (g.float() * factor).to(o.dtype))
+
+
+@pytest.mark.parametrize("count, apart", [(608, True), (609, True), (1152, False), (1153, False), (1300, True)])
+def test_lists_that_fill_a_launch(ft, count, apart):
+    """Dense tensors, or windows of wider matrices among them; every one is clipped once."""
+    gradients, wide = [], []
+    for i in range(count):
+        matrix = make([(3, 5 + i % 9)], TYPES[i % 3], seed=i)[0]
+        wide.append((matrix, matrix.clone()))
+        gradients.append(matrix[:, :4] if apart and i % 2 else matrix)
+    originals = [g.clone() for g in gradients]
+    norm = exact_norm(originals)
+    check_norm(ft.grad_norm(gradients), norm)
+    check_norm(ft.clip_grads(gradients, 1.0), norm)
+    for i, (g, original) in enumerate(zip(gradients, originals)):
+        check_clipped(g, original, norm, 1.0)
+        if apart and i % 2:
+            assert torch.equal(wide[i][0][:, 4:], wide[i][1][:, 4:])
