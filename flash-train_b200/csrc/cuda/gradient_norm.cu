@@ -32,7 +32,8 @@ constexpr int kSumCtasPerSm       = 4;
 constexpr int kScaleCtasPerSm     = 4;
 constexpr int kSumBatch           = 4;  // packs of 16 bytes that a thread asks for at a time, twice over
 constexpr int kScaleBatch         = 4;
-constexpr int kScaleSingles       = 8;  // ... or single elements, where the two sides' alignment differs
+constexpr int kScaleShifted       = 3;  // ... or pairs of packs, where the two sides' alignment differs
+constexpr int kScaleSingles       = 8;  // ... or single elements, where their types' sizes do as well
 constexpr std::uint32_t kChunk    = 16 * kThreads;  // elements
 // Tensors of one launch: what nearly fills the 32764 bytes that a kernel's parameters may take; and few of them, whose table is quicker
 // to hand over.
@@ -149,9 +150,10 @@ template<typename T> __device__ __forceinline__ std::uint32_t misaligned(const T
 }
 
 // Goes over `count` packs with all threads of the CTA, from the last one back with kBack, kBatch at a time for each: the next batch is asked
-// for before `use` is called for the packs of the one at hand, so that loads are always on their way.
-template<int kBatch, bool kBack, typename P, typename Use>
-__device__ __forceinline__ void stream(const P* from, std::uint64_t count, const Use& use) {
+// for (by `load`) before `use` is called for the packs of the one at hand, so that loads are always on their way.
+template<int kBatch, bool kBack, typename Load, typename Use>
+__device__ __forceinline__ void stream(const Load& load, std::uint64_t count, const Use& use) {
+    using P = decltype(load(std::int64_t{0}));
     constexpr std::int64_t kStep  = kBack ? -kBatch * kThreads : kBatch * kThreads;
     constexpr std::int64_t kEach  = kBack ? -kThreads : kThreads;
     const std::uint64_t batches   = count / (kBatch * kThreads);
@@ -159,12 +161,12 @@ __device__ __forceinline__ void stream(const P* from, std::uint64_t count, const
     if (batches != 0) {
         P now[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) { now[i] = from[at + i * kEach]; }
+        for (int i = 0; i < kBatch; ++i) { now[i] = load(at + i * kEach); }
 #pragma unroll 1
         for (std::uint64_t batch = 1; batch < batches; ++batch) {
             P next[kBatch];
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) { next[i] = from[at + kStep + i * kEach]; }
+            for (int i = 0; i < kBatch; ++i) { next[i] = load(at + kStep + i * kEach); }
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) { use(at + i * kEach, now[i]); }
 #pragma unroll
@@ -177,7 +179,7 @@ __device__ __forceinline__ void stream(const P* from, std::uint64_t count, const
     }
 #pragma unroll 1
     for (; kBack ? at >= 0 : at < static_cast<std::int64_t>(count); at += kEach) {
-        const P one = from[at];
+        const P one = load(at);
         use(at, one);
     }
 }
@@ -207,7 +209,8 @@ template<typename T, typename Sum> __device__ __forceinline__ void sumRow(const 
         const float x[1] = {Element<T>::widen(row[threadIdx.x < head ? threadIdx.x : rest + (threadIdx.x - head)])};
         sum.add(x);
     }
-    stream<kSumBatch, false>(reinterpret_cast<const P*>(row + head), packs, [&](std::int64_t, const P& pack) {
+    const P* const from = reinterpret_cast<const P*>(row + head);
+    stream<kSumBatch, false>([&](std::int64_t at) { return from[at]; }, packs, [&](std::int64_t, const P& pack) {
         float x[kEach];
 #pragma unroll
         for (int j = 0; j < kEach; ++j) { x[j] = Element<T>::widen(pack.at[j]); }
@@ -216,7 +219,7 @@ template<typename T, typename Sum> __device__ __forceinline__ void sumRow(const 
 }
 
 // out = row * factor. Packs of four elements (eight where both sides have 16 bits) where both sides are aligned for them at the same element: a
-// warp's accesses are neighbours on both sides then. Otherwise one element at a time.
+// warp's accesses are neighbours on both sides then. Otherwise shifted packs, or one element at a time.
 template<typename T, typename U>
 __device__ __forceinline__ void scaleRow(const T* row, U* out, std::uint64_t count, float factor) {
     constexpr int kEach      = 16 / (sizeof(T) > sizeof(U) ? sizeof(T) : sizeof(U));
@@ -233,14 +236,52 @@ __device__ __forceinline__ void scaleRow(const T* row, U* out, std::uint64_t cou
             out[at]                = Element<U>::narrow(Element<T>::widen(row[at]) * factor);
         }
         Q* const to = reinterpret_cast<Q*>(out + head);
-        stream<kScaleBatch, true>(reinterpret_cast<const P*>(row + head), packs, [&](std::int64_t at, const P& pack) {
+        const P* const from = reinterpret_cast<const P*>(row + head);
+        stream<kScaleBatch, true>([&](std::int64_t at) { return from[at]; }, packs, [&](std::int64_t at, const P& pack) {
+            Q o;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) { o.at[j] = Element<U>::narrow(Element<T>::widen(pack.at[j]) * factor); }
+            storeStreaming(to + at, o);
+        });
+    } else if (sizeof(T) == sizeof(U) && row != static_cast<const void*>(out)) {
+        // Packs of both sides, the input's shifted: pack k of the output lies across two of the input's, whose words are moved down by `shift` bytes. The second one
+        // of them a neighbour reads as well.
+        const std::uint32_t first  = misaligned(row);
+        const std::uint32_t start  = misaligned(out) >= first ? misaligned(out) : misaligned(out) + kEach;
+        const std::uint64_t whole  = count > first ? (count - first) / kEach : 0;
+        const std::uint64_t packs  = whole > 1 ? whole - 1 : 0;
+        const std::uint64_t rest   = start + packs * kEach;
+        const std::uint32_t ends   = packs != 0 ? start + static_cast<std::uint32_t>(count - rest) : static_cast<std::uint32_t>(count);  // fewer than four packs
+        const std::uint32_t shift  = (start - first) * static_cast<std::uint32_t>(sizeof(T));
+        const uint4* const from    = reinterpret_cast<const uint4*>(row + first);
+        Q* const to                = reinterpret_cast<Q*>(out + start);
+        if (threadIdx.x < ends) {
+            const std::uint64_t at = packs == 0 || threadIdx.x < start ? threadIdx.x : rest + (threadIdx.x - start);
+            out[at]                = Element<U>::narrow(Element<T>::widen(row[at]) * factor);
+        }
+        struct Two {
+            uint4 low, high;
+        };
+        stream<kScaleShifted, true>([&](std::int64_t at) { return Two{from[at], from[at + 1]}; }, packs, [&](std::int64_t at, const Two& two) {
+            std::uint32_t words[8] = {two.low.x, two.low.y, two.low.z, two.low.w, two.high.x, two.high.y, two.high.z, two.high.w};
+#pragma unroll
+            for (int by = 2; by > 0; by /= 2) {
+                if ((shift / 4 & by) != 0) {
+#pragma unroll
+                    for (int i = 0; i + by < 8; ++i) { words[i] = words[i + by]; }
+                }
+            }
+            std::uint32_t moved[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { moved[i] = __funnelshift_r(words[i], words[i + 1], shift % 4 * 8); }
+            const P pack = *reinterpret_cast<const P*>(moved);
             Q o;
 #pragma unroll
             for (int j = 0; j < kEach; ++j) { o.at[j] = Element<U>::narrow(Element<T>::widen(pack.at[j]) * factor); }
             storeStreaming(to + at, o);
         });
     } else {
-        stream<kScaleSingles, true>(row, count, [&](std::int64_t at, const T& x) { storeStreaming(out + at, Element<U>::narrow(Element<T>::widen(x) * factor)); });
+        stream<kScaleSingles, true>([&](std::int64_t at) { return row[at]; }, count, [&](std::int64_t at, const T& x) { storeStreaming(out + at, Element<U>::narrow(Element<T>::widen(x) * factor)); });
     }
 }
 
