@@ -191,19 +191,19 @@ bool encodeTensorMap2d(CUtensorMap* map, const void* base, std::uint64_t inner, 
     return true;
 }
 
-bool encodeMap16(CUtensorMap* map, bool bf16, const void* base, std::uint64_t inner, std::uint64_t outer, std::uint64_t row_pitch_bytes,
-                 std::uint32_t box_outer, char* message, std::size_t capacity) {
+bool encodeMap16(CUtensorMap* map, bool bf16, const void* base, std::uint64_t inner, std::uint64_t outer, std::uint64_t planes,
+                 std::uint64_t row_pitch_bytes, std::uint64_t plane_bytes, std::uint32_t box_outer, char* message, std::size_t capacity) {
     const PFN_cuTensorMapEncodeTiled_v12000 encode = tensorMapEncoder();
     if (encode == nullptr) {
         fail(message, capacity, 1, "the CUDA driver does not provide cuTensorMapEncodeTiled");
         return false;
     }
-    const cuuint64_t dims[2]     = {inner, outer};
-    const cuuint64_t strides[1]  = {row_pitch_bytes};
-    const cuuint32_t box[2]      = {64, box_outer};
-    const cuuint32_t elements[2] = {1, 1};
+    const cuuint64_t dims[3]     = {inner, outer, planes};
+    const cuuint64_t strides[2]  = {row_pitch_bytes, plane_bytes};
+    const cuuint32_t box[3]      = {64, box_outer, 1};
+    const cuuint32_t elements[3] = {1, 1, 1};
     const CUresult result = encodeInContext([&] {
-        return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, elements,
+        return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, elements,
                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     });
     if (result != CUDA_SUCCESS) {

@@ -117,9 +117,9 @@ void countLaunches(std::uint64_t launches);
 // 3-D FP16 map over a split operand: `rows` rows of `blocks` 64-element blocks, 128-byte swizzle, box 64 x box_rows x 2.
 bool encodeSplitMap(CUtensorMap* map, const void* base, std::uint64_t rows, std::uint64_t blocks, std::uint32_t box_rows,
                     char* message, std::size_t capacity);
-// 2-D map over a matrix of 16-bit elements: `outer` rows of `inner` neighbours, 128-byte swizzle, box 64 x box_outer.
-bool encodeMap16(CUtensorMap* map, bool bf16, const void* base, std::uint64_t inner, std::uint64_t outer, std::uint64_t row_pitch_bytes,
-                 std::uint32_t box_outer, char* message, std::size_t capacity);
+// 3-D map over `planes` matrices of 16-bit elements: `outer` rows of `inner` neighbours each, 128-byte swizzle, box 64 x box_outer x 1.
+bool encodeMap16(CUtensorMap* map, bool bf16, const void* base, std::uint64_t inner, std::uint64_t outer, std::uint64_t planes,
+                 std::uint64_t row_pitch_bytes, std::uint64_t plane_bytes, std::uint32_t box_outer, char* message, std::size_t capacity);
 bool replaceMapAddress(CUtensorMap* map, void* base);
 
 // True when `base`/strides describe a matrix TMA can fetch with `contiguous`

@@ -13,14 +13,16 @@
 // makes what the padding holds irrelevant (a NaN there would reach dW through 0 * NaN), spares the products those rows, and gives
 // the tensor cores an aligned operand whatever H's strides. How many there are only the GPU knows; the kernels read it there.
 //
-// BF16 and FP16 operands go through loss_products.cu; FP32 ones through the library's own FP32 products, chosen by the same rules as the
-// host pipeline's (gemm_choice.hpp), with Z of a piece in the workspace and a pass over it for the statistics or dZ.
+// BF16 and FP16 operands go through loss_products.cu, and FP32 ones as sums of three BF16, which takes six products for each. Where the library's
+// own FP32 products in their prepared form (three FP16 products) are ahead, FP32 operands go through those instead, chosen by the same rules as the
+// host pipeline's (gemm_choice.hpp), with Z of a piece in the workspace and a pass over it for the statistics or dZ: see libraryPays.
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "gemm_choice.hpp"
 #include "loss_products.hpp"
@@ -172,6 +174,29 @@ __global__ void __launch_bounds__(kGatherThreads) copyRows16(const std::uint16_t
     to += blockIdx.x * pitch;
 #pragma unroll 4
     for (std::uint32_t i = threadIdx.x; i < depth; i += kGatherThreads) { to[i] = from[i]; }
+}
+
+// An FP32 matrix's rows as three BF16 matrices, `plane` elements apart. With `rows`, those of the live tokens, and zeros behind the last one.
+__global__ void __launch_bounds__(kGatherThreads) splitRows(const LiveRows rows, bool gathered, const float* from, std::int64_t stride, std::uint16_t* to,
+                                                            std::uint64_t pitch, std::uint64_t plane, std::uint32_t depth) {
+    gridDependencyWait();
+    gridDependencyLaunchDependents();
+    const std::uint32_t row  = blockIdx.x;
+    const std::uint32_t live = gathered ? *rows.count : 0xFFFFFFFFU;
+    if (gathered && row >= (max(live, 1U) + loss::kTileRows - 1) / loss::kTileRows * loss::kTileRows) { return; }
+    if (row < live) { from += static_cast<std::int64_t>(gathered ? rows.token[row] : static_cast<std::int32_t>(row)) * stride; }
+    to += row * pitch;
+    // Two elements a thread: the planes' rows begin at multiples of 16 bytes and have room for one more.
+#pragma unroll 2
+    for (std::uint32_t i = 2 * threadIdx.x; i < depth; i += 2 * kGatherThreads) {
+        float low[3] = {0.0F, 0.0F, 0.0F}, high[3] = {0.0F, 0.0F, 0.0F};
+        if (row < live) {
+            training::splitPlanes(from[i], low);
+            training::splitPlanes(i + 1 < depth ? from[i + 1] : 0.0F, high);
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) { *reinterpret_cast<__nv_bfloat162*>(to + p * plane + i) = __floats2bfloat162_rn(low[p], high[p]); }
+    }
 }
 
 // Two partial results of a row: sums of 2^(x - base), with the bases.
@@ -335,12 +360,22 @@ struct KeptParams {
     LiveRows rows;
     const float2* partials;  // [piece][capacity]
     std::uint32_t pieces, width, capacity;
-    std::uint64_t pitch;
+    std::uint64_t pitch, plane;
 };
+
+// Of a piece's row: what its exponentials are multiplied by to be slopes.
+__device__ __forceinline__ float keptFactor(const KeptParams& p, std::uint32_t piece, std::uint32_t row) {
+    const float base = p.partials[static_cast<std::uint64_t>(piece) * p.capacity + row].x;
+    // (A piece of -inf alone kept zeros; against a sum of nothing, or of NaN, NaN comes out.)
+    const float lse2 = p.rows.lse2[row];
+    return p.rows.scale[row] * (base == -INFINITY && lse2 > -INFINITY ? 0.0F : exp2f(base - lse2));
+}
 
 // What the product kept becomes dZ, in place: 2^(logit - piece's largest) 2^(that - lse), less the target's one; zeros in the neutral rows. A thread
 // takes eight columns of a row at a time, neighbouring threads neighbouring ones.
-template<typename T> __global__ void __launch_bounds__(256) keptSlopes(const KeptParams p, __half* kept) {
+// kPlanes: from FP32 to the three BF16 matrices at `planes`, T being float; otherwise from FP16 to T.
+template<typename T> __global__ void __launch_bounds__(256) keptSlopes(const KeptParams p, void* kept, std::uint16_t* planes) {
+    constexpr bool kPlanes = std::is_same<T, float>::value;
     __shared__ float factors[kKeptPieces][kKeptRows];
     gridDependencyWait();
     gridDependencyLaunchDependents();
@@ -351,12 +386,7 @@ template<typename T> __global__ void __launch_bounds__(256) keptSlopes(const Kep
     const std::uint32_t pieces = min(p.pieces - piece0, static_cast<std::uint32_t>(kKeptPieces));
     if (threadIdx.x < kKeptPieces * kKeptRows) {
         const std::uint32_t piece = threadIdx.x / kKeptRows, row = row0 + threadIdx.x % kKeptRows;
-        if (piece < pieces && row < live) {
-            const float base = p.partials[static_cast<std::uint64_t>(piece0 + piece) * p.capacity + row].x;
-            // (A piece of -inf alone kept zeros; against a sum of nothing, or of NaN, NaN comes out.)
-            const float lse2 = p.rows.lse2[row];
-            factors[piece][threadIdx.x % kKeptRows] = p.rows.scale[row] * (1.0F / loss::kKeptScale) * (base == -INFINITY && lse2 > -INFINITY ? 0.0F : exp2f(base - lse2));
-        }
+        if (piece < pieces && row < live) { factors[piece][threadIdx.x % kKeptRows] = keptFactor(p, piece0 + piece, row) * (kPlanes ? 1.0F : 1.0F / loss::kKeptScale); }
     }
     __syncthreads();
     const std::uint32_t each  = p.width / 8;  // packs of a piece's row
@@ -364,23 +394,33 @@ template<typename T> __global__ void __launch_bounds__(256) keptSlopes(const Kep
     for (std::uint32_t i = threadIdx.x; i < packs * kKeptRows; i += 256) {
         const std::uint32_t in_row = i / packs, pack = i - in_row * packs;
         const std::uint32_t row    = row0 + in_row, col = piece0 * p.width + pack * 8;
-        uint4* const at            = reinterpret_cast<uint4*>(kept + row * p.pitch + col);
-        if (row >= live) {
-            *at = make_uint4(0, 0, 0, 0);
-            continue;
-        }
-        const float factor        = factors[pack / each][in_row];
-        const std::int32_t hit    = p.rows.target[row] - static_cast<std::int32_t>(col);
-        alignas(16) __half from[8];
-        alignas(16) T to[8];
-        *reinterpret_cast<uint4*>(from) = *at;
+        const std::uint64_t at     = row * p.pitch + col;
+        const bool on              = row < live;
+        const float factor         = on ? factors[pack / each][in_row] : 0.0F;
+        const float scale          = on ? p.rows.scale[row] : 0.0F;
+        const std::int32_t hit     = on ? p.rows.target[row] - static_cast<std::int32_t>(col) : -1;
+        if constexpr (kPlanes) {
+            alignas(16) float from[8];
+            alignas(16) __nv_bfloat16 to[3][8];
+            for (int j = 0; j < 8; j += 4) { *reinterpret_cast<float4*>(from + j) = *reinterpret_cast<const float4*>(static_cast<const float*>(kept) + at + j); }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float slope = factor * __half2float(from[j]);
-            if (j == hit) { slope -= p.rows.scale[row]; }
-            to[j] = Element<T>::narrow(slope);
+            for (int j = 0; j < 8; ++j) {
+                float parts[3];
+                training::splitPlanes(on ? factor * from[j] - (j == hit ? scale : 0.0F) : 0.0F, parts);
+#pragma unroll
+                for (int plane = 0; plane < 3; ++plane) { to[plane][j] = __float2bfloat16_rn(parts[plane]); }
+            }
+#pragma unroll
+            for (int plane = 0; plane < 3; ++plane) { *reinterpret_cast<uint4*>(planes + plane * p.plane + at) = *reinterpret_cast<const uint4*>(to[plane]); }
+        } else {
+            uint4* const words = reinterpret_cast<uint4*>(static_cast<__half*>(kept) + at);
+            alignas(16) __half from[8];
+            alignas(16) T to[8];
+            *reinterpret_cast<uint4*>(from) = *words;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { to[j] = Element<T>::narrow(on ? factor * __half2float(from[j]) - (j == hit ? scale : 0.0F) : 0.0F); }
+            *words = *reinterpret_cast<const uint4*>(to);
         }
-        *at = *reinterpret_cast<const uint4*>(to);
     }
 }
 
@@ -407,15 +447,17 @@ __global__ void __launch_bounds__(kGatherThreads) spreadHidden(const LiveRows ro
 // ---------------------------------------------------------------- host: layout of the workspace
 
 struct Layout {
+    bool library;                 // FP32 through the library's products
+    bool planes;                  // ... or as three BF16 matrices
     std::uint64_t capacity;       // rows, a multiple of kTileRows
     std::uint64_t copy_pitch;     // of the hidden states' copy, elements
-    std::uint64_t weight_pitch;   // of the weight's copy, 0: none
+    std::uint64_t weight_pitch;   // of the weight's copy or planes, 0: none
     std::uint64_t columns;        // of a piece
     std::uint64_t piece_pitch;    // of Z or dZ, elements
     std::uint64_t pieces;         // partial statistics of a row
     std::uint32_t splits;         // of the sums for dH
     std::uint64_t sums_pitch;
-    std::uint64_t count, unit, token, target, scale, lse2, picked, row_loss, slot, hidden, weight, partials, piece, sums, product, product_bytes;
+    std::uint64_t count, unit, token, target, scale, lse2, picked, row_loss, slot, hidden, weight, partials, piece, kept, sums, product, product_bytes;
     std::uint64_t total;
 };
 
@@ -516,26 +558,44 @@ FtcudaGemmDesc describeWeight(const FtcudaLinearCrossEntropy& q, const Layout& l
 // What a call computes: the loss, the gradients from a loss that is known, or both at once.
 enum class Form { kLoss, kGradients, kStep };
 
+// Whether FP32 operands are better off with the library's products. Measured (a step, library / three BF16 matrices, microseconds): large products
+// of a depth from 768 on, where the prepared form is what they take (2048 x 2048 x 32000 2300 / 3240, 4096 x 1024 x 16000 1413 / 1666,
+// 700 x 2048 x 20000 749 / 851, 768 x 768 x 30000 524 / 529, but 2048 x 512 x 8000 349 / 281, 600 x 4096 x 6000 521 / 489, 896 x 72 x 45256
+// 1275 / 424); and few tokens, which read the weight once and would have it split for nothing else (64 x 1024 x 32000 280 / 302, 64 x 4096 x 32000 741 / 932,
+// but 96 x 1024 x 32000 337 / 308, 129 x 512 x 8191 145 / 92), a few more for the loss alone (96 x 4096 x 32000 202 / 512).
+bool libraryPays(const FtcudaLinearCrossEntropy& q, Form form) {
+    if (!isFp32(q)) { return false; }
+    return q.tokens <= (form == Form::kLoss ? 128U : 64U) || (q.depth >= 768 && preparedFormPays(q.tokens, q.vocabulary, q.depth));
+}
+
+// What a logit takes of the workspace while it is there, in bytes: its slope, and in the step call its exponential as well where that cannot
+// be in the same place.
+std::uint64_t logitBytes(const FtcudaLinearCrossEntropy& q, Form form) {
+    if (!isFp32(q)) { return 2; }
+    return libraryPays(q, form) ? 4 : form == Form::kStep ? 2 * loss::kPlanes + 4 : 2 * loss::kPlanes;
+}
+
 // What the step call holds of all logits at once, in bytes.
 std::uint64_t stepBytes(const FtcudaLinearCrossEntropy& q) {
-    return roundUp(std::max<std::uint64_t>(q.tokens, 1), loss::kTileRows) * roundUp(q.vocabulary, 256) * training::elementBytes(q.element);
+    return roundUp(std::max<std::uint64_t>(q.tokens, 1), loss::kTileRows) * roundUp(q.vocabulary, 256) * logitBytes(q, Form::kStep);
 }
 
 int layOut(const FtcudaLinearCrossEntropy& q, Form form, int sms, Layout& l, char* message, std::size_t capacity) {
     const bool gradients      = form != Form::kLoss;
-    const std::uint64_t bytes = training::elementBytes(q.element);
-    const bool fp32           = isFp32(q);
     l                         = Layout{};
+    l.library                 = libraryPays(q, form);
+    l.planes                  = isFp32(q) && !l.library;
+    const std::uint64_t bytes = logitBytes(q, form);
     l.capacity                = roundUp(std::max<std::uint64_t>(q.tokens, 1), loss::kTileRows);
-    l.copy_pitch              = roundUp(q.depth, 16 / bytes);
-    l.weight_pitch            = !fp32 && !weightFits(q) ? roundUp(q.depth, 8) : 0;
+    l.copy_pitch              = roundUp(q.depth, 8);
+    l.weight_pitch            = l.planes || (!l.library && !weightFits(q)) ? roundUp(q.depth, 8) : 0;
     const std::uint64_t fill  = roundUp(q.vocabulary, 256);
     l.columns                 = form == Form::kStep ? fill : std::min(fill, std::max(kLeastColumns, kPieceBytes / (l.capacity * bytes) / 256 * 256));
     l.columns                 = roundUp(ceilDiv(fill, ceilDiv(fill, l.columns)), 256);  // pieces of about one size
     l.piece_pitch             = l.columns;
-    l.pieces                  = fp32 ? ceilDiv(q.vocabulary, l.columns) : loss::statisticsPieces(static_cast<std::uint32_t>(q.vocabulary));
+    l.pieces                  = l.library ? ceilDiv(q.vocabulary, l.columns) : loss::statisticsPieces(static_cast<std::uint32_t>(q.vocabulary));
     l.sums_pitch              = roundUp(q.depth, 8);
-    l.splits                  = fp32 ? 1 : loss::hiddenSplits(static_cast<std::uint32_t>(l.capacity), static_cast<std::uint32_t>(q.depth),
+    l.splits                  = l.library ? 1 : loss::hiddenSplits(static_cast<std::uint32_t>(l.capacity), static_cast<std::uint32_t>(q.depth),
                                                               static_cast<std::uint32_t>(std::min(l.columns, q.vocabulary)), sms);
     std::uint64_t at = 0;
     const auto take  = [&](std::uint64_t size) {
@@ -548,8 +608,8 @@ int layOut(const FtcudaLinearCrossEntropy& q, Form form, int sms, Layout& l, cha
     l.token  = take(4 * l.capacity);
     l.target = take(4 * l.capacity);
     l.slot   = take(4 * l.capacity);
-    l.hidden = take(bytes * l.capacity * l.copy_pitch);
-    if (l.weight_pitch != 0) { l.weight = take(2 * q.vocabulary * l.weight_pitch); }
+    l.hidden = take((l.planes ? 2 * loss::kPlanes : training::elementBytes(q.element)) * l.capacity * l.copy_pitch);
+    if (l.weight_pitch != 0) { l.weight = take((l.planes ? 2 * loss::kPlanes : 2) * q.vocabulary * l.weight_pitch); }
     if (gradients) {
         l.scale = take(4 * l.capacity);
         l.lse2  = take(4 * l.capacity);
@@ -560,8 +620,9 @@ int layOut(const FtcudaLinearCrossEntropy& q, Form form, int sms, Layout& l, cha
         l.row_loss = take(4 * l.capacity);
         l.partials = take(8 * l.capacity * l.pieces);
     }
-    if (gradients || fp32) { l.piece = take(bytes * l.capacity * l.piece_pitch); }
-    if (fp32 && q.tokens != 0) {
+    if (gradients || l.library) { l.piece = take((l.planes ? 2 * loss::kPlanes : training::elementBytes(q.element)) * l.capacity * l.piece_pitch); }
+    if (l.planes && form == Form::kStep) { l.kept = take(4 * l.capacity * l.piece_pitch); }
+    if (l.library && q.tokens != 0) {
         // The most that any product of any piece wants. (The addresses are not known yet, but how they are aligned is.)
         l.product            = at;
         auto* const stand_in = reinterpret_cast<unsigned char*>(std::uintptr_t{1} << 40);
@@ -627,8 +688,8 @@ class Call final {
         rows_.scale  = at<float>(l_.scale);
         rows_.lse2   = at<float>(l_.lse2);
         rows_.picked = at<float>(l_.picked);
-        products_    = loss::ProductCall{q_.element == FTCUDA_ELEMENT_BF16, static_cast<std::uint32_t>(l_.capacity), static_cast<std::uint32_t>(q_.depth), rows_,
-                                      {base_ + l_.hidden, l_.copy_pitch}, status, sms_, stream_, message_, capacity_};
+        products_    = loss::ProductCall{l_.planes || q_.element == FTCUDA_ELEMENT_BF16, l_.planes, static_cast<std::uint32_t>(l_.capacity), static_cast<std::uint32_t>(q_.depth), rows_,
+                                      {base_ + l_.hidden, l_.copy_pitch, l_.capacity * l_.copy_pitch}, status, sms_, stream_, message_, capacity_};
         if (message_ != nullptr && capacity_ != 0) { message_[0] = '\0'; }
         return 0;
     }
@@ -642,7 +703,7 @@ class Call final {
         cudaError_t error = started();
         if (error == cudaSuccess) { error = gather(); }
         float2* const partials = at<float2>(l_.partials);
-        if (!isFp32(q_)) {
+        if (!l_.library) {
             if (error == cudaSuccess) { error = loss::launchStatistics(products_, weight(0), static_cast<std::uint32_t>(q_.vocabulary), partials); }
         } else {
             std::uint64_t piece = 0;
@@ -666,21 +727,22 @@ class Call final {
         if (error == cudaSuccess) { error = gather(); }
         float2* const partials        = at<float2>(l_.partials);
         const std::uint32_t columns   = static_cast<std::uint32_t>(q_.vocabulary);
-        if (error == cudaSuccess && !isFp32(q_)) { error = loss::launchKept(products_, weight(0), columns, partials, base_ + l_.piece, l_.piece_pitch); }
-        if (isFp32(q_)) {
+        void* const kept              = base_ + (l_.planes ? l_.kept : l_.piece);
+        if (error == cudaSuccess && !l_.library) { error = loss::launchKept(products_, weight(0), columns, partials, kept, l_.piece_pitch); }
+        if (l_.library) {
             if (error == cudaSuccess) { error = multiply(describeLogits(q_, l_, base_, 0, columns), false); }
             if (error == cudaSuccess) { error = training::launchOverlapped(rowStatistics, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(0, columns, partials)); }
         }
         if (error == cudaSuccess) { error = join(loss, nullptr, true); }
         if (error != cudaSuccess) { return error; }
-        if (isFp32(q_)) {
+        if (l_.library) {
             error = training::launchOverlapped(rowSlopes, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(0, columns, nullptr));
         } else {
-            const KeptParams kept{rows_, partials, static_cast<std::uint32_t>(l_.pieces), loss::statisticsWidth(columns), static_cast<std::uint32_t>(l_.capacity),
-                                  l_.piece_pitch};
+            const KeptParams params{rows_, partials, static_cast<std::uint32_t>(l_.pieces), loss::statisticsWidth(columns), static_cast<std::uint32_t>(l_.capacity),
+                                    l_.piece_pitch, slopesPlane()};
             const dim3 grid(static_cast<unsigned>(ceilDiv(l_.pieces, kKeptPieces)), static_cast<unsigned>(l_.capacity / kKeptRows));
-            error = training::launchOverlapped(q_.element == FTCUDA_ELEMENT_FP16 ? keptSlopes<__half> : keptSlopes<__nv_bfloat16>, grid, dim3(256), 0, stream_, kept,
-                                               at<__half>(l_.piece));
+            const auto kernel = l_.planes ? keptSlopes<float> : q_.element == FTCUDA_ELEMENT_FP16 ? keptSlopes<__half> : keptSlopes<__nv_bfloat16>;
+            error             = training::launchOverlapped(kernel, grid, dim3(256), 0, stream_, params, kept, at<std::uint16_t>(l_.piece));
         }
         if (error == cudaSuccess) { error = multiplySlopes(0, columns, grad_hidden != nullptr, grad_weight, weight_stride, grad_element); }
         return error == cudaSuccess && grad_hidden != nullptr ? spreadTyped(grad_hidden, hidden_stride, grad_element) : error;
@@ -711,6 +773,9 @@ class Call final {
         return error;
     }
 
+    // Elements between the planes of the slopes.
+    std::uint64_t slopesPlane() const { return l_.capacity * l_.piece_pitch; }
+
     // FP16's exponents do not hold small probabilities unless the largest slope is near 2^13.
     std::int32_t scaleBits() const { return isFp32(q_) ? INT32_MIN : q_.element == FTCUDA_ELEMENT_FP16 ? 13 : 0; }
 
@@ -732,9 +797,19 @@ class Call final {
 
     // The live hidden states, and the weight where TMA cannot fetch it as it is.
     cudaError_t gather() const {
+        if (l_.planes) {
+            const std::uint32_t depth = static_cast<std::uint32_t>(q_.depth);
+            cudaError_t error = training::launchOverlapped(splitRows, dim3(static_cast<unsigned>(l_.capacity)), dim3(kGatherThreads), 0, stream_, rows_, true,
+                                                           static_cast<const float*>(q_.hidden), q_.hidden_row_stride, at<std::uint16_t>(l_.hidden), l_.copy_pitch,
+                                                           l_.capacity * l_.copy_pitch, depth);
+            if (error != cudaSuccess) { return error; }
+            return training::launchOverlapped(splitRows, dim3(static_cast<unsigned>(q_.vocabulary)), dim3(kGatherThreads), 0, stream_, rows_, false,
+                                              static_cast<const float*>(q_.weight), q_.vocabulary == 1 ? std::int64_t{0} : q_.weight_row_stride, at<std::uint16_t>(l_.weight),
+                                              l_.weight_pitch, q_.vocabulary * l_.weight_pitch, depth);
+        }
         const std::uint64_t bytes = training::elementBytes(q_.element);
-        // The FP32 products go over all rows, the others over whole tiles of live ones.
-        const std::uint32_t zero_to = isFp32(q_) ? static_cast<std::uint32_t>(q_.tokens) : 0;
+        // The library's products go over all rows, the others over whole tiles of live ones.
+        const std::uint32_t zero_to = l_.library ? static_cast<std::uint32_t>(q_.tokens) : 0;
         const auto run = [&](auto word) {
             using W                   = decltype(word);
             const std::uint64_t ratio = sizeof(W) / bytes;
@@ -757,7 +832,7 @@ class Call final {
         const bool copied         = l_.weight_pitch != 0;
         const std::uint64_t pitch = copied ? l_.weight_pitch : weightStride(q_);
         const void* const from    = copied ? base_ + l_.weight : q_.weight;
-        return loss::Matrix16{static_cast<const unsigned char*>(from) + 2 * first * pitch, pitch};
+        return loss::Matrix16{static_cast<const unsigned char*>(from) + 2 * first * pitch, pitch, q_.vocabulary * pitch};
     }
 
     // One FP32 product.
@@ -790,7 +865,7 @@ class Call final {
     // dZ of a piece of the vocabulary, to the workspace.
     cudaError_t slopes(std::uint64_t first, std::uint64_t columns) const {
         const std::uint32_t first32 = static_cast<std::uint32_t>(first), columns32 = static_cast<std::uint32_t>(columns);
-        if (!isFp32(q_)) { return loss::launchSlopes(products_, weight(first), first32, columns32, base_ + l_.piece, l_.piece_pitch); }
+        if (!l_.library) { return loss::launchSlopes(products_, weight(first), first32, columns32, base_ + l_.piece, l_.piece_pitch, slopesPlane()); }
         const cudaError_t error = multiply(describeLogits(q_, l_, base_, first, columns), false);
         if (error != cudaSuccess) { return error; }
         return training::launchOverlapped(rowSlopes, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(first, columns, nullptr));
@@ -798,7 +873,7 @@ class Call final {
 
     // What dZ of a piece is multiplied with.
     cudaError_t multiplySlopes(std::uint64_t first, std::uint64_t columns, bool hidden, void* grad_weight, std::int64_t weight_stride, std::int32_t grad_element) const {
-        if (!isFp32(q_)) {
+        if (!l_.library) {
             loss::Gradients gradients{};
             gradients.sums                  = hidden ? at<float>(l_.sums) : nullptr;
             gradients.sums_pitch            = l_.sums_pitch;
@@ -810,7 +885,7 @@ class Call final {
                 gradients.weight_gradient =
                     static_cast<unsigned char*>(grad_weight) + static_cast<std::int64_t>(training::elementBytes(grad_element) * first) * weight_stride;
             }
-            return loss::launchGradients(products_, weight(first), static_cast<std::uint32_t>(columns), base_ + l_.piece, l_.piece_pitch, gradients);
+            return loss::launchGradients(products_, weight(first), static_cast<std::uint32_t>(columns), loss::Matrix16{base_ + l_.piece, l_.piece_pitch, slopesPlane()}, gradients);
         }
         cudaError_t error = cudaSuccess;
         if (hidden) { error = multiply(describeHidden(q_, l_, base_, first, columns), true); }

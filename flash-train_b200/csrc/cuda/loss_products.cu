@@ -1,4 +1,5 @@
-// The products of the linear cross entropy on BF16 or FP16 operands, each with its epilogue (linear_cross_entropy.cu has the whole).
+// The products of the linear cross entropy on BF16 or FP16 operands, or on FP32 ones as sums of three BF16 (loss_products.hpp), each with
+// its epilogue (linear_cross_entropy.cu has the whole).
 //
 //   statistics   Z = H W^T; of a tile of Z nothing is kept but the rows' maxima and sums of exponentials
 //   kept         the same, and the exponentials go to memory in FP16, each against its row's maximum in 128 columns
@@ -17,8 +18,13 @@
 //   warp 1       MMA issuer (one thread, in the first CTA, for both CTAs' tensor cores)
 //   warps 4-11   epilogue, 32 rows x half of the columns each
 //
+// An FP32 product is six BF16 ones (kTermsA, kTermsB say which planes), a K block's one after another in the same accumulator: a sixth of
+// the rate that the tensor cores have for BF16, with no scaling and no case that it is not exact enough for.
+//
 // Tensor memory holds two accumulators of 256 columns: one is filled while the other is read. What the epilogue reads goes to registers at once
-// and the accumulator back to the issuer; a thread has one row, so maxima, sums and the target's column need no
+// and the accumulator back to the issuer, at the end of an item or, where the sum is to be FP32's, more often: the tensor cores cut off
+// below the last bit of the sum so far, so a sum of many steps is short by 2^-25 or so for each, and the parts are added to nearest. Logits
+// are read every kLogitBlocks blocks of K, sums of FP32 operands every kFp32Blocks; a thread has one row, so maxima, sums and the target's column need no
 // exchange between threads, and its output is 256 neighbouring bytes, written 32 at a time.
 //
 // A K block is 512 cycles of MMAs, and the threads that feed them must need less. One producer for both operands, with its parameters read again for
@@ -48,7 +54,12 @@ namespace {
 
 constexpr std::uint32_t kBlockK = 64;  // 128 bytes, one swizzle row
 constexpr std::uint32_t kTileN  = 256;
-constexpr std::uint32_t kItemBlocks = 12;
+constexpr std::uint32_t kItemBlocks  = 12;
+constexpr std::uint32_t kLogitBlocks = 16;
+constexpr std::uint32_t kFp32Blocks  = 2;
+constexpr std::uint32_t kTerms       = 6;         // of an FP32 product: which plane of A and of B, four bits for each term
+constexpr std::uint32_t kTermsA      = 0x201100;
+constexpr std::uint32_t kTermsB      = 0x021010;
 constexpr int kStages           = 5;  // seven are no faster; what is left is the stores' L1
 constexpr int kThreads          = 384;
 constexpr int kOperandBytes     = 128 * 128;  // a CTA's share of A, and of a B of 256 columns
@@ -93,11 +104,13 @@ struct ProductParams {
     std::uint32_t problems, band;
     std::uint32_t instruction;  // the operands' type
     std::uint32_t bf16, capacity;
+    std::uint32_t terms;        // products for each block of K: 1, or kTerms
+    std::uint32_t chunk;        // blocks of K between two readings of a sum
     std::uint32_t first;        // column of the vocabulary that column 0 is
     LiveRows rows;
     float2* partials;
     void* slopes;               // or what is kept
-    std::uint64_t slopes_pitch;
+    std::uint64_t slopes_pitch, slopes_plane;
     float* sums;
     std::uint64_t sums_pitch;
     std::uint32_t accumulate;
@@ -141,7 +154,7 @@ __device__ __forceinline__ Work workOf(const ProductParams& p, std::uint32_t liv
     w.late  = w.items[0] % pairs;
     // (An item costs about kItemBlocks blocks' time beside its own.)
     const std::uint32_t first = p.problem[0].splits == 1 ? w.blocks[0] : p.problem[0].blocks_per_split;
-    w.early                   = w.items[1] != 0 && w.late != 0 ? (first + kItemBlocks) / (w.blocks[1] + kItemBlocks) : 0;
+    w.early                   = w.items[1] != 0 && w.late != 0 ? (first * p.terms + kItemBlocks) / (w.blocks[1] * p.terms + kItemBlocks) : 0;
     return w;
 }
 
@@ -199,6 +212,27 @@ __device__ __forceinline__ std::uint32_t pack16(float low, float high, bool bf16
     return *reinterpret_cast<const std::uint32_t*>(&pair);
 }
 
+// This thread's row of FP32 numbers as three BF16 matrices with room for whole tiles.
+__device__ __forceinline__ void storePlanes(const ProductParams& p, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, float scale, bool on, const float (&v)[128]) {
+    unsigned char* const out = static_cast<unsigned char*>(p.slopes) + (static_cast<std::uint64_t>(row) * p.slopes_pitch + col) * 2;
+#pragma unroll
+    for (int j = 0; j < 128; j += 16) {
+        if (j < 64 || pieces == 4) {
+            std::uint32_t packed[kPlanes][8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float low[kPlanes], high[kPlanes];
+                training::splitPlanes(on ? scale * v[j + 2 * i] : 0.0F, low);
+                training::splitPlanes(on ? scale * v[j + 2 * i + 1] : 0.0F, high);
+#pragma unroll
+                for (std::uint32_t plane = 0; plane < kPlanes; ++plane) { packed[plane][i] = pack16(low[plane], high[plane], true); }
+            }
+#pragma unroll
+            for (std::uint32_t plane = 0; plane < kPlanes; ++plane) { storeGlobal8(out + 2 * (plane * p.slopes_plane + j), packed[plane]); }
+        }
+    }
+}
+
 // This thread's row of a 16-bit matrix that has room for whole tiles; what lies beyond the columns is never fetched.
 __device__ __forceinline__ void storeRow(const ProductParams& p, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, float scale, bool on, bool bf16,
                                          const float (&v)[128]) {
@@ -250,7 +284,19 @@ __device__ __forceinline__ void finishStatistics(const ProductParams& p, const I
     }
     const std::uint32_t piece = 2 * (w.col / p.problem[0].tile_n) + half;
     p.partials[static_cast<std::uint64_t>(piece) * p.capacity + row] = make_float2(none ? -INFINITY : base, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-    if (kKeep) { storeRow(p, row, col, pieces, kKeptScale, true, false, v); }
+    if (kKeep && p.terms == 1) { storeRow(p, row, col, pieces, kKeptScale, true, false, v); }
+    if (kKeep && p.terms != 1) {
+        float* const out = static_cast<float*>(p.slopes) + static_cast<std::uint64_t>(row) * p.slopes_pitch + col;
+#pragma unroll
+        for (int j = 0; j < 128; j += 8) {
+            if (j < 64 || pieces == 4) {
+                float o[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { o[i] = v[j + i]; }
+                storeGlobal8(out + j, o);
+            }
+        }
+    }
 }
 
 __device__ __forceinline__ void finishSlopes(const ProductParams& p, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, std::uint32_t live,
@@ -266,7 +312,11 @@ __device__ __forceinline__ void finishSlopes(const ProductParams& p, std::uint32
 #pragma unroll
         for (int j = 0; j < 128; ++j) { v[j] = j == at ? v[j] - 1.0F : v[j]; }
     }
-    storeRow(p, row, col, pieces, scale, on, p.bf16 != 0, v);
+    if (p.terms == 1) {
+        storeRow(p, row, col, pieces, scale, on, p.bf16 != 0, v);
+    } else {
+        storePlanes(p, row, col, pieces, scale, on, v);
+    }
 }
 
 __device__ __forceinline__ void finishSums(const ProductParams& p, const Item& w, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, float (&v)[128]) {
@@ -394,32 +444,34 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
         const float unit              = kMode == kGradients ? *p.rows.unit : 1.0F;
         std::uint32_t sums = 0;
         bool ok = true;
-        for (std::uint32_t item; ok && (item = itemOf(work, pair, pairs, sums)) != kNoItem; ++sums) {
+        for (std::uint32_t n = 0, item; ok && (item = itemOf(work, pair, pairs, n)) != kNoItem; ++n) {
             const Item w                 = decode(p, work, item);
             const Problem& problem       = p.problem[w.problem];
             const std::uint32_t pieces   = problem.tile_n / 64;  // of 32 columns, for this warp
-            const std::uint32_t which    = sums & 1;
             const std::uint32_t row      = w.row + rank * 128 + in_tile + lane;
             const std::uint32_t col      = w.col + half * 32 * pieces;
-            ok = mbarrierWait(&bars->sum_full[which], (sums >> 1) & 1, abort_flag);
-            if (!ok) { break; }
-            tcgen05FenceAfterSync();
             float v[128];
 #pragma unroll
-            for (std::uint32_t q = 0; q < 4; ++q) {
-                if (q < pieces) {
-                    float part[32];
-                    tmemLoad32(tmem_row + which * kTileN + half * 32 * pieces + q * 32, part);
+            for (int j = 0; j < 128; ++j) { v[j] = 0.0F; }
+            for (std::uint32_t kb = 0; kb < w.blocks; kb += min(p.chunk, w.blocks - kb), ++sums) {
+                const std::uint32_t which = sums & 1;
+                ok = mbarrierWait(&bars->sum_full[which], (sums >> 1) & 1, abort_flag);
+                if (!ok) { break; }
+                tcgen05FenceAfterSync();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) { v[q * 32 + j] = part[j]; }
-                } else {
+                for (std::uint32_t q = 0; q < 4; ++q) {
+                    if (q < pieces) {
+                        float part[32];
+                        tmemLoad32(tmem_row + which * kTileN + half * 32 * pieces + q * 32, part);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) { v[q * 32 + j] = 0.0F; }
+                        for (int j = 0; j < 32; ++j) { v[q * 32 + j] += part[j]; }
+                    }
                 }
+                tcgen05FenceBeforeSync();
+                __syncwarp();
+                if (lane == 0) { mbarrierArriveCluster(sum_empty[which]); }
             }
-            tcgen05FenceBeforeSync();
-            __syncwarp();
-            if (lane == 0) { mbarrierArriveCluster(sum_empty[which]); }
+            if (!ok) { break; }
             if (kMode == kStatistics) {
                 finishStatistics<false>(p, w, row, col, pieces, half, live, v);
             } else if (kMode == kKept) {
@@ -457,16 +509,22 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
                     const std::int32_t step_x = along ? 0 : static_cast<std::int32_t>(kBlockK), step_y = along ? static_cast<std::int32_t>(kBlockK) : 0;
                     const std::uint32_t bytes    = 2 * (kOperandBytes + problem.tile_n / 2 * 128);
                     std::int32_t x = along ? row : first, y = along ? first : row;
-                    for (std::uint32_t kb = 0; kb < w.blocks; ++kb, ++filled, ring.next()) {
+                    const std::uint32_t terms = p.terms, loads = w.blocks * terms, planes = terms == 1 ? 0 : second ? kTermsB : kTermsA;
+                    std::uint32_t term        = 0;
+                    for (std::uint32_t load = 0; load < loads; ++load, ++filled, ring.next()) {
+                        const std::int32_t plane = static_cast<std::int32_t>(planes >> (4 * term) & 0xF);
                         ok = mbarrierWait(&bars->empty[ring.slot], (ring.round & 1) ^ 1, abort_flag);
                         if (!ok) { break; }
                         // The bytes of both CTAs count on the first CTA's barrier, which that CTA arms. (The other's
                         // may land first: the phase cannot complete before it has been armed.)
                         if (arms) { mbarrierArriveExpectTx(&bars->full[ring.slot], bytes); }
-                        tmaLoad2dPair(to + ring.slot * kStageBytes, map, full + ring.slot * 8, x, y);
-                        if (two) { tmaLoad2dPair(to + ring.slot * kStageBytes + kBoxBytes, map, full + ring.slot * 8, x + 64, y); }
-                        x += step_x;
-                        y += step_y;
+                        tmaLoad3dPair(to + ring.slot * kStageBytes, map, full + ring.slot * 8, x, y, plane);
+                        if (two) { tmaLoad3dPair(to + ring.slot * kStageBytes + kBoxBytes, map, full + ring.slot * 8, x + 64, y, plane); }
+                        if (++term == terms) {
+                            term = 0;
+                            x += step_x;
+                            y += step_y;
+                        }
                     }
                 }
                 // Neither CTA leaves before the last commits have arrived on its barriers.
@@ -485,7 +543,7 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
             Ring ring;
             std::uint32_t sums = 0;
             bool ok            = true;
-            for (std::uint32_t item; ok && (item = itemOf(work, pair, pairs, sums)) != kNoItem; ++sums) {
+            for (std::uint32_t n = 0, item; ok && (item = itemOf(work, pair, pairs, n)) != kNoItem; ++n) {
                 const Item w           = decode(p, work, item);
                 const Problem& problem = p.problem[w.problem];
                 const bool a_mn = problem.a_along_rows != 0, b_mn = problem.b_along_rows != 0;
@@ -495,28 +553,32 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
                 const std::uint64_t a_step = a_mn ? 16 * 128 >> 4 : 2, b_step = b_mn ? 16 * 128 >> 4 : 2;
                 const std::uint32_t instruction =
                     p.instruction | umaInstructionF16(kTileRows, problem.tile_n) | (a_mn ? kUmaAMnMajor : 0) | (b_mn ? kUmaBMnMajor : 0);
-                const std::uint32_t which = sums & 1;
-                const std::uint32_t d     = tmem_base + which * kTileN;
-                ok = mbarrierWait(&bars->sum_empty[which], ((sums >> 1) & 1) ^ 1, abort_flag);
-                if (!ok) { break; }
-                tcgen05FenceAfterSync();
-                for (std::uint32_t kb = 0; kb < w.blocks; ++kb, ring.next()) {
-                    ok = mbarrierWait(&bars->full[ring.slot], ring.round & 1, abort_flag);
+                for (std::uint32_t kb = 0, blocks; kb < w.blocks && ok; kb += blocks, ++sums) {
+                    blocks                    = min(p.chunk, w.blocks - kb);
+                    const std::uint32_t loads = blocks * p.terms;
+                    const std::uint32_t which = sums & 1;
+                    const std::uint32_t d     = tmem_base + which * kTileN;
+                    ok = mbarrierWait(&bars->sum_empty[which], ((sums >> 1) & 1) ^ 1, abort_flag);
                     if (!ok) { break; }
                     tcgen05FenceAfterSync();
-                    const std::uint64_t a = a0 + ring.slot * stage_step, b = b0 + ring.slot * stage_step;
-                    if (leads) {
+                    for (std::uint32_t load = 0; load < loads; ++load, ring.next()) {
+                        ok = mbarrierWait(&bars->full[ring.slot], ring.round & 1, abort_flag);
+                        if (!ok) { break; }
+                        tcgen05FenceAfterSync();
+                        const std::uint64_t a = a0 + ring.slot * stage_step, b = b0 + ring.slot * stage_step;
+                        if (leads) {
 #pragma unroll
-                        for (std::uint32_t step = 0; step < kBlockK / 16; ++step) {
-                            umaF16Pair(d, a + step * a_step, b + step * b_step, instruction, kb != 0 || step != 0 ? 1U : 0U);
+                            for (std::uint32_t step = 0; step < kBlockK / 16; ++step) {
+                                umaF16Pair(d, a + step * a_step, b + step * b_step, instruction, load != 0 || step != 0 ? 1U : 0U);
+                            }
+                            umaCommitPair(&bars->empty[ring.slot]);
                         }
-                        umaCommitPair(&bars->empty[ring.slot]);
+                        __syncwarp();
                     }
+                    if (!ok) { break; }
+                    if (leads) { umaCommitPair(&bars->sum_full[which]); }
                     __syncwarp();
                 }
-                if (!ok) { break; }
-                if (leads) { umaCommitPair(&bars->sum_full[which]); }
-                __syncwarp();
             }
             if (!ok && leads) {
                 *abort_flag = 1;
@@ -561,8 +623,9 @@ std::uint32_t tileColumns(std::uint32_t columns) { return columns <= 128 ? 128 :
 
 // An operand whose rows (of the product) are `rows` and whose depth is `k`: neighbours along K, or along the rows.
 bool encodeOperand(CUtensorMap* map, const ProductCall& call, Matrix16 matrix, bool along_rows, std::uint32_t rows, std::uint32_t k, std::uint32_t tile_rows) {
-    return along_rows ? encodeMap16(map, call.bf16, matrix.at, rows, k, matrix.pitch * 2, 64, call.message, call.message_capacity)
-                      : encodeMap16(map, call.bf16, matrix.at, k, rows, matrix.pitch * 2, tile_rows, call.message, call.message_capacity);
+    const std::uint64_t planes = call.planes ? kPlanes : 1, apart = call.planes ? matrix.plane * 2 : matrix.pitch * 2;
+    return along_rows ? encodeMap16(map, call.bf16, matrix.at, rows, k, planes, matrix.pitch * 2, apart, 64, call.message, call.message_capacity)
+                      : encodeMap16(map, call.bf16, matrix.at, k, rows, planes, matrix.pitch * 2, apart, tile_rows, call.message, call.message_capacity);
 }
 
 template<int kMode> cudaError_t launch(const ProductCall& call, const ProductMaps& maps, const ProductParams& p, std::uint64_t items) {
@@ -578,6 +641,8 @@ ProductParams paramsFor(const ProductCall& call) {
     p.band           = 16;
     p.instruction    = call.bf16 ? kUmaBf16 : 0;
     p.bf16           = call.bf16 ? 1 : 0;
+    p.terms          = call.planes ? kTerms : 1;
+    p.chunk          = call.planes ? kFp32Blocks : 0xFFFFFFFFU;
     p.capacity       = call.capacity;
     p.rows           = call.rows;
     p.status         = call.status;
@@ -587,6 +652,7 @@ ProductParams paramsFor(const ProductCall& call) {
 
 // Z = H W^T over `columns` rows of the weight.
 bool describeLogits(const ProductCall& call, Matrix16 weight, std::uint32_t columns, ProductMaps& maps, ProductParams& p) {
+    if (!call.planes) { p.chunk = kLogitBlocks; }
     Problem& problem          = p.problem[0];
     problem.columns           = columns;
     problem.tile_n            = tileColumns(columns);
@@ -621,12 +687,14 @@ cudaError_t launchKept(const ProductCall& call, Matrix16 weight, std::uint32_t v
     return launch<kKept>(call, maps, p, static_cast<std::uint64_t>(call.capacity / kTileRows) * p.problem[0].tiles_n);
 }
 
-cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, std::uint64_t slopes_pitch) {
+cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, std::uint64_t slopes_pitch,
+                         std::uint64_t slopes_plane) {
     ProductMaps maps;
     ProductParams p = paramsFor(call);
     p.first         = first;
     p.slopes        = slopes;
     p.slopes_pitch  = slopes_pitch;
+    p.slopes_plane  = slopes_plane;
     if (!describeLogits(call, weight, columns, maps, p)) { return cudaErrorInvalidValue; }
     return launch<kSlopes>(call, maps, p, static_cast<std::uint64_t>(call.capacity / kTileRows) * p.problem[0].tiles_n);
 }
@@ -640,12 +708,10 @@ std::uint32_t hiddenSplits(std::uint32_t capacity, std::uint32_t depth, std::uin
     return divideUp(blocks, divideUp(blocks, wanted));  // none of them empty
 }
 
-cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint32_t columns, const void* slopes, std::uint64_t slopes_pitch,
-                            const Gradients& gradients) {
+cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint32_t columns, Matrix16 slopes, const Gradients& gradients) {
     ProductMaps maps;
     ProductParams p = paramsFor(call);
     p.problems      = 0;
-    const Matrix16 slope_matrix{slopes, slopes_pitch};
     std::uint64_t items        = 0;
     const std::uint32_t tile_n = tileColumns(call.depth), tiles_n = divideUp(call.depth, tile_n);
     bool encoded = true;
@@ -661,7 +727,7 @@ cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint3
         p.sums                    = gradients.sums;
         p.sums_pitch              = gradients.sums_pitch;
         p.accumulate              = gradients.accumulate ? 1 : 0;
-        encoded = encodeOperand(&maps.a[p.problems], call, slope_matrix, false, call.capacity, columns, 128) &&
+        encoded = encodeOperand(&maps.a[p.problems], call, slopes, false, call.capacity, columns, 128) &&
                   encodeOperand(&maps.b[p.problems], call, weight, true, call.depth, columns, 64);
         items += static_cast<std::uint64_t>(call.capacity / kTileRows) * tiles_n * problem.splits;
         ++p.problems;
@@ -684,7 +750,7 @@ cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint3
             return call.depth % n == 0 && gradients.weight_gradient_pitch % n == 0 && training::aligned(gradients.weight_gradient, bytes * n);
         };
         p.weight_vector = !gradients.weight_gradient_fp32 && fits(16) ? 16 : fits(8) ? 8 : 1;
-        encoded = encodeOperand(&maps.a[p.problems], call, slope_matrix, true, columns, call.capacity, 128) &&
+        encoded = encodeOperand(&maps.a[p.problems], call, slopes, true, columns, call.capacity, 128) &&
                   encodeOperand(&maps.b[p.problems], call, call.hidden, true, call.depth, call.capacity, 64);
         items += static_cast<std::uint64_t>(divideUp(columns, kTileRows)) * tiles_n;
         ++p.problems;

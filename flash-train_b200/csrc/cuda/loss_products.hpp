@@ -1,4 +1,4 @@
-// The products of the linear cross entropy on 16-bit operands (loss_products.cu), as linear_cross_entropy.cu calls them.
+// The products of the linear cross entropy on the tensor cores (loss_products.cu), as linear_cross_entropy.cu calls them.
 #ifndef FTCUDA_LOSS_PRODUCTS_HPP_
 #define FTCUDA_LOSS_PRODUCTS_HPP_
 
@@ -27,14 +27,20 @@ struct LiveRows {
 };
 constexpr std::int32_t kBadTarget = -2;
 
-// A matrix of 16-bit elements in memory, rows of neighbours.
+// A matrix of 16-bit elements in memory, rows of neighbours; or an FP32 matrix as three of them, whose sum it is (kPlanes).
 struct Matrix16 {
     const void* at;
     std::uint64_t pitch;  // elements between rows
+    std::uint64_t plane;  // elements between matrices; any for one
 };
+
+// An FP32 number is the sum of three BF16 ones to within its own rounding: x = h + m + l, h = bf16(x), m = bf16(x - h), l = bf16(x - h - m), whatever
+// its exponent. Of the nine products of two such sums, six are 2^-16 or more of the whole.
+constexpr std::uint32_t kPlanes = 3;
 
 struct ProductCall {
     bool bf16;
+    bool planes;              // FP32 operands, as kPlanes BF16 matrices each; the slopes come and go the same way, all other results are FP32
     std::uint32_t capacity;   // rows that the live arrays have room for, a multiple of kTileRows
     std::uint32_t depth;      // elements of a hidden state
     LiveRows rows;
@@ -54,14 +60,15 @@ std::uint32_t statisticsPieces(std::uint32_t columns);
 // partials[piece][capacity]; and the target's logit to rows.picked.
 cudaError_t launchStatistics(const ProductCall& call, Matrix16 weight, std::uint32_t vocabulary, float2* partials);
 
-// slopes[row][column - first] = scale (2^(logit log2 e - lse2) - [column is the target]) for `columns` columns from `first` on;
-// `weight` starts at row `first`. The pitch is a multiple of 256.
-cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, std::uint64_t slopes_pitch);
-
-// The same, and kept[row][column] = 2^(logit log2 e - its piece's largest), times kKeptScale, in FP16 whatever the operands' type: against the
-// largest of its piece a number needs no more range, and BF16 would round 2^3 times as much. The pitch is a multiple of 256.
+// The same, and kept[row][column] = 2^(logit log2 e - its piece's largest): FP32 for FP32 operands, else times kKeptScale in FP16 whatever the
+// operands' type: against the largest of its piece a number needs no more range, and BF16 would round 2^3 times as much. The pitch is a multiple of 256.
 constexpr float kKeptScale = 8192.0F;
 cudaError_t launchKept(const ProductCall& call, Matrix16 weight, std::uint32_t vocabulary, float2* partials, void* kept, std::uint64_t kept_pitch);
+
+// slopes[row][column - first] = scale (2^(logit log2 e - lse2) - [column is the target]) for `columns` columns from `first` on;
+// `weight` starts at row `first`. The pitch is a multiple of 256.
+cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, std::uint64_t slopes_pitch,
+                         std::uint64_t slopes_plane);
 
 // How many parts the sum over `columns` columns is cut into for the gradient of the hidden states. (Over fewer columns
 // launchGradients may fill fewer of them, never more.)
@@ -78,8 +85,7 @@ struct Gradients {
     std::int64_t weight_gradient_pitch;
     bool weight_gradient_fp32;  // or of the operands' type
 };
-cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint32_t columns, const void* slopes, std::uint64_t slopes_pitch,
-                            const Gradients& gradients);
+cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint32_t columns, Matrix16 slopes, const Gradients& gradients);
 
 }  // namespace loss
 }  // namespace ftcuda

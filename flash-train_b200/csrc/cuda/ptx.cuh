@@ -462,15 +462,6 @@ __device__ __forceinline__ void tmaLoad3dPair(void* smem_destination, const void
         : "memory");
 }
 
-// The same for a 2-D tile; x * the element's size must be a multiple of 16 bytes.
-__device__ __forceinline__ void tmaLoad2dPair(void* smem_destination, const void* tensor_map, std::uint32_t barrier, std::int32_t x, std::int32_t y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(smemAddress(smem_destination)),
-        "l"(reinterpret_cast<std::uint64_t>(tensor_map)), "r"(barrier), "r"(x), "r"(y)
-        : "memory");
-}
-
 // Shared-memory operand descriptor for an MN-major tile of 16-bit elements with the 128-byte swizzle: rows of 128 bytes hold 64
 // consecutive MN elements at one k; eight consecutive k form a swizzle atom of 1024 bytes (what a TMA load of a box of 64 (MN) x 8j (K)
 // leaves, j atoms one after another). `mn_atom_bytes` is the distance to the next 64 MN elements ("leading" offset, bits

@@ -31,6 +31,21 @@ template<> struct Element<__nv_bfloat16> {
     static __device__ __forceinline__ __nv_bfloat16 narrow(float x) { return __float2bfloat16_rn(x); }
 };
 
+// An FP32 number as three BF16 ones, x = h + m + l to within its own rounding. A number that BF16 would round to infinity has the largest
+// finite h; an infinity has that too, and itself in l, which meets the other operand's h alone in a product: the result is the
+// infinity that FP32 arithmetic gives, or NaN against zero.
+__device__ __forceinline__ void splitPlanes(float x, float (&parts)[3]) {
+    constexpr float kLargest = 3.38953138925153547590e38F;
+    float high = __bfloat162float(__float2bfloat16_rn(x));
+    if (fabsf(high) > kLargest) { high = copysignf(kLargest, x); }
+    const float rest   = x - high;
+    const float middle = __bfloat162float(__float2bfloat16_rn(rest));
+    const bool bounded = fabsf(rest) <= kLargest;
+    parts[0]           = high;
+    parts[1]           = bounded ? middle : 0.0F;
+    parts[2]           = bounded ? rest - middle : rest;
+}
+
 // Bytes of an element, 0 for a type that the operators do not take.
 inline std::uint64_t elementBytes(std::int32_t element) {
     return element == FTCUDA_ELEMENT_FP32 ? 4 : element == FTCUDA_ELEMENT_FP16 || element == FTCUDA_ELEMENT_BF16 ? 2 : 0;
