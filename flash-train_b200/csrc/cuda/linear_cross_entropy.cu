@@ -380,7 +380,8 @@ template<typename T> __global__ void __launch_bounds__(256) keptSlopes(const Kep
     gridDependencyWait();
     gridDependencyLaunchDependents();
     const std::uint32_t live   = *p.rows.count;
-    const std::uint32_t row0   = blockIdx.y * kKeptRows, piece0 = blockIdx.x * kKeptPieces;
+    const std::uint32_t across = (p.pieces + kKeptPieces - 1) / kKeptPieces;  // CTAs side by side
+    const std::uint32_t row0   = blockIdx.x / across * kKeptRows, piece0 = blockIdx.x % across * kKeptPieces;
     const std::uint32_t padded = (max(live, 1U) + loss::kTileRows - 1) / loss::kTileRows * loss::kTileRows;
     if (row0 >= padded) { return; }
     const std::uint32_t pieces = min(p.pieces - piece0, static_cast<std::uint32_t>(kKeptPieces));
@@ -740,7 +741,7 @@ class Call final {
         } else {
             const KeptParams params{rows_, partials, static_cast<std::uint32_t>(l_.pieces), loss::statisticsWidth(columns), static_cast<std::uint32_t>(l_.capacity),
                                     l_.piece_pitch, slopesPlane()};
-            const dim3 grid(static_cast<unsigned>(ceilDiv(l_.pieces, kKeptPieces)), static_cast<unsigned>(l_.capacity / kKeptRows));
+            const dim3 grid(static_cast<unsigned>(ceilDiv(l_.pieces, kKeptPieces) * (l_.capacity / kKeptRows)));  // (of x, which takes any number)
             const auto kernel = l_.planes ? keptSlopes<float> : q_.element == FTCUDA_ELEMENT_FP16 ? keptSlopes<__half> : keptSlopes<__nv_bfloat16>;
             error             = training::launchOverlapped(kernel, grid, dim3(256), 0, stream_, params, kept, at<std::uint16_t>(l_.piece));
         }

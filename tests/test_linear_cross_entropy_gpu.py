@@ -485,3 +485,11 @@ def test_what_the_step_refuses(ft, capi):
         capi.linear_cross_entropy_step(problem(), out.data_ptr(), 7, 0, 0, 0, 0, workspace.data_ptr(), size)
     with pytest.raises(capi.FTrainError, match="workspace of"):
         capi.linear_cross_entropy_step(problem(), out.data_ptr(), 8, 0, 0, 0, 0, workspace.data_ptr(), size - 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_tokens_of_a_small_vocabulary(ft, dtype):
+    """More rows of 32 than a grid's second dimension takes (FP32: more logits than the step call takes)."""
+    hidden, weight, target = make(32 * 65535 + 1, 8, 3, dtype, seed=14)
+    target[::5] = -100
+    run_and_check(ft, hidden, weight, target, scale=1024.0)
