@@ -936,6 +936,17 @@ const char* checkStep(const FtcudaLinearCrossEntropy& q) {
     return nullptr;
 }
 
+// Memory from an operand's first byte up to its last one.
+struct Extent {
+    std::uintptr_t begin, end;
+};
+Extent extentOf(const void* at, std::uint64_t rows, std::uint64_t cols, std::int64_t stride, std::uint64_t bytes) {
+    const std::uintptr_t begin = reinterpret_cast<std::uintptr_t>(at);
+    if (at == nullptr || rows == 0) { return {0, 0}; }
+    return {begin, begin + ((rows - 1) * static_cast<std::uint64_t>(rows > 1 ? stride : 0) + cols) * bytes};
+}
+bool meet(const Extent& a, const Extent& b) { return a.begin < b.end && b.begin < a.end; }
+
 // nullptr, or what is wrong with where the gradients go. The weight's stride comes out as one that rows can have.
 const char* checkGradients(const FtcudaLinearCrossEntropy& q, std::uint64_t bytes, const void* grad_hidden, std::int64_t hidden_stride, const void* grad_weight,
                            std::int64_t& weight_stride) {
@@ -950,7 +961,12 @@ const char* checkGradients(const FtcudaLinearCrossEntropy& q, std::uint64_t byte
         return "the rows of the weight's gradient overlap, or lie too far apart";
     }
     if (q.vocabulary == 1) { weight_stride = depth; }
-    return nullptr;
+    const Extent hidden_out = extentOf(grad_hidden, q.tokens, q.depth, hidden_stride, bytes), weight_out = extentOf(grad_weight, q.vocabulary, q.depth, weight_stride, bytes);
+    const Extent in[]       = {extentOf(q.hidden, q.tokens, q.depth, q.hidden_row_stride, training::elementBytes(q.element)),
+                               extentOf(q.weight, q.vocabulary, q.depth, q.weight_row_stride, training::elementBytes(q.element)), extentOf(q.target, 1, q.tokens, 0, 8)};
+    bool apart = !meet(hidden_out, weight_out);
+    for (const Extent& operand : in) { apart = apart && !meet(hidden_out, operand) && !meet(weight_out, operand); }
+    return apart ? nullptr : "a gradient lies across the other one or an operand";
 }
 
 int workspaceBytes(const FtcudaLinearCrossEntropy* problem, Form form, std::uint64_t* bytes, char* message, std::size_t capacity) {

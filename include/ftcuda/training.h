@@ -69,7 +69,8 @@ FTCUDA_API int ftcuda_linear_cross_entropy(const FtcudaLinearCrossEntropy* probl
 
 /*
  * The gradients of hidden and weight, each of the operands' type and dense along the depth; either may be NULL (not wanted).
- * grad_loss: FP32 on the device, in the loss's shape. They are written, not added to.
+ * grad_loss: FP32 on the device, in the loss's shape. They are written, not added to. From its first byte to its last one, a gradient's memory may
+ * not meet the other's or an operand's (refused).
  */
 FTCUDA_API int ftcuda_linear_cross_entropy_backward(const FtcudaLinearCrossEntropy* problem, const float* lse, const float* grad_loss, void* grad_hidden,
                                                     int64_t grad_hidden_row_stride, void* grad_weight, int64_t grad_weight_row_stride,

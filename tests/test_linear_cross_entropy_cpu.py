@@ -39,3 +39,31 @@ def test_addresses_that_cannot_be(capi):
     refuse(capi, "a gradient's address", back, q, 0x40000000, 0x50000000, 0x70000000, 64, 0x80000001, 64, 0x60000000, 1 << 40)
     refuse(capi, "hidden states' gradient overlap", back, q, 0x40000000, 0x50000000, 0x70000000, 63, 0x80000000, 64, 0x60000000, 1 << 40)
     refuse(capi, "weight's gradient overlap", back, q, 0x40000000, 0x50000000, 0x70000000, 64, 0x80000000, 63, 0x60000000, 1 << 40)
+
+
+@pytest.mark.parametrize("grad_hidden, grad_weight", [(0x10000000, 0x80000000), (0x70000000, 0x20000000), (0x10000000 + 12798, 0), (0, 0x20000000 + 127998),
+                                                      (0x70000000, 0x70000000 + 12798), (0x70000000, 0x30000000), (0x30000000 - 12798, 0)])
+def test_gradients_across_other_memory(capi, grad_hidden, grad_weight):
+    q = problem(capi)
+    refuse(capi, "lies across", capi.linear_cross_entropy_backward, q, 0x40000000, 0x50000000, grad_hidden, 64, grad_weight, 64, 0x60000000, 1 << 40)
+    refuse(capi, "lies across", capi.linear_cross_entropy_step, q, 0x40000000, 8, grad_hidden, 64, grad_weight, 64, 0x60000000, 1 << 40)
+
+
+@pytest.mark.parametrize("change, reason", [
+    ({"reduction": 0}, "without reduction"), ({"tokens": 0}, "no tokens"), ({"tokens": 1 << 16, "vocabulary": 1 << 15}, "2 GiB"), ({"element": 1}, "FP32, FP16 or BF16"),
+    ({"hidden": None}, "hidden states have no address"), ({"weight_row_stride": 1}, "weight's rows overlap"),
+])
+def test_what_the_step_does_not_take(capi, change, reason):
+    q = problem(capi, **change)
+    refuse(capi, reason, capi.linear_cross_entropy_step, q, 0x40000000, 8, 0x70000000, 64, 0x80000000, 64, 0x60000000, 1 << 40)
+    refuse(capi, reason, capi.linear_cross_entropy_step_workspace_bytes, q)
+
+
+def test_where_the_step_does_not_write(capi):
+    q, step = problem(capi), capi.linear_cross_entropy_step
+    refuse(capi, "operands' type", step, q, 0x40000000, 7, 0x70000000, 64, 0x80000000, 64, 0x60000000, 1 << 40)
+    refuse(capi, "the loss has no address", step, q, 0, 8, 0x70000000, 64, 0x80000000, 64, 0x60000000, 1 << 40)
+    refuse(capi, "the loss has no address", step, q, 0x40000001, 8, 0x70000000, 64, 0x80000000, 64, 0x60000000, 1 << 40)
+    refuse(capi, "a gradient's address", step, q, 0x40000000, 4, 0x70000002, 64, 0x80000000, 64, 0x60000000, 1 << 40)
+    refuse(capi, "hidden states' gradient overlap", step, q, 0x40000000, 8, 0x70000000, 63, 0x80000000, 64, 0x60000000, 1 << 40)
+    refuse(capi, "weight's gradient overlap", step, q, 0x40000000, 8, 0x70000000, 64, 0x80000000, -64, 0x60000000, 1 << 40)
