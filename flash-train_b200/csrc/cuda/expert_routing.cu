@@ -468,7 +468,7 @@ template<typename T, int kItems, bool kVector> __global__ void __launch_bounds__
         if (t < p.tokens) {
             Place::load(static_cast<const T*>(p.logits) + static_cast<std::int64_t>(t) * p.row_stride, p.experts, lane, ahead);
             if (lane < static_cast<int>(p.top_k)) {
-                ahead_mine     = p.chosen[t * p.top_k + lane];
+                ahead_mine     = min(p.chosen[t * p.top_k + lane], static_cast<std::int32_t>(p.experts) - 1);  // (never beyond, whatever stands there)
                 ahead_weight   = p.weights[t * p.top_k + lane];
                 ahead_upstream = p.grad_weights != nullptr ? p.grad_weights[t * p.top_k + lane] : 0.0F;
             }
