@@ -10,6 +10,10 @@
 // a maximum over the warp of keys that order as the logits do. Sums over tokens: each lane keeps its experts' p over all of its
 // warp's tokens, a CTA joins its warps and leaves one row of partial sums, and a cluster of eight CTAs adds the rows up; the counts are whole
 // numbers in shared memory. One CTA alone (few tokens) finishes by itself, without the second launch.
+//
+// What bounds it: with few experts latency and HBM (16384 x 64 FP32, top 8: 21.5 us forward, 12.3 backward, 1.5 us of bytes), with many the forward kernel's
+// whole-number instructions (65535 x 256 BF16, top 8: 52 us forward at 0.69 TB/s, the ALU pipe busy for 70 % of the time), the backward one's latency
+// (32.8 us, 2.2 TB/s).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -29,6 +33,10 @@ using training::Element;
 constexpr int kWarps              = 16;  // of the forward kernel's CTA
 constexpr int kBackwardWarps      = 8;
 constexpr int kCtasPerSm          = 2;
+// CTAs of the backward kernel that an SM holds: where a lane has up to 16 bytes of a row few registers are enough, and more rows are on their way
+// (65535 x 256 BF16: 36.8 us with four, 32.8 with six; 65536 x 128 FP16: 30.7, 24.6). With more, six are no faster (32768 x 256 FP32: 21.2, 22.7; 16384 x 512
+// BF16: 23.0, 24.0).
+__host__ __device__ constexpr int backwardCtasPerSm(std::uint64_t bytes) { return bytes <= 16 ? 6 : 4; }
 constexpr std::uint32_t kMaxExperts = 1024;
 constexpr std::uint32_t kMaxTopK    = 32;
 constexpr std::uint32_t kMaxRows    = 512;  // CTAs of the forward kernel at most
@@ -137,101 +145,121 @@ template<typename T, int kItems, bool kVector> struct Share {
     }
 };
 
-// The largest keys of a warp, one after another, the lowest index first among equal ones. next() gives a key, or false where only -inf is
-// left; value() and index() say what a key stands for.
+// The k largest logits of a warp's row, the lowest index first among equal ones: lane i gets the key of the i-th, and `first` is the first one's. take()
+// gives how many there are above -inf; value() and index() say what a key stands for. A row is -inf beyond the last expert.
 template<typename T, int kItems> struct TopK;
 
 // FP32: a round is two reductions, for the key and for the index.
 template<int kItems> struct TopK<float, kItems> {
     using Key = std::uint64_t;
-    std::uint32_t keys[kItems];
-    template<typename Place> __device__ __forceinline__ void set(const float (&x)[kItems], std::uint32_t experts, int lane) {
+    template<typename Place> static __device__ __forceinline__ std::uint32_t take(const float (&x)[kItems], std::uint32_t top_k, int lane, Key& kept, Key& first) {
+        std::uint32_t keys[kItems];
 #pragma unroll
-        for (int i = 0; i < kItems; ++i) { keys[i] = Place::index(i, lane) < experts ? orderOf(x[i]) : 0; }
-    }
-    template<typename Place> __device__ __forceinline__ bool next(int lane, Key& key) {
-        std::uint32_t best = keys[0];
+        for (int i = 0; i < kItems; ++i) { keys[i] = orderOf(x[i]); }
+        std::uint32_t round = 0;
+        for (; round < top_k; ++round) {
+            std::uint32_t best = keys[0];
 #pragma unroll
-        for (int i = 1; i < kItems; ++i) { best = max(best, keys[i]); }
-        best = __reduce_max_sync(kAll, best);
-        if (best <= kDead) { return false; }
-        std::uint32_t at = 0xFFFFFFFFU;
+            for (int i = 1; i < kItems; ++i) { best = max(best, keys[i]); }
+            best = __reduce_max_sync(kAll, best);
+            if (best <= kDead) { break; }
+            std::uint32_t at = 0xFFFFFFFFU;
 #pragma unroll
-        for (int i = kItems - 1; i >= 0; --i) { at = keys[i] == best ? Place::index(i, lane) : at; }
-        at = __reduce_min_sync(kAll, at);
+            for (int i = kItems - 1; i >= 0; --i) { at = keys[i] == best ? Place::index(i, lane) : at; }
+            at = __reduce_min_sync(kAll, at);
 #pragma unroll
-        for (int i = 0; i < kItems; ++i) { keys[i] = at == Place::index(i, lane) ? 0 : keys[i]; }
-        key = static_cast<Key>(best) << 32 | at;
-        return true;
+            for (int i = 0; i < kItems; ++i) { keys[i] = at == Place::index(i, lane) ? 0 : keys[i]; }
+            const Key key = static_cast<Key>(best) << 32 | at;
+            first         = round == 0 ? key : first;
+            kept          = lane == static_cast<int>(round) ? key : kept;
+        }
+        return round;
     }
     static __device__ __forceinline__ float value(Key key) { return valueOf(static_cast<std::uint32_t>(key >> 32)); }
     static __device__ __forceinline__ std::uint32_t index(Key key) { return static_cast<std::uint32_t>(key); }
 };
 
-// 16 bits: a word holds the number's order and, upside down, its index, and one reduction does a round. No two words are equal. Up to eight
-// words a lane are sorted first, so that a round only looks at each lane's first one, and the lane it belonged to moves its others
-// up; more are gone through in each round.
+// 16 bits: a word holds the number's order and, upside down, its index, and one reduction does a round (65535 x 256, top 8: 60 us with all lanes' words
+// moved and a question after each round, 52 as here). No two words are equal. Up to eight
+// words a lane are sorted first, so that a round only looks at each lane's first one, and the lane it belonged to moves its others up, as many
+// as the rounds to come can ask for; more are gone through in each round. No round asks whether anything is left: what comes behind the last one above -inf
+// is not above it either.
 template<typename T, int kItems> struct TopK {
-    using Key = std::uint32_t;
-    static constexpr bool kSorted = kItems <= 8;
-    static constexpr Key kDead16  = std::is_same<T, __half>::value ? 0x03FFFFFFU : 0x007FFFFFU;  // the largest of -inf
-    Key keys[kItems];
+    using Key = std::int32_t;
+    static constexpr bool kSorted       = kItems <= 8;
+    static constexpr Key kDead16        = (std::is_same<T, __half>::value ? -0x7C010000 : -0x7F810000) | 0xFFFF;  // the largest of -inf
+    static constexpr std::uint32_t kEnd = 8;  // rounds that are written out
     // Adding zero makes -0 the other zero and every NaN the one with all bits but the sign's.
     static __device__ __forceinline__ std::uint32_t bits(T x) {
         const T sum = __hadd(x, Element<T>::narrow(0.0F));
         return *reinterpret_cast<const unsigned short*>(&sum);
     }
-    template<typename Place> __device__ __forceinline__ void set(const T (&x)[kItems], std::uint32_t experts, int lane) {
-#pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-            const std::uint32_t word  = bits(x[i]) << 16;
-            const std::uint32_t order = word ^ (static_cast<std::uint32_t>(static_cast<std::int32_t>(word) >> 31) | 0x80000000U);
-            keys[i] = Place::index(i, lane) < experts ? (order & 0xFFFF0000U) | (0xFFFFU - Place::index(i, lane)) : 0;
-        }
-        if (!kSorted) { return; }
-        // Odd-even merging (Batcher's network).
-#pragma unroll
-        for (int size = 1; size < kItems; size *= 2) {
-#pragma unroll
-            for (int gap = size; gap > 0; gap /= 2) {
-#pragma unroll
-                for (int start = gap % size; start + gap < kItems; start += 2 * gap) {
-#pragma unroll
-                    for (int i = 0; i < gap; ++i) {
-                        if (i + start + gap < kItems && (i + start) / (2 * size) == (i + start + gap) / (2 * size)) {
-                            const Key low = keys[i + start], high = keys[i + start + gap];
-                            keys[i + start]       = max(low, high);
-                            keys[i + start + gap] = min(low, high);
-                        }
-                    }
-                }
-            }
-        }
-    }
-    template<typename Place> __device__ __forceinline__ bool next(int, Key& key) {
+    template<bool kMove> static __device__ __forceinline__ Key next(Key (&keys)[kItems], int moved) {
         Key first = keys[0];
         if (!kSorted) {
 #pragma unroll
             for (int i = 1; i < kItems; ++i) { first = max(first, keys[i]); }
         }
-        key = __reduce_max_sync(kAll, first);
-        if (key <= kDead16) { return false; }
+        const Key key = __reduce_max_sync(kAll, first);
+        if (!kMove) { return key; }
         if (kSorted) {
             const bool mine = first == key;
 #pragma unroll
-            for (int i = 0; i < kItems - 1; ++i) { keys[i] = mine ? keys[i + 1] : keys[i]; }
-            keys[kItems - 1] = mine ? 0 : keys[kItems - 1];
+            for (int i = 0; i < kItems; ++i) {
+                if (i < moved) { keys[i] = mine ? i + 1 < kItems ? keys[i + 1] : INT32_MIN : keys[i]; }
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < kItems; ++i) { keys[i] = keys[i] == key ? 0 : keys[i]; }
+            for (int i = 0; i < kItems; ++i) { keys[i] = keys[i] == key ? INT32_MIN : keys[i]; }
         }
-        return true;
+        return key;
+    }
+    template<typename Place> static __device__ __forceinline__ std::uint32_t take(const T (&x)[kItems], std::uint32_t top_k, int lane, Key& kept, Key& first) {
+        Key keys[kItems];
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const Key word = static_cast<Key>(bits(x[i]) << 16 | (0xFFFFU - Place::index(i, lane)));
+            keys[i]        = word ^ (word >> 31 & 0x7FFF0000);  // negative numbers the other way round
+        }
+        if (kSorted) {
+            // Odd-even merging (Batcher's network).
+#pragma unroll
+            for (int size = 1; size < kItems; size *= 2) {
+#pragma unroll
+                for (int gap = size; gap > 0; gap /= 2) {
+#pragma unroll
+                    for (int start = gap % size; start + gap < kItems; start += 2 * gap) {
+#pragma unroll
+                        for (int i = 0; i < gap; ++i) {
+                            if (i + start + gap < kItems && (i + start) / (2 * size) == (i + start + gap) / (2 * size)) {
+                                const Key low = keys[i + start], high = keys[i + start + gap];
+                                keys[i + start]       = max(low, high);
+                                keys[i + start + gap] = min(low, high);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        kept                = INT32_MIN;
+        std::uint32_t round = 0;
+        const auto note     = [&](Key key) {
+            first = round == 0 ? key : first;
+            kept  = lane == static_cast<int>(round) ? key : kept;
+            ++round;
+        };
+        for (; round + kEnd < top_k;) { note(next<true>(keys, kItems)); }
+#pragma unroll
+        for (std::uint32_t left = kEnd; left > 0; --left) {  // as many as there still can be
+            if (round + left == top_k) { left == 1 ? note(next<false>(keys, 0)) : note(next<true>(keys, static_cast<int>(left) - 1)); }
+        }
+        return static_cast<std::uint32_t>(__popc(__ballot_sync(kAll, kept > kDead16)));
     }
     static __device__ __forceinline__ float value(Key key) {
-        const unsigned short word = static_cast<unsigned short>((key & 0x80000000U) != 0 ? key >> 16 & 0x7FFFU : ~(key >> 16));
+        const unsigned short word = static_cast<unsigned short>((key ^ (key >> 31 & 0x7FFF0000)) >> 16);
         return Element<T>::widen(*reinterpret_cast<const T*>(&word));
     }
-    static __device__ __forceinline__ std::uint32_t index(Key key) { return 0xFFFFU - (key & 0xFFFFU); }
+    static __device__ __forceinline__ std::uint32_t index(Key key) { return 0xFFFFU - (static_cast<std::uint32_t>(key) & 0xFFFFU); }
 };
 
 // e^x, within a few units of the last place for the arguments that a softmax has (|x| 2^-24 more for large ones).
@@ -256,32 +284,26 @@ template<typename T, int kItems, bool kVector> __global__ void __launch_bounds__
 #pragma unroll
     for (int i = 0; i < kItems; ++i) { sums[i] = 0.0F; }
     std::int32_t live = 0;
+    T raw[kItems];  // -inf beyond the last expert
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) { raw[i] = Element<T>::narrow(-INFINITY); }
     const std::uint64_t step = static_cast<std::uint64_t>(gridDim.x) * kWarps;
     for (std::uint64_t token = static_cast<std::uint64_t>(blockIdx.x) * kWarps + warp; token < p.tokens; token += step) {
-        T raw[kItems];
         Place::load(static_cast<const T*>(p.logits) + static_cast<std::int64_t>(token) * p.row_stride, p.experts, lane, raw);
         const bool on = p.mask == nullptr || p.mask[token] != 0;
         std::int32_t mine  = -1;
         float value        = 0.0F, weight = 0.0F;
         if (on) {
-            Top top;
-            top.template set<Place>(raw, p.experts, lane);
             typename Top::Key kept = 0, first = 0;
-            std::uint32_t round    = 0;
-            for (; round < p.top_k; ++round) {
-                typename Top::Key key;
-                if (!top.template next<Place>(lane, key)) { break; }
-                first = round == 0 ? key : first;
-                kept  = lane == static_cast<int>(round) ? key : kept;
-            }
-            if (lane < static_cast<int>(round)) {
+            const std::uint32_t found = Top::template take<Place>(raw, p.top_k, lane, kept, first);
+            if (lane < static_cast<int>(found)) {
                 mine  = static_cast<std::int32_t>(Top::index(kept));
                 value = Top::value(kept);
             }
-            const float largest = round != 0 ? Top::value(first) : -INFINITY;
+            const float largest = found != 0 ? Top::value(first) : -INFINITY;
             float x[kItems];
 #pragma unroll
-            for (int i = 0; i < kItems; ++i) { x[i] = Place::index(i, lane) < p.experts ? Element<T>::widen(raw[i]) : -INFINITY; }
+            for (int i = 0; i < kItems; ++i) { x[i] = Element<T>::widen(raw[i]); }
             if (largest != -INFINITY) {  // (not a number included)
                 float total = 0.0F;
 #pragma unroll
@@ -440,7 +462,7 @@ struct RouteGradient {
     void* grad_logits;
 };
 
-template<typename T, int kItems, bool kVector> __global__ void __launch_bounds__(kBackwardWarps * 32) routeGradient(const RouteGradient p) {
+template<typename T, int kItems, bool kVector> __global__ void __launch_bounds__(kBackwardWarps * 32, backwardCtasPerSm(kItems * sizeof(T)) == 6 ? 6 : 1) routeGradient(const RouteGradient p) {
     using Place = Share<T, kItems, kVector>;
     extern __shared__ unsigned char memory[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -461,7 +483,9 @@ template<typename T, int kItems, bool kVector> __global__ void __launch_bounds__
     // What the next token needs is on its way while this one is worked on.
     const std::uint64_t step = static_cast<std::uint64_t>(gridDim.x) * kBackwardWarps;
     std::uint64_t token      = static_cast<std::uint64_t>(blockIdx.x) * kBackwardWarps + warp;
-    T ahead[kItems];
+    T ahead[kItems];  // -inf beyond the last expert
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) { ahead[i] = Element<T>::narrow(-INFINITY); }
     std::int32_t ahead_mine = -1;
     float ahead_weight = 0.0F, ahead_upstream = 0.0F;
     const auto ask = [&](std::uint64_t t) {
@@ -491,7 +515,7 @@ template<typename T, int kItems, bool kVector> __global__ void __launch_bounds__
         }
         float x[kItems];
 #pragma unroll
-        for (int i = 0; i < kItems; ++i) { x[i] = Place::index(i, lane) < p.experts ? Element<T>::widen(raw[i]) : -INFINITY; }
+        for (int i = 0; i < kItems; ++i) { x[i] = Element<T>::widen(raw[i]); }
         float largest = x[0];
 #pragma unroll
         for (int i = 1; i < kItems; ++i) { largest = fmaxf(largest, x[i]); }
@@ -545,7 +569,7 @@ std::uint32_t forwardRows(std::uint64_t tokens, std::uint32_t sms) {
 }
 
 // One of the kernels' instantiations: by type, experts for each lane, and whether the lanes' runs of experts (two, four, or 16 bytes' worth) are whole
-// and aligned in every row that the call names. (65535 x 256 BF16, top 8, forward: 60 us with runs of eight, 68 one by one.)
+// and aligned in every row that the call names. (65535 x 256 BF16, top 8, forward: 60 us with runs of eight, 68 one by one; 52 since TopK was made shorter.)
 template<template<typename, int, bool> class Pick, typename Kernel> Kernel choose(std::int32_t element, std::uint32_t experts, bool vector) {
     const auto typed = [&](auto sample) -> Kernel {
         using T          = decltype(sample);
@@ -666,7 +690,7 @@ extern "C" int ftcuda_expert_routing_backward(const FtcudaRouting* routing, cons
     p.grad_logits     = grad_logits;
     const auto kernel              = choose<Backward, void (*)(RouteGradient)>(r.element, r.experts, wholeRuns(r.logits, r.tokens, r.row_stride, r.experts, r.element) &&
                                                                                                                          wholeRuns(grad_logits, r.tokens, grad_row_stride, r.experts, r.element));
-    const std::uint32_t grid       = static_cast<std::uint32_t>(std::min<std::uint64_t>(ceilDiv(r.tokens, kBackwardWarps), static_cast<std::uint64_t>(sms) * 4));
+    const std::uint32_t grid       = static_cast<std::uint32_t>(std::min<std::uint64_t>(ceilDiv(r.tokens, kBackwardWarps), static_cast<std::uint64_t>(sms) * backwardCtasPerSm(ceilDiv(r.experts, 32) * training::elementBytes(r.element))));
     const std::size_t shared_bytes = r.experts * 4ULL * kBackwardWarps;
     kernel<<<grid, kBackwardWarps * 32, shared_bytes, static_cast<cudaStream_t>(stream)>>>(p);
     const cudaError_t error = cudaGetLastError();
