@@ -35,15 +35,18 @@ enum {
 
 /*
  * logits[t][v] = hidden[t] . weight[v],  loss[t] = log(sum_v exp(logits[t][v])) - logits[t][target[t]].
- * The logits are never in memory, but for a piece of the vocabulary at a time in the backward call (and, for FP32 operands, the forward
- * call), or, in 16 bits and at most 2 GiB of them, for the time of a step call.
+ * The logits are never all in memory: a piece of the vocabulary's gradients of them at a time is in the backward call (and a piece of FP32 logits in the forward
+ * call where FP32 operands go through the library's products), or, in a step call, their exponentials, at most 2 GiB of them.
  *   - hidden [tokens][depth], weight [vocabulary][depth]: unit stride along the depth, the others any that keep rows apart; both
- *     of one type. BF16 and FP16 are multiplied by the tensor cores with FP32 sums; FP32 by the library's FP32 products.
+ *     of one type. BF16 and FP16 are multiplied by the tensor cores with FP32 sums; FP32 to FP32's precision, as sums of three BF16 matrices (which
+ *     the workspace then holds, six bytes an element of the weight) or by the library's FP32 products, whichever is faster for the sizes.
  *   - target [tokens]: INT64. A token whose target is ignore_index takes no part: its loss and gradient are 0, whatever its hidden
- *     state holds, and (BF16, FP16) nothing is computed for it. Any other target outside of [0, vocabulary) makes the token's loss NaN, and
- *     the gradients too.
+ *     state holds, and but for the library's FP32 products nothing is computed for it. Any other target outside of [0, vocabulary) makes the token's loss
+ *     NaN, and the gradients too.
+ *   - infinities and NaN in what takes part reach the token's loss and the gradients as NaN (a logit of -inf is a probability of 0).
  *   - a gradient's rounding: with BF16 and FP16 operands the logits' gradients are rounded to that type before they are
- *     multiplied, at a scale that keeps FP16's range, and the products' sums once at the end.
+ *     multiplied, at a scale that keeps FP16's range, and the products' sums once at the end. In the step call their exponentials are FP16 before that,
+ *     against the largest of 128 neighbours.
  * Sums are in an order that depends on the sizes and on which tokens take part alone: equal calls give equal bits.
  */
 typedef struct {
@@ -130,8 +133,8 @@ FTCUDA_API int ftcuda_gradient_scale(const FtcudaGradient* gradients, uint64_t c
 
 /*
  * The loss, and the gradients for an upstream gradient of 1, in one call that computes the logits once: three quarters of the work of the
- * two calls above. Their exponentials (FP32: the logits) are in the workspace meanwhile. With a reduction only, and only where they take at most
- * 2 GiB; ftcuda_linear_cross_entropy_step_workspace_bytes answers with a failure where that is not so.
+ * two calls above. Their exponentials (FP32: the logits, or exponentials and slopes, 10 bytes each) are in the workspace meanwhile. With a reduction only, and
+ * only where they take at most 2 GiB; ftcuda_linear_cross_entropy_step_workspace_bytes answers with a failure where that is not so.
  * grad_element: the operands' type, or FP32, for a caller that multiplies by an upstream gradient afterwards and wants nothing rounded (or, with
  * FP16, lost) before. Either gradient may be NULL.
  */
@@ -180,7 +183,8 @@ FTCUDA_API int ftcuda_expert_routing(const FtcudaRouting* routing, float* weight
 
 /*
  * grad_logits (of the logits' type, grad_row_stride elements between tokens) from grad_weights (FP32 [tokens][top_k], dense) and *grad_loss (one FP32 on the
- * device), either of which may be NULL, meaning zero; the other arguments as the forward call took and left them. Needs no workspace.
+ * device), either of which may be NULL, meaning zero; the other arguments as the forward call took and left them (an expert's number beyond the last one
+ * is taken for the last one). grad_logits may be the logits themselves, with their stride; otherwise it may not meet what the call reads. Needs no workspace.
  */
 FTCUDA_API int ftcuda_expert_routing_backward(const FtcudaRouting* routing, const float* weights, const int32_t* experts, const int32_t* counts,
                                               const int32_t* routed, const float* grad_weights, const float* grad_loss,

@@ -296,3 +296,42 @@ def test_refusals(ft):
     ]:
         with pytest.raises(RuntimeError, match=reason):
             call()
+
+
+def test_another_device_than_the_current_one(ft, capi):
+    x, out = make(10, 16, torch.float32), torch.empty(1 << 20, device="cuda")
+    r = capi.Routing(logits=x.data_ptr(), mask=None, tokens=10, row_stride=16, experts=16, top_k=2, normalize=1, element=4, device=1)
+    weights, experts, counts, routed, loss, workspace, gw, gl, gx = (out.data_ptr() + 65536 * i for i in range(9))
+    with pytest.raises(capi.FTrainError, match="device 1 must be current"):
+        capi.expert_routing(r, weights, experts, counts, routed, loss, workspace, 65536)
+    with pytest.raises(capi.FTrainError, match="device 1 must be current"):
+        capi.expert_routing_backward(r, weights, experts, counts, routed, gw, gl, gx, 16)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("experts, k", [(40, 3), (256, 8), (1000, 20)])
+def test_gradient_over_the_logits_themselves(ft, capi, dtype, experts, k):
+    """grad_logits may be the logits, with their stride."""
+    tokens, code = 3001, {torch.float32: 4, torch.float16: 7, torch.bfloat16: 8}[dtype]
+    x = make(tokens, experts, dtype, seed=8)
+    routing = ft.expert_routing(x, k)
+    r = capi.Routing(logits=x.data_ptr(), mask=None, tokens=tokens, row_stride=experts, experts=experts, top_k=k, normalize=1, element=code, device=0)
+    routed = torch.tensor(tokens, dtype=torch.int32, device="cuda")
+    gw, gl = torch.randn(tokens, k, device="cuda"), torch.tensor(0.5, device="cuda")
+    apart = torch.empty_like(x)
+    for to in (apart, x):
+        capi.expert_routing_backward(r, routing.weights.data_ptr(), routing.experts.data_ptr(), routing.counts.data_ptr(), routed.data_ptr(), gw.data_ptr(), gl.data_ptr(),
+                                     to.data_ptr(), experts, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(apart, x) and torch.isfinite(x).all() and x.any()
+
+
+def test_slots_that_nothing_takes_with_many_rounds(ft):
+    """More slots than experts that can be chosen, below and above the rounds that are written out one by one."""
+    for dtype in TYPES:
+        for experts, k in ((40, 32), (256, 8), (256, 9), (600, 20)):
+            x = make(77, experts, dtype, seed=k)
+            x[:, torch.randperm(experts, device="cuda")[: experts - 5]] = -math.inf
+            x[5] = -math.inf
+            x[6, 3:] = -math.inf
+            run_and_check(ft, x, k)

@@ -290,3 +290,11 @@ def test_lists_that_fill_a_launch(ft, count, apart):
         check_clipped(g, original, norm, 1.0)
         if apart and i % 2:
             assert torch.equal(wide[i][0][:, 4:], wide[i][1][:, 4:])
+
+
+def test_another_device_than_the_current_one(ft, capi):
+    g, out = torch.ones(100, device="cuda"), torch.empty(1 << 16, device="cuda")
+    gradients = [capi.Gradient(data=g.data_ptr(), out=g.data_ptr(), rows=1, cols=100, row_stride=0, out_row_stride=0, element=4, out_element=4)]
+    with pytest.raises(capi.FTrainError, match="device 1 must be current"):
+        capi.gradient_scale(gradients, out.data_ptr(), device=1)
+    assert (g == 1).all()

@@ -493,3 +493,61 @@ def test_many_tokens_of_a_small_vocabulary(ft, dtype):
     hidden, weight, target = make(32 * 65535 + 1, 8, 3, dtype, seed=14)
     target[::5] = -100
     run_and_check(ft, hidden, weight, target, scale=1024.0)
+
+
+def test_another_device_than_the_current_one(ft, capi):
+    hidden, weight, target = make(10, 16, 20, torch.bfloat16)
+    q = capi.LinearCrossEntropy(hidden=hidden.data_ptr(), weight=weight.data_ptr(), target=target.data_ptr(), tokens=10, vocabulary=20, depth=16, hidden_row_stride=16,
+                                weight_row_stride=16, ignore_index=-100, element=8, reduction=1, device=1)
+    out = torch.empty(1 << 20, device="cuda")
+    loss, lse, grad_loss, dh, dw, workspace = (out.data_ptr() + 65536 * i for i in range(6))
+    with pytest.raises(capi.FTrainError, match="device 1 must be current"):
+        capi.linear_cross_entropy(q, loss, lse, workspace, 1 << 21)
+    with pytest.raises(capi.FTrainError, match="device 1 must be current"):
+        capi.linear_cross_entropy_backward(q, lse, grad_loss, dh, 16, dw, 16, workspace, 1 << 21)
+    with pytest.raises(capi.FTrainError, match="device 1 must be current"):
+        capi.linear_cross_entropy_step(q, loss, 8, dh, 16, dw, 16, workspace, 1 << 21)
+
+
+def test_two_calls_at_once(ft):
+    """Two streams, each with its own workspace from the allocator; and in one process two threads' backward passes."""
+    cases = [make(700, 256, 5000, torch.bfloat16, seed=30), make(300, 128, 9001, torch.float16, seed=31), make(400, 96, 3001, torch.float32, seed=32)]
+    alone = [run(ft, *case) for case in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        together = []
+        for case, stream in zip(cases, streams):
+            with torch.cuda.stream(stream):
+                together.append(run(ft, *case))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for one, other in zip(alone, together) for a, b in zip(one, other))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_graphs_with_a_pool_in_common(ft, dtype):
+    """Captured one after the other into one memory pool, so that the second one's workspace may be the first one's; replayed in turn and after new inputs."""
+    hidden, weight, target = make(300, 96, 2000, dtype, seed=33)
+    inputs = [tuple(x.clone() for x in (hidden, weight, target)) for _ in range(2)]
+    leaves = [(h.requires_grad_(), w.requires_grad_(), t) for h, w, t in inputs]
+    pool, graphs, results = torch.cuda.graph_pool_handle(), [], []
+    for h, w, t in leaves:
+        torch.autograd.grad(ft.linear_cross_entropy(h, w, t), (h, w))
+    torch.cuda.synchronize()
+    for h, w, t in leaves:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            loss = ft.linear_cross_entropy(h, w, t)
+            results.append((loss.detach(), *torch.autograd.grad(loss, (h, w))))
+        graphs.append(graph)
+    for seed in (40, 41):
+        for i, (h, w, t) in enumerate(leaves):
+            fresh = make(300, 96, 2000, dtype, seed=seed + 10 * i)
+            with torch.no_grad():
+                h.copy_(fresh[0]), w.copy_(fresh[1])
+            t.copy_(fresh[2])
+            t[::3 + i] = -100
+            graphs[i].replay()
+            got = [x.clone() for x in results[i]]
+            expected = run(ft, h.detach(), w.detach(), t)
+            assert all(torch.equal(a, b) for a, b in zip(got, expected))
