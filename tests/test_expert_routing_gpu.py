@@ -335,3 +335,22 @@ def test_slots_that_nothing_takes_with_many_rounds(ft):
             x[5] = -math.inf
             x[6, 3:] = -math.inf
             run_and_check(ft, x, k)
+
+
+def test_logits_past_32_bits(ft):
+    """More than 2^32 logits: the last tokens come out as they do alone, and every slot is counted."""
+    tokens, experts, k = (1 << 22) + 1001, 1024, 4
+    x = torch.empty(tokens, experts, device="cuda", dtype=torch.bfloat16)
+    for piece in x.split(1 << 18):
+        piece.copy_(torch.randn(piece.shape, device="cuda"))
+    x.requires_grad_()
+    tail = x.detach()[-3000:].clone().requires_grad_()
+    routing, alone = ft.expert_routing(x, k), ft.expert_routing(tail, k)
+    assert torch.equal(routing.experts[-3000:], alone.experts) and torch.equal(routing.weights[-3000:], alone.weights)
+    assert torch.equal(routing.counts.long(), torch.bincount(routing.experts.flatten(), minlength=experts))
+    # Sums over 900 tokens of a warp one after another, whose softmax values are all about 1 / 1024: the loss is 1 within their rounding and what chance leaves.
+    assert abs(routing.balance_loss.item() - 1.0) < 1e-2
+    upstream = torch.randn(tokens, k, device="cuda")
+    grad, = torch.autograd.grad(routing.weights, x, upstream)
+    expected, = torch.autograd.grad(alone.weights, tail, upstream[-3000:].contiguous())
+    assert torch.equal(grad[-3000:], expected)

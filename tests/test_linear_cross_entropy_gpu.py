@@ -551,3 +551,43 @@ def test_two_graphs_with_a_pool_in_common(ft, dtype):
             got = [x.clone() for x in results[i]]
             expected = run(ft, h.detach(), w.detach(), t)
             assert all(torch.equal(a, b) for a, b in zip(got, expected))
+
+
+@pytest.mark.parametrize("dtype, tokens, vocabulary, reduction", [(torch.bfloat16, 16, 530001, "sum"), (torch.float16, 16, 530001, "none"), (torch.float32, 80, 270001, "sum"),
+                                                                  (torch.float32, 20, 530001, "none")])
+def test_a_weight_past_32_bits(ft, dtype, tokens, vocabulary, reduction):
+    """More than 2^31 elements (or 2^32 bytes of them), against the formula piece by piece: the sums over the vocabulary, and rows of the weight's gradient from both ends."""
+    depth = 4096
+    hidden, _, _ = make(tokens, depth, 2, dtype, seed=50)
+    weight = torch.empty(vocabulary, depth, device="cuda", dtype=dtype)
+    for piece in weight.split(65536):
+        piece.copy_(torch.randn(piece.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(piece.shape[0])) * depth ** -0.5)
+    target = torch.randint(0, vocabulary, (tokens,), device="cuda")
+    target[0], target[1], target[2] = 0, vocabulary - 1, vocabulary // 2
+    loss, grad_hidden, grad_weight = run(ft, hidden, weight, target, reduction)
+    h = hidden.double()
+    z = torch.cat([h @ piece.double().T for piece in weight.split(65536)], 1)
+    size = max((h.abs() @ piece.double().abs().T).max().item() for piece in weight.split(65536))
+    lse = torch.logsumexp(z, 1)
+    # The bounds of Oracle, with the largest of all tokens for each.
+    relative = 2 * (depth / 8 + 8) * 2 * STEP * size + (32 + 4 * (z.abs().max() + lse.abs().max()).item()) * 2 * STEP
+    expected = lse - z.gather(1, target[:, None])[:, 0]
+    if reduction == "sum":
+        check(loss, expected.sum(), tokens * relative + 2 * STEP * expected.sum(), "loss")
+    else:
+        check(loss, expected, torch.full_like(expected, relative), "loss")
+    slope = torch.exp(z - lse[:, None])
+    half_step = torch.finfo(dtype).eps / 2
+    error = slope * (relative + 2.0 ** -11 * (dtype != torch.float32) + half_step + 4 * STEP) + 2.0 ** -38 * (dtype != torch.float32) + 2.0 ** -49 * (dtype == torch.float32)
+    slope[torch.arange(tokens), target] -= 1.0
+    error[torch.arange(tokens), target] += half_step + 4 * STEP
+    value, bound = torch.zeros_like(h), torch.zeros_like(h)
+    for s, e, piece in zip(slope.split(65536, 1), error.split(65536, 1), weight.split(65536)):
+        value += s @ piece.double()
+        bound += (e + (vocabulary / 8 + 24) * 2 * STEP * s.abs()) @ piece.double().abs()
+    finfo = torch.finfo(dtype)
+    check(grad_hidden, value, bound + 1.01 * half_step * value.abs() + finfo.smallest_normal * finfo.eps, "hidden's gradient")
+    for rows in (slice(0, 3000), slice(vocabulary // 2 - 1500, vocabulary // 2 + 1500), slice(vocabulary - 3000, vocabulary)):
+        value = slope[:, rows].T @ h
+        bound = (error[:, rows].T + (tokens / 8 + 24) * 2 * STEP * slope[:, rows].T.abs()) @ h.abs()
+        check(grad_weight[rows], value, bound + 1.01 * half_step * value.abs() + finfo.smallest_normal * finfo.eps, "weight's gradient")
