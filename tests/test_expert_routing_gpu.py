@@ -1,4 +1,5 @@
 """expert_routing and its gradient against the definition in 64 bits."""
+import gc
 import math
 
 import pytest
@@ -20,6 +21,14 @@ def ft(native_library):
     import flash_train.torch
 
     return flash_train.torch
+
+
+@pytest.fixture
+def memory_given_back():
+    """What a large test took goes back to the device, so that no later test's small tensor sits in a piece of it and keeps the rest."""
+    yield
+    gc.collect()
+    torch.cuda.empty_cache()
 
 
 def oracle(logits, k, normalize=True, mask=None):
@@ -337,7 +346,7 @@ def test_slots_that_nothing_takes_with_many_rounds(ft):
             run_and_check(ft, x, k)
 
 
-def test_logits_past_32_bits(ft):
+def test_logits_past_32_bits(ft, memory_given_back):
     """More than 2^32 logits: the last tokens come out as they do alone, and every slot is counted."""
     tokens, experts, k = (1 << 22) + 1001, 1024, 4
     x = torch.empty(tokens, experts, device="cuda", dtype=torch.bfloat16)

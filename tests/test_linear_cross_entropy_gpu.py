@@ -1,4 +1,5 @@
 """linear_cross_entropy and its gradients against the definition in 64 bits."""
+import gc
 import math
 
 import pytest
@@ -21,6 +22,14 @@ def ft(native_library):
     import flash_train.torch
 
     return flash_train.torch
+
+
+@pytest.fixture
+def memory_given_back():
+    """What a large test took goes back to the device, so that no later test's small tensor sits in a piece of it and keeps the rest."""
+    yield
+    gc.collect()
+    torch.cuda.empty_cache()
 
 
 def make(tokens, depth, vocabulary, dtype, seed=0, spread=2.0):
@@ -221,7 +230,7 @@ def test_infinities_and_nan_show(ft, dtype):
 
 
 @pytest.mark.parametrize("dtype, tokens, vocabulary", [(torch.bfloat16, 4096, 140001), (torch.float16, 4500, 131072), (torch.float32, 4096, 70001)])
-def test_several_pieces_of_the_vocabulary(ft, dtype, tokens, vocabulary):
+def test_several_pieces_of_the_vocabulary(ft, memory_given_back, dtype, tokens, vocabulary):
     hidden, weight, target = make(tokens, 40, vocabulary, dtype, seed=10)
     target[::7] = -100
     target[1], target[2] = 0, vocabulary - 1
@@ -488,7 +497,7 @@ def test_what_the_step_refuses(ft, capi):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_many_tokens_of_a_small_vocabulary(ft, dtype):
+def test_many_tokens_of_a_small_vocabulary(ft, memory_given_back, dtype):
     """More rows of 32 than a grid's second dimension takes (FP32: more logits than the step call takes)."""
     hidden, weight, target = make(32 * 65535 + 1, 8, 3, dtype, seed=14)
     target[::5] = -100
@@ -555,7 +564,7 @@ def test_two_graphs_with_a_pool_in_common(ft, dtype):
 
 @pytest.mark.parametrize("dtype, tokens, vocabulary, reduction", [(torch.bfloat16, 16, 530001, "sum"), (torch.float16, 16, 530001, "none"), (torch.float32, 80, 270001, "sum"),
                                                                   (torch.float32, 20, 530001, "none")])
-def test_a_weight_past_32_bits(ft, dtype, tokens, vocabulary, reduction):
+def test_a_weight_past_32_bits(ft, memory_given_back, dtype, tokens, vocabulary, reduction):
     """More than 2^31 elements (or 2^32 bytes of them), against the formula piece by piece: the sums over the vocabulary, and rows of the weight's gradient from both ends."""
     depth = 4096
     hidden, _, _ = make(tokens, depth, 2, dtype, seed=50)
