@@ -37,6 +37,7 @@ using training::Element;
 
 constexpr int kListThreads             = 1024;
 constexpr int kGatherThreads           = 256;
+constexpr int kSplitCtasPerSm          = 8;
 constexpr int kJoinRows                = 32;   // rows of a CTA that joins statistics ...
 constexpr int kJoinWarps               = 32;   // ... each of its warps some of the pieces
 constexpr int kRowThreads              = 256;  // FP32: threads that go over a row of logits
@@ -46,6 +47,7 @@ constexpr std::uint64_t kStepBytes     = 2ULL << 30;    // that the step call's 
 constexpr std::uint64_t kAlign         = 256;
 constexpr int kKeptRows                = 32;            // rows of a CTA that turns exponentials into slopes ...
 constexpr int kKeptPieces              = 4;             // ... and pieces of the statistics
+constexpr int kKeptBatch               = 2;             // packs that a thread asks for at a time
 
 // ---------------------------------------------------------------- kernels
 
@@ -176,26 +178,42 @@ __global__ void __launch_bounds__(kGatherThreads) copyRows16(const std::uint16_t
     for (std::uint32_t i = threadIdx.x; i < depth; i += kGatherThreads) { to[i] = from[i]; }
 }
 
-// An FP32 matrix's rows as three BF16 matrices, `plane` elements apart. With `rows`, those of the live tokens, and zeros behind the last one.
-__global__ void __launch_bounds__(kGatherThreads) splitRows(const LiveRows rows, bool gathered, const float* from, std::int64_t stride, std::uint16_t* to,
+// An FP32 matrix's rows as three BF16 matrices, `plane` elements apart, eight elements a thread. With `gathered`, the rows are those of the live tokens, and
+// zeros behind the last one. (16384 x 512: two elements a thread and a CTA a row 4 us more.) kWide: the rows begin at multiples of 16 bytes. (The planes' rows do, and have room for whole packs.)
+template<bool kWide>
+__global__ void __launch_bounds__(kGatherThreads) splitRows(const LiveRows rows, bool gathered, std::uint32_t count, const float* matrix, std::int64_t stride, std::uint16_t* to,
                                                             std::uint64_t pitch, std::uint64_t plane, std::uint32_t depth) {
     gridDependencyWait();
     gridDependencyLaunchDependents();
-    const std::uint32_t row  = blockIdx.x;
-    const std::uint32_t live = gathered ? *rows.count : 0xFFFFFFFFU;
-    if (gathered && row >= (max(live, 1U) + loss::kTileRows - 1) / loss::kTileRows * loss::kTileRows) { return; }
-    if (row < live) { from += static_cast<std::int64_t>(gathered ? rows.token[row] : static_cast<std::int32_t>(row)) * stride; }
-    to += row * pitch;
-    // Two elements a thread: the planes' rows begin at multiples of 16 bytes and have room for one more.
-#pragma unroll 2
-    for (std::uint32_t i = 2 * threadIdx.x; i < depth; i += 2 * kGatherThreads) {
-        float low[3] = {0.0F, 0.0F, 0.0F}, high[3] = {0.0F, 0.0F, 0.0F};
+    const std::uint32_t live   = gathered ? *rows.count : count;
+    const std::uint32_t padded = gathered ? (max(live, 1U) + loss::kTileRows - 1) / loss::kTileRows * loss::kTileRows : count;
+    const std::uint32_t packs  = (depth + 7) / 8;
+    const std::uint64_t all    = static_cast<std::uint64_t>(padded) * packs, step = static_cast<std::uint64_t>(gridDim.x) * kGatherThreads;
+    for (std::uint64_t i = static_cast<std::uint64_t>(blockIdx.x) * kGatherThreads + threadIdx.x; i < all; i += step) {
+        const std::uint32_t row = static_cast<std::uint32_t>(i / packs), first = static_cast<std::uint32_t>(i - static_cast<std::uint64_t>(row) * packs) * 8;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { x[j] = 0.0F; }
         if (row < live) {
-            training::splitPlanes(from[i], low);
-            training::splitPlanes(i + 1 < depth ? from[i + 1] : 0.0F, high);
+            const float* const from = matrix + static_cast<std::int64_t>(gathered ? rows.token[row] : static_cast<std::int32_t>(row)) * stride + first;
+            if (kWide && first + 8 <= depth) {
+                const float4 low = *reinterpret_cast<const float4*>(from), high = *reinterpret_cast<const float4*>(from + 4);
+                x[0] = low.x, x[1] = low.y, x[2] = low.z, x[3] = low.w, x[4] = high.x, x[5] = high.y, x[6] = high.z, x[7] = high.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { x[j] = first + j < depth ? from[j] : 0.0F; }
+            }
+        }
+        alignas(16) __nv_bfloat16 parts[3][8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float three[3];
+            training::splitPlanes(x[j], three);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) { parts[p][j] = __float2bfloat16_rn(three[p]); }
         }
 #pragma unroll
-        for (int p = 0; p < 3; ++p) { *reinterpret_cast<__nv_bfloat162*>(to + p * plane + i) = __floats2bfloat162_rn(low[p], high[p]); }
+        for (int p = 0; p < 3; ++p) { *reinterpret_cast<uint4*>(to + p * plane + row * pitch + first) = *reinterpret_cast<const uint4*>(parts[p]); }
     }
 }
 
@@ -371,6 +389,7 @@ __device__ __forceinline__ float keptFactor(const KeptParams& p, std::uint32_t p
     return p.rows.scale[row] * (base == -INFINITY && lse2 > -INFINITY ? 0.0F : exp2f(base - lse2));
 }
 
+// (Of 4096 x 32768 in 16 bits 94 us with a pack at a time, 80 with two asked for before the first is written, the rate of a copy.)
 // What the product kept becomes dZ, in place: 2^(logit - piece's largest) 2^(that - lse), less the target's one; zeros in the neutral rows. A thread
 // takes eight columns of a row at a time, neighbouring threads neighbouring ones.
 // kPlanes: from FP32 to the three BF16 matrices at `planes`, T being float; otherwise from FP16 to T.
@@ -391,41 +410,52 @@ template<typename T> __global__ void __launch_bounds__(256) keptSlopes(const Kep
     }
     __syncthreads();
     const std::uint32_t each  = p.width / 8;  // packs of a piece's row
-    const std::uint32_t packs = pieces * each;
-    for (std::uint32_t i = threadIdx.x; i < packs * kKeptRows; i += 256) {
-        const std::uint32_t in_row = i / packs, pack = i - in_row * packs;
-        const std::uint32_t row    = row0 + in_row, col = piece0 * p.width + pack * 8;
-        const std::uint64_t at     = row * p.pitch + col;
-        const bool on              = row < live;
-        const float factor         = on ? factors[pack / each][in_row] : 0.0F;
-        const float scale          = on ? p.rows.scale[row] : 0.0F;
-        const std::int32_t hit     = on ? p.rows.target[row] - static_cast<std::int32_t>(col) : -1;
-        if constexpr (kPlanes) {
-            alignas(16) float from[8];
-            alignas(16) __nv_bfloat16 to[3][8];
-            for (int j = 0; j < 8; j += 4) { *reinterpret_cast<float4*>(from + j) = *reinterpret_cast<const float4*>(static_cast<const float*>(kept) + at + j); }
+    const std::uint32_t packs = pieces * each, all = packs * kKeptRows;
+    using From = typename std::conditional<kPlanes, float, __half>::type;
+    struct alignas(16) Pack {
+        From at[8];
+    };
+    // A batch is asked for before the first of it is written.
+    for (std::uint32_t first = threadIdx.x; first < all; first += kKeptBatch * 256) {
+        Pack batch[kKeptBatch];
+        const auto place = [&](std::uint32_t i) { return (row0 + i / packs) * p.pitch + piece0 * p.width + i % packs * 8; };
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float parts[3];
-                training::splitPlanes(on ? factor * from[j] - (j == hit ? scale : 0.0F) : 0.0F, parts);
+        for (int b = 0; b < kKeptBatch; ++b) {
+            const std::uint32_t i = first + b * 256;
+            if (i < all) { batch[b] = *reinterpret_cast<const Pack*>(static_cast<const From*>(kept) + place(i)); }
+        }
 #pragma unroll
-                for (int plane = 0; plane < 3; ++plane) { to[plane][j] = __float2bfloat16_rn(parts[plane]); }
+        for (int b = 0; b < kKeptBatch; ++b) {
+            const std::uint32_t i = first + b * 256;
+            if (i >= all) { break; }
+            const std::uint32_t in_row = i / packs, pack = i - in_row * packs, row = row0 + in_row;
+            const std::uint64_t at     = place(i);
+            const bool on              = row < live;
+            const float factor         = on ? factors[pack / each][in_row] : 0.0F;
+            const float scale          = on ? p.rows.scale[row] : 0.0F;
+            const std::int32_t hit     = on ? p.rows.target[row] - static_cast<std::int32_t>(piece0 * p.width + pack * 8) : -1;
+            if constexpr (kPlanes) {
+                alignas(16) __nv_bfloat16 to[3][8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float parts[3];
+                    training::splitPlanes(on ? factor * batch[b].at[j] - (j == hit ? scale : 0.0F) : 0.0F, parts);
+#pragma unroll
+                    for (int plane = 0; plane < 3; ++plane) { to[plane][j] = __float2bfloat16_rn(parts[plane]); }
+                }
+#pragma unroll
+                for (int plane = 0; plane < 3; ++plane) { *reinterpret_cast<uint4*>(planes + plane * p.plane + at) = *reinterpret_cast<const uint4*>(to[plane]); }
+            } else {
+                alignas(16) T to[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { to[j] = Element<T>::narrow(on ? factor * __half2float(batch[b].at[j]) - (j == hit ? scale : 0.0F) : 0.0F); }
+                *reinterpret_cast<uint4*>(static_cast<__half*>(kept) + at) = *reinterpret_cast<const uint4*>(to);
             }
-#pragma unroll
-            for (int plane = 0; plane < 3; ++plane) { *reinterpret_cast<uint4*>(planes + plane * p.plane + at) = *reinterpret_cast<const uint4*>(to[plane]); }
-        } else {
-            uint4* const words = reinterpret_cast<uint4*>(static_cast<__half*>(kept) + at);
-            alignas(16) __half from[8];
-            alignas(16) T to[8];
-            *reinterpret_cast<uint4*>(from) = *words;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) { to[j] = Element<T>::narrow(on ? factor * __half2float(from[j]) - (j == hit ? scale : 0.0F) : 0.0F); }
-            *words = *reinterpret_cast<const uint4*>(to);
         }
     }
 }
 
-// grad_hidden[t] = unit * (the sums' parts added up), 0 for a token that takes no part.
+// grad_hidden[t] = unit * (the sums' parts added up), 0 for a token that takes no part. Few tokens have many parts, and several CTAs each.
 template<typename T>
 __global__ void __launch_bounds__(kGatherThreads) spreadHidden(const LiveRows rows, const std::int32_t* slot, const float* sums, std::uint64_t part, std::uint64_t pitch,
                                                                std::uint32_t splits, std::uint32_t depth, T* out, std::int64_t stride) {
@@ -436,9 +466,10 @@ __global__ void __launch_bounds__(kGatherThreads) spreadHidden(const LiveRows ro
     T* const to            = out + static_cast<std::int64_t>(blockIdx.x) * stride;
     const float* const from = sums + static_cast<std::uint64_t>(max(row, 0)) * pitch;
 #pragma unroll 2
-    for (std::uint32_t i = threadIdx.x; i < depth; i += kGatherThreads) {
+    for (std::uint32_t i = blockIdx.y * kGatherThreads + threadIdx.x; i < depth; i += gridDim.y * kGatherThreads) {
         float sum = 0.0F;
         if (row >= 0) {
+#pragma unroll 8
             for (std::uint32_t s = 0; s < splits; ++s) { sum += from[s * part + i]; }
         }
         to[i] = Element<T>::narrow(unit * sum);
@@ -796,17 +827,21 @@ class Call final {
         return RowParams{rows_, at<float>(l_.piece), l_.piece_pitch, static_cast<std::uint32_t>(first), static_cast<std::uint32_t>(columns), partials};
     }
 
+    // An operand as three BF16 matrices, `rows` rows of it at most.
+    cudaError_t split(bool gathered, std::uint64_t rows, const float* from, std::int64_t stride, std::uint64_t to, std::uint64_t pitch) const {
+        const std::uint64_t threads = rows * ceilDiv(q_.depth, 8), most = static_cast<std::uint64_t>(sms_) * kSplitCtasPerSm;
+        const dim3 grid(static_cast<unsigned>(std::min(most, ceilDiv(threads, kGatherThreads))));
+        const auto kernel = training::aligned(from, 16) && stride % 4 == 0 ? splitRows<true> : splitRows<false>;
+        return training::launchOverlapped(kernel, grid, dim3(kGatherThreads), 0, stream_, rows_, gathered, static_cast<std::uint32_t>(rows), from, stride, at<std::uint16_t>(to), pitch,
+                                          rows * pitch, static_cast<std::uint32_t>(q_.depth));
+    }
+
     // The live hidden states, and the weight where TMA cannot fetch it as it is.
     cudaError_t gather() const {
         if (l_.planes) {
-            const std::uint32_t depth = static_cast<std::uint32_t>(q_.depth);
-            cudaError_t error = training::launchOverlapped(splitRows, dim3(static_cast<unsigned>(l_.capacity)), dim3(kGatherThreads), 0, stream_, rows_, true,
-                                                           static_cast<const float*>(q_.hidden), q_.hidden_row_stride, at<std::uint16_t>(l_.hidden), l_.copy_pitch,
-                                                           l_.capacity * l_.copy_pitch, depth);
-            if (error != cudaSuccess) { return error; }
-            return training::launchOverlapped(splitRows, dim3(static_cast<unsigned>(q_.vocabulary)), dim3(kGatherThreads), 0, stream_, rows_, false,
-                                              static_cast<const float*>(q_.weight), q_.vocabulary == 1 ? std::int64_t{0} : q_.weight_row_stride, at<std::uint16_t>(l_.weight),
-                                              l_.weight_pitch, q_.vocabulary * l_.weight_pitch, depth);
+            const cudaError_t error = split(true, l_.capacity, static_cast<const float*>(q_.hidden), q_.tokens <= 1 ? 0 : q_.hidden_row_stride, l_.hidden, l_.copy_pitch);
+            return error == cudaSuccess ? split(false, q_.vocabulary, static_cast<const float*>(q_.weight), q_.vocabulary == 1 ? 0 : q_.weight_row_stride, l_.weight, l_.weight_pitch)
+                                        : error;
         }
         const std::uint64_t bytes = training::elementBytes(q_.element);
         // The library's products go over all rows, the others over whole tiles of live ones.
@@ -903,7 +938,9 @@ class Call final {
     }
 
     template<typename T> cudaError_t spread(T* out, std::int64_t stride) const {
-        return training::launchOverlapped(spreadHidden<T>, dim3(static_cast<unsigned>(q_.tokens)), dim3(kGatherThreads), 0, stream_, rows_,
+        // (64 x 2048 in 16 parts: 14 us with a CTA for each token, 5 with eight; 4096 x 512 in one: 14, and 20 with two.)
+        const std::uint64_t each = std::min(ceilDiv(q_.depth, kGatherThreads), std::max<std::uint64_t>(1, static_cast<std::uint64_t>(sms_) * 4 / q_.tokens));
+        return training::launchOverlapped(spreadHidden<T>, dim3(static_cast<unsigned>(q_.tokens), static_cast<unsigned>(each)), dim3(kGatherThreads), 0, stream_, rows_,
                                           static_cast<const std::int32_t*>(at<std::int32_t>(l_.slot)), static_cast<const float*>(at<float>(l_.sums)), l_.capacity * l_.sums_pitch,
                                           l_.sums_pitch, l_.splits, static_cast<std::uint32_t>(q_.depth), out, stride);
     }
