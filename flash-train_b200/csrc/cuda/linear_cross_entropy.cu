@@ -625,10 +625,10 @@ int layOut(const FtcudaLinearCrossEntropy& q, Form form, int sms, Layout& l, cha
     l.columns                 = form == Form::kStep ? fill : std::min(fill, std::max(kLeastColumns, kPieceBytes / (l.capacity * bytes) / 256 * 256));
     l.columns                 = roundUp(ceilDiv(fill, ceilDiv(fill, l.columns)), 256);  // pieces of about one size
     l.piece_pitch             = l.columns;
-    l.pieces                  = l.library ? ceilDiv(q.vocabulary, l.columns) : loss::statisticsPieces(static_cast<std::uint32_t>(q.vocabulary));
+    l.pieces                  = l.library ? ceilDiv(q.vocabulary, l.columns) : loss::statisticsPieces(static_cast<std::uint32_t>(q.vocabulary), static_cast<std::uint32_t>(l.capacity), sms);
     l.sums_pitch              = roundUp(q.depth, 8);
-    l.splits                  = l.library ? 1 : loss::hiddenSplits(static_cast<std::uint32_t>(l.capacity), static_cast<std::uint32_t>(q.depth),
-                                                              static_cast<std::uint32_t>(std::min(l.columns, q.vocabulary)), sms);
+    l.splits                  = l.library ? 1 : loss::hiddenSplits(static_cast<std::uint32_t>(std::max<std::uint64_t>(q.tokens, 1)), static_cast<std::uint32_t>(q.depth),
+                                                              static_cast<std::uint32_t>(std::min(l.columns, q.vocabulary)), l.planes, sms);
     std::uint64_t at = 0;
     const auto take  = [&](std::uint64_t size) {
         const std::uint64_t here = at;
@@ -770,7 +770,7 @@ class Call final {
         if (l_.library) {
             error = training::launchOverlapped(rowSlopes, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(0, columns, nullptr));
         } else {
-            const KeptParams params{rows_, partials, static_cast<std::uint32_t>(l_.pieces), loss::statisticsWidth(columns), static_cast<std::uint32_t>(l_.capacity),
+            const KeptParams params{rows_, partials, static_cast<std::uint32_t>(l_.pieces), loss::statisticsWidth(columns, static_cast<std::uint32_t>(l_.capacity), sms_), static_cast<std::uint32_t>(l_.capacity),
                                     l_.piece_pitch, slopesPlane()};
             const dim3 grid(static_cast<unsigned>(ceilDiv(l_.pieces, kKeptPieces) * (l_.capacity / kKeptRows)));  // (of x, which takes any number)
             const auto kernel = l_.planes ? keptSlopes<float> : q_.element == FTCUDA_ELEMENT_FP16 ? keptSlopes<__half> : keptSlopes<__nv_bfloat16>;

@@ -2,7 +2,7 @@
 // its epilogue (linear_cross_entropy.cu has the whole).
 //
 //   statistics   Z = H W^T; of a tile of Z nothing is kept but the rows' maxima and sums of exponentials
-//   kept         the same, and the exponentials go to memory in FP16, each against its row's maximum in 128 columns
+//   kept         the same, and the exponentials go to memory in FP16, each against its row's maximum in 64 or 128 columns
 //   slopes       Z once more; dZ = scale (exp(Z - lse) - onehot), rounded to the operands' type, goes to memory for a piece of the vocabulary
 //   gradients    dH (+)= dZ W and dW = dZ^T H of that piece, in one launch
 //
@@ -55,7 +55,10 @@ namespace {
 
 constexpr std::uint32_t kBlockK = 64;  // 128 bytes, one swizzle row
 constexpr std::uint32_t kTileN  = 256;
-constexpr std::uint32_t kItemBlocks  = 12;
+constexpr std::uint32_t kItemBlocks  = 12;  // of an item: what it costs beside its own
+constexpr std::uint32_t kMostSplits  = 16;
+constexpr std::uint64_t kStreamTokens = 400;         // at which the tensor cores take as long as HBM does (times an FP32 product's terms)
+constexpr std::uint64_t kStreamBytes  = 64ULL << 20;  // half of L2
 constexpr std::uint32_t kSumBlocks   = 16;
 constexpr std::uint32_t kFp32Blocks  = 2;
 constexpr std::uint32_t kTerms       = 6;         // of an FP32 product: which plane of A and of B, four bits for each term
@@ -139,6 +142,25 @@ struct Work {
     std::uint32_t late, early;
 };
 
+// How long that takes, an item of the first problem taking `first`, one of the second `second`.
+__host__ __device__ __forceinline__ std::uint64_t makespan(std::uint32_t first_items, std::uint32_t first, std::uint32_t second_items, std::uint32_t second, std::uint32_t pairs,
+                                                           std::uint32_t early) {
+    const std::uint32_t own = first_items / pairs, late = first_items % pairs, others = pairs - late;
+    const std::uint64_t all   = static_cast<std::uint64_t>(early) * others;
+    const std::uint32_t taken = all < second_items ? static_cast<std::uint32_t>(all) : second_items, rest = second_items - taken;
+    const std::uint32_t before = (taken + others - 1) / others;
+    const std::uint64_t most  = static_cast<std::uint64_t>(own + (late != 0 ? 1 : 0)) * first + static_cast<std::uint64_t>((rest + pairs - 1) / pairs) * second;
+    const std::uint64_t least = static_cast<std::uint64_t>(own) * first + static_cast<std::uint64_t>(before + (rest > late ? (rest - late + pairs - 1) / pairs : 0)) * second;
+    return most > least ? most : least;
+}
+
+// The better one of the two numbers of early items next to an even share.
+__host__ __device__ __forceinline__ std::uint32_t earlyItems(std::uint32_t first_items, std::uint32_t first, std::uint32_t second_items, std::uint32_t second, std::uint32_t pairs) {
+    if (second_items == 0 || first_items % pairs == 0) { return 0; }
+    const std::uint32_t fewer = first / second;
+    return makespan(first_items, first, second_items, second, pairs, fewer + 1) < makespan(first_items, first, second_items, second, pairs, fewer) ? fewer + 1 : fewer;
+}
+
 __device__ __forceinline__ Work workOf(const ProductParams& p, std::uint32_t live, std::uint32_t pairs) {
     live = max(live, 1U);
     Work w;
@@ -155,7 +177,7 @@ __device__ __forceinline__ Work workOf(const ProductParams& p, std::uint32_t liv
     w.late  = w.items[0] % pairs;
     // (An item costs about kItemBlocks blocks' time beside its own.)
     const std::uint32_t first = p.problem[0].splits == 1 ? w.blocks[0] : p.problem[0].blocks_per_split;
-    w.early                   = w.items[1] != 0 && w.late != 0 ? (first * p.terms + kItemBlocks) / (w.blocks[1] * p.terms + kItemBlocks) : 0;
+    w.early                   = w.items[1] == 0 ? 0 : earlyItems(w.items[0], first * p.terms + kItemBlocks, w.items[1], w.blocks[1] * p.terms + kItemBlocks, pairs);
     return w;
 }
 
@@ -622,6 +644,12 @@ std::uint32_t divideUp(std::uint32_t x, std::uint32_t y) { return (x + y - 1) / 
 // 128 columns where that is all there are: B's tile is half as wide then.
 std::uint32_t tileColumns(std::uint32_t columns) { return columns <= 128 ? 128 : kTileN; }
 
+// Of the logits: and where that does not give a pair of SMs two tiles.
+std::uint32_t logitTileColumns(std::uint32_t columns, std::uint32_t capacity, int sms) {
+    const std::uint64_t tiles = static_cast<std::uint64_t>(capacity / kTileRows) * divideUp(columns, kTileN);
+    return 2 * tiles <= static_cast<std::uint64_t>(std::max(1, sms / 2)) ? 128 : tileColumns(columns);
+}
+
 // An operand whose rows (of the product) are `rows` and whose depth is `k`: neighbours along K, or along the rows.
 bool encodeOperand(CUtensorMap* map, const ProductCall& call, Matrix16 matrix, bool along_rows, std::uint32_t rows, std::uint32_t k, std::uint32_t tile_rows) {
     const std::uint64_t planes = call.planes ? kPlanes : 1, apart = call.planes ? matrix.plane * 2 : matrix.pitch * 2;
@@ -655,7 +683,7 @@ ProductParams paramsFor(const ProductCall& call) {
 bool describeLogits(const ProductCall& call, Matrix16 weight, std::uint32_t columns, ProductMaps& maps, ProductParams& p) {
     Problem& problem          = p.problem[0];
     problem.columns           = columns;
-    problem.tile_n            = tileColumns(columns);
+    problem.tile_n            = logitTileColumns(columns, call.capacity, call.sms);
     problem.tiles_n           = divideUp(columns, problem.tile_n);
     problem.blocks            = divideUp(call.depth, kBlockK);
     problem.splits            = 1;
@@ -666,8 +694,8 @@ bool describeLogits(const ProductCall& call, Matrix16 weight, std::uint32_t colu
 
 }  // namespace
 
-std::uint32_t statisticsWidth(std::uint32_t columns) { return tileColumns(columns) / 2; }
-std::uint32_t statisticsPieces(std::uint32_t columns) { return 2 * divideUp(columns, tileColumns(columns)); }
+std::uint32_t statisticsWidth(std::uint32_t columns, std::uint32_t capacity, int sms) { return logitTileColumns(columns, capacity, sms) / 2; }
+std::uint32_t statisticsPieces(std::uint32_t columns, std::uint32_t capacity, int sms) { return 2 * divideUp(columns, logitTileColumns(columns, capacity, sms)); }
 
 cudaError_t launchStatistics(const ProductCall& call, Matrix16 weight, std::uint32_t vocabulary, float2* partials) {
     ProductMaps maps;
@@ -699,13 +727,32 @@ cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t
     return launch<kSlopes>(call, maps, p, static_cast<std::uint64_t>(call.capacity / kTileRows) * p.problem[0].tiles_n);
 }
 
-// With few tiles the sum over the columns is cut until there are about two items for each pair of SMs, eight K blocks each at least.
-std::uint32_t hiddenSplits(std::uint32_t capacity, std::uint32_t depth, std::uint32_t columns, int sms) {
-    const std::uint32_t tiles = capacity / kTileRows * divideUp(depth, tileColumns(depth));
-    const std::uint32_t pairs = static_cast<std::uint32_t>(std::max(1, sms / 2));
-    const std::uint32_t blocks = divideUp(columns, kBlockK);
-    const std::uint32_t wanted = std::min({std::max(1U, blocks / 8), 16U, std::max(1U, 2 * pairs / tiles)});
-    return divideUp(blocks, divideUp(blocks, wanted));  // none of them empty
+// The sum over the columns is cut into as many parts as let both gradients' items end soonest (all tokens taken for live), a part's way through memory and
+// back counted as well. Where the weight streams through (too large for L2, and too few tokens to be bound by anything else), into as many as make two items
+// for each pair of SMs, so that all of them fetch it. Measured, a step, always the latter / as here: 700 x 700 x 3000 FP32 133 / 104 us, 1024 x 600 x 9000 FP32 250 / 224,
+// 4096 x 512 x 32768 BF16 471 / 445; 257 x 4096 x 131072 BF16 920, and 1016 where the items alone decide, 64 x 2048 x 50257 205 and 218.
+std::uint32_t hiddenSplits(std::uint32_t tokens, std::uint32_t depth, std::uint32_t columns, bool planes, int sms) {
+    const std::uint32_t across = divideUp(depth, tileColumns(depth)), tiles = divideUp(tokens, kTileRows) * across;
+    const std::uint32_t pairs  = static_cast<std::uint32_t>(std::max(1, sms / 2));
+    const std::uint32_t blocks = divideUp(columns, kBlockK), terms = planes ? kTerms : 1;
+    if (static_cast<std::uint64_t>(tokens) * terms <= kStreamTokens && static_cast<std::uint64_t>(columns) * depth * 2 * (planes ? kPlanes : 1) > kStreamBytes) {
+        const std::uint32_t wanted = std::min({std::max(1U, blocks / 8), kMostSplits, std::max(1U, 2 * pairs / tiles)});
+        return divideUp(blocks, divideUp(blocks, wanted));
+    }
+    const std::uint32_t weight_items = divideUp(columns, kTileRows) * across, weight = divideUp(tokens, kBlockK) * terms + kItemBlocks;
+    const std::uint64_t apart  = static_cast<std::uint64_t>(tokens) * depth >> 19;  // a block's 512 cycles are the time of 2^21 bytes or so
+    std::uint32_t best         = 1;
+    std::uint64_t least        = ~std::uint64_t{0};
+    for (std::uint32_t wanted = 1; wanted <= std::min(blocks, kMostSplits); ++wanted) {
+        const std::uint32_t each = divideUp(blocks, wanted), splits = divideUp(blocks, each);  // none of them empty
+        const std::uint32_t part = each * terms + kItemBlocks;
+        const std::uint64_t time = makespan(tiles * splits, part, weight_items, weight, pairs, earlyItems(tiles * splits, part, weight_items, weight, pairs)) + splits * apart;
+        if (time < least) {
+            least = time;
+            best  = splits;
+        }
+    }
+    return best;
 }
 
 cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint32_t columns, Matrix16 slopes, const Gradients& gradients) {

@@ -53,8 +53,8 @@ struct ProductCall {
 };
 
 // Columns of the vocabulary that one partial result of the statistics covers, and how many of those there are.
-std::uint32_t statisticsWidth(std::uint32_t columns);
-std::uint32_t statisticsPieces(std::uint32_t columns);
+std::uint32_t statisticsWidth(std::uint32_t columns, std::uint32_t capacity, int sms);
+std::uint32_t statisticsPieces(std::uint32_t columns, std::uint32_t capacity, int sms);
 
 // For every live row and piece of columns: {largest logit times log2 e, sum of 2^(logit log2 e - that)} to
 // partials[piece][capacity]; and the target's logit to rows.picked.
@@ -72,7 +72,7 @@ cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t
 
 // How many parts the sum over `columns` columns is cut into for the gradient of the hidden states. (Over fewer columns
 // launchGradients may fill fewer of them, never more.)
-std::uint32_t hiddenSplits(std::uint32_t capacity, std::uint32_t depth, std::uint32_t columns, int sms);
+std::uint32_t hiddenSplits(std::uint32_t tokens, std::uint32_t depth, std::uint32_t columns, bool planes, int sms);
 
 struct Gradients {
     // hidden: sums[split][capacity][pitch] (+)= slopes times weight; NULL when not wanted.
