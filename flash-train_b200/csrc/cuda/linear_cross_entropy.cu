@@ -590,14 +590,18 @@ FtcudaGemmDesc describeWeight(const FtcudaLinearCrossEntropy& q, const Layout& l
 // What a call computes: the loss, the gradients from a loss that is known, or both at once.
 enum class Form { kLoss, kGradients, kStep };
 
-// Whether FP32 operands are better off with the library's products. Measured (a step, library / three BF16 matrices, microseconds): large products
-// of a depth from 768 on, where the prepared form is what they take (2048 x 2048 x 32000 2300 / 3240, 4096 x 1024 x 16000 1413 / 1666,
-// 700 x 2048 x 20000 749 / 851, 768 x 768 x 30000 524 / 529, but 2048 x 512 x 8000 349 / 281, 600 x 4096 x 6000 521 / 489, 896 x 72 x 45256
-// 1275 / 424); and few tokens, which read the weight once and would have it split for nothing else (64 x 1024 x 32000 280 / 302, 64 x 4096 x 32000 741 / 932,
-// but 96 x 1024 x 32000 337 / 308, 129 x 512 x 8191 145 / 92), a few more for the loss alone (96 x 4096 x 32000 202 / 512).
+// Whether FP32 operands are better off with the library's products. Measured (library / three BF16 matrices, microseconds):
+//   large products that take the prepared form; a step of 2048 x 2048 x 32000 2501 / 3231, 4096 x 1024 x 16000 1476 / 1666, 700 x 2048 x 20000 743 / 837, 1200 x 1200 x 9000
+//   379 / 407, but 1024 x 1024 x 4096 165 / 150, 768 x 768 x 30000 558 / 521, 512 x 2048 x 32000 963 / 971, 256 x 1024 x 32000 424 / 324, and 2048 x 512 x 8000 349 / 281;
+//   few tokens, which read the weight once and would have it split for nothing else: a step of 64 x 4096 x 32000 790 / 916, 32 x 2048 x 128 41 / 77, 64 x 1024 x 32000 275 / 282,
+//   8 x 512 x 16000 94 / 107, but 64 x 512 x 8000 77 / 73, 48 x 512 x 16000 118 / 109, 20 x 512 x 5000 73 / 63, 96 x 1024 x 32000 333 / 289;
+//   the loss alone, more of both: 96 x 4096 x 32000 225 / 505, 128 x 1024 x 20000 67 / 117, 300 x 2048 x 50000 442 / 580, 512 x 4096 x 32000 641 / 785, but 256 x 1024 x 32000 151 / 146,
+//   768 x 768 x 30000 193 / 179.
 bool libraryPays(const FtcudaLinearCrossEntropy& q, Form form) {
     if (!isFp32(q)) { return false; }
-    return q.tokens <= (form == Form::kLoss ? 128U : 64U) || (q.depth >= 768 && preparedFormPays(q.tokens, q.vocabulary, q.depth));
+    const bool large = q.depth >= 768 && q.tokens * q.depth >= 1400000 && preparedFormPays(q.tokens, q.vocabulary, q.depth);
+    if (form == Form::kLoss) { return large || q.tokens <= 128 || q.depth >= 2048; }
+    return large || q.tokens <= 8 || (q.tokens <= 64 && q.depth >= 1024);
 }
 
 // What a logit takes of the workspace while it is there, in bytes: its slope, and in the step call its exponential as well where that cannot
