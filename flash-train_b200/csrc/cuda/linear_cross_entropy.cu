@@ -5,9 +5,9 @@
 //
 // The forward call is one pass over the vocabulary, 2 T V D operations; the backward call goes through the vocabulary piece by
 // piece and computes Z of a piece again: dZ of it, then dH += dZ W and dW = dZ^T H, 6 T V D. A piece is as wide as kPieceBytes of dZ allow, so that
-// the passes over dH (one for each piece) and the launches weigh little. The step call does both for an upstream gradient of 1 without
-// computing Z twice, 6 T V D in all, where kStepBytes have room for all of Z's exponentials, 16 bits each (FP32: for Z), during the call:
-// a pass over them, two bytes read and two written for each, makes them dZ.
+// the passes over dH (one for each piece) and the launches weigh little. The step call does both without
+// computing Z twice, 6 T V D in all, where kStepBytes have room for all of Z's exponentials, 16 bits each (FP32: for Z):
+// a pass over them, two bytes read and two written for each, makes them dZ for an upstream gradient of 1, and what comes from it is multiplied by the one there is.
 //
 // Tokens without a target are left out first: the others' hidden states are gathered into the workspace, which costs one pass over H,
 // makes what the padding holds irrelevant (a NaN there would reach dW through 0 * NaN), spares the products those rows, and gives
@@ -455,14 +455,15 @@ template<typename T> __global__ void __launch_bounds__(256) keptSlopes(const Kep
     }
 }
 
-// grad_hidden[t] = unit * (the sums' parts added up), 0 for a token that takes no part. Few tokens have many parts, and several CTAs each.
+// grad_hidden[t] = unit * upstream * (the sums' parts added up), 0 for a token that takes no part. Few tokens have many parts, and several CTAs each.
 template<typename T>
 __global__ void __launch_bounds__(kGatherThreads) spreadHidden(const LiveRows rows, const std::int32_t* slot, const float* sums, std::uint64_t part, std::uint64_t pitch,
-                                                               std::uint32_t splits, std::uint32_t depth, T* out, std::int64_t stride) {
+                                                               std::uint32_t capacity, std::uint32_t splits, std::uint32_t depth, const float* upstream, T* out,
+                                                               std::int64_t stride) {
     gridDependencyWait();
     gridDependencyLaunchDependents();
-    const std::int32_t row = slot[blockIdx.x];
-    const float unit       = *rows.unit;
+    const std::int32_t row = min(slot[blockIdx.x], static_cast<std::int32_t>(capacity) - 1);  // (never beyond, whatever stands there)
+    const float unit       = *rows.unit * (upstream != nullptr ? *upstream : 1.0F);
     T* const to            = out + static_cast<std::int64_t>(blockIdx.x) * stride;
     const float* const from = sums + static_cast<std::uint64_t>(max(row, 0)) * pitch;
 #pragma unroll 2
@@ -725,7 +726,7 @@ class Call final {
         rows_.lse2   = at<float>(l_.lse2);
         rows_.picked = at<float>(l_.picked);
         products_    = loss::ProductCall{l_.planes || q_.element == FTCUDA_ELEMENT_BF16, l_.planes, static_cast<std::uint32_t>(l_.capacity), static_cast<std::uint32_t>(q_.depth), rows_,
-                                      {base_ + l_.hidden, l_.copy_pitch, l_.capacity * l_.copy_pitch}, status, sms_, stream_, message_, capacity_};
+                                      {base_ + l_.hidden, l_.copy_pitch, l_.capacity * l_.copy_pitch}, status, sms_, stream_, message_, capacity_, false};
         if (message_ != nullptr && capacity_ != 0) { message_[0] = '\0'; }
         return 0;
     }
@@ -754,8 +755,8 @@ class Call final {
         return error == cudaSuccess ? join(loss, lse, false) : error;
     }
 
-    // The loss, and the gradients for an upstream gradient of 1, with the logits computed once.
-    cudaError_t step(float* loss, void* grad_hidden, std::int64_t hidden_stride, void* grad_weight, std::int64_t weight_stride, std::int32_t grad_element) {
+    // The loss and, for an upstream gradient of 1, the slopes, with the logits computed once.
+    cudaError_t stepLoss(float* loss) {
         ListParams list = listParams();
         list.scale_bits = scaleBits();
         listTokens<true><<<1, kListThreads, 0, stream_>>>(list);
@@ -772,16 +773,31 @@ class Call final {
         if (error == cudaSuccess) { error = join(loss, nullptr, true); }
         if (error != cudaSuccess) { return error; }
         if (l_.library) {
-            error = training::launchOverlapped(rowSlopes, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(0, columns, nullptr));
+            return training::launchOverlapped(rowSlopes, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(0, columns, nullptr));
         } else {
             const KeptParams params{rows_, partials, static_cast<std::uint32_t>(l_.pieces), loss::statisticsWidth(columns, static_cast<std::uint32_t>(l_.capacity), sms_), static_cast<std::uint32_t>(l_.capacity),
                                     l_.piece_pitch, slopesPlane()};
             const dim3 grid(static_cast<unsigned>(ceilDiv(l_.pieces, kKeptPieces) * (l_.capacity / kKeptRows)));  // (of x, which takes any number)
             const auto kernel = l_.planes ? keptSlopes<float> : q_.element == FTCUDA_ELEMENT_FP16 ? keptSlopes<__half> : keptSlopes<__nv_bfloat16>;
-            error             = training::launchOverlapped(kernel, grid, dim3(256), 0, stream_, params, kept, at<std::uint16_t>(l_.piece));
+            return training::launchOverlapped(kernel, grid, dim3(256), 0, stream_, params, kept, at<std::uint16_t>(l_.piece));
         }
-        if (error == cudaSuccess) { error = multiplySlopes(0, columns, grad_hidden != nullptr, grad_weight, weight_stride, grad_element); }
-        return error == cudaSuccess && grad_hidden != nullptr ? spreadTyped(grad_hidden, hidden_stride, grad_element) : error;
+    }
+
+    // The gradients from the slopes that stepLoss left in the workspace, for an upstream gradient of *upstream (NULL: 1).
+    cudaError_t stepGradients(const float* upstream, void* grad_hidden, std::int64_t hidden_stride, void* grad_weight, std::int64_t weight_stride, std::int32_t grad_element,
+                              bool starts) {
+        products_.starts  = starts;
+        cudaError_t error = multiplySlopes(0, q_.vocabulary, grad_hidden != nullptr, grad_weight, weight_stride, grad_element, upstream);
+        if (error == cudaSuccess && grad_hidden != nullptr) { error = spreadTyped(grad_hidden, hidden_stride, grad_element, upstream); }
+        if (error != cudaSuccess || !l_.library || grad_weight == nullptr || upstream == nullptr) { return error; }
+        // (The library's products take a factor from the host alone.)
+        FtcudaGradient all{};
+        all.data = all.out = grad_weight;
+        all.rows           = q_.vocabulary;
+        all.cols           = q_.depth;
+        all.row_stride = all.out_row_stride = weight_stride;
+        all.element = all.out_element = grad_element;
+        return ftcuda_gradient_scale(&all, 1, upstream, q_.device, stream_, message_, capacity_) == 0 ? cudaSuccess : cudaErrorUnknown;
     }
 
     cudaError_t backward(const float* lse, const float* grad_loss, void* grad_hidden, std::int64_t hidden_stride, void* grad_weight, std::int64_t weight_stride) {
@@ -795,9 +811,9 @@ class Call final {
         for (std::uint64_t first = 0; first < q_.vocabulary && error == cudaSuccess; first += l_.columns) {
             const std::uint64_t columns = std::min(l_.columns, q_.vocabulary - first);
             error                       = slopes(first, columns);
-            if (error == cudaSuccess) { error = multiplySlopes(first, columns, grad_hidden != nullptr, grad_weight, weight_stride, q_.element); }
+            if (error == cudaSuccess) { error = multiplySlopes(first, columns, grad_hidden != nullptr, grad_weight, weight_stride, q_.element, nullptr); }
         }
-        return error == cudaSuccess && grad_hidden != nullptr ? spreadTyped(grad_hidden, hidden_stride, q_.element) : error;
+        return error == cudaSuccess && grad_hidden != nullptr ? spreadTyped(grad_hidden, hidden_stride, q_.element, nullptr) : error;
     }
 
   private:
@@ -912,7 +928,8 @@ class Call final {
     }
 
     // What dZ of a piece is multiplied with.
-    cudaError_t multiplySlopes(std::uint64_t first, std::uint64_t columns, bool hidden, void* grad_weight, std::int64_t weight_stride, std::int32_t grad_element) const {
+    cudaError_t multiplySlopes(std::uint64_t first, std::uint64_t columns, bool hidden, void* grad_weight, std::int64_t weight_stride, std::int32_t grad_element,
+                               const float* upstream) const {
         if (!l_.library) {
             loss::Gradients gradients{};
             gradients.sums                  = hidden ? at<float>(l_.sums) : nullptr;
@@ -921,6 +938,7 @@ class Call final {
             gradients.accumulate            = first != 0;
             gradients.weight_gradient_fp32  = grad_element == FTCUDA_ELEMENT_FP32;
             gradients.weight_gradient_pitch = weight_stride;
+            gradients.upstream              = upstream;
             if (grad_weight != nullptr) {
                 gradients.weight_gradient =
                     static_cast<unsigned char*>(grad_weight) + static_cast<std::int64_t>(training::elementBytes(grad_element) * first) * weight_stride;
@@ -933,20 +951,20 @@ class Call final {
         return error;
     }
 
-    cudaError_t spreadTyped(void* out, std::int64_t stride, std::int32_t element) const {
+    cudaError_t spreadTyped(void* out, std::int64_t stride, std::int32_t element, const float* upstream) const {
         switch (element) {
-            case FTCUDA_ELEMENT_FP32: return spread(static_cast<float*>(out), stride);
-            case FTCUDA_ELEMENT_FP16: return spread(static_cast<__half*>(out), stride);
-            default: return spread(static_cast<__nv_bfloat16*>(out), stride);
+            case FTCUDA_ELEMENT_FP32: return spread(static_cast<float*>(out), stride, upstream);
+            case FTCUDA_ELEMENT_FP16: return spread(static_cast<__half*>(out), stride, upstream);
+            default: return spread(static_cast<__nv_bfloat16*>(out), stride, upstream);
         }
     }
 
-    template<typename T> cudaError_t spread(T* out, std::int64_t stride) const {
+    template<typename T> cudaError_t spread(T* out, std::int64_t stride, const float* upstream) const {
         // (64 x 2048 in 16 parts: 14 us with a CTA for each token, 5 with eight; 4096 x 512 in one: 14, and 20 with two.)
         const std::uint64_t each = std::min(ceilDiv(q_.depth, kGatherThreads), std::max<std::uint64_t>(1, static_cast<std::uint64_t>(sms_) * 4 / q_.tokens));
         return training::launchOverlapped(spreadHidden<T>, dim3(static_cast<unsigned>(q_.tokens), static_cast<unsigned>(each)), dim3(kGatherThreads), 0, stream_, rows_,
                                           static_cast<const std::int32_t*>(at<std::int32_t>(l_.slot)), static_cast<const float*>(at<float>(l_.sums)), l_.capacity * l_.sums_pitch,
-                                          l_.sums_pitch, l_.splits, static_cast<std::uint32_t>(q_.depth), out, stride);
+                                          l_.sums_pitch, static_cast<std::uint32_t>(l_.capacity), l_.splits, static_cast<std::uint32_t>(q_.depth), upstream, out, stride);
     }
 
     const FtcudaLinearCrossEntropy& q_;
@@ -1047,7 +1065,40 @@ extern "C" int ftcuda_linear_cross_entropy_step(const FtcudaLinearCrossEntropy* 
     if (reason != nullptr) { return fail(message, message_capacity, 1, "%s", reason); }
     Call call(*problem, message, message_capacity);
     if (const int status = call.begin(Form::kStep, workspace, workspace_bytes, stream)) { return status; }
-    return finish(call.step(loss, grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride, grad_element), message, message_capacity);
+    cudaError_t error = call.stepLoss(loss);
+    if (error == cudaSuccess) { error = call.stepGradients(nullptr, grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride, grad_element, false); }
+    return finish(error, message, message_capacity);
+}
+
+extern "C" int ftcuda_linear_cross_entropy_step_loss(const FtcudaLinearCrossEntropy* problem, float* loss, void* workspace, uint64_t workspace_bytes, void* stream, char* message,
+                                                     size_t message_capacity) {
+    using namespace ftcuda;
+    if (problem == nullptr) { return fail(message, message_capacity, 1, "null problem"); }
+    const char* reason = check(*problem);
+    if (reason == nullptr) { reason = checkStep(*problem); }
+    if (reason == nullptr && !wordAligned(loss)) { reason = "the loss has no address, or one that is not a multiple of four"; }
+    if (reason != nullptr) { return fail(message, message_capacity, 1, "%s", reason); }
+    Call call(*problem, message, message_capacity);
+    if (const int status = call.begin(Form::kStep, workspace, workspace_bytes, stream)) { return status; }
+    return finish(call.stepLoss(loss), message, message_capacity);
+}
+
+extern "C" int ftcuda_linear_cross_entropy_step_gradients(const FtcudaLinearCrossEntropy* problem, const float* grad_loss, void* grad_hidden, int64_t grad_hidden_row_stride,
+                                                          void* grad_weight, int64_t grad_weight_row_stride, void* workspace, uint64_t workspace_bytes, void* stream,
+                                                          char* message, size_t message_capacity) {
+    using namespace ftcuda;
+    if (problem == nullptr) { return fail(message, message_capacity, 1, "null problem"); }
+    const char* reason = check(*problem);
+    if (reason == nullptr) { reason = checkStep(*problem); }
+    if (reason == nullptr && !wordAligned(grad_loss)) { reason = "the loss's gradient has no address, or one that is not a multiple of four"; }
+    if (reason == nullptr) {
+        reason = checkGradients(*problem, training::elementBytes(problem->element), grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride);
+    }
+    if (reason != nullptr) { return fail(message, message_capacity, 1, "%s", reason); }
+    if (grad_hidden == nullptr && grad_weight == nullptr) { return 0; }
+    Call call(*problem, message, message_capacity);
+    if (const int status = call.begin(Form::kStep, workspace, workspace_bytes, stream)) { return status; }
+    return finish(call.stepGradients(grad_loss, grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride, problem->element, true), message, message_capacity);
 }
 
 extern "C" int ftcuda_linear_cross_entropy(const FtcudaLinearCrossEntropy* problem, float* loss, float* lse, void* workspace, uint64_t workspace_bytes, void* stream,

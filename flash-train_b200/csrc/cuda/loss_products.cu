@@ -123,6 +123,7 @@ struct ProductParams {
     std::int64_t weight_gradient_pitch;
     std::uint32_t weight_fp32;
     std::uint32_t weight_vector;   // elements of it that one aligned store takes: 16, 8, or 1
+    const float* upstream;         // NULL: 1
     int* status;
 };
 
@@ -454,7 +455,7 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
     // Launched with programmatic stream serialization: what is above overlaps the predecessor's tail.
     gridDependencyWait();
     gridDependencyLaunchDependents();
-    const std::uint32_t live = *p.rows.count;
+    const std::uint32_t live = min(*p.rows.count, p.capacity);  // (never beyond, whatever stands there)
     const Work work          = workOf(p, live, pairs);
 
     if (warp >= kFirstEpilogue) {
@@ -464,7 +465,7 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
         const std::uint32_t in_tile   = static_cast<std::uint32_t>(32 * (warp & 3));  // the tensor-memory lanes a warp can read
         const std::uint32_t tmem_row  = tmem_base + (in_tile << 16);
         const std::uint32_t sum_empty[2] = {mapToRank(&bars->sum_empty[0], 0), mapToRank(&bars->sum_empty[1], 0)};
-        const float unit              = kMode == kGradients ? *p.rows.unit : 1.0F;
+        const float unit              = kMode != kGradients ? 1.0F : *p.rows.unit * (p.upstream != nullptr ? *p.upstream : 1.0F);
         std::uint32_t sums = 0;
         bool ok = true;
         for (std::uint32_t n = 0, item; ok && (item = itemOf(work, pair, pairs, n)) != kNoItem; ++n) {
@@ -661,7 +662,7 @@ template<int kMode> cudaError_t launch(const ProductCall& call, const ProductMap
     cudaError_t error = cudaFuncSetAttribute(lossProduct<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (error != cudaSuccess) { return error; }
     const std::uint64_t pairs = std::max<std::uint64_t>(1, std::min<std::uint64_t>(static_cast<std::uint64_t>(call.sms) / 2, items));
-    return training::launchOverlapped(lossProduct<kMode>, dim3(static_cast<unsigned>(2 * pairs)), dim3(kThreads), kSmemBytes, call.stream, maps, p);
+    return training::launchKernel(!call.starts, lossProduct<kMode>, dim3(static_cast<unsigned>(2 * pairs)), dim3(kThreads), kSmemBytes, call.stream, maps, p);
 }
 
 ProductParams paramsFor(const ProductCall& call) {
@@ -759,6 +760,7 @@ cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint3
     ProductMaps maps;
     ProductParams p = paramsFor(call);
     p.problems      = 0;
+    p.upstream      = gradients.upstream;
     std::uint64_t items        = 0;
     const std::uint32_t tile_n = tileColumns(call.depth), tiles_n = divideUp(call.depth, tile_n);
     bool encoded = true;

@@ -50,6 +50,7 @@ struct ProductCall {
     cudaStream_t stream;
     char* message;
     std::size_t message_capacity;
+    bool starts;              // a call with this product: an ordinary launch, which waits for all that came before in the stream
 };
 
 // Columns of the vocabulary that one partial result of the statistics covers, and how many of those there are.
@@ -84,6 +85,7 @@ struct Gradients {
     void* weight_gradient;
     std::int64_t weight_gradient_pitch;
     bool weight_gradient_fp32;  // or of the operands' type
+    const float* upstream;      // a number that the weight's gradient is multiplied by as well; NULL: 1
 };
 cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint32_t columns, Matrix16 slopes, const Gradients& gradients);
 

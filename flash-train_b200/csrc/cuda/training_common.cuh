@@ -68,10 +68,10 @@ inline bool deviceIsCurrent(std::int32_t device, char* message, std::size_t capa
     return true;
 }
 
-// A kernel launch that may start while the stream's preceding kernel ends (which the kernel waits for by gridDependencyWait).
+// A kernel launch; `overlapped`: one that may start while the stream's preceding kernel ends (which the kernel waits for by gridDependencyWait).
 template<typename... Parameters, typename... Arguments>
-cudaError_t launchOverlapped(void (*kernel)(Parameters...), dim3 grid, dim3 block, std::size_t shared, cudaStream_t stream,
-                             const Arguments&... arguments) {
+cudaError_t launchKernel(bool overlapped, void (*kernel)(Parameters...), dim3 grid, dim3 block, std::size_t shared, cudaStream_t stream,
+                         const Arguments&... arguments) {
     cudaLaunchConfig_t config{};
     config.gridDim          = grid;
     config.blockDim         = block;
@@ -81,10 +81,16 @@ cudaError_t launchOverlapped(void (*kernel)(Parameters...), dim3 grid, dim3 bloc
     attribute.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;
     config.attrs                                         = &attribute;
-    config.numAttrs                                      = 1;
+    config.numAttrs                                      = overlapped ? 1 : 0;
     const cudaError_t error = cudaLaunchKernelEx(&config, kernel, arguments...);
     if (error == cudaSuccess) { countLaunches(1); }
     return error;
+}
+
+template<typename... Parameters, typename... Arguments>
+cudaError_t launchOverlapped(void (*kernel)(Parameters...), dim3 grid, dim3 block, std::size_t shared, cudaStream_t stream,
+                             const Arguments&... arguments) {
+    return launchKernel(true, kernel, grid, block, shared, stream, arguments...);
 }
 
 }  // namespace training

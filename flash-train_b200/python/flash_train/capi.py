@@ -56,7 +56,8 @@ PLATFORM_SYMBOLS = (
     "ftcuda_grouped_gemm_launch ftcuda_grouped_gemm_destroy ftcuda_gradient_norm_workspace_bytes ftcuda_gradient_norm "
     "ftcuda_gradient_clip ftcuda_expert_routing_workspace_bytes ftcuda_expert_routing ftcuda_expert_routing_backward "
     "ftcuda_linear_cross_entropy_workspace_bytes ftcuda_linear_cross_entropy ftcuda_linear_cross_entropy_backward "
-    "ftcuda_linear_cross_entropy_step_workspace_bytes ftcuda_linear_cross_entropy_step ftcuda_gradient_scale"
+    "ftcuda_linear_cross_entropy_step_workspace_bytes ftcuda_linear_cross_entropy_step ftcuda_gradient_scale "
+    "ftcuda_linear_cross_entropy_step_loss ftcuda_linear_cross_entropy_step_gradients"
 ).split()
 
 
@@ -672,11 +673,14 @@ def _declare_training(lib) -> None:
     lib.ftcuda_linear_cross_entropy.argtypes = problem + [c_void_p] * 2 + work
     lib.ftcuda_linear_cross_entropy_step_workspace_bytes.argtypes = problem + [POINTER(c_uint64)] + message
     lib.ftcuda_linear_cross_entropy_step.argtypes = problem + [c_void_p, ctypes.c_int32, c_void_p, c_int64, c_void_p, c_int64] + work
+    lib.ftcuda_linear_cross_entropy_step_loss.argtypes = problem + [c_void_p] + work
+    lib.ftcuda_linear_cross_entropy_step_gradients.argtypes = problem + [c_void_p] * 2 + [c_int64, c_void_p, c_int64] + work
     lib.ftcuda_gradient_scale.argtypes = [POINTER(Gradient), c_uint64, c_void_p, ctypes.c_int32, c_void_p] + message
     lib.ftcuda_linear_cross_entropy_backward.argtypes = problem + [c_void_p] * 3 + [c_int64, c_void_p, c_int64] + work
     for name in ("ftcuda_gradient_norm", "ftcuda_gradient_clip", "ftcuda_expert_routing", "ftcuda_expert_routing_backward",
                  "ftcuda_linear_cross_entropy_workspace_bytes", "ftcuda_linear_cross_entropy", "ftcuda_linear_cross_entropy_backward",
-                 "ftcuda_linear_cross_entropy_step_workspace_bytes", "ftcuda_linear_cross_entropy_step", "ftcuda_gradient_scale"):
+                 "ftcuda_linear_cross_entropy_step_workspace_bytes", "ftcuda_linear_cross_entropy_step", "ftcuda_gradient_scale",
+                 "ftcuda_linear_cross_entropy_step_loss", "ftcuda_linear_cross_entropy_step_gradients"):
         getattr(lib, name).restype = ctypes.c_int
 
 
@@ -753,6 +757,18 @@ def linear_cross_entropy_step(problem: LinearCrossEntropy, loss: int, grad_eleme
                               grad_weight_row_stride: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
     """ftcuda_linear_cross_entropy_step: the loss, and the gradients for an upstream gradient of 1; 0 for one that is not wanted."""
     _run_training(lib.ftcuda_linear_cross_entropy_step, byref(problem), loss, grad_element, grad_hidden, grad_hidden_row_stride, grad_weight,
+                  grad_weight_row_stride, workspace, workspace_bytes, stream)
+
+
+def linear_cross_entropy_step_loss(problem: LinearCrossEntropy, loss: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    """ftcuda_linear_cross_entropy_step_loss: the loss, and in the workspace what its gradients are made of."""
+    _run_training(lib.ftcuda_linear_cross_entropy_step_loss, byref(problem), loss, workspace, workspace_bytes, stream)
+
+
+def linear_cross_entropy_step_gradients(problem: LinearCrossEntropy, grad_loss: int, grad_hidden: int, grad_hidden_row_stride: int, grad_weight: int,
+                                        grad_weight_row_stride: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    """ftcuda_linear_cross_entropy_step_gradients from the workspace that linear_cross_entropy_step_loss left; 0 for a gradient that is not wanted."""
+    _run_training(lib.ftcuda_linear_cross_entropy_step_gradients, byref(problem), grad_loss, grad_hidden, grad_hidden_row_stride, grad_weight,
                   grad_weight_row_stride, workspace, workspace_bytes, stream)
 
 

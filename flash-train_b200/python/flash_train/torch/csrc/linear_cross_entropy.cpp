@@ -3,11 +3,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/engine.h>
-#include <torch/csrc/autograd/graph_task.h>
 
 #include <string>
-#include <vector>
 
 #include <ftcuda/training.h>
 
@@ -91,57 +88,40 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
     }
 };
 
-// Both at once, for an upstream gradient of 1; the backward pass only multiplies by the one that comes. FP16 operands' gradients
-// wait in FP32: without the loss's scale, which comes then, many of them are too small for FP16.
+// The logits are computed once: the forward pass leaves in its workspace what the gradients are made of, which the graph keeps until the backward pass.
 class LinearCrossEntropyStep : public torch::autograd::Function<LinearCrossEntropyStep> {
   public:
     static at::Tensor forward(AutogradContext* context, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, std::int64_t ignore_index,
                               std::int64_t reduction, std::int64_t workspace_bytes) {
         const c10::cuda::CUDAGuard guard(hidden.device());
         const FtcudaLinearCrossEntropy q = describe(hidden, weight, target, ignore_index, reduction);
-        const auto floats                = hidden.options().dtype(at::kFloat).requires_grad(false);
-        const auto kept                  = hidden.scalar_type() == at::kHalf ? floats : hidden.options().requires_grad(false);
-        at::Tensor loss                  = at::empty({}, floats);
-        at::Tensor grad_hidden, grad_weight;
-        if (hidden.requires_grad()) { grad_hidden = at::empty(hidden.sizes(), kept); }
-        if (weight.requires_grad()) { grad_weight = at::empty(weight.sizes(), kept); }
-        const at::Tensor workspace = workspaceFor(static_cast<std::uint64_t>(workspace_bytes), hidden);
+        at::Tensor loss                  = at::empty({}, hidden.options().dtype(at::kFloat).requires_grad(false));
+        const at::Tensor workspace       = workspaceFor(static_cast<std::uint64_t>(workspace_bytes), hidden);
         Message message;
-        const int status = ftcuda_linear_cross_entropy_step(&q, loss.data_ptr<float>(), elementOf(grad_hidden.defined() ? grad_hidden : grad_weight), addressOf(grad_hidden),
-                                                            hidden.size(1), addressOf(grad_weight), hidden.size(1), workspace.data_ptr(),
-                                                            static_cast<std::uint64_t>(workspace_bytes), streamOf(q), message.text, sizeof message.text);
+        const int status = ftcuda_linear_cross_entropy_step_loss(&q, loss.data_ptr<float>(), workspace.data_ptr(), static_cast<std::uint64_t>(workspace_bytes), streamOf(q),
+                                                                 message.text, sizeof message.text);
         TORCH_CHECK(status == 0, "flash_train linear_cross_entropy failed: ", message.text);
-        context->save_for_backward({grad_hidden, grad_weight});
-        context->saved_data["type"] = hidden.scalar_type();
+        context->save_for_backward({hidden, weight, target, workspace});
+        context->saved_data["ignore_index"] = ignore_index;
+        context->saved_data["reduction"]    = reduction;
         return loss;
     }
 
     static variable_list backward(AutogradContext* context, const variable_list& gradients) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "linear_cross_entropy has no second derivative (create_graph=True)");
-        const variable_list saved  = context->get_saved_variables();
-        const at::ScalarType type  = context->saved_data["type"].toScalarType();
+        const variable_list saved = context->get_saved_variables();
+        const at::Tensor &hidden = saved[0], &weight = saved[1], &target = saved[2], &workspace = saved[3];
         const at::Tensor grad_loss = gradients[0].to(at::kFloat).contiguous();
-        const c10::cuda::CUDAGuard guard(grad_loss.device());
-        // Without another backward pass to come, what waited is the result's memory as well.
-        const bool last = !torch::autograd::get_current_graph_task_keep_graph();
+        const c10::cuda::CUDAGuard guard(hidden.device());
+        const FtcudaLinearCrossEntropy q =
+            describe(hidden, weight, target, context->saved_data["ignore_index"].toInt(), context->saved_data["reduction"].toInt());
         variable_list out(6);
-        std::vector<FtcudaGradient> described;
-        for (std::size_t i = 0; i < 2; ++i) {
-            const at::Tensor& from = saved[i];
-            if (!from.defined() || !context->needs_input_grad(i)) { continue; }
-            out[i] = last && from.scalar_type() == type ? from : at::empty(from.sizes(), from.options().dtype(type));
-            FtcudaGradient g{};
-            g.data        = from.data_ptr();
-            g.out         = out[i].data_ptr();
-            g.rows        = 1;
-            g.cols        = static_cast<std::uint64_t>(from.numel());
-            g.element     = elementOf(from);
-            g.out_element = elementOf(out[i]);
-            described.push_back(g);
-        }
+        if (context->needs_input_grad(0)) { out[0] = at::empty(hidden.sizes(), hidden.options().requires_grad(false)); }
+        if (context->needs_input_grad(1)) { out[1] = at::empty(weight.sizes(), weight.options().requires_grad(false)); }
         Message message;
-        const int status = ftcuda_gradient_scale(described.data(), described.size(), grad_loss.data_ptr<float>(), grad_loss.device().index(),
-                                                 c10::cuda::getCurrentCUDAStream(grad_loss.device().index()).stream(), message.text, sizeof message.text);
+        const int status = ftcuda_linear_cross_entropy_step_gradients(&q, grad_loss.data_ptr<float>(), addressOf(out[0]), hidden.size(1), addressOf(out[1]), hidden.size(1),
+                                                                      workspace.data_ptr(), static_cast<std::uint64_t>(workspace.numel()), streamOf(q), message.text,
+                                                                      sizeof message.text);
         TORCH_CHECK(status == 0, "flash_train linear_cross_entropy's gradient failed: ", message.text);
         return out;
     }

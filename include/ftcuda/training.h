@@ -145,6 +145,18 @@ FTCUDA_API int ftcuda_linear_cross_entropy_step(const FtcudaLinearCrossEntropy* 
                                                 void* workspace, uint64_t workspace_bytes, void* stream, char* message,
                                                 size_t message_capacity);
 
+/*
+ * The step call in two: the loss first, and the gradients when the upstream gradient (*grad_loss, FP32 on the device) is known, of the operands' type and
+ * rounded once. In between the workspace keeps what they are made of, for the same problem, and so does the weight; the hidden states and the targets are not looked at again.
+ * The second call may be made any number of times.
+ */
+FTCUDA_API int ftcuda_linear_cross_entropy_step_loss(const FtcudaLinearCrossEntropy* problem, float* loss, void* workspace, uint64_t workspace_bytes,
+                                                     void* stream, char* message, size_t message_capacity);
+FTCUDA_API int ftcuda_linear_cross_entropy_step_gradients(const FtcudaLinearCrossEntropy* problem, const float* grad_loss, void* grad_hidden,
+                                                          int64_t grad_hidden_row_stride, void* grad_weight, int64_t grad_weight_row_stride,
+                                                          void* workspace, uint64_t workspace_bytes, void* stream, char* message,
+                                                          size_t message_capacity);
+
 /* ---- the experts' router ---- */
 
 /*

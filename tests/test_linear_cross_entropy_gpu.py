@@ -600,3 +600,50 @@ def test_a_weight_past_32_bits(ft, memory_given_back, dtype, tokens, vocabulary,
         value = slope[:, rows].T @ h
         bound = (error[:, rows].T + (tokens / 8 + 24) * 2 * STEP * slope[:, rows].T.abs()) @ h.abs()
         check(grad_weight[rows], value, bound + 1.01 * half_step * value.abs() + finfo.smallest_normal * finfo.eps, "weight's gradient")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens, depth, vocabulary", [(1, 64, 128), (64, 1024, 700), (300, 96, 1500), (900, 1600, 2000), (1537, 200, 4001)])
+def test_the_step_in_two(ft, capi, tokens, depth, vocabulary, dtype):
+    """The loss first and gradients twice, with operands and gradients whose rows lie apart: as the step in one where the upstream gradient is 1, and for another one
+    against the definition."""
+    hidden, weight, target = make(tokens, depth, vocabulary, dtype, seed=60)
+    target[2::5] = -100
+    wide = torch.full((tokens, depth + 24), math.nan, device="cuda", dtype=dtype)
+    wide[:, :depth] = hidden
+    q = capi.LinearCrossEntropy(hidden=wide.data_ptr(), weight=weight.data_ptr(), target=target.data_ptr(), tokens=tokens, vocabulary=vocabulary, depth=depth,
+                                hidden_row_stride=depth + 24, weight_row_stride=depth, ignore_index=-100, element={torch.float32: 4, torch.float16: 7, torch.bfloat16: 8}[dtype],
+                                reduction=1, device=0)
+    stream = torch.cuda.current_stream().cuda_stream
+    size = capi.linear_cross_entropy_step_workspace_bytes(q)
+    workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+    losses, upstreams = torch.full((2,), math.nan, device="cuda"), torch.tensor([1.0, 37.5], device="cuda")
+    out = [(torch.full((tokens, depth + 8), 7.0, device="cuda", dtype=dtype), torch.full((vocabulary, depth + 16), 7.0, device="cuda", dtype=dtype)) for _ in range(3)]
+    capi.linear_cross_entropy_step(q, losses.data_ptr(), q.element, out[0][0].data_ptr(), depth + 8, out[0][1].data_ptr(), depth + 16, workspace.data_ptr(), size, stream)
+    workspace.fill_(255)
+    capi.linear_cross_entropy_step_loss(q, losses.data_ptr() + 4, workspace.data_ptr(), size, stream)
+    for i in (1, 2):
+        capi.linear_cross_entropy_step_gradients(q, upstreams.data_ptr() + 4 * (i - 1), out[i][0].data_ptr(), depth + 8, out[i][1].data_ptr(), depth + 16, workspace.data_ptr(),
+                                                 size, stream)
+    torch.cuda.synchronize()
+    assert torch.equal(losses[0], losses[1]) and torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+    assert all((x[:, depth:] == 7).all() for pair in out for x in pair)  # nothing beside the rows
+    oracle = Oracle(hidden, weight, target)
+    live = max(1, int(oracle.live.sum()))
+    dh, dh_bound, dw, dw_bound = oracle.gradients(torch.full((tokens,), 37.5 / live, device="cuda", dtype=torch.float64), dtype)
+    # (FP32 by the library's products: one more rounding, by the factor.)
+    check(out[2][0][:, :depth], dh, dh_bound + 2 * STEP * dh.abs(), "hidden's gradient")
+    check(out[2][1][:, :depth], dw, dw_bound + 2 * STEP * dw.abs(), "weight's gradient")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_what_changes_between_the_passes(ft, dtype):
+    """An operand that is overwritten between the passes is noticed, as torch's own operators do."""
+    for which in range(3):
+        operands = make(100, 64, 300, dtype, seed=61)
+        h, w = operands[0].clone().requires_grad_(), operands[1].clone().requires_grad_()
+        loss = ft.linear_cross_entropy(h, w, operands[2])
+        with torch.no_grad():
+            (h, w, operands[2])[which].add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(loss, (h, w))
