@@ -56,7 +56,8 @@ namespace {
 constexpr std::uint32_t kBlockK = 64;  // 128 bytes, one swizzle row
 constexpr std::uint32_t kTileN  = 256;
 constexpr std::uint32_t kItemBlocks  = 12;  // of an item: what it costs beside its own
-constexpr std::uint32_t kMostSplits  = 16;
+constexpr std::uint32_t kMostSplits  = 96;
+constexpr std::uint32_t kStreamSplits = 16;          // where the weight streams through; 96 are no faster there (1 x 512 x 131072 BF16: 183 us, 189)
 constexpr std::uint64_t kStreamTokens = 400;         // at which the tensor cores take as long as HBM does (times an FP32 product's terms)
 constexpr std::uint64_t kStreamBytes  = 64ULL << 20;  // half of L2
 constexpr std::uint32_t kSumBlocks   = 16;
@@ -731,13 +732,13 @@ cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t
 // The sum over the columns is cut into as many parts as let both gradients' items end soonest (all tokens taken for live), a part's way through memory and
 // back counted as well. Where the weight streams through (too large for L2, and too few tokens to be bound by anything else), into as many as make two items
 // for each pair of SMs, so that all of them fetch it. Measured, a step, always the latter / as here: 700 x 700 x 3000 FP32 133 / 104 us, 1024 x 600 x 9000 FP32 250 / 224,
-// 4096 x 512 x 32768 BF16 471 / 445; 257 x 4096 x 131072 BF16 920, and 1016 where the items alone decide, 64 x 2048 x 50257 205 and 218.
+// 4096 x 512 x 32768 BF16 471 / 445; with 16 parts at most, 256 x 104 x 99422 FP32 331, with up to 96 267; 257 x 4096 x 131072 BF16 920, and 1016 where the items alone decide, 64 x 2048 x 50257 205 and 218.
 std::uint32_t hiddenSplits(std::uint32_t tokens, std::uint32_t depth, std::uint32_t columns, bool planes, int sms) {
     const std::uint32_t across = divideUp(depth, tileColumns(depth)), tiles = divideUp(tokens, kTileRows) * across;
     const std::uint32_t pairs  = static_cast<std::uint32_t>(std::max(1, sms / 2));
     const std::uint32_t blocks = divideUp(columns, kBlockK), terms = planes ? kTerms : 1;
     if (static_cast<std::uint64_t>(tokens) * terms <= kStreamTokens && static_cast<std::uint64_t>(columns) * depth * 2 * (planes ? kPlanes : 1) > kStreamBytes) {
-        const std::uint32_t wanted = std::min({std::max(1U, blocks / 8), kMostSplits, std::max(1U, 2 * pairs / tiles)});
+        const std::uint32_t wanted = std::min({std::max(1U, blocks / 8), kStreamSplits, std::max(1U, 2 * pairs / tiles)});
         return divideUp(blocks, divideUp(blocks, wanted));
     }
     const std::uint32_t weight_items = divideUp(columns, kTileRows) * across, weight = divideUp(tokens, kBlockK) * terms + kItemBlocks;
