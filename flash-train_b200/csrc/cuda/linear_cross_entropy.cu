@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kGatherThreads) copyRows16(const std::uint16_t
 }
 
 // An FP32 matrix's rows as three BF16 matrices, `plane` elements apart, eight elements a thread. With `gathered`, the rows are those of the live tokens, and
-// zeros behind the last one. (16384 x 512: two elements a thread and a CTA a row 4 us more.) kWide: the rows begin at multiples of 16 bytes. (The planes' rows do, and have room for whole packs.)
+// zeros behind the last one. (16384 x 512: 14.5 us, 22.3 with two elements a thread and a CTA a row.) kWide: the rows begin at multiples of 16 bytes. (The planes' rows do, and have room for whole packs.)
 template<bool kWide>
 __global__ void __launch_bounds__(kGatherThreads) splitRows(const LiveRows rows, bool gathered, std::uint32_t count, const float* matrix, std::int64_t stride, std::uint16_t* to,
                                                             std::uint64_t pitch, std::uint64_t plane, std::uint32_t depth) {

@@ -291,11 +291,13 @@ __device__ __forceinline__ void finishStatistics(const ProductParams& p, const I
 #pragma unroll
         for (int j = 0; j < 128; ++j) { v[j] = col + j < columns ? v[j] : -INFINITY; }
     }
-    float largest = -INFINITY;
+    // (Four chains each: there are two warps a scheduler to hide what an instruction takes.)
+    float tops[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-    for (int j = 0; j < 128; ++j) {
-        if (j < 64 || pieces == 4) { largest = fmaxf(largest, v[j]); }
+    for (int j = 4; j < 128; ++j) {
+        if (j < 64 || pieces == 4) { tops[j % 4] = fmaxf(tops[j % 4], v[j]); }
     }
+    const float largest = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), -INFINITY);  // not NaN
     const bool none  = largest == -INFINITY;  // and no reference to subtract; sums of nothing (or of NaN) come out
     const float base = none ? 0.0F : largest * kLog2E;
     float sum[4] = {0.0F, 0.0F, 0.0F, 0.0F};
