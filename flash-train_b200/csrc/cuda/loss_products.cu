@@ -747,8 +747,12 @@ std::uint32_t hiddenSplits(std::uint32_t tokens, std::uint32_t depth, std::uint3
     const std::uint64_t apart  = static_cast<std::uint64_t>(tokens) * depth >> 19;  // a block's 512 cycles are the time of 2^21 bytes or so
     std::uint32_t best         = 1;
     std::uint64_t least        = ~std::uint64_t{0};
-    for (std::uint32_t wanted = 1; wanted <= std::min(blocks, kMostSplits); ++wanted) {
+    std::uint32_t before       = 0;
+    // (All numbers up to eight, then about every eighth part more: the host has this to do in every call.)
+    for (std::uint32_t wanted = 1; wanted <= std::min(blocks, kMostSplits); wanted += std::max(1U, wanted / 8)) {
         const std::uint32_t each = divideUp(blocks, wanted), splits = divideUp(blocks, each);  // none of them empty
+        if (splits == before) { continue; }
+        before                   = splits;
         const std::uint32_t part = each * terms + kItemBlocks;
         const std::uint64_t time = makespan(tiles * splits, part, weight_items, weight, pairs, earlyItems(tiles * splits, part, weight_items, weight, pairs)) + splits * apart;
         if (time < least) {
