@@ -167,15 +167,43 @@ __global__ void __launch_bounds__(kGatherThreads) gatherHidden(const LiveRows ro
     }
 }
 
-// A 16-bit weight that TMA cannot describe, copied with rows at multiples of 16 bytes.
-__global__ void __launch_bounds__(kGatherThreads) copyRows16(const std::uint16_t* from, std::int64_t stride, std::uint16_t* to, std::uint64_t pitch,
+// A 16-bit weight that TMA cannot describe, copied with rows at multiples of 16 bytes, eight elements a thread: out of the two packs of 16 bytes that they lie across
+// where both are between the weight's first and last element, else one by one. (What gets behind a row's last element is never fetched.) 13632 x 2311: 39 us less than
+// element by element, 60001 x 3967 286 less.
+__global__ void __launch_bounds__(kGatherThreads) copyRows16(const std::uint16_t* matrix, std::int64_t stride, std::uint32_t rows, std::uint16_t* to, std::uint64_t pitch,
                                                              std::uint32_t depth) {
     gridDependencyWait();
     gridDependencyLaunchDependents();
-    from += static_cast<std::int64_t>(blockIdx.x) * stride;
-    to += blockIdx.x * pitch;
-#pragma unroll 4
-    for (std::uint32_t i = threadIdx.x; i < depth; i += kGatherThreads) { to[i] = from[i]; }
+    const std::uintptr_t begin = reinterpret_cast<std::uintptr_t>(matrix), end = reinterpret_cast<std::uintptr_t>(matrix + static_cast<std::int64_t>(rows - 1) * stride + depth);
+    const std::uint32_t packs  = (depth + 7) / 8;
+    const std::uint64_t all    = static_cast<std::uint64_t>(rows) * packs, step = static_cast<std::uint64_t>(gridDim.x) * kGatherThreads;
+    for (std::uint64_t i = static_cast<std::uint64_t>(blockIdx.x) * kGatherThreads + threadIdx.x; i < all; i += step) {
+        const std::uint32_t row = static_cast<std::uint32_t>(i / packs), first = static_cast<std::uint32_t>(i - static_cast<std::uint64_t>(row) * packs) * 8;
+        const std::uint16_t* const from = matrix + static_cast<std::int64_t>(row) * stride + first;
+        const std::uintptr_t at         = reinterpret_cast<std::uintptr_t>(from), low = at & ~std::uintptr_t{15};
+        std::uint32_t out[4];
+        if (low >= begin && low + 32 <= end) {
+            const uint4 a = *reinterpret_cast<const uint4*>(low), b = *reinterpret_cast<const uint4*>(low + 16);
+            std::uint32_t words[8]    = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            const std::uint32_t shift = static_cast<std::uint32_t>(at - low);
+#pragma unroll
+            for (int by = 2; by > 0; by /= 2) {
+                if ((shift / 4 & by) != 0) {
+#pragma unroll
+                    for (int j = 0; j + by < 8; ++j) { words[j] = words[j + by]; }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { out[j] = __funnelshift_r(words[j], words[j + 1], shift % 4 * 8); }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const std::uint32_t left = first + 2 * j < depth ? from[2 * j] : 0, right = first + 2 * j + 1 < depth ? from[2 * j + 1] : 0;
+                out[j]                   = left | right << 16;
+            }
+        }
+        *reinterpret_cast<uint4*>(to + row * pitch + first) = make_uint4(out[0], out[1], out[2], out[3]);
+    }
 }
 
 // An FP32 matrix's rows as three BF16 matrices, `plane` elements apart, eight elements a thread. With `gathered`, the rows are those of the live tokens, and
@@ -877,8 +905,10 @@ class Call final {
         const bool wide          = row % 16 == 0 && training::aligned(q_.hidden, 16) && (q_.tokens <= 1 || static_cast<std::uint64_t>(q_.hidden_row_stride) * bytes % 16 == 0);
         cudaError_t error        = wide ? run(uint4{}) : bytes == 4 ? run(std::uint32_t{}) : run(std::uint16_t{});
         if (error == cudaSuccess && l_.weight_pitch != 0) {
-            error = training::launchOverlapped(copyRows16, dim3(static_cast<unsigned>(q_.vocabulary)), dim3(kGatherThreads), 0, stream_, static_cast<const std::uint16_t*>(q_.weight),
-                                               q_.weight_row_stride, at<std::uint16_t>(l_.weight), l_.weight_pitch, static_cast<std::uint32_t>(q_.depth));
+            const std::uint64_t ctas = std::min(ceilDiv(q_.vocabulary * ceilDiv(q_.depth, 8), kGatherThreads), static_cast<std::uint64_t>(sms_) * kSplitCtasPerSm);
+            error = training::launchOverlapped(copyRows16, dim3(static_cast<unsigned>(ctas)), dim3(kGatherThreads), 0, stream_, static_cast<const std::uint16_t*>(q_.weight),
+                                               q_.vocabulary == 1 ? std::int64_t{0} : q_.weight_row_stride, static_cast<std::uint32_t>(q_.vocabulary), at<std::uint16_t>(l_.weight),
+                                               l_.weight_pitch, static_cast<std::uint32_t>(q_.depth));
         }
         return error;
     }

@@ -70,8 +70,9 @@ constexpr int kThreads          = 384;
 constexpr int kOperandBytes     = 128 * 128;  // a CTA's share of A, and of a B of 256 columns
 constexpr int kStageBytes       = 2 * kOperandBytes;
 constexpr int kBarrierOffset    = kStages * kStageBytes;
-constexpr int kSmemBytes        = kBarrierOffset + 256 + 1024;
-static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
+constexpr int kScratchOffset    = kBarrierOffset + 256;
+constexpr int kScratchRow       = 33;  // words: rows of 32 numbers that neither rows nor columns have bank conflicts in
+constexpr int kScratchBytes     = 32 * kScratchRow * 4;  // of an epilogue warp
 constexpr std::uint32_t kBoxBytes = 64 * 128;  // 64 rows of 128 bytes: one box of an MN-major operand
 
 constexpr int kRegsLight = 72;   // producer, issuer (warpgroup 0)
@@ -84,6 +85,8 @@ constexpr int kFirstEpilogue = 4;
 constexpr std::uint32_t kTmemColumns = 512;
 
 enum Mode : int { kStatistics, kKept, kSlopes, kGradients };
+constexpr int smemBytes(int mode) { return kScratchOffset + 1024 + (mode == kGradients ? 8 * kScratchBytes : 0); }
+static_assert(smemBytes(kGradients) <= 232448, "shared memory of one CTA");
 
 struct Barriers {
     std::uint64_t full[kStages];  // used in the pair's first CTA
@@ -365,6 +368,35 @@ __device__ __forceinline__ void finishSums(const ProductParams& p, const Item& w
     }
 }
 
+// A gradient whose rows no aligned store fits (an odd depth, say): 32 columns at a time are turned in shared memory, so that a warp writes neighbours. (A thread writing
+// its own row element by element touches 32 rows with every store: a step of 72 x 2311 x 13632 FP16 took 502 us so and takes 140, of 1000 x 1001 x 20000 BF16 412 and 158.)
+__device__ __forceinline__ void finishWeightTurned(const ProductParams& p, const Problem& problem, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, float unit,
+                                                   float* scratch, float (&v)[128]) {
+    const std::uint32_t lane = threadIdx.x & 31, row0 = row - lane;
+    const std::uint32_t rows = row0 < problem.rows ? min(32U, problem.rows - row0) : 0;
+#pragma unroll
+    for (std::uint32_t q = 0; q < 4; ++q) {
+        if (q < pieces) {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) { scratch[lane * kScratchRow + j] = unit * v[q * 32 + j]; }
+            __syncwarp();
+            const std::uint32_t at = col + q * 32 + lane;
+            if (at < problem.columns) {
+                for (std::uint32_t i = 0; i < rows; ++i) {
+                    const float x            = scratch[i * kScratchRow + lane];
+                    const std::int64_t place = static_cast<std::int64_t>(row0 + i) * p.weight_gradient_pitch + at;
+                    if (p.weight_fp32 != 0) {
+                        static_cast<float*>(p.weight_gradient)[place] = x;
+                    } else {
+                        static_cast<std::uint16_t*>(p.weight_gradient)[place] = static_cast<std::uint16_t>(pack16(x, 0.0F, p.bf16 != 0));
+                    }
+                }
+            }
+        }
+    }
+}
+
 __device__ __forceinline__ void finishWeight(const ProductParams& p, const Problem& problem, std::uint32_t row, std::uint32_t col, std::uint32_t pieces,
                                              float unit, float (&v)[128]) {
     if (row >= problem.rows) { return; }
@@ -376,14 +408,7 @@ __device__ __forceinline__ void finishWeight(const ProductParams& p, const Probl
                 float o[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) { o[i] = unit * v[j + i]; }
-                if (p.weight_vector == 8) {
-                    if (col + j < problem.columns) { storeGlobal8(at + j, o); }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (col + j + i < problem.columns) { at[j + i] = o[i]; }
-                    }
-                }
+                if (col + j < problem.columns) { storeGlobal8(at + j, o); }
             }
         }
         return;
@@ -397,18 +422,11 @@ __device__ __forceinline__ void finishWeight(const ProductParams& p, const Probl
             for (int i = 0; i < 8; ++i) { packed[i] = pack16(unit * v[j + 2 * i], unit * v[j + 2 * i + 1], p.bf16 != 0); }
             if (p.weight_vector == 16) {
                 if (col + j < problem.columns) { storeGlobal8(at + 2 * j, packed); }
-            } else if (p.weight_vector == 8) {
+            } else {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if (col + j + 8 * i < problem.columns) {
                         *reinterpret_cast<uint4*>(at + 2 * j + 16 * i) = make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if (col + j + i < problem.columns) {
-                        *reinterpret_cast<std::uint16_t*>(at + 2 * (j + i)) = static_cast<std::uint16_t>(packed[i / 2] >> (16 * (i % 2)));
                     }
                 }
             }
@@ -506,7 +524,11 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
             } else if (kMode == kSlopes) {
                 finishSlopes(p, row, col, pieces, live, v);
             } else if (w.problem == p.weight_problem) {
-                finishWeight(p, problem, row, col, pieces, unit, v);
+                if (p.weight_vector != 1) {
+                    finishWeight(p, problem, row, col, pieces, unit, v);
+                } else {
+                    finishWeightTurned(p, problem, row, col, pieces, unit, reinterpret_cast<float*>(smem + kScratchOffset + e * kScratchBytes), v);
+                }
             } else {
                 finishSums(p, w, row, col, pieces, v);
             }
@@ -662,10 +684,10 @@ bool encodeOperand(CUtensorMap* map, const ProductCall& call, Matrix16 matrix, b
 }
 
 template<int kMode> cudaError_t launch(const ProductCall& call, const ProductMaps& maps, const ProductParams& p, std::uint64_t items) {
-    cudaError_t error = cudaFuncSetAttribute(lossProduct<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    cudaError_t error = cudaFuncSetAttribute(lossProduct<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, smemBytes(kMode));
     if (error != cudaSuccess) { return error; }
     const std::uint64_t pairs = std::max<std::uint64_t>(1, std::min<std::uint64_t>(static_cast<std::uint64_t>(call.sms) / 2, items));
-    return training::launchKernel(!call.starts, lossProduct<kMode>, dim3(static_cast<unsigned>(2 * pairs)), dim3(kThreads), kSmemBytes, call.stream, maps, p);
+    return training::launchKernel(!call.starts, lossProduct<kMode>, dim3(static_cast<unsigned>(2 * pairs)), dim3(kThreads), smemBytes(kMode), call.stream, maps, p);
 }
 
 ProductParams paramsFor(const ProductCall& call) {
