@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kGatherThreads) gatherHidden(const LiveRows ro
     }
 }
 
-// A 16-bit weight that TMA cannot describe, copied with rows at multiples of 16 bytes, eight elements a thread: out of the two packs of 16 bytes that they lie across
+// A weight that TMA cannot describe, copied with rows at multiples of 16 bytes, eight 16-bit elements (or halves of FP32 ones) a thread: out of the two packs of 16 bytes that they lie across
 // where both are between the weight's first and last element, else one by one. (What gets behind a row's last element is never fetched.) 13632 x 2311: 39 us less than
 // element by element, 60001 x 3967 286 less.
 __global__ void __launch_bounds__(kGatherThreads) copyRows16(const std::uint16_t* matrix, std::int64_t stride, std::uint32_t rows, std::uint16_t* to, std::uint64_t pitch,
@@ -527,7 +527,9 @@ std::uint64_t roundUp(std::uint64_t x, std::uint64_t unit) { return (x + unit - 
 bool isFp32(const FtcudaLinearCrossEntropy& q) { return q.element == FTCUDA_ELEMENT_FP32; }
 
 // Whether TMA can fetch the weight as it is.
-bool weightFits(const FtcudaLinearCrossEntropy& q) { return training::aligned(q.weight, 16) && (q.vocabulary == 1 || q.weight_row_stride % 8 == 0); }
+bool weightFits(const FtcudaLinearCrossEntropy& q) {
+    return training::aligned(q.weight, 16) && (q.vocabulary == 1 || q.weight_row_stride % (16 / static_cast<std::int64_t>(training::elementBytes(q.element))) == 0);
+}
 
 std::uint64_t weightStride(const FtcudaLinearCrossEntropy& q) {
     return q.vocabulary == 1 ? roundUp(q.depth, 8) : static_cast<std::uint64_t>(q.weight_row_stride);
@@ -566,7 +568,8 @@ int configureProduct(const FtcudaGemmDesc& desc, bool slopes, int sms, std::uint
 FtcudaGemmDesc describeLogits(const FtcudaLinearCrossEntropy& q, const Layout& l, unsigned char* base, std::uint64_t first, std::uint64_t columns) {
     FtcudaGemmDesc d{};
     d.a            = reinterpret_cast<const float*>(base + l.hidden);
-    d.b            = static_cast<const float*>(q.weight) + static_cast<std::int64_t>(first) * q.weight_row_stride;
+    d.b            = l.weight_pitch != 0 ? reinterpret_cast<const float*>(base + l.weight) + first * l.weight_pitch
+                                         : static_cast<const float*>(q.weight) + static_cast<std::int64_t>(first) * q.weight_row_stride;
     d.d            = reinterpret_cast<float*>(base + l.piece);
     d.alpha        = 1.0F;
     d.m            = q.tokens;
@@ -575,7 +578,7 @@ FtcudaGemmDesc describeLogits(const FtcudaLinearCrossEntropy& q, const Layout& l
     d.a_row_stride = static_cast<std::int64_t>(l.copy_pitch);
     d.a_col_stride = 1;
     d.b_row_stride = 1;
-    d.b_col_stride = q.vocabulary == 1 ? static_cast<std::int64_t>(q.depth) : q.weight_row_stride;
+    d.b_col_stride = l.weight_pitch != 0 ? static_cast<std::int64_t>(l.weight_pitch) : q.vocabulary == 1 ? static_cast<std::int64_t>(q.depth) : q.weight_row_stride;
     d.d_row_stride = static_cast<std::int64_t>(l.piece_pitch);
     d.d_col_stride = 1;
     d.device       = q.device;
@@ -653,7 +656,10 @@ int layOut(const FtcudaLinearCrossEntropy& q, Form form, int sms, Layout& l, cha
     const std::uint64_t bytes = logitBytes(q, form);
     l.capacity                = roundUp(std::max<std::uint64_t>(q.tokens, 1), loss::kTileRows);
     l.copy_pitch              = roundUp(q.depth, 8);
-    l.weight_pitch            = l.planes || (!l.library && !weightFits(q)) ? roundUp(q.depth, 8) : 0;
+    // (The prepared products split the weight whatever its rows' alignment; the others would copy it for each product, element by element: a step of 8 x 3967 x 60001 FP32
+    // 3166 us, 1309 with one copy; 1000 x 2311 x 20000, prepared, the loss 384, with a copy 411.)
+    const bool splits         = l.library && preparedFormPays(q.tokens, q.vocabulary, q.depth);
+    l.weight_pitch            = l.planes || (!splits && !weightFits(q)) ? roundUp(q.depth, 8) : 0;
     const std::uint64_t fill  = roundUp(q.vocabulary, 256);
     l.columns                 = form == Form::kStep ? fill : std::min(fill, std::max(kLeastColumns, kPieceBytes / (l.capacity * bytes) / 256 * 256));
     l.columns                 = roundUp(ceilDiv(fill, ceilDiv(fill, l.columns)), 256);  // pieces of about one size
@@ -674,7 +680,7 @@ int layOut(const FtcudaLinearCrossEntropy& q, Form form, int sms, Layout& l, cha
     l.target = take(4 * l.capacity);
     l.slot   = take(4 * l.capacity);
     l.hidden = take((l.planes ? 2 * loss::kPlanes : training::elementBytes(q.element)) * l.capacity * l.copy_pitch);
-    if (l.weight_pitch != 0) { l.weight = take((l.planes ? 2 * loss::kPlanes : 2) * q.vocabulary * l.weight_pitch); }
+    if (l.weight_pitch != 0) { l.weight = take((l.planes ? 2 * loss::kPlanes : training::elementBytes(q.element)) * q.vocabulary * l.weight_pitch); }
     if (gradients) {
         l.scale = take(4 * l.capacity);
         l.lse2  = take(4 * l.capacity);
@@ -905,10 +911,10 @@ class Call final {
         const bool wide          = row % 16 == 0 && training::aligned(q_.hidden, 16) && (q_.tokens <= 1 || static_cast<std::uint64_t>(q_.hidden_row_stride) * bytes % 16 == 0);
         cudaError_t error        = wide ? run(uint4{}) : bytes == 4 ? run(std::uint32_t{}) : run(std::uint16_t{});
         if (error == cudaSuccess && l_.weight_pitch != 0) {
-            const std::uint64_t ctas = std::min(ceilDiv(q_.vocabulary * ceilDiv(q_.depth, 8), kGatherThreads), static_cast<std::uint64_t>(sms_) * kSplitCtasPerSm);
+            const std::uint64_t words = bytes / 2, ctas = std::min(ceilDiv(q_.vocabulary * ceilDiv(words * q_.depth, 8), kGatherThreads), static_cast<std::uint64_t>(sms_) * kSplitCtasPerSm);
             error = training::launchOverlapped(copyRows16, dim3(static_cast<unsigned>(ctas)), dim3(kGatherThreads), 0, stream_, static_cast<const std::uint16_t*>(q_.weight),
-                                               q_.vocabulary == 1 ? std::int64_t{0} : q_.weight_row_stride, static_cast<std::uint32_t>(q_.vocabulary), at<std::uint16_t>(l_.weight),
-                                               l_.weight_pitch, static_cast<std::uint32_t>(q_.depth));
+                                               q_.vocabulary == 1 ? std::int64_t{0} : static_cast<std::int64_t>(words) * q_.weight_row_stride, static_cast<std::uint32_t>(q_.vocabulary),
+                                               at<std::uint16_t>(l_.weight), words * l_.weight_pitch, static_cast<std::uint32_t>(words * q_.depth));
         }
         return error;
     }

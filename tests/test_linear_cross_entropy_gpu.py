@@ -647,3 +647,16 @@ def test_what_changes_between_the_passes(ft, dtype):
             (h, w, operands[2])[which].add_(1)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(loss, (h, w))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens, depth, vocabulary, offset, gap", [(5, 1027, 517, 1, 0), (5, 131, 90, 2, 3), (70, 1025, 300, 3, 2), (130, 127, 1001, 5, 4), (300, 2051, 700, 7, 1),
+                                                                    (40, 1024, 600, 1, 7), (513, 259, 777, 6, 0), (1, 9, 3, 3, 1)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_weight_at_any_address(ft, dtype, tokens, depth, vocabulary, offset, gap, reduction):
+    """Rows at any distance from any element on, in a buffer whose other elements are NaN: copies take whole packs where they can, and nothing of the others is used."""
+    hidden, weight, target = make(tokens, depth, vocabulary, dtype, seed=70 + offset)
+    buffer = torch.full((offset + vocabulary * (depth + gap),), math.nan, device="cuda", dtype=dtype)
+    view = buffer[offset:].view(vocabulary, depth + gap)[:, :depth]
+    view.copy_(weight)
+    run_and_check(ft, hidden, view, target, reduction)
