@@ -490,7 +490,8 @@ __global__ void __launch_bounds__(kGatherThreads) spreadHidden(const LiveRows ro
                                                                std::int64_t stride) {
     gridDependencyWait();
     gridDependencyLaunchDependents();
-    const std::int32_t row = min(slot[blockIdx.x], static_cast<std::int32_t>(capacity) - 1);  // (never beyond, whatever stands there)
+    // (Never beyond, whatever stands there. Without slots every row is its own: the weight's gradient.)
+    const std::int32_t row = slot != nullptr ? min(slot[blockIdx.x], static_cast<std::int32_t>(capacity) - 1) : static_cast<std::int32_t>(blockIdx.x);
     const float unit       = *rows.unit * (upstream != nullptr ? *upstream : 1.0F);
     T* const to            = out + static_cast<std::int64_t>(blockIdx.x) * stride;
     const float* const from = sums + static_cast<std::uint64_t>(max(row, 0)) * pitch;
@@ -517,8 +518,10 @@ struct Layout {
     std::uint64_t piece_pitch;    // of Z or dZ, elements
     std::uint64_t pieces;         // partial statistics of a row
     std::uint32_t splits;         // of the sums for dH
+    std::uint32_t weight_splits;  // ... for dW, 1: it needs none
+    std::uint32_t weight_rows;    // rows of a part of those
     std::uint64_t sums_pitch;
-    std::uint64_t count, unit, token, target, scale, lse2, picked, row_loss, slot, hidden, weight, partials, piece, kept, sums, product, product_bytes;
+    std::uint64_t count, unit, token, target, scale, lse2, picked, row_loss, slot, hidden, weight, partials, piece, kept, sums, weight_sums, product, product_bytes;
     std::uint64_t total;
 };
 
@@ -658,16 +661,20 @@ int layOut(const FtcudaLinearCrossEntropy& q, Form form, int sms, Layout& l, cha
     l.copy_pitch              = roundUp(q.depth, 8);
     // (The prepared products split the weight whatever its rows' alignment; the others would copy it for each product, element by element: a step of 8 x 3967 x 60001 FP32
     // 3166 us, 1309 with one copy; 1000 x 2311 x 20000, prepared, the loss 384, with a copy 411.)
-    const bool splits         = l.library && preparedFormPays(q.tokens, q.vocabulary, q.depth);
-    l.weight_pitch            = l.planes || (!splits && !weightFits(q)) ? roundUp(q.depth, 8) : 0;
+    const bool split_anyway   = l.library && preparedFormPays(q.tokens, q.vocabulary, q.depth);
+    l.weight_pitch            = l.planes || (!split_anyway && !weightFits(q)) ? roundUp(q.depth, 8) : 0;
     const std::uint64_t fill  = roundUp(q.vocabulary, 256);
     l.columns                 = form == Form::kStep ? fill : std::min(fill, std::max(kLeastColumns, kPieceBytes / (l.capacity * bytes) / 256 * 256));
     l.columns                 = roundUp(ceilDiv(fill, ceilDiv(fill, l.columns)), 256);  // pieces of about one size
     l.piece_pitch             = l.columns;
     l.pieces                  = l.library ? ceilDiv(q.vocabulary, l.columns) : loss::statisticsPieces(static_cast<std::uint32_t>(q.vocabulary), static_cast<std::uint32_t>(l.capacity), sms);
     l.sums_pitch              = roundUp(q.depth, 8);
-    l.splits                  = l.library ? 1 : loss::hiddenSplits(static_cast<std::uint32_t>(std::max<std::uint64_t>(q.tokens, 1)), static_cast<std::uint32_t>(q.depth),
-                                                              static_cast<std::uint32_t>(std::min(l.columns, q.vocabulary)), l.planes, sms);
+    l.weight_rows             = static_cast<std::uint32_t>(roundUp(std::min(l.columns, q.vocabulary), loss::kTileRows));
+    const loss::GradientSplits splits = l.library ? loss::GradientSplits{1, 1}
+                                                  : loss::gradientSplits(static_cast<std::uint32_t>(std::max<std::uint64_t>(q.tokens, 1)), static_cast<std::uint32_t>(q.depth),
+                                                                         static_cast<std::uint32_t>(std::min(l.columns, q.vocabulary)), l.planes, sms);
+    l.splits                  = splits.hidden;
+    l.weight_splits           = splits.weight;
     std::uint64_t at = 0;
     const auto take  = [&](std::uint64_t size) {
         const std::uint64_t here = at;
@@ -685,6 +692,7 @@ int layOut(const FtcudaLinearCrossEntropy& q, Form form, int sms, Layout& l, cha
         l.scale = take(4 * l.capacity);
         l.lse2  = take(4 * l.capacity);
         l.sums  = take(4 * l.capacity * l.sums_pitch * l.splits);
+        if (l.weight_splits > 1) { l.weight_sums = take(4 * static_cast<std::uint64_t>(l.weight_rows) * l.sums_pitch * l.weight_splits); }
     }
     if (form != Form::kGradients) {
         l.picked   = take(4 * l.capacity);
@@ -822,7 +830,7 @@ class Call final {
                               bool starts) {
         products_.starts  = starts;
         cudaError_t error = multiplySlopes(0, q_.vocabulary, grad_hidden != nullptr, grad_weight, weight_stride, grad_element, upstream);
-        if (error == cudaSuccess && grad_hidden != nullptr) { error = spreadTyped(grad_hidden, hidden_stride, grad_element, upstream); }
+        if (error == cudaSuccess && grad_hidden != nullptr) { error = spreadTyped(hiddenParts(hidden_stride, upstream), grad_hidden, grad_element); }
         if (error != cudaSuccess || !l_.library || grad_weight == nullptr || upstream == nullptr) { return error; }
         // (The library's products take a factor from the host alone.)
         FtcudaGradient all{};
@@ -847,7 +855,7 @@ class Call final {
             error                       = slopes(first, columns);
             if (error == cudaSuccess) { error = multiplySlopes(first, columns, grad_hidden != nullptr, grad_weight, weight_stride, q_.element, nullptr); }
         }
-        return error == cudaSuccess && grad_hidden != nullptr ? spreadTyped(grad_hidden, hidden_stride, q_.element, nullptr) : error;
+        return error == cudaSuccess && grad_hidden != nullptr ? spreadTyped(hiddenParts(hidden_stride, nullptr), grad_hidden, q_.element) : error;
     }
 
   private:
@@ -975,11 +983,18 @@ class Call final {
             gradients.weight_gradient_fp32  = grad_element == FTCUDA_ELEMENT_FP32;
             gradients.weight_gradient_pitch = weight_stride;
             gradients.upstream              = upstream;
+            if (l_.weight_splits > 1 && grad_weight != nullptr) {
+                gradients.weight_sums   = at<float>(l_.weight_sums);
+                gradients.weight_splits = l_.weight_splits;
+                gradients.weight_rows   = l_.weight_rows;
+            }
             if (grad_weight != nullptr) {
                 gradients.weight_gradient =
                     static_cast<unsigned char*>(grad_weight) + static_cast<std::int64_t>(training::elementBytes(grad_element) * first) * weight_stride;
             }
-            return loss::launchGradients(products_, weight(first), static_cast<std::uint32_t>(columns), loss::Matrix16{base_ + l_.piece, l_.piece_pitch, slopesPlane()}, gradients);
+            const cudaError_t error = loss::launchGradients(products_, weight(first), static_cast<std::uint32_t>(columns), loss::Matrix16{base_ + l_.piece, l_.piece_pitch, slopesPlane()}, gradients);
+            if (error != cudaSuccess || gradients.weight_sums == nullptr) { return error; }
+            return spreadTyped(Spread{columns, nullptr, gradients.weight_sums, l_.weight_rows, l_.weight_splits, weight_stride, upstream}, gradients.weight_gradient, grad_element);
         }
         cudaError_t error = cudaSuccess;
         if (hidden) { error = multiply(describeHidden(q_, l_, base_, first, columns), true); }
@@ -987,20 +1002,34 @@ class Call final {
         return error;
     }
 
-    cudaError_t spreadTyped(void* out, std::int64_t stride, std::int32_t element, const float* upstream) const {
+    // Parts of sums to be added up.
+    struct Spread {
+        std::uint64_t rows;
+        const std::int32_t* slot;
+        const float* sums;
+        std::uint64_t capacity;
+        std::uint32_t splits;
+        std::int64_t stride;
+        const float* upstream;
+    };
+    Spread hiddenParts(std::int64_t stride, const float* upstream) const {
+        return Spread{q_.tokens, at<std::int32_t>(l_.slot), at<float>(l_.sums), l_.capacity, l_.splits, stride, upstream};
+    }
+
+    cudaError_t spreadTyped(const Spread& parts, void* out, std::int32_t element) const {
         switch (element) {
-            case FTCUDA_ELEMENT_FP32: return spread(static_cast<float*>(out), stride, upstream);
-            case FTCUDA_ELEMENT_FP16: return spread(static_cast<__half*>(out), stride, upstream);
-            default: return spread(static_cast<__nv_bfloat16*>(out), stride, upstream);
+            case FTCUDA_ELEMENT_FP32: return spread(parts, static_cast<float*>(out));
+            case FTCUDA_ELEMENT_FP16: return spread(parts, static_cast<__half*>(out));
+            default: return spread(parts, static_cast<__nv_bfloat16*>(out));
         }
     }
 
-    template<typename T> cudaError_t spread(T* out, std::int64_t stride, const float* upstream) const {
+    template<typename T> cudaError_t spread(const Spread& parts, T* out) const {
         // (64 x 2048 in 16 parts: 14 us with a CTA for each token, 5 with eight; 4096 x 512 in one: 14, and 20 with two.)
-        const std::uint64_t each = std::min(ceilDiv(q_.depth, kGatherThreads), std::max<std::uint64_t>(1, static_cast<std::uint64_t>(sms_) * 4 / q_.tokens));
-        return training::launchOverlapped(spreadHidden<T>, dim3(static_cast<unsigned>(q_.tokens), static_cast<unsigned>(each)), dim3(kGatherThreads), 0, stream_, rows_,
-                                          static_cast<const std::int32_t*>(at<std::int32_t>(l_.slot)), static_cast<const float*>(at<float>(l_.sums)), l_.capacity * l_.sums_pitch,
-                                          l_.sums_pitch, static_cast<std::uint32_t>(l_.capacity), l_.splits, static_cast<std::uint32_t>(q_.depth), upstream, out, stride);
+        const std::uint64_t each = std::min(ceilDiv(q_.depth, kGatherThreads), std::max<std::uint64_t>(1, static_cast<std::uint64_t>(sms_) * 4 / parts.rows));
+        return training::launchOverlapped(spreadHidden<T>, dim3(static_cast<unsigned>(parts.rows), static_cast<unsigned>(each)), dim3(kGatherThreads), 0, stream_, rows_, parts.slot,
+                                          parts.sums, parts.capacity * l_.sums_pitch, l_.sums_pitch, static_cast<std::uint32_t>(parts.capacity), parts.splits,
+                                          static_cast<std::uint32_t>(q_.depth), parts.upstream, out, parts.stride);
     }
 
     const FtcudaLinearCrossEntropy& q_;

@@ -57,6 +57,8 @@ constexpr std::uint32_t kBlockK = 64;  // 128 bytes, one swizzle row
 constexpr std::uint32_t kTileN  = 256;
 constexpr std::uint32_t kItemBlocks  = 12;  // of an item: what it costs beside its own
 constexpr std::uint32_t kMostSplits  = 96;
+constexpr std::uint32_t kMostWeightSplits = 16;
+constexpr std::uint32_t kLaunchBlocks = 12;          // of one more launch
 constexpr std::uint32_t kStreamSplits = 16;          // where the weight streams through; 96 are no faster there (1 x 512 x 131072 BF16: 183 us, 189)
 constexpr std::uint64_t kStreamTokens = 400;         // at which the tensor cores take as long as HBM does (times an FP32 product's terms)
 constexpr std::uint64_t kStreamBytes  = 64ULL << 20;  // half of L2
@@ -120,7 +122,9 @@ struct ProductParams {
     void* slopes;               // or what is kept
     std::uint64_t slopes_pitch, slopes_plane;
     float* sums;
+    float* weight_sums;         // NULL: the weight's gradient is written as it is
     std::uint64_t sums_pitch;
+    std::uint32_t weight_rows;
     std::uint32_t accumulate;
     std::uint32_t weight_problem;  // which of the problems is the weight's gradient
     void* weight_gradient;
@@ -182,7 +186,11 @@ __device__ __forceinline__ Work workOf(const ProductParams& p, std::uint32_t liv
     w.late  = w.items[0] % pairs;
     // (An item costs about kItemBlocks blocks' time beside its own.)
     const std::uint32_t first = p.problem[0].splits == 1 ? w.blocks[0] : p.problem[0].blocks_per_split;
-    w.early                   = w.items[1] == 0 ? 0 : earlyItems(w.items[0], first * p.terms + kItemBlocks, w.items[1], w.blocks[1] * p.terms + kItemBlocks, pairs);
+    w.early                   = 0;
+    if (w.items[1] != 0) {
+        const std::uint32_t second = p.problem[1].splits == 1 ? w.blocks[1] : p.problem[1].blocks_per_split;
+        w.early                    = earlyItems(w.items[0], first * p.terms + kItemBlocks, w.items[1], second * p.terms + kItemBlocks, pairs);
+    }
     return w;
 }
 
@@ -217,7 +225,8 @@ __device__ __forceinline__ Item decode(const ProductParams& p, const Work& work,
     w.row                       = (first + rest % rows) * kTileRows;
     w.col                       = rest / rows * problem.tile_n;
     w.first_block               = w.split * problem.blocks_per_split;
-    w.blocks                    = problem.splits == 1 ? blocks : min(blocks - w.first_block, problem.blocks_per_split);
+    // (Few live rows may leave a part nothing.)
+    w.blocks                    = problem.splits == 1 ? blocks : w.first_block < blocks ? min(blocks - w.first_block, problem.blocks_per_split) : 0;
     return w;
 }
 
@@ -349,13 +358,14 @@ __device__ __forceinline__ void finishSlopes(const ProductParams& p, std::uint32
     }
 }
 
-__device__ __forceinline__ void finishSums(const ProductParams& p, const Item& w, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, float (&v)[128]) {
-    float* const at = p.sums + (static_cast<std::uint64_t>(w.split) * p.capacity + row) * p.sums_pitch + col;
+__device__ __forceinline__ void finishSums(const ProductParams& p, const Item& w, float* sums, std::uint32_t rows, bool accumulate, std::uint32_t row, std::uint32_t col,
+                                           std::uint32_t pieces, float (&v)[128]) {
+    float* const at = sums + (static_cast<std::uint64_t>(w.split) * rows + row) * p.sums_pitch + col;
 #pragma unroll
     for (int j = 0; j < 128; j += 8) {
         if ((j < 64 || pieces == 4) && col + j < p.sums_pitch) {
             float o[8];
-            if (p.accumulate != 0) {
+            if (accumulate) {
                 loadGlobal8(at + j, o);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) { o[i] += v[j + i]; }
@@ -523,6 +533,8 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
                 finishStatistics<true>(p, w, row, col, pieces, half, live, v);
             } else if (kMode == kSlopes) {
                 finishSlopes(p, row, col, pieces, live, v);
+            } else if (w.problem == p.weight_problem && p.weight_sums != nullptr) {
+                finishSums(p, w, p.weight_sums, p.weight_rows, false, row, col, pieces, v);
             } else if (w.problem == p.weight_problem) {
                 if (p.weight_vector != 1) {
                     finishWeight(p, problem, row, col, pieces, unit, v);
@@ -530,7 +542,7 @@ lossProduct(const __grid_constant__ ProductMaps maps, const __grid_constant__ Pr
                     finishWeightTurned(p, problem, row, col, pieces, unit, reinterpret_cast<float*>(smem + kScratchOffset + e * kScratchBytes), v);
                 }
             } else {
-                finishSums(p, w, row, col, pieces, v);
+                finishSums(p, w, p.sums, p.capacity, p.accumulate != 0, row, col, pieces, v);
             }
         }
         if (!ok) { *abort_flag = 1; }
@@ -757,29 +769,38 @@ cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t
 // back counted as well. Where the weight streams through (too large for L2, and too few tokens to be bound by anything else), into as many as make two items
 // for each pair of SMs, so that all of them fetch it. Measured, a step, always the latter / as here: 700 x 700 x 3000 FP32 133 / 104 us, 1024 x 600 x 9000 FP32 250 / 224,
 // 4096 x 512 x 32768 BF16 471 / 445; with 16 parts at most, 256 x 104 x 99422 FP32 331, with up to 96 267; 257 x 4096 x 131072 BF16 920, and 1016 where the items alone decide, 64 x 2048 x 50257 205 and 218.
-std::uint32_t hiddenSplits(std::uint32_t tokens, std::uint32_t depth, std::uint32_t columns, bool planes, int sms) {
+// The weight's gradient is cut over the tokens where its items are few and long (many tokens, a small vocabulary), against a launch that adds the parts up: a step of
+// 7424 x 432 x 1526 FP32 320 us, 228 so, of 16384 x 1024 x 500 BF16 224 and 183, of 4000 x 200 x 900 FP16 70 and 56.
+GradientSplits gradientSplits(std::uint32_t tokens, std::uint32_t depth, std::uint32_t columns, bool planes, int sms) {
     const std::uint32_t across = divideUp(depth, tileColumns(depth)), tiles = divideUp(tokens, kTileRows) * across;
     const std::uint32_t pairs  = static_cast<std::uint32_t>(std::max(1, sms / 2));
-    const std::uint32_t blocks = divideUp(columns, kBlockK), terms = planes ? kTerms : 1;
+    const std::uint32_t blocks = divideUp(columns, kBlockK), rows = divideUp(tokens, kBlockK), terms = planes ? kTerms : 1;
     if (static_cast<std::uint64_t>(tokens) * terms <= kStreamTokens && static_cast<std::uint64_t>(columns) * depth * 2 * (planes ? kPlanes : 1) > kStreamBytes) {
         const std::uint32_t wanted = std::min({std::max(1U, blocks / 8), kStreamSplits, std::max(1U, 2 * pairs / tiles)});
-        return divideUp(blocks, divideUp(blocks, wanted));
+        return {divideUp(blocks, divideUp(blocks, wanted)), 1};
     }
-    const std::uint32_t weight_items = divideUp(columns, kTileRows) * across, weight = divideUp(tokens, kBlockK) * terms + kItemBlocks;
+    const std::uint32_t weight_items = divideUp(columns, kTileRows) * across;
     const std::uint64_t apart  = static_cast<std::uint64_t>(tokens) * depth >> 19;  // a block's 512 cycles are the time of 2^21 bytes or so
-    std::uint32_t best         = 1;
+    const std::uint64_t weight_apart = (static_cast<std::uint64_t>(columns) * depth >> 19) + 1;
+    GradientSplits best        = {1, 1};
     std::uint64_t least        = ~std::uint64_t{0};
-    std::uint32_t before       = 0;
-    // (All numbers up to eight, then about every eighth part more: the host has this to do in every call.)
-    for (std::uint32_t wanted = 1; wanted <= std::min(blocks, kMostSplits); wanted += std::max(1U, wanted / 8)) {
-        const std::uint32_t each = divideUp(blocks, wanted), splits = divideUp(blocks, each);  // none of them empty
-        if (splits == before) { continue; }
-        before                   = splits;
-        const std::uint32_t part = each * terms + kItemBlocks;
-        const std::uint64_t time = makespan(tiles * splits, part, weight_items, weight, pairs, earlyItems(tiles * splits, part, weight_items, weight, pairs)) + splits * apart;
-        if (time < least) {
-            least = time;
-            best  = splits;
+    const std::uint32_t most   = 2 * weight_items <= pairs ? std::min(rows, kMostWeightSplits) : 1;
+    for (std::uint32_t parts = 1; parts <= most; parts *= 2) {
+        const std::uint32_t weight = divideUp(rows, parts) * terms + kItemBlocks;
+        const std::uint64_t extra  = parts == 1 ? 0 : parts * weight_apart + kLaunchBlocks;
+        std::uint32_t before       = 0;
+        // (All numbers up to eight, then about every eighth part more: the host has this to do in every call.)
+        for (std::uint32_t wanted = 1; wanted <= std::min(blocks, kMostSplits); wanted += std::max(1U, wanted / 8)) {
+            const std::uint32_t each = divideUp(blocks, wanted), splits = divideUp(blocks, each);  // none of them empty
+            if (splits == before) { continue; }
+            before                   = splits;
+            const std::uint32_t part = each * terms + kItemBlocks, items = weight_items * parts;
+            std::uint64_t time       = makespan(tiles * splits, part, items, weight, pairs, earlyItems(tiles * splits, part, items, weight, pairs)) + splits * apart + extra;
+            time += parts == 1 ? 0 : time / 8;  // (what is cut has to be well ahead: 5000 x 300 x 4000 FP32 289 us as one, 299 in two parts)
+            if (time < least) {
+                least = time;
+                best  = {splits, parts};
+            }
         }
     }
     return best;
@@ -816,7 +837,11 @@ cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint3
         problem.columns           = call.depth;
         problem.tile_n            = tile_n;
         problem.tiles_n           = tiles_n;
-        problem.splits            = 1;
+        problem.splits            = gradients.weight_sums != nullptr ? gradients.weight_splits : 1;
+        problem.blocks_per_split  = divideUp(call.capacity / kBlockK, problem.splits);
+        p.weight_sums             = gradients.weight_sums;
+        p.weight_rows             = gradients.weight_rows;
+        p.sums_pitch              = gradients.sums_pitch;
         problem.a_along_rows      = 1;
         problem.b_along_rows      = 1;
         p.weight_problem          = p.problems;
@@ -830,7 +855,7 @@ cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint3
         p.weight_vector = !gradients.weight_gradient_fp32 && fits(16) ? 16 : fits(8) ? 8 : 1;
         encoded = encodeOperand(&maps.a[p.problems], call, slopes, true, columns, call.capacity, 128) &&
                   encodeOperand(&maps.b[p.problems], call, call.hidden, true, call.depth, call.capacity, 64);
-        items += static_cast<std::uint64_t>(divideUp(columns, kTileRows)) * tiles_n;
+        items += static_cast<std::uint64_t>(divideUp(columns, kTileRows)) * tiles_n * problem.splits;
         ++p.problems;
     }
     if (!encoded) { return cudaErrorInvalidValue; }

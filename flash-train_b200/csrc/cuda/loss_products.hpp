@@ -71,9 +71,12 @@ cudaError_t launchKept(const ProductCall& call, Matrix16 weight, std::uint32_t v
 cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, std::uint64_t slopes_pitch,
                          std::uint64_t slopes_plane);
 
-// How many parts the sum over `columns` columns is cut into for the gradient of the hidden states. (Over fewer columns
-// launchGradients may fill fewer of them, never more.)
-std::uint32_t hiddenSplits(std::uint32_t tokens, std::uint32_t depth, std::uint32_t columns, bool planes, int sms);
+// How many parts the sums are cut into: over `columns` columns for the gradient of the hidden states (over fewer columns
+// launchGradients may fill fewer of them, never more), and over the tokens for that of the weight.
+struct GradientSplits {
+    std::uint32_t hidden, weight;
+};
+GradientSplits gradientSplits(std::uint32_t tokens, std::uint32_t depth, std::uint32_t columns, bool planes, int sms);
 
 struct Gradients {
     // hidden: sums[split][capacity][pitch] (+)= slopes times weight; NULL when not wanted.
@@ -86,6 +89,9 @@ struct Gradients {
     std::int64_t weight_gradient_pitch;
     bool weight_gradient_fp32;  // or of the operands' type
     const float* upstream;      // a number that the weight's gradient is multiplied by as well; NULL: 1
+    // With weight_splits > 1 its parts are left in weight_sums[split][weight_rows][sums_pitch] instead, without either factor.
+    float* weight_sums;
+    std::uint32_t weight_splits, weight_rows;  // rows: a multiple of kTileRows
 };
 cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint32_t columns, Matrix16 slopes, const Gradients& gradients);
 

@@ -660,3 +660,18 @@ def test_a_weight_at_any_address(ft, dtype, tokens, depth, vocabulary, offset, g
     view = buffer[offset:].view(vocabulary, depth + gap)[:, :depth]
     view.copy_(weight)
     run_and_check(ft, hidden, view, target, reduction)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens, depth, vocabulary, live", [(3000, 72, 300, 1.0), (3000, 72, 300, 0.02), (2000, 257, 129, 0.5), (5000, 128, 1000, 0.0), (6000, 40, 5, 1.0)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_many_tokens_of_few_classes(ft, dtype, tokens, depth, vocabulary, live, reduction):
+    """The weight's gradient is summed up in parts over the tokens, of which few live ones leave some empty; together with the other gradient and alone."""
+    hidden, weight, target = make(tokens, depth, vocabulary, dtype, seed=80)
+    target[torch.rand(tokens, device="cuda", generator=torch.Generator(device="cuda").manual_seed(81)) >= live] = -100
+    _, _, grad_weight = run_and_check(ft, hidden, weight, target, reduction, scale=16.0)
+    w = weight.clone().requires_grad_()
+    loss = ft.linear_cross_entropy(hidden, w, target, reduction=reduction)
+    upstream = torch.randn(tokens, device="cuda", generator=torch.Generator(device="cuda").manual_seed(9)) * 16.0 if reduction == "none" else torch.tensor(16.0, device="cuda")
+    alone, = torch.autograd.grad(loss, w, upstream)
+    assert torch.equal(alone, grad_weight)
