@@ -24,10 +24,12 @@ _IGNORED = -100
 
 
 def _framework():
-    if "flash_train.torch" not in sys.modules:
-        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "flash-train_b200" / "python"))
-        import flash_train.torch  # noqa: F401
-    return sys.modules["flash_train.torch"]
+    path = str(Path(__file__).resolve().parents[1] / "flash-train_b200" / "python")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import flash_train.torch as ft
+
+    return ft
 
 
 def listed():
