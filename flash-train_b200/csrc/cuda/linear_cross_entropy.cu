@@ -508,12 +508,17 @@ __global__ void __launch_bounds__(kGatherThreads) spreadHidden(const LiveRows ro
 
 // ---------------------------------------------------------------- host: layout of the workspace
 
+// Offsets in two memories: one that the step call keeps from the loss to the gradients, and one of the call's own. What lies where in the kept one goes by sizes alone, so
+// that the weight may be at another address when the gradients are made (saved-tensor hooks of torch hand back a copy): a copy of the weight for TMA, which depends on
+// its address, is the last thing there, and the memory's size says whether there is one.
 struct Layout {
     bool library;                 // FP32 through the library's products
     bool planes;                  // ... or as three BF16 matrices
     std::uint64_t capacity;       // rows, a multiple of kTileRows
     std::uint64_t copy_pitch;     // of the hidden states' copy, elements
     std::uint64_t weight_pitch;   // of the weight's copy or planes, 0: none
+    bool weight_kept;             // ... which are in the kept memory
+    bool weight_made;             // ... since the loss: the gradients need not make them
     std::uint64_t columns;        // of a piece
     std::uint64_t piece_pitch;    // of Z or dZ, elements
     std::uint64_t pieces;         // partial statistics of a row
@@ -521,8 +526,10 @@ struct Layout {
     std::uint32_t weight_splits;  // ... for dW, 1: it needs none
     std::uint32_t weight_rows;    // rows of a part of those
     std::uint64_t sums_pitch;
-    std::uint64_t count, unit, token, target, scale, lse2, picked, row_loss, slot, hidden, weight, partials, piece, kept, sums, weight_sums, product, product_bytes;
-    std::uint64_t total;
+    std::uint64_t count, unit, slot, hidden, piece;  // kept
+    std::uint64_t weight;
+    std::uint64_t token, target, scale, lse2, picked, row_loss, partials, exponentials, sums, weight_sums, product, product_bytes;
+    std::uint64_t kept_bytes, bytes;
 };
 
 std::uint64_t roundUp(std::uint64_t x, std::uint64_t unit) { return (x + unit - 1) / unit * unit; }
@@ -567,13 +574,20 @@ int configureProduct(const FtcudaGemmDesc& desc, bool slopes, int sms, std::uint
     return fail(message, capacity, 1, "no FP32 product takes the problem");
 }
 
+// The two memories that a call has.
+struct Memory {
+    unsigned char* kept;
+    unsigned char* own;
+    unsigned char* weight(const Layout& l) const { return (l.weight_kept ? kept : own) + l.weight; }
+};
+
 // The three FP32 products of a piece of `columns` columns from `first` on.
-FtcudaGemmDesc describeLogits(const FtcudaLinearCrossEntropy& q, const Layout& l, unsigned char* base, std::uint64_t first, std::uint64_t columns) {
+FtcudaGemmDesc describeLogits(const FtcudaLinearCrossEntropy& q, const Layout& l, const Memory& memory, std::uint64_t first, std::uint64_t columns) {
     FtcudaGemmDesc d{};
-    d.a            = reinterpret_cast<const float*>(base + l.hidden);
-    d.b            = l.weight_pitch != 0 ? reinterpret_cast<const float*>(base + l.weight) + first * l.weight_pitch
+    d.a            = reinterpret_cast<const float*>(memory.kept + l.hidden);
+    d.b            = l.weight_pitch != 0 ? reinterpret_cast<const float*>(memory.weight(l)) + first * l.weight_pitch
                                          : static_cast<const float*>(q.weight) + static_cast<std::int64_t>(first) * q.weight_row_stride;
-    d.d            = reinterpret_cast<float*>(base + l.piece);
+    d.d            = reinterpret_cast<float*>(memory.kept + l.piece);
     d.alpha        = 1.0F;
     d.m            = q.tokens;
     d.n            = columns;
@@ -587,10 +601,10 @@ FtcudaGemmDesc describeLogits(const FtcudaLinearCrossEntropy& q, const Layout& l
     d.device       = q.device;
     return d;
 }
-FtcudaGemmDesc describeHidden(const FtcudaLinearCrossEntropy& q, const Layout& l, unsigned char* base, std::uint64_t first, std::uint64_t columns) {
-    FtcudaGemmDesc d = describeLogits(q, l, base, first, columns);
+FtcudaGemmDesc describeHidden(const FtcudaLinearCrossEntropy& q, const Layout& l, const Memory& memory, std::uint64_t first, std::uint64_t columns) {
+    FtcudaGemmDesc d = describeLogits(q, l, memory, first, columns);
     d.a              = d.d;
-    d.d              = reinterpret_cast<float*>(base + l.sums);
+    d.d              = reinterpret_cast<float*>(memory.own + l.sums);
     d.n              = q.depth;
     d.k              = columns;
     d.a_row_stride   = static_cast<std::int64_t>(l.piece_pitch);
@@ -605,9 +619,9 @@ FtcudaGemmDesc describeHidden(const FtcudaLinearCrossEntropy& q, const Layout& l
     }
     return d;
 }
-FtcudaGemmDesc describeWeight(const FtcudaLinearCrossEntropy& q, const Layout& l, unsigned char* base, std::uint64_t first, std::uint64_t columns, void* grad_weight,
+FtcudaGemmDesc describeWeight(const FtcudaLinearCrossEntropy& q, const Layout& l, const Memory& memory, std::uint64_t first, std::uint64_t columns, void* grad_weight,
                               std::int64_t stride) {
-    FtcudaGemmDesc d = describeLogits(q, l, base, first, columns);
+    FtcudaGemmDesc d = describeLogits(q, l, memory, first, columns);
     d.b              = d.a;
     d.a              = d.d;
     d.d              = static_cast<float*>(grad_weight) + static_cast<std::int64_t>(first) * stride;
@@ -622,8 +636,9 @@ FtcudaGemmDesc describeWeight(const FtcudaLinearCrossEntropy& q, const Layout& l
     return d;
 }
 
-// What a call computes: the loss, the gradients from a loss that is known, or both at once.
-enum class Form { kLoss, kGradients, kStep };
+// What a call computes: the loss, the gradients from a loss that is known (and logits computed again), or one of the two halves of a step.
+enum class Form { kLoss, kGradients, kStepLoss, kStepGradients };
+constexpr bool isStep(Form form) { return form == Form::kStepLoss || form == Form::kStepGradients; }
 
 // Whether FP32 operands are better off with the library's products. Measured (library / three BF16 matrices, microseconds):
 //   large products that take the prepared form; a step of 2048 x 2048 x 32000 2501 / 3231, 4096 x 1024 x 16000 1476 / 1666, 700 x 2048 x 20000 743 / 837, 1200 x 1200 x 9000
@@ -643,83 +658,108 @@ bool libraryPays(const FtcudaLinearCrossEntropy& q, Form form) {
 // be in the same place.
 std::uint64_t logitBytes(const FtcudaLinearCrossEntropy& q, Form form) {
     if (!isFp32(q)) { return 2; }
-    return libraryPays(q, form) ? 4 : form == Form::kStep ? 2 * loss::kPlanes + 4 : 2 * loss::kPlanes;
+    return libraryPays(q, form) ? 4 : isStep(form) ? 2 * loss::kPlanes + 4 : 2 * loss::kPlanes;
 }
 
 // What the step call holds of all logits at once, in bytes.
 std::uint64_t stepBytes(const FtcudaLinearCrossEntropy& q) {
-    return roundUp(std::max<std::uint64_t>(q.tokens, 1), loss::kTileRows) * roundUp(q.vocabulary, 256) * logitBytes(q, Form::kStep);
+    return roundUp(std::max<std::uint64_t>(q.tokens, 1), loss::kTileRows) * roundUp(q.vocabulary, 256) * logitBytes(q, Form::kStepLoss);
 }
 
-int layOut(const FtcudaLinearCrossEntropy& q, Form form, int sms, Layout& l, char* message, std::size_t capacity) {
-    const bool gradients      = form != Form::kLoss;
+// Hands out offsets of a memory.
+struct Room {
+    std::uint64_t at = 0;
+    std::uint64_t take(std::uint64_t size) {
+        const std::uint64_t here = at;
+        at += roundUp(size, kAlign);
+        return here;
+    }
+};
+
+constexpr std::uint64_t kAny = ~std::uint64_t{0};
+
+// `kept_bytes`: of the memory that a step's loss left for these gradients; kAny in the other calls.
+int layOut(const FtcudaLinearCrossEntropy& q, Form form, std::uint64_t kept_bytes, int sms, Layout& l, char* message, std::size_t capacity) {
+    const bool gradients      = form != Form::kLoss && form != Form::kStepLoss;
+    const bool statistics     = form != Form::kGradients && form != Form::kStepGradients;
     l                         = Layout{};
     l.library                 = libraryPays(q, form);
     l.planes                  = isFp32(q) && !l.library;
-    const std::uint64_t bytes = logitBytes(q, form);
+    const std::uint64_t bytes = logitBytes(q, form), element = l.planes ? 2 * loss::kPlanes : training::elementBytes(q.element);
     l.capacity                = roundUp(std::max<std::uint64_t>(q.tokens, 1), loss::kTileRows);
     l.copy_pitch              = roundUp(q.depth, 8);
-    // (The prepared products split the weight whatever its rows' alignment; the others would copy it for each product, element by element: a step of 8 x 3967 x 60001 FP32
-    // 3166 us, 1309 with one copy; 1000 x 2311 x 20000, prepared, the loss 384, with a copy 411.)
-    const bool split_anyway   = l.library && preparedFormPays(q.tokens, q.vocabulary, q.depth);
-    l.weight_pitch            = l.planes || (!split_anyway && !weightFits(q)) ? roundUp(q.depth, 8) : 0;
     const std::uint64_t fill  = roundUp(q.vocabulary, 256);
-    l.columns                 = form == Form::kStep ? fill : std::min(fill, std::max(kLeastColumns, kPieceBytes / (l.capacity * bytes) / 256 * 256));
+    l.columns                 = isStep(form) ? fill : std::min(fill, std::max(kLeastColumns, kPieceBytes / (l.capacity * bytes) / 256 * 256));
     l.columns                 = roundUp(ceilDiv(fill, ceilDiv(fill, l.columns)), 256);  // pieces of about one size
     l.piece_pitch             = l.columns;
     l.pieces                  = l.library ? ceilDiv(q.vocabulary, l.columns) : loss::statisticsPieces(static_cast<std::uint32_t>(q.vocabulary), static_cast<std::uint32_t>(l.capacity), sms);
     l.sums_pitch              = roundUp(q.depth, 8);
     l.weight_rows             = static_cast<std::uint32_t>(roundUp(std::min(l.columns, q.vocabulary), loss::kTileRows));
-    const loss::GradientSplits splits = l.library ? loss::GradientSplits{1, 1}
+    const loss::GradientSplits splits = l.library || !gradients ? loss::GradientSplits{1, 1}
                                                   : loss::gradientSplits(static_cast<std::uint32_t>(std::max<std::uint64_t>(q.tokens, 1)), static_cast<std::uint32_t>(q.depth),
                                                                          static_cast<std::uint32_t>(std::min(l.columns, q.vocabulary)), l.planes, sms);
     l.splits                  = splits.hidden;
     l.weight_splits           = splits.weight;
-    std::uint64_t at = 0;
-    const auto take  = [&](std::uint64_t size) {
-        const std::uint64_t here = at;
-        at += roundUp(size, kAlign);
-        return here;
-    };
-    l.count  = take(4);
-    l.unit   = take(4);
-    l.token  = take(4 * l.capacity);
-    l.target = take(4 * l.capacity);
-    l.slot   = take(4 * l.capacity);
-    l.hidden = take((l.planes ? 2 * loss::kPlanes : training::elementBytes(q.element)) * l.capacity * l.copy_pitch);
-    if (l.weight_pitch != 0) { l.weight = take((l.planes ? 2 * loss::kPlanes : training::elementBytes(q.element)) * q.vocabulary * l.weight_pitch); }
+    Room kept, own;
+    l.count  = kept.take(4);
+    l.unit   = kept.take(4);
+    l.slot   = kept.take(4 * l.capacity);
+    l.hidden = kept.take(element * l.capacity * l.copy_pitch);
+    if (form != Form::kLoss || l.library) { l.piece = kept.take(element * l.capacity * l.piece_pitch); }
+    // (The prepared products split the weight whatever its rows' alignment; the others would copy it for each product, element by element: a step of 8 x 3967 x 60001 FP32
+    // 3166 us, 1309 with one copy; 1000 x 2311 x 20000, prepared, the loss 384, with a copy 411.)
+    const bool split_anyway = l.library && preparedFormPays(q.tokens, q.vocabulary, q.depth);
+    Room with_copy          = kept;
+    const std::uint64_t at  = with_copy.take(element * q.vocabulary * l.copy_pitch);
+    if (l.planes || (kept_bytes == with_copy.at && !split_anyway) || (!split_anyway && !weightFits(q))) {
+        l.weight_pitch = l.copy_pitch;
+        l.weight_kept  = isStep(form) && (kept_bytes == kAny || kept_bytes == with_copy.at);
+        l.weight_made  = form == Form::kStepGradients && l.weight_kept;
+        l.weight       = l.weight_kept ? at : own.take(element * q.vocabulary * l.copy_pitch);
+        if (l.weight_kept) { kept = with_copy; }
+    }
+    l.kept_bytes = kept.at;
+    if (kept_bytes != kAny && kept_bytes != l.kept_bytes) {
+        return fail(message, capacity, 1, "the kept memory has %llu bytes, which is not what the loss of this problem leaves", static_cast<unsigned long long>(kept_bytes));
+    }
+    if (form != Form::kStepGradients) {
+        l.token  = own.take(4 * l.capacity);
+        l.target = own.take(4 * l.capacity);
+        l.scale  = own.take(4 * l.capacity);
+        l.lse2   = own.take(4 * l.capacity);
+    }
+    if (statistics) {
+        l.picked   = own.take(4 * l.capacity);
+        l.row_loss = own.take(4 * l.capacity);
+        l.partials = own.take(8 * l.capacity * l.pieces);
+    }
+    if (l.planes && isStep(form) && statistics) { l.exponentials = own.take(4 * l.capacity * l.piece_pitch); }
     if (gradients) {
-        l.scale = take(4 * l.capacity);
-        l.lse2  = take(4 * l.capacity);
-        l.sums  = take(4 * l.capacity * l.sums_pitch * l.splits);
-        if (l.weight_splits > 1) { l.weight_sums = take(4 * static_cast<std::uint64_t>(l.weight_rows) * l.sums_pitch * l.weight_splits); }
+        l.sums = own.take(4 * l.capacity * l.sums_pitch * l.splits);
+        if (l.weight_splits > 1) { l.weight_sums = own.take(4 * static_cast<std::uint64_t>(l.weight_rows) * l.sums_pitch * l.weight_splits); }
     }
-    if (form != Form::kGradients) {
-        l.picked   = take(4 * l.capacity);
-        l.row_loss = take(4 * l.capacity);
-        l.partials = take(8 * l.capacity * l.pieces);
-    }
-    if (gradients || l.library) { l.piece = take((l.planes ? 2 * loss::kPlanes : training::elementBytes(q.element)) * l.capacity * l.piece_pitch); }
-    if (l.planes && form == Form::kStep) { l.kept = take(4 * l.capacity * l.piece_pitch); }
     if (l.library && q.tokens != 0) {
         // The most that any product of any piece wants. (The addresses are not known yet, but how they are aligned is.)
-        l.product            = at;
+        l.product            = own.at;
         auto* const stand_in = reinterpret_cast<unsigned char*>(std::uintptr_t{1} << 40);
+        const Memory memory{stand_in, stand_in};
         for (std::uint64_t first = 0; first < q.vocabulary; first += l.columns) {
             const std::uint64_t columns = std::min(l.columns, q.vocabulary - first);
             if (first != 0 && columns == l.columns && first != l.columns) { continue; }  // like the piece before
             Product product;
-            if (configureProduct(describeLogits(q, l, stand_in, first, columns), false, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
-            l.product_bytes = std::max(l.product_bytes, product.bytes);
+            if (form != Form::kStepGradients) {
+                if (configureProduct(describeLogits(q, l, memory, first, columns), false, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
+                l.product_bytes = std::max(l.product_bytes, product.bytes);
+            }
             if (!gradients) { continue; }
-            if (configureProduct(describeHidden(q, l, stand_in, first, columns), true, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
+            if (configureProduct(describeHidden(q, l, memory, first, columns), true, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
             l.product_bytes = std::max(l.product_bytes, product.bytes);
-            if (configureProduct(describeWeight(q, l, stand_in, first, columns, stand_in, static_cast<std::int64_t>(q.depth)), true, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
+            if (configureProduct(describeWeight(q, l, memory, first, columns, stand_in, static_cast<std::int64_t>(q.depth)), true, sms, ~std::uint64_t{0}, product, message, capacity) != 0) { return 1; }
             l.product_bytes = std::max(l.product_bytes, product.bytes);
         }
-        take(l.product_bytes);
+        own.take(l.product_bytes);
     }
-    l.total = at;
+    l.bytes = own.at;
     return 0;
 }
 
@@ -745,12 +785,23 @@ class Call final {
   public:
     Call(const FtcudaLinearCrossEntropy& problem, char* message, std::size_t capacity) : q_(problem), message_(message), capacity_(capacity) {}
 
-    // Everything that is the same in both directions; 0 or a failure that has its message.
-    int begin(Form form, void* workspace, std::uint64_t workspace_bytes, void* stream) {
+    // Everything that is the same in both directions; 0 or a failure that has its message. The halves of a step have their kept memory; the other calls' is the workspace's beginning.
+    int begin(Form form, void* kept_memory, std::uint64_t kept_bytes, void* workspace, std::uint64_t workspace_bytes, void* stream) {
         if (!training::deviceIsCurrent(q_.device, message_, capacity_) || !deviceSmCount(q_.device, &sms_, message_, capacity_)) { return 1; }
-        if (layOut(q_, form, sms_, l_, message_, capacity_) != 0) { return 1; }
-        if (workspace == nullptr || workspace_bytes < l_.total || !training::aligned(workspace, kAlign)) {
-            return fail(message_, capacity_, 1, "workspace of %llu bytes needed, at a multiple of 256", static_cast<unsigned long long>(l_.total));
+        if (layOut(q_, form, form == Form::kStepGradients ? kept_bytes : kAny, sms_, l_, message_, capacity_) != 0) { return 1; }
+        if (!isStep(form)) {
+            if (workspace == nullptr || workspace_bytes < l_.kept_bytes + l_.bytes || !training::aligned(workspace, kAlign)) {
+                return fail(message_, capacity_, 1, "workspace of %llu bytes needed, at a multiple of 256", static_cast<unsigned long long>(l_.kept_bytes + l_.bytes));
+            }
+            memory_ = Memory{static_cast<unsigned char*>(workspace), static_cast<unsigned char*>(workspace) + l_.kept_bytes};
+        } else {
+            if (kept_memory == nullptr || kept_bytes != l_.kept_bytes || !training::aligned(kept_memory, kAlign)) {
+                return fail(message_, capacity_, 1, "kept memory of %llu bytes needed, no more and no less, at a multiple of 256", static_cast<unsigned long long>(l_.kept_bytes));
+            }
+            if (workspace == nullptr || workspace_bytes < l_.bytes || !training::aligned(workspace, kAlign)) {
+                return fail(message_, capacity_, 1, "workspace of %llu bytes needed, at a multiple of 256", static_cast<unsigned long long>(l_.bytes));
+            }
+            memory_ = Memory{static_cast<unsigned char*>(kept_memory), static_cast<unsigned char*>(workspace)};
         }
         int* status              = nullptr;
         volatile int* host       = nullptr;
@@ -758,17 +809,16 @@ class Call final {
         if (const int code = takeDeviceStatus(host)) {
             return fail(message_, capacity_, 1, "an earlier kernel reported a timed-out wait (code %d)", code);
         }
-        base_        = static_cast<unsigned char*>(workspace);
         stream_      = static_cast<cudaStream_t>(stream);
-        rows_.count  = at<std::uint32_t>(l_.count);
-        rows_.unit   = at<float>(l_.unit);
-        rows_.token  = at<std::int32_t>(l_.token);
-        rows_.target = at<std::int32_t>(l_.target);
-        rows_.scale  = at<float>(l_.scale);
-        rows_.lse2   = at<float>(l_.lse2);
-        rows_.picked = at<float>(l_.picked);
+        rows_.count  = kept<std::uint32_t>(l_.count);
+        rows_.unit   = kept<float>(l_.unit);
+        rows_.token  = own<std::int32_t>(l_.token);
+        rows_.target = own<std::int32_t>(l_.target);
+        rows_.scale  = own<float>(l_.scale);
+        rows_.lse2   = own<float>(l_.lse2);
+        rows_.picked = own<float>(l_.picked);
         products_    = loss::ProductCall{l_.planes || q_.element == FTCUDA_ELEMENT_BF16, l_.planes, static_cast<std::uint32_t>(l_.capacity), static_cast<std::uint32_t>(q_.depth), rows_,
-                                      {base_ + l_.hidden, l_.copy_pitch, l_.capacity * l_.copy_pitch}, status, sms_, stream_, message_, capacity_, false};
+                                      {memory_.kept + l_.hidden, l_.copy_pitch, l_.capacity * l_.copy_pitch}, status, sms_, stream_, message_, capacity_, false};
         if (message_ != nullptr && capacity_ != 0) { message_[0] = '\0'; }
         return 0;
     }
@@ -781,14 +831,14 @@ class Call final {
         listTokens<false><<<1, kListThreads, 0, stream_>>>(list);
         cudaError_t error = started();
         if (error == cudaSuccess) { error = gather(); }
-        float2* const partials = at<float2>(l_.partials);
+        float2* const partials = own<float2>(l_.partials);
         if (!l_.library) {
             if (error == cudaSuccess) { error = loss::launchStatistics(products_, weight(0), static_cast<std::uint32_t>(q_.vocabulary), partials); }
         } else {
             std::uint64_t piece = 0;
             for (std::uint64_t first = 0; first < q_.vocabulary && error == cudaSuccess; first += l_.columns, ++piece) {
                 const std::uint64_t columns = std::min(l_.columns, q_.vocabulary - first);
-                error                       = multiply(describeLogits(q_, l_, base_, first, columns), false);
+                error                       = multiply(describeLogits(q_, l_, memory_, first, columns), false);
                 if (error == cudaSuccess) {
                     error = training::launchOverlapped(rowStatistics, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(first, columns, partials + piece * l_.capacity));
                 }
@@ -804,12 +854,12 @@ class Call final {
         listTokens<true><<<1, kListThreads, 0, stream_>>>(list);
         cudaError_t error = started();
         if (error == cudaSuccess) { error = gather(); }
-        float2* const partials        = at<float2>(l_.partials);
+        float2* const partials        = own<float2>(l_.partials);
         const std::uint32_t columns   = static_cast<std::uint32_t>(q_.vocabulary);
-        void* const kept              = base_ + (l_.planes ? l_.kept : l_.piece);
-        if (error == cudaSuccess && !l_.library) { error = loss::launchKept(products_, weight(0), columns, partials, kept, l_.piece_pitch); }
+        void* const exponentials      = l_.planes ? memory_.own + l_.exponentials : memory_.kept + l_.piece;
+        if (error == cudaSuccess && !l_.library) { error = loss::launchKept(products_, weight(0), columns, partials, exponentials, l_.piece_pitch); }
         if (l_.library) {
-            if (error == cudaSuccess) { error = multiply(describeLogits(q_, l_, base_, 0, columns), false); }
+            if (error == cudaSuccess) { error = multiply(describeLogits(q_, l_, memory_, 0, columns), false); }
             if (error == cudaSuccess) { error = training::launchOverlapped(rowStatistics, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(0, columns, partials)); }
         }
         if (error == cudaSuccess) { error = join(loss, nullptr, true); }
@@ -821,15 +871,16 @@ class Call final {
                                     l_.piece_pitch, slopesPlane()};
             const dim3 grid(static_cast<unsigned>(ceilDiv(l_.pieces, kKeptPieces) * (l_.capacity / kKeptRows)));  // (of x, which takes any number)
             const auto kernel = l_.planes ? keptSlopes<float> : q_.element == FTCUDA_ELEMENT_FP16 ? keptSlopes<__half> : keptSlopes<__nv_bfloat16>;
-            return training::launchOverlapped(kernel, grid, dim3(256), 0, stream_, params, kept, at<std::uint16_t>(l_.piece));
+            return training::launchOverlapped(kernel, grid, dim3(256), 0, stream_, params, exponentials, kept<std::uint16_t>(l_.piece));
         }
     }
 
-    // The gradients from the slopes that stepLoss left in the workspace, for an upstream gradient of *upstream (NULL: 1).
-    cudaError_t stepGradients(const float* upstream, void* grad_hidden, std::int64_t hidden_stride, void* grad_weight, std::int64_t weight_stride, std::int32_t grad_element,
-                              bool starts) {
-        products_.starts  = starts;
-        cudaError_t error = multiplySlopes(0, q_.vocabulary, grad_hidden != nullptr, grad_weight, weight_stride, grad_element, upstream);
+    // The gradients from the slopes that stepLoss left in the kept memory, for an upstream gradient of *upstream (NULL: 1).
+    cudaError_t stepGradients(const float* upstream, void* grad_hidden, std::int64_t hidden_stride, void* grad_weight, std::int64_t weight_stride, std::int32_t grad_element) {
+        const bool copies = l_.weight_pitch != 0 && !l_.weight_made;
+        products_.starts  = !copies;
+        cudaError_t error = copies ? copyWeight(true) : cudaSuccess;
+        if (error == cudaSuccess) { error = multiplySlopes(0, q_.vocabulary, grad_hidden != nullptr, grad_weight, weight_stride, grad_element, upstream); }
         if (error == cudaSuccess && grad_hidden != nullptr) { error = spreadTyped(hiddenParts(hidden_stride, upstream), grad_hidden, grad_element); }
         if (error != cudaSuccess || !l_.library || grad_weight == nullptr || upstream == nullptr) { return error; }
         // (The library's products take a factor from the host alone.)
@@ -859,7 +910,8 @@ class Call final {
     }
 
   private:
-    template<typename T> T* at(std::uint64_t offset) const { return reinterpret_cast<T*>(base_ + offset); }
+    template<typename T> T* kept(std::uint64_t offset) const { return reinterpret_cast<T*>(memory_.kept + offset); }
+    template<typename T> T* own(std::uint64_t offset) const { return reinterpret_cast<T*>(memory_.own + offset); }
 
     static cudaError_t started() {
         const cudaError_t error = cudaGetLastError();
@@ -881,57 +933,63 @@ class Call final {
         list.tokens       = static_cast<std::uint32_t>(q_.tokens);
         list.reduction    = q_.reduction;
         list.rows         = rows_;
-        list.slot         = at<std::int32_t>(l_.slot);
+        list.slot         = kept<std::int32_t>(l_.slot);
         return list;
     }
 
     RowParams rowParams(std::uint64_t first, std::uint64_t columns, float2* partials) const {
-        return RowParams{rows_, at<float>(l_.piece), l_.piece_pitch, static_cast<std::uint32_t>(first), static_cast<std::uint32_t>(columns), partials};
+        return RowParams{rows_, kept<float>(l_.piece), l_.piece_pitch, static_cast<std::uint32_t>(first), static_cast<std::uint32_t>(columns), partials};
     }
 
-    // An operand as three BF16 matrices, `rows` rows of it at most.
-    cudaError_t split(bool gathered, std::uint64_t rows, const float* from, std::int64_t stride, std::uint64_t to, std::uint64_t pitch) const {
+    // An operand as three BF16 matrices, `rows` rows of it at most. `starts`: the first kernel of a call.
+    cudaError_t split(bool starts, bool gathered, std::uint64_t rows, const float* from, std::int64_t stride, unsigned char* to, std::uint64_t pitch) const {
         const std::uint64_t threads = rows * ceilDiv(q_.depth, 8), most = static_cast<std::uint64_t>(sms_) * kSplitCtasPerSm;
         const dim3 grid(static_cast<unsigned>(std::min(most, ceilDiv(threads, kGatherThreads))));
         const auto kernel = training::aligned(from, 16) && stride % 4 == 0 ? splitRows<true> : splitRows<false>;
-        return training::launchOverlapped(kernel, grid, dim3(kGatherThreads), 0, stream_, rows_, gathered, static_cast<std::uint32_t>(rows), from, stride, at<std::uint16_t>(to), pitch,
-                                          rows * pitch, static_cast<std::uint32_t>(q_.depth));
+        return training::launchKernel(!starts, kernel, grid, dim3(kGatherThreads), 0, stream_, rows_, gathered, static_cast<std::uint32_t>(rows), from, stride,
+                                      reinterpret_cast<std::uint16_t*>(to), pitch, rows * pitch, static_cast<std::uint32_t>(q_.depth));
     }
 
     // The live hidden states, and the weight where TMA cannot fetch it as it is.
     cudaError_t gather() const {
+        cudaError_t error = cudaSuccess;
         if (l_.planes) {
-            const cudaError_t error = split(true, l_.capacity, static_cast<const float*>(q_.hidden), q_.tokens <= 1 ? 0 : q_.hidden_row_stride, l_.hidden, l_.copy_pitch);
-            return error == cudaSuccess ? split(false, q_.vocabulary, static_cast<const float*>(q_.weight), q_.vocabulary == 1 ? 0 : q_.weight_row_stride, l_.weight, l_.weight_pitch)
-                                        : error;
+            error = split(false, true, l_.capacity, static_cast<const float*>(q_.hidden), q_.tokens <= 1 ? 0 : q_.hidden_row_stride, memory_.kept + l_.hidden, l_.copy_pitch);
+        } else {
+            const std::uint64_t bytes = training::elementBytes(q_.element);
+            // The library's products go over all rows, the others over whole tiles of live ones.
+            const std::uint32_t zero_to = l_.library ? static_cast<std::uint32_t>(q_.tokens) : 0;
+            const auto run = [&](auto word) {
+                using W                   = decltype(word);
+                const std::uint64_t ratio = sizeof(W) / bytes;
+                return training::launchOverlapped(gatherHidden<W>, dim3(static_cast<unsigned>(l_.capacity)), dim3(kGatherThreads), 0, stream_, rows_, zero_to,
+                                                  static_cast<const W*>(q_.hidden), static_cast<std::int64_t>(q_.hidden_row_stride / static_cast<std::int64_t>(ratio)),
+                                                  kept<W>(l_.hidden), l_.copy_pitch / ratio, static_cast<std::uint32_t>(q_.depth / ratio));
+            };
+            const std::uint64_t row = q_.depth * bytes;
+            const bool wide         = row % 16 == 0 && training::aligned(q_.hidden, 16) && (q_.tokens <= 1 || static_cast<std::uint64_t>(q_.hidden_row_stride) * bytes % 16 == 0);
+            error                   = wide ? run(uint4{}) : bytes == 4 ? run(std::uint32_t{}) : run(std::uint16_t{});
         }
-        const std::uint64_t bytes = training::elementBytes(q_.element);
-        // The library's products go over all rows, the others over whole tiles of live ones.
-        const std::uint32_t zero_to = l_.library ? static_cast<std::uint32_t>(q_.tokens) : 0;
-        const auto run = [&](auto word) {
-            using W                   = decltype(word);
-            const std::uint64_t ratio = sizeof(W) / bytes;
-            return training::launchOverlapped(gatherHidden<W>, dim3(static_cast<unsigned>(l_.capacity)), dim3(kGatherThreads), 0, stream_, rows_, zero_to,
-                                              static_cast<const W*>(q_.hidden), static_cast<std::int64_t>(q_.hidden_row_stride / static_cast<std::int64_t>(ratio)), at<W>(l_.hidden),
-                                              l_.copy_pitch / ratio, static_cast<std::uint32_t>(q_.depth / ratio));
-        };
-        const std::uint64_t row  = q_.depth * bytes;
-        const bool wide          = row % 16 == 0 && training::aligned(q_.hidden, 16) && (q_.tokens <= 1 || static_cast<std::uint64_t>(q_.hidden_row_stride) * bytes % 16 == 0);
-        cudaError_t error        = wide ? run(uint4{}) : bytes == 4 ? run(std::uint32_t{}) : run(std::uint16_t{});
-        if (error == cudaSuccess && l_.weight_pitch != 0) {
-            const std::uint64_t words = bytes / 2, ctas = std::min(ceilDiv(q_.vocabulary * ceilDiv(words * q_.depth, 8), kGatherThreads), static_cast<std::uint64_t>(sms_) * kSplitCtasPerSm);
-            error = training::launchOverlapped(copyRows16, dim3(static_cast<unsigned>(ctas)), dim3(kGatherThreads), 0, stream_, static_cast<const std::uint16_t*>(q_.weight),
-                                               q_.vocabulary == 1 ? std::int64_t{0} : static_cast<std::int64_t>(words) * q_.weight_row_stride, static_cast<std::uint32_t>(q_.vocabulary),
-                                               at<std::uint16_t>(l_.weight), words * l_.weight_pitch, static_cast<std::uint32_t>(words * q_.depth));
+        return error == cudaSuccess && l_.weight_pitch != 0 ? copyWeight(false) : error;
+    }
+
+    // The weight's planes, or its copy for TMA.
+    cudaError_t copyWeight(bool starts) const {
+        if (l_.planes) {
+            return split(starts, false, q_.vocabulary, static_cast<const float*>(q_.weight), q_.vocabulary == 1 ? 0 : q_.weight_row_stride, memory_.weight(l_), l_.weight_pitch);
         }
-        return error;
+        const std::uint64_t words = training::elementBytes(q_.element) / 2;
+        const std::uint64_t ctas  = std::min(ceilDiv(q_.vocabulary * ceilDiv(words * q_.depth, 8), kGatherThreads), static_cast<std::uint64_t>(sms_) * kSplitCtasPerSm);
+        return training::launchKernel(!starts, copyRows16, dim3(static_cast<unsigned>(ctas)), dim3(kGatherThreads), 0, stream_, static_cast<const std::uint16_t*>(q_.weight),
+                                      q_.vocabulary == 1 ? std::int64_t{0} : static_cast<std::int64_t>(words) * q_.weight_row_stride, static_cast<std::uint32_t>(q_.vocabulary),
+                                      reinterpret_cast<std::uint16_t*>(memory_.weight(l_)), words * l_.weight_pitch, static_cast<std::uint32_t>(words * q_.depth));
     }
 
     // The weight from row `first` on, as the 16-bit products fetch it.
     loss::Matrix16 weight(std::uint64_t first) const {
         const bool copied         = l_.weight_pitch != 0;
         const std::uint64_t pitch = copied ? l_.weight_pitch : weightStride(q_);
-        const void* const from    = copied ? base_ + l_.weight : q_.weight;
+        const void* const from    = copied ? memory_.weight(l_) : q_.weight;
         return loss::Matrix16{static_cast<const unsigned char*>(from) + 2 * first * pitch, pitch, q_.vocabulary * pitch};
     }
 
@@ -939,7 +997,7 @@ class Call final {
     cudaError_t multiply(const FtcudaGemmDesc& desc, bool slopes) const {
         Product product;
         if (configureProduct(desc, slopes, sms_, l_.product_bytes, product, message_, capacity_) != 0 ||
-            ftcuda_gemm_launch(&product.launch, base_ + l_.product, l_.product_bytes, stream_, message_, capacity_) != 0) {
+            ftcuda_gemm_launch(&product.launch, memory_.own + l_.product, l_.product_bytes, stream_, message_, capacity_) != 0) {
             return cudaErrorUnknown;  // the message says which
         }
         return cudaSuccess;
@@ -949,24 +1007,24 @@ class Call final {
     cudaError_t join(float* loss, float* lse, bool keep) const {
         JoinParams join{};
         join.rows     = rows_;
-        join.partials = at<float2>(l_.partials);
+        join.partials = own<float2>(l_.partials);
         join.pieces   = static_cast<std::uint32_t>(l_.pieces);
         join.capacity = static_cast<std::uint32_t>(l_.capacity);
-        join.row_loss = at<float>(l_.row_loss);
+        join.row_loss = own<float>(l_.row_loss);
         join.loss     = q_.reduction == FTCUDA_REDUCTION_NONE ? loss : nullptr;
         join.lse      = lse;
         join.keep     = keep;
         const cudaError_t error = training::launchOverlapped(joinStatistics, dim3(static_cast<unsigned>(l_.capacity / kJoinRows)), dim3(kJoinWarps * 32), 0, stream_, join);
         if (error != cudaSuccess || q_.reduction == FTCUDA_REDUCTION_NONE) { return error; }
-        return training::launchOverlapped(sumLosses, dim3(1), dim3(kListThreads), 0, stream_, rows_, static_cast<const float*>(at<float>(l_.row_loss)),
+        return training::launchOverlapped(sumLosses, dim3(1), dim3(kListThreads), 0, stream_, rows_, static_cast<const float*>(own<float>(l_.row_loss)),
                                           q_.reduction == FTCUDA_REDUCTION_MEAN, loss);
     }
 
     // dZ of a piece of the vocabulary, to the workspace.
     cudaError_t slopes(std::uint64_t first, std::uint64_t columns) const {
         const std::uint32_t first32 = static_cast<std::uint32_t>(first), columns32 = static_cast<std::uint32_t>(columns);
-        if (!l_.library) { return loss::launchSlopes(products_, weight(first), first32, columns32, base_ + l_.piece, l_.piece_pitch, slopesPlane()); }
-        const cudaError_t error = multiply(describeLogits(q_, l_, base_, first, columns), false);
+        if (!l_.library) { return loss::launchSlopes(products_, weight(first), first32, columns32, memory_.kept + l_.piece, l_.piece_pitch, slopesPlane()); }
+        const cudaError_t error = multiply(describeLogits(q_, l_, memory_, first, columns), false);
         if (error != cudaSuccess) { return error; }
         return training::launchOverlapped(rowSlopes, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(first, columns, nullptr));
     }
@@ -976,7 +1034,7 @@ class Call final {
                                const float* upstream) const {
         if (!l_.library) {
             loss::Gradients gradients{};
-            gradients.sums                  = hidden ? at<float>(l_.sums) : nullptr;
+            gradients.sums                  = hidden ? own<float>(l_.sums) : nullptr;
             gradients.sums_pitch            = l_.sums_pitch;
             gradients.splits                = l_.splits;
             gradients.accumulate            = first != 0;
@@ -984,7 +1042,7 @@ class Call final {
             gradients.weight_gradient_pitch = weight_stride;
             gradients.upstream              = upstream;
             if (l_.weight_splits > 1 && grad_weight != nullptr) {
-                gradients.weight_sums   = at<float>(l_.weight_sums);
+                gradients.weight_sums   = own<float>(l_.weight_sums);
                 gradients.weight_splits = l_.weight_splits;
                 gradients.weight_rows   = l_.weight_rows;
             }
@@ -992,13 +1050,13 @@ class Call final {
                 gradients.weight_gradient =
                     static_cast<unsigned char*>(grad_weight) + static_cast<std::int64_t>(training::elementBytes(grad_element) * first) * weight_stride;
             }
-            const cudaError_t error = loss::launchGradients(products_, weight(first), static_cast<std::uint32_t>(columns), loss::Matrix16{base_ + l_.piece, l_.piece_pitch, slopesPlane()}, gradients);
+            const cudaError_t error = loss::launchGradients(products_, weight(first), static_cast<std::uint32_t>(columns), loss::Matrix16{memory_.kept + l_.piece, l_.piece_pitch, slopesPlane()}, gradients);
             if (error != cudaSuccess || gradients.weight_sums == nullptr) { return error; }
             return spreadTyped(Spread{columns, nullptr, gradients.weight_sums, l_.weight_rows, l_.weight_splits, weight_stride, upstream}, gradients.weight_gradient, grad_element);
         }
         cudaError_t error = cudaSuccess;
-        if (hidden) { error = multiply(describeHidden(q_, l_, base_, first, columns), true); }
-        if (error == cudaSuccess && grad_weight != nullptr) { error = multiply(describeWeight(q_, l_, base_, first, columns, grad_weight, weight_stride), true); }
+        if (hidden) { error = multiply(describeHidden(q_, l_, memory_, first, columns), true); }
+        if (error == cudaSuccess && grad_weight != nullptr) { error = multiply(describeWeight(q_, l_, memory_, first, columns, grad_weight, weight_stride), true); }
         return error;
     }
 
@@ -1013,7 +1071,7 @@ class Call final {
         const float* upstream;
     };
     Spread hiddenParts(std::int64_t stride, const float* upstream) const {
-        return Spread{q_.tokens, at<std::int32_t>(l_.slot), at<float>(l_.sums), l_.capacity, l_.splits, stride, upstream};
+        return Spread{q_.tokens, kept<std::int32_t>(l_.slot), own<float>(l_.sums), l_.capacity, l_.splits, stride, upstream};
     }
 
     cudaError_t spreadTyped(const Spread& parts, void* out, std::int32_t element) const {
@@ -1037,7 +1095,7 @@ class Call final {
     std::size_t capacity_;
     int sms_ = 0;
     Layout l_{};
-    unsigned char* base_ = nullptr;
+    Memory memory_{};
     cudaStream_t stream_ = nullptr;
     LiveRows rows_{};
     loss::ProductCall products_{};
@@ -1093,15 +1151,55 @@ const char* checkGradients(const FtcudaLinearCrossEntropy& q, std::uint64_t byte
     return apart ? nullptr : "a gradient lies across the other one or an operand";
 }
 
-int workspaceBytes(const FtcudaLinearCrossEntropy* problem, Form form, std::uint64_t* bytes, char* message, std::size_t capacity) {
-    if (problem == nullptr || bytes == nullptr) { return fail(message, capacity, 1, "null argument"); }
+const char* checkAddress(const void* loss, const char* reason) { return wordAligned(loss) ? nullptr : reason; }
+constexpr const char* kNoLoss     = "the loss has no address, or one that is not a multiple of four";
+constexpr const char* kNoUpstream = "the loss's gradient has no address, or one that is not a multiple of four";
+
+// What a call needs: 0, or a failure with its message.
+int layOutChecked(const FtcudaLinearCrossEntropy* problem, Form form, std::uint64_t kept_bytes, Layout& layout, char* message, std::size_t capacity) {
+    if (problem == nullptr) { return fail(message, capacity, 1, "null problem"); }
     const char* reason = check(*problem);
-    if (reason == nullptr && form == Form::kStep) { reason = checkStep(*problem); }
+    if (reason == nullptr && isStep(form)) { reason = checkStep(*problem); }
     if (reason != nullptr) { return fail(message, capacity, 1, "%s", reason); }
     int sms = 0;
-    Layout layout;
-    if (!deviceSmCount(problem->device, &sms, message, capacity) || layOut(*problem, form, sms, layout, message, capacity) != 0) { return 1; }
-    *bytes = layout.total;
+    return deviceSmCount(problem->device, &sms, message, capacity) && layOut(*problem, form, kept_bytes, sms, layout, message, capacity) == 0 ? 0 : 1;
+}
+
+// Of a step with both memories in one workspace, the kept one first: how much that is, and how much both are.
+int stepBytesInOne(const FtcudaLinearCrossEntropy* problem, std::uint64_t& kept_bytes, std::uint64_t& bytes, char* message, std::size_t capacity) {
+    Layout first, second;
+    if (layOutChecked(problem, Form::kStepLoss, kAny, first, message, capacity) != 0) { return 1; }
+    if (layOutChecked(problem, Form::kStepGradients, first.kept_bytes, second, message, capacity) != 0) { return 1; }
+    kept_bytes = first.kept_bytes;
+    bytes      = first.kept_bytes + std::max(first.bytes, second.bytes);
+    return 0;
+}
+
+// The halves of a step; what they are given is checked but for the memories.
+int stepLoss(const FtcudaLinearCrossEntropy& problem, float* loss, void* kept, std::uint64_t kept_bytes, void* workspace, std::uint64_t workspace_bytes, void* stream, char* message,
+             std::size_t capacity) {
+    Call call(problem, message, capacity);
+    if (const int status = call.begin(Form::kStepLoss, kept, kept_bytes, workspace, workspace_bytes, stream)) { return status; }
+    return finish(call.stepLoss(loss), message, capacity);
+}
+int stepGradients(const FtcudaLinearCrossEntropy& problem, const float* grad_loss, std::int32_t grad_element, void* grad_hidden, std::int64_t hidden_stride, void* grad_weight,
+                  std::int64_t weight_stride, void* kept, std::uint64_t kept_bytes, void* workspace, std::uint64_t workspace_bytes, void* stream, char* message,
+                  std::size_t capacity) {
+    if (grad_hidden == nullptr && grad_weight == nullptr) { return 0; }
+    Call call(problem, message, capacity);
+    if (const int status = call.begin(Form::kStepGradients, kept, kept_bytes, workspace, workspace_bytes, stream)) { return status; }
+    return finish(call.stepGradients(grad_loss, grad_hidden, hidden_stride, grad_weight, weight_stride, grad_element), message, capacity);
+}
+
+// The kept part at the beginning of a workspace for both; 0, or a failure with its message. `exactly`: a size that another problem's would be is refused.
+int splitWorkspace(const FtcudaLinearCrossEntropy& problem, void* workspace, std::uint64_t workspace_bytes, bool exactly, std::uint64_t& kept_bytes, char* message,
+                   std::size_t capacity) {
+    if (!training::deviceIsCurrent(problem.device, message, capacity)) { return 1; }
+    std::uint64_t bytes = 0;
+    if (stepBytesInOne(&problem, kept_bytes, bytes, message, capacity) != 0) { return 1; }
+    if (workspace == nullptr || workspace_bytes < bytes || (exactly && workspace_bytes != bytes) || !training::aligned(workspace, kAlign)) {
+        return fail(message, capacity, 1, "workspace of %llu bytes needed, %sat a multiple of 256", static_cast<unsigned long long>(bytes), exactly ? "no more and no less, " : "");
+    }
     return 0;
 }
 
@@ -1110,11 +1208,40 @@ int workspaceBytes(const FtcudaLinearCrossEntropy* problem, Form form, std::uint
 
 extern "C" int ftcuda_linear_cross_entropy_workspace_bytes(const FtcudaLinearCrossEntropy* problem, int backward, uint64_t* workspace_bytes, char* message,
                                                            size_t message_capacity) {
-    return ftcuda::workspaceBytes(problem, backward != 0 ? ftcuda::Form::kGradients : ftcuda::Form::kLoss, workspace_bytes, message, message_capacity);
+    using namespace ftcuda;
+    if (workspace_bytes == nullptr) { return fail(message, message_capacity, 1, "null argument"); }
+    Layout layout;
+    if (layOutChecked(problem, backward != 0 ? Form::kGradients : Form::kLoss, kAny, layout, message, message_capacity) != 0) { return 1; }
+    *workspace_bytes = layout.kept_bytes + layout.bytes;
+    return 0;
 }
 
 extern "C" int ftcuda_linear_cross_entropy_step_workspace_bytes(const FtcudaLinearCrossEntropy* problem, uint64_t* workspace_bytes, char* message, size_t message_capacity) {
-    return ftcuda::workspaceBytes(problem, ftcuda::Form::kStep, workspace_bytes, message, message_capacity);
+    using namespace ftcuda;
+    if (workspace_bytes == nullptr) { return fail(message, message_capacity, 1, "null argument"); }
+    std::uint64_t kept_bytes = 0;
+    return stepBytesInOne(problem, kept_bytes, *workspace_bytes, message, message_capacity);
+}
+
+extern "C" int ftcuda_linear_cross_entropy_step_loss_bytes(const FtcudaLinearCrossEntropy* problem, uint64_t* kept_bytes, uint64_t* workspace_bytes, char* message,
+                                                           size_t message_capacity) {
+    using namespace ftcuda;
+    if (kept_bytes == nullptr || workspace_bytes == nullptr) { return fail(message, message_capacity, 1, "null argument"); }
+    Layout layout;
+    if (layOutChecked(problem, Form::kStepLoss, kAny, layout, message, message_capacity) != 0) { return 1; }
+    *kept_bytes      = layout.kept_bytes;
+    *workspace_bytes = layout.bytes;
+    return 0;
+}
+
+extern "C" int ftcuda_linear_cross_entropy_step_gradients_bytes(const FtcudaLinearCrossEntropy* problem, uint64_t kept_bytes, uint64_t* workspace_bytes, char* message,
+                                                                size_t message_capacity) {
+    using namespace ftcuda;
+    if (workspace_bytes == nullptr) { return fail(message, message_capacity, 1, "null argument"); }
+    Layout layout;
+    if (layOutChecked(problem, Form::kStepGradients, kept_bytes, layout, message, message_capacity) != 0) { return 1; }
+    *workspace_bytes = layout.bytes;
+    return 0;
 }
 
 extern "C" int ftcuda_linear_cross_entropy_step(const FtcudaLinearCrossEntropy* problem, float* loss, int32_t grad_element, void* grad_hidden, int64_t grad_hidden_row_stride,
@@ -1125,14 +1252,15 @@ extern "C" int ftcuda_linear_cross_entropy_step(const FtcudaLinearCrossEntropy* 
     const char* reason = check(*problem);
     if (reason == nullptr) { reason = checkStep(*problem); }
     if (reason == nullptr && grad_element != problem->element && grad_element != FTCUDA_ELEMENT_FP32) { reason = "the gradients are of the operands' type, or FP32"; }
-    if (reason == nullptr && !wordAligned(loss)) { reason = "the loss has no address, or one that is not a multiple of four"; }
+    if (reason == nullptr) { reason = checkAddress(loss, kNoLoss); }
     if (reason == nullptr) { reason = checkGradients(*problem, training::elementBytes(grad_element), grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride); }
     if (reason != nullptr) { return fail(message, message_capacity, 1, "%s", reason); }
-    Call call(*problem, message, message_capacity);
-    if (const int status = call.begin(Form::kStep, workspace, workspace_bytes, stream)) { return status; }
-    cudaError_t error = call.stepLoss(loss);
-    if (error == cudaSuccess) { error = call.stepGradients(nullptr, grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride, grad_element, false); }
-    return finish(error, message, message_capacity);
+    std::uint64_t kept = 0;
+    if (const int status = splitWorkspace(*problem, workspace, workspace_bytes, false, kept, message, message_capacity)) { return status; }
+    void* const own = static_cast<unsigned char*>(workspace) + kept;
+    if (const int status = stepLoss(*problem, loss, workspace, kept, own, workspace_bytes - kept, stream, message, message_capacity)) { return status; }
+    return stepGradients(*problem, nullptr, grad_element, grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride, workspace, kept, own, workspace_bytes - kept, stream,
+                         message, message_capacity);
 }
 
 extern "C" int ftcuda_linear_cross_entropy_step_loss(const FtcudaLinearCrossEntropy* problem, float* loss, void* workspace, uint64_t workspace_bytes, void* stream, char* message,
@@ -1141,11 +1269,11 @@ extern "C" int ftcuda_linear_cross_entropy_step_loss(const FtcudaLinearCrossEntr
     if (problem == nullptr) { return fail(message, message_capacity, 1, "null problem"); }
     const char* reason = check(*problem);
     if (reason == nullptr) { reason = checkStep(*problem); }
-    if (reason == nullptr && !wordAligned(loss)) { reason = "the loss has no address, or one that is not a multiple of four"; }
+    if (reason == nullptr) { reason = checkAddress(loss, kNoLoss); }
     if (reason != nullptr) { return fail(message, message_capacity, 1, "%s", reason); }
-    Call call(*problem, message, message_capacity);
-    if (const int status = call.begin(Form::kStep, workspace, workspace_bytes, stream)) { return status; }
-    return finish(call.stepLoss(loss), message, message_capacity);
+    std::uint64_t kept = 0;
+    if (const int status = splitWorkspace(*problem, workspace, workspace_bytes, false, kept, message, message_capacity)) { return status; }
+    return stepLoss(*problem, loss, workspace, kept, static_cast<unsigned char*>(workspace) + kept, workspace_bytes - kept, stream, message, message_capacity);
 }
 
 extern "C" int ftcuda_linear_cross_entropy_step_gradients(const FtcudaLinearCrossEntropy* problem, const float* grad_loss, void* grad_hidden, int64_t grad_hidden_row_stride,
@@ -1155,15 +1283,42 @@ extern "C" int ftcuda_linear_cross_entropy_step_gradients(const FtcudaLinearCros
     if (problem == nullptr) { return fail(message, message_capacity, 1, "null problem"); }
     const char* reason = check(*problem);
     if (reason == nullptr) { reason = checkStep(*problem); }
-    if (reason == nullptr && !wordAligned(grad_loss)) { reason = "the loss's gradient has no address, or one that is not a multiple of four"; }
+    if (reason == nullptr) { reason = checkAddress(grad_loss, kNoUpstream); }
     if (reason == nullptr) {
         reason = checkGradients(*problem, training::elementBytes(problem->element), grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride);
     }
     if (reason != nullptr) { return fail(message, message_capacity, 1, "%s", reason); }
-    if (grad_hidden == nullptr && grad_weight == nullptr) { return 0; }
-    Call call(*problem, message, message_capacity);
-    if (const int status = call.begin(Form::kStep, workspace, workspace_bytes, stream)) { return status; }
-    return finish(call.stepGradients(grad_loss, grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride, problem->element, true), message, message_capacity);
+    std::uint64_t kept = 0;
+    if (const int status = splitWorkspace(*problem, workspace, workspace_bytes, true, kept, message, message_capacity)) { return status; }
+    return stepGradients(*problem, grad_loss, problem->element, grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride, workspace, kept,
+                         static_cast<unsigned char*>(workspace) + kept, workspace_bytes - kept, stream, message, message_capacity);
+}
+
+extern "C" int ftcuda_linear_cross_entropy_step_loss_kept(const FtcudaLinearCrossEntropy* problem, float* loss, void* kept, uint64_t kept_bytes, void* workspace,
+                                                          uint64_t workspace_bytes, void* stream, char* message, size_t message_capacity) {
+    using namespace ftcuda;
+    if (problem == nullptr) { return fail(message, message_capacity, 1, "null problem"); }
+    const char* reason = check(*problem);
+    if (reason == nullptr) { reason = checkStep(*problem); }
+    if (reason == nullptr) { reason = checkAddress(loss, kNoLoss); }
+    if (reason != nullptr) { return fail(message, message_capacity, 1, "%s", reason); }
+    return stepLoss(*problem, loss, kept, kept_bytes, workspace, workspace_bytes, stream, message, message_capacity);
+}
+
+extern "C" int ftcuda_linear_cross_entropy_step_gradients_kept(const FtcudaLinearCrossEntropy* problem, const float* grad_loss, void* grad_hidden, int64_t grad_hidden_row_stride,
+                                                               void* grad_weight, int64_t grad_weight_row_stride, void* kept, uint64_t kept_bytes, void* workspace,
+                                                               uint64_t workspace_bytes, void* stream, char* message, size_t message_capacity) {
+    using namespace ftcuda;
+    if (problem == nullptr) { return fail(message, message_capacity, 1, "null problem"); }
+    const char* reason = check(*problem);
+    if (reason == nullptr) { reason = checkStep(*problem); }
+    if (reason == nullptr) { reason = checkAddress(grad_loss, kNoUpstream); }
+    if (reason == nullptr) {
+        reason = checkGradients(*problem, training::elementBytes(problem->element), grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride);
+    }
+    if (reason != nullptr) { return fail(message, message_capacity, 1, "%s", reason); }
+    return stepGradients(*problem, grad_loss, problem->element, grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride, kept, kept_bytes, workspace, workspace_bytes,
+                         stream, message, message_capacity);
 }
 
 extern "C" int ftcuda_linear_cross_entropy(const FtcudaLinearCrossEntropy* problem, float* loss, float* lse, void* workspace, uint64_t workspace_bytes, void* stream,
@@ -1172,10 +1327,10 @@ extern "C" int ftcuda_linear_cross_entropy(const FtcudaLinearCrossEntropy* probl
     if (problem == nullptr) { return fail(message, message_capacity, 1, "null problem"); }
     if (const char* reason = check(*problem)) { return fail(message, message_capacity, 1, "%s", reason); }
     const bool empty = problem->tokens == 0;
-    if (!(empty && problem->reduction == FTCUDA_REDUCTION_NONE) && !wordAligned(loss)) { return fail(message, message_capacity, 1, "the loss has no address, or one that is not a multiple of four"); }
+    if (!(empty && problem->reduction == FTCUDA_REDUCTION_NONE) && !wordAligned(loss)) { return fail(message, message_capacity, 1, "%s", kNoLoss); }
     if (!empty && !wordAligned(lse)) { return fail(message, message_capacity, 1, "lse has no address, or one that is not a multiple of four"); }
     Call call(*problem, message, message_capacity);
-    if (const int status = call.begin(Form::kLoss, workspace, workspace_bytes, stream)) { return status; }
+    if (const int status = call.begin(Form::kLoss, nullptr, 0, workspace, workspace_bytes, stream)) { return status; }
     if (empty) {
         return finish(problem->reduction == FTCUDA_REDUCTION_NONE ? cudaSuccess : cudaMemsetAsync(loss, 0, sizeof(float), static_cast<cudaStream_t>(stream)), message,
                       message_capacity);
@@ -1196,7 +1351,7 @@ extern "C" int ftcuda_linear_cross_entropy_backward(const FtcudaLinearCrossEntro
         return fail(message, message_capacity, 1, "%s", reason);
     }
     Call call(*problem, message, message_capacity);
-    if (const int status = call.begin(Form::kGradients, workspace, workspace_bytes, stream)) { return status; }
+    if (const int status = call.begin(Form::kGradients, nullptr, 0, workspace, workspace_bytes, stream)) { return status; }
     if (empty) {
         if (grad_weight == nullptr) { return 0; }
         return finish(cudaMemset2DAsync(grad_weight, static_cast<std::size_t>(grad_weight_row_stride) * bytes, 0, problem->depth * bytes, problem->vocabulary,

@@ -57,7 +57,8 @@ PLATFORM_SYMBOLS = (
     "ftcuda_gradient_clip ftcuda_expert_routing_workspace_bytes ftcuda_expert_routing ftcuda_expert_routing_backward "
     "ftcuda_linear_cross_entropy_workspace_bytes ftcuda_linear_cross_entropy ftcuda_linear_cross_entropy_backward "
     "ftcuda_linear_cross_entropy_step_workspace_bytes ftcuda_linear_cross_entropy_step ftcuda_gradient_scale "
-    "ftcuda_linear_cross_entropy_step_loss ftcuda_linear_cross_entropy_step_gradients"
+    "ftcuda_linear_cross_entropy_step_loss ftcuda_linear_cross_entropy_step_gradients ftcuda_linear_cross_entropy_step_loss_bytes "
+    "ftcuda_linear_cross_entropy_step_gradients_bytes ftcuda_linear_cross_entropy_step_loss_kept ftcuda_linear_cross_entropy_step_gradients_kept"
 ).split()
 
 
@@ -675,12 +676,17 @@ def _declare_training(lib) -> None:
     lib.ftcuda_linear_cross_entropy_step.argtypes = problem + [c_void_p, ctypes.c_int32, c_void_p, c_int64, c_void_p, c_int64] + work
     lib.ftcuda_linear_cross_entropy_step_loss.argtypes = problem + [c_void_p] + work
     lib.ftcuda_linear_cross_entropy_step_gradients.argtypes = problem + [c_void_p] * 2 + [c_int64, c_void_p, c_int64] + work
+    lib.ftcuda_linear_cross_entropy_step_loss_bytes.argtypes = problem + [POINTER(c_uint64)] * 2 + message
+    lib.ftcuda_linear_cross_entropy_step_gradients_bytes.argtypes = problem + [c_uint64, POINTER(c_uint64)] + message
+    lib.ftcuda_linear_cross_entropy_step_loss_kept.argtypes = problem + [c_void_p, c_void_p, c_uint64] + work
+    lib.ftcuda_linear_cross_entropy_step_gradients_kept.argtypes = problem + [c_void_p] * 2 + [c_int64, c_void_p, c_int64, c_void_p, c_uint64] + work
     lib.ftcuda_gradient_scale.argtypes = [POINTER(Gradient), c_uint64, c_void_p, ctypes.c_int32, c_void_p] + message
     lib.ftcuda_linear_cross_entropy_backward.argtypes = problem + [c_void_p] * 3 + [c_int64, c_void_p, c_int64] + work
     for name in ("ftcuda_gradient_norm", "ftcuda_gradient_clip", "ftcuda_expert_routing", "ftcuda_expert_routing_backward",
                  "ftcuda_linear_cross_entropy_workspace_bytes", "ftcuda_linear_cross_entropy", "ftcuda_linear_cross_entropy_backward",
                  "ftcuda_linear_cross_entropy_step_workspace_bytes", "ftcuda_linear_cross_entropy_step", "ftcuda_gradient_scale",
-                 "ftcuda_linear_cross_entropy_step_loss", "ftcuda_linear_cross_entropy_step_gradients"):
+                 "ftcuda_linear_cross_entropy_step_loss", "ftcuda_linear_cross_entropy_step_gradients", "ftcuda_linear_cross_entropy_step_loss_bytes",
+                 "ftcuda_linear_cross_entropy_step_gradients_bytes", "ftcuda_linear_cross_entropy_step_loss_kept", "ftcuda_linear_cross_entropy_step_gradients_kept"):
         getattr(lib, name).restype = ctypes.c_int
 
 
@@ -770,6 +776,31 @@ def linear_cross_entropy_step_gradients(problem: LinearCrossEntropy, grad_loss: 
     """ftcuda_linear_cross_entropy_step_gradients from the workspace that linear_cross_entropy_step_loss left; 0 for a gradient that is not wanted."""
     _run_training(lib.ftcuda_linear_cross_entropy_step_gradients, byref(problem), grad_loss, grad_hidden, grad_hidden_row_stride, grad_weight,
                   grad_weight_row_stride, workspace, workspace_bytes, stream)
+
+
+def linear_cross_entropy_step_loss_bytes(problem: LinearCrossEntropy) -> tuple:
+    """Bytes of the kept memory and of the workspace for linear_cross_entropy_step_loss_kept."""
+    kept, size = c_uint64(), c_uint64()
+    _run_training(lib.ftcuda_linear_cross_entropy_step_loss_bytes, byref(problem), byref(kept), byref(size))
+    return int(kept.value), int(size.value)
+
+
+def linear_cross_entropy_step_gradients_bytes(problem: LinearCrossEntropy, kept_bytes: int) -> int:
+    size = c_uint64()
+    _run_training(lib.ftcuda_linear_cross_entropy_step_gradients_bytes, byref(problem), kept_bytes, byref(size))
+    return int(size.value)
+
+
+def linear_cross_entropy_step_loss_kept(problem: LinearCrossEntropy, loss: int, kept: int, kept_bytes: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    """ftcuda_linear_cross_entropy_step_loss_kept: the loss, and in the kept memory what its gradients are made of."""
+    _run_training(lib.ftcuda_linear_cross_entropy_step_loss_kept, byref(problem), loss, kept, kept_bytes, workspace, workspace_bytes, stream)
+
+
+def linear_cross_entropy_step_gradients_kept(problem: LinearCrossEntropy, grad_loss: int, grad_hidden: int, grad_hidden_row_stride: int, grad_weight: int,
+                                             grad_weight_row_stride: int, kept: int, kept_bytes: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    """ftcuda_linear_cross_entropy_step_gradients_kept from what linear_cross_entropy_step_loss_kept left; 0 for a gradient that is not wanted."""
+    _run_training(lib.ftcuda_linear_cross_entropy_step_gradients_kept, byref(problem), grad_loss, grad_hidden, grad_hidden_row_stride, grad_weight, grad_weight_row_stride, kept,
+                  kept_bytes, workspace, workspace_bytes, stream)
 
 
 def gradient_scale(gradients, factor: int, device: int = 0, stream: int = 0) -> None:

@@ -88,20 +88,22 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
     }
 };
 
-// The logits are computed once: the forward pass leaves in its workspace what the gradients are made of, which the graph keeps until the backward pass.
+// The logits are computed once: the forward pass leaves what the gradients are made of in a tensor that the graph keeps until the backward pass. (The weight is the graph's too, and may
+// come back from a saved-tensor hook as another copy; only the kept tensor's size has to stay.)
 class LinearCrossEntropyStep : public torch::autograd::Function<LinearCrossEntropyStep> {
   public:
     static at::Tensor forward(AutogradContext* context, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, std::int64_t ignore_index,
-                              std::int64_t reduction, std::int64_t workspace_bytes) {
+                              std::int64_t reduction, std::int64_t kept_bytes, std::int64_t workspace_bytes) {
         const c10::cuda::CUDAGuard guard(hidden.device());
         const FtcudaLinearCrossEntropy q = describe(hidden, weight, target, ignore_index, reduction);
         at::Tensor loss                  = at::empty({}, hidden.options().dtype(at::kFloat).requires_grad(false));
+        const at::Tensor kept            = workspaceFor(static_cast<std::uint64_t>(kept_bytes), hidden);
         const at::Tensor workspace       = workspaceFor(static_cast<std::uint64_t>(workspace_bytes), hidden);
         Message message;
-        const int status = ftcuda_linear_cross_entropy_step_loss(&q, loss.data_ptr<float>(), workspace.data_ptr(), static_cast<std::uint64_t>(workspace_bytes), streamOf(q),
-                                                                 message.text, sizeof message.text);
+        const int status = ftcuda_linear_cross_entropy_step_loss_kept(&q, loss.data_ptr<float>(), kept.data_ptr(), static_cast<std::uint64_t>(kept_bytes), workspace.data_ptr(),
+                                                                      static_cast<std::uint64_t>(workspace_bytes), streamOf(q), message.text, sizeof message.text);
         TORCH_CHECK(status == 0, "flash_train linear_cross_entropy failed: ", message.text);
-        context->save_for_backward({hidden, weight, target, workspace});
+        context->save_for_backward({hidden, weight, target, kept});
         context->saved_data["ignore_index"] = ignore_index;
         context->saved_data["reduction"]    = reduction;
         return loss;
@@ -110,18 +112,22 @@ class LinearCrossEntropyStep : public torch::autograd::Function<LinearCrossEntro
     static variable_list backward(AutogradContext* context, const variable_list& gradients) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "linear_cross_entropy has no second derivative (create_graph=True)");
         const variable_list saved = context->get_saved_variables();
-        const at::Tensor &hidden = saved[0], &weight = saved[1], &target = saved[2], &workspace = saved[3];
+        const at::Tensor &hidden = saved[0], &weight = saved[1], &target = saved[2], &kept = saved[3];
         const at::Tensor grad_loss = gradients[0].to(at::kFloat).contiguous();
         const c10::cuda::CUDAGuard guard(hidden.device());
         const FtcudaLinearCrossEntropy q =
             describe(hidden, weight, target, context->saved_data["ignore_index"].toInt(), context->saved_data["reduction"].toInt());
-        variable_list out(6);
+        variable_list out(7);
         if (context->needs_input_grad(0)) { out[0] = at::empty(hidden.sizes(), hidden.options().requires_grad(false)); }
         if (context->needs_input_grad(1)) { out[1] = at::empty(weight.sizes(), weight.options().requires_grad(false)); }
+        const std::uint64_t kept_bytes = static_cast<std::uint64_t>(kept.numel());
+        std::uint64_t bytes            = 0;
         Message message;
-        const int status = ftcuda_linear_cross_entropy_step_gradients(&q, grad_loss.data_ptr<float>(), addressOf(out[0]), hidden.size(1), addressOf(out[1]), hidden.size(1),
-                                                                      workspace.data_ptr(), static_cast<std::uint64_t>(workspace.numel()), streamOf(q), message.text,
-                                                                      sizeof message.text);
+        int status = ftcuda_linear_cross_entropy_step_gradients_bytes(&q, kept_bytes, &bytes, message.text, sizeof message.text);
+        TORCH_CHECK(status == 0, "flash_train linear_cross_entropy's gradient failed: ", message.text);
+        const at::Tensor workspace = workspaceFor(bytes, hidden);
+        status = ftcuda_linear_cross_entropy_step_gradients_kept(&q, grad_loss.data_ptr<float>(), addressOf(out[0]), hidden.size(1), addressOf(out[1]), hidden.size(1), kept.data_ptr(),
+                                                                 kept_bytes, workspace.data_ptr(), bytes, streamOf(q), message.text, sizeof message.text);
         TORCH_CHECK(status == 0, "flash_train linear_cross_entropy's gradient failed: ", message.text);
         return out;
     }
@@ -147,9 +153,9 @@ at::Tensor linearCrossEntropy(const at::Tensor& hidden, const at::Tensor& weight
     const at::Tensor indices = target.reshape({-1}).contiguous();
     if (at::GradMode::is_enabled() && (flat.requires_grad() || weight.requires_grad())) {
         const FtcudaLinearCrossEntropy q = describe(flat, weight, indices, ignore_index, kind);
-        std::uint64_t bytes              = 0;
-        if (ftcuda_linear_cross_entropy_step_workspace_bytes(&q, &bytes, nullptr, 0) == 0) {
-            return LinearCrossEntropyStep::apply(flat, weight, indices, ignore_index, kind, static_cast<std::int64_t>(bytes));
+        std::uint64_t kept = 0, bytes = 0;
+        if (ftcuda_linear_cross_entropy_step_loss_bytes(&q, &kept, &bytes, nullptr, 0) == 0) {
+            return LinearCrossEntropyStep::apply(flat, weight, indices, ignore_index, kind, static_cast<std::int64_t>(kept), static_cast<std::int64_t>(bytes));
         }
     }
     const at::Tensor loss = LinearCrossEntropy::apply(flat, weight, indices, ignore_index, kind);

@@ -148,7 +148,7 @@ FTCUDA_API int ftcuda_linear_cross_entropy_step(const FtcudaLinearCrossEntropy* 
 /*
  * The step call in two: the loss first, and the gradients when the upstream gradient (*grad_loss, FP32 on the device) is known, of the operands' type and
  * rounded once. In between the workspace keeps what they are made of, for the same problem, and so does the weight; the hidden states and the targets are not looked at again.
- * The second call may be made any number of times.
+ * The second call may be made any number of times, with the workspace_bytes that ftcuda_linear_cross_entropy_step_workspace_bytes says, no more and no less.
  */
 FTCUDA_API int ftcuda_linear_cross_entropy_step_loss(const FtcudaLinearCrossEntropy* problem, float* loss, void* workspace, uint64_t workspace_bytes,
                                                      void* stream, char* message, size_t message_capacity);
@@ -156,6 +156,22 @@ FTCUDA_API int ftcuda_linear_cross_entropy_step_gradients(const FtcudaLinearCros
                                                           int64_t grad_hidden_row_stride, void* grad_weight, int64_t grad_weight_row_stride,
                                                           void* workspace, uint64_t workspace_bytes, void* stream, char* message,
                                                           size_t message_capacity);
+
+/*
+ * The same two calls with what is kept in a memory of its own, so that each call's workspace is free again behind it. `kept` and the workspaces start at multiples of 256;
+ * kept_bytes is what ftcuda_linear_cross_entropy_step_loss_bytes says for the problem of the loss, no more and no less, in both calls. When the gradients are made
+ * the weight's values have to be the same; its address and strides need not.
+ */
+FTCUDA_API int ftcuda_linear_cross_entropy_step_loss_bytes(const FtcudaLinearCrossEntropy* problem, uint64_t* kept_bytes, uint64_t* workspace_bytes, char* message,
+                                                           size_t message_capacity);
+FTCUDA_API int ftcuda_linear_cross_entropy_step_gradients_bytes(const FtcudaLinearCrossEntropy* problem, uint64_t kept_bytes, uint64_t* workspace_bytes, char* message,
+                                                                size_t message_capacity);
+FTCUDA_API int ftcuda_linear_cross_entropy_step_loss_kept(const FtcudaLinearCrossEntropy* problem, float* loss, void* kept, uint64_t kept_bytes, void* workspace,
+                                                          uint64_t workspace_bytes, void* stream, char* message, size_t message_capacity);
+FTCUDA_API int ftcuda_linear_cross_entropy_step_gradients_kept(const FtcudaLinearCrossEntropy* problem, const float* grad_loss, void* grad_hidden,
+                                                               int64_t grad_hidden_row_stride, void* grad_weight, int64_t grad_weight_row_stride, void* kept,
+                                                               uint64_t kept_bytes, void* workspace, uint64_t workspace_bytes, void* stream, char* message,
+                                                               size_t message_capacity);
 
 /* ---- the experts' router ---- */
 

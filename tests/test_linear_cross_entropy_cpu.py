@@ -89,3 +89,24 @@ def test_where_the_step_in_two_does_not_write(capi):
     refuse(capi, "a gradient's address", step, q, 0x40000000, 0x70000001, 64, 0x80000000, 64, 0x60000000, 1 << 40)
     refuse(capi, "weight's gradient overlap", step, q, 0x40000000, 0x70000000, 64, 0x80000000, 63, 0x60000000, 1 << 40)
     refuse(capi, "lies across", step, q, 0x40000000, 0x70000000, 64, 0x20000000, 64, 0x60000000, 1 << 40)
+
+
+@pytest.mark.parametrize("change, reason", [
+    ({"reduction": 0}, "without reduction"), ({"tokens": 0}, "no tokens"), ({"tokens": 1 << 16, "vocabulary": 1 << 15}, "2 GiB"), ({"element": 1}, "FP32, FP16 or BF16"),
+    ({"target": 0x30000004}, "targets"), ({"weight": None}, "the weight has no address"),
+])
+def test_what_the_step_with_a_kept_memory_does_not_take(capi, change, reason):
+    q = problem(capi, **change)
+    refuse(capi, reason, capi.linear_cross_entropy_step_loss_bytes, q)
+    refuse(capi, reason, capi.linear_cross_entropy_step_gradients_bytes, q, 1 << 20)
+    refuse(capi, reason, capi.linear_cross_entropy_step_loss_kept, q, 0x40000000, 0x50000000, 1 << 20, 0x60000000, 1 << 40)
+    refuse(capi, reason, capi.linear_cross_entropy_step_gradients_kept, q, 0x40000000, 0x70000000, 64, 0x80000000, 64, 0x50000000, 1 << 20, 0x60000000, 1 << 40)
+
+
+def test_where_the_step_with_a_kept_memory_does_not_write(capi):
+    q = problem(capi)
+    loss, step = capi.linear_cross_entropy_step_loss_kept, capi.linear_cross_entropy_step_gradients_kept
+    refuse(capi, "the loss has no address", loss, q, 0, 0x50000000, 1 << 20, 0x60000000, 1 << 40)
+    refuse(capi, "gradient has no address", step, q, 0x40000001, 0x70000000, 64, 0x80000000, 64, 0x50000000, 1 << 20, 0x60000000, 1 << 40)
+    refuse(capi, "a gradient's address", step, q, 0x40000000, 0x70000001, 64, 0x80000000, 64, 0x50000000, 1 << 20, 0x60000000, 1 << 40)
+    refuse(capi, "lies across", step, q, 0x40000000, 0x70000000, 64, 0x20000000, 64, 0x50000000, 1 << 20, 0x60000000, 1 << 40)

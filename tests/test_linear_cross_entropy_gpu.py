@@ -675,3 +675,76 @@ def test_many_tokens_of_few_classes(ft, dtype, tokens, depth, vocabulary, live, 
     upstream = torch.randn(tokens, device="cuda", generator=torch.Generator(device="cuda").manual_seed(9)) * 16.0 if reduction == "none" else torch.tensor(16.0, device="cuda")
     alone, = torch.autograd.grad(loss, w, upstream)
     assert torch.equal(alone, grad_weight)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens, depth, vocabulary, offset, gap", [(70, 1024, 300, 1, 0), (300, 96, 1501, 3, 0), (40, 136, 700, 0, 5), (90, 1027, 601, 0, 5), (130, 129, 515, 1, 0),
+                                                                    (64, 1024, 300, 0, 8), (8, 130, 400, 0, 6),
+                                                                    (64, 1024, 300, 1, 0), (8, 131, 400, 2, 0)])
+def test_a_weight_that_comes_back_from_elsewhere(ft, dtype, tokens, depth, vocabulary, offset, gap):
+    """What a saved-tensor hook hands back is another copy: a weight at an odd address or with rows at an odd distance comes back dense and aligned, and one that TMA takes with
+    rows that it does not."""
+    hidden, weight, target = make(tokens, depth, vocabulary, dtype, seed=90)
+    target[::6] = -100
+    buffer = torch.full((offset + vocabulary * (depth + gap),), math.nan, device="cuda", dtype=dtype)
+    view = buffer[offset:].view(vocabulary, depth + gap)[:, :depth]
+    view.copy_(weight)
+    expected = run(ft, hidden, view, target)
+    h, w = hidden.clone().requires_grad_(), view.detach().requires_grad_()
+    with torch.autograd.graph.save_on_cpu():
+        loss = ft.linear_cross_entropy(h, w, target)
+    grad_hidden, grad_weight = torch.autograd.grad(loss, (h, w))
+    assert torch.equal(loss.detach(), expected[0])
+    oracle = Oracle(hidden, weight, target)
+    each = torch.full((tokens,), 1.0 / int(oracle.live.sum()), device="cuda", dtype=torch.float64)
+    dh, dh_bound, dw, dw_bound = oracle.gradients(each, dtype)
+    check(grad_hidden, dh, dh_bound, "hidden's gradient")
+    check(grad_weight, dw, dw_bound, "weight's gradient")
+
+
+@pytest.mark.parametrize("dtype, tokens, depth, vocabulary", [(torch.bfloat16, 2048, 512, 32768), (torch.float16, 600, 512, 50000), (torch.float32, 400, 512, 32768), (torch.float32, 1200, 1200, 9000)])
+def test_what_waits_in_the_graph(ft, memory_given_back, dtype, tokens, depth, vocabulary):
+    """From the forward pass to the backward one: the slopes (FP32 operands: three halves each, or one number where they go through the library's products), the hidden states, a
+    copy of an FP32 weight; not what one of the passes needs for itself."""
+    hidden, weight, target = make(tokens, depth, vocabulary, dtype, seed=98)
+    h, w = hidden.requires_grad_(), weight.requires_grad_()
+    before = torch.cuda.memory_allocated()
+    loss = ft.linear_cross_entropy(h, w, target)
+    kept = torch.cuda.memory_allocated() - before
+    rows, columns, bytes = -(-tokens // 256) * 256, -(-vocabulary // 256) * 256, {torch.float32: 6, torch.float16: 2, torch.bfloat16: 2}[dtype]
+    pitch = -(-depth // 8) * 8
+    limit = rows * columns * bytes + rows * pitch * bytes + (vocabulary * pitch * 6 if dtype == torch.float32 else 0)
+    assert kept <= limit + (4 << 20)  # (the lists, and what the allocator rounds up to)
+    loss.backward()
+
+
+def test_what_the_kept_memory_has_to_be(ft, capi):
+    hidden, weight, target = make(10, 16, 20, torch.bfloat16)
+    buffer = torch.zeros(20 * 17, device="cuda", dtype=torch.bfloat16)
+
+    def problem(weight, stride=16):
+        return capi.LinearCrossEntropy(hidden=hidden.data_ptr(), weight=weight.data_ptr(), target=target.data_ptr(), tokens=10, vocabulary=20, depth=16, hidden_row_stride=16,
+                                       weight_row_stride=stride, ignore_index=-100, element=8, reduction=1, device=0)
+
+    q, odd = problem(weight), problem(buffer, 17)
+    kept, size = capi.linear_cross_entropy_step_loss_bytes(q)
+    with_copy, _ = capi.linear_cross_entropy_step_loss_bytes(odd)
+    assert with_copy > kept
+    memory, out = torch.empty(1 << 20, dtype=torch.uint8, device="cuda"), torch.empty(4096, device="cuda")
+    loss, at = out.data_ptr(), memory.data_ptr()
+    for bytes, where, workspace, reason in ((kept - 1, at, size, "kept memory of"), (kept + 256, at, size, "kept memory of"), (kept, at + 128, size, "kept memory of"),
+                                            (kept, 0, size, "kept memory of"), (kept, at, size - 1, "workspace of")):
+        with pytest.raises(capi.FTrainError, match=reason):
+            capi.linear_cross_entropy_step_loss_kept(q, loss, where, bytes, at + (1 << 19), workspace)
+    for p in (q, odd):  # either size is one that a loss can have left, whatever the weight's address is by now
+        for bytes in (kept, with_copy):
+            assert capi.linear_cross_entropy_step_gradients_bytes(p, bytes) > 0
+        with pytest.raises(capi.FTrainError, match="kept memory has"):
+            capi.linear_cross_entropy_step_gradients_bytes(p, kept + 256)
+        with pytest.raises(capi.FTrainError, match="kept memory has"):
+            capi.linear_cross_entropy_step_gradients_kept(p, loss, loss + 1024, 16, loss + 2048, 16, at, with_copy + 256, at + (1 << 19), 1 << 19)
+    # With both in one workspace its size says what was kept.
+    whole = capi.linear_cross_entropy_step_workspace_bytes(q)
+    for bytes in (whole - 1, whole + 1, capi.linear_cross_entropy_step_workspace_bytes(odd)):
+        with pytest.raises(capi.FTrainError, match="no more and no less"):
+            capi.linear_cross_entropy_step_gradients(q, loss, loss + 1024, 16, loss + 2048, 16, at, bytes)
