@@ -709,11 +709,14 @@ int layOut(const FtcudaLinearCrossEntropy& q, Form form, std::uint64_t kept_byte
     // (The prepared products split the weight whatever its rows' alignment; the others would copy it for each product, element by element: a step of 8 x 3967 x 60001 FP32
     // 3166 us, 1309 with one copy; 1000 x 2311 x 20000, prepared, the loss 384, with a copy 411.)
     const bool split_anyway = l.library && preparedFormPays(q.tokens, q.vocabulary, q.depth);
+    // What waits for the gradients is no more than the logits' limit with the weight's copy either: a larger one is made again. (256 x 4096 x 131072 FP32 4.74 ms with 3.2 GB of planes
+    // waiting, 5.65 made again, 300 x 4096 x 90000 4.95 and 5.57; in a step of 600 x 512 x 16384, where they wait, another splitting would take 14 us of 269.)
     Room with_copy          = kept;
     const std::uint64_t at  = with_copy.take(element * q.vocabulary * l.copy_pitch);
-    if (l.planes || (kept_bytes == with_copy.at && !split_anyway) || (!split_anyway && !weightFits(q))) {
+    const bool may_keep     = isStep(form) && stepBytes(q) + element * q.vocabulary * l.copy_pitch <= kStepBytes, keeps = may_keep && kept_bytes == with_copy.at;
+    if (l.planes || (keeps && !split_anyway) || (!split_anyway && !weightFits(q))) {
         l.weight_pitch = l.copy_pitch;
-        l.weight_kept  = isStep(form) && (kept_bytes == kAny || kept_bytes == with_copy.at);
+        l.weight_kept  = keeps || (may_keep && kept_bytes == kAny);
         l.weight_made  = form == Form::kStepGradients && l.weight_kept;
         l.weight       = l.weight_kept ? at : own.take(element * q.vocabulary * l.copy_pitch);
         if (l.weight_kept) { kept = with_copy; }

@@ -748,3 +748,23 @@ def test_what_the_kept_memory_has_to_be(ft, capi):
     for bytes in (whole - 1, whole + 1, capi.linear_cross_entropy_step_workspace_bytes(odd)):
         with pytest.raises(capi.FTrainError, match="no more and no less"):
             capi.linear_cross_entropy_step_gradients(q, loss, loss + 1024, 16, loss + 2048, 16, at, bytes)
+
+
+@pytest.mark.parametrize("dtype, depth, vocabulary", [(torch.float32, 4096, 90001), (torch.bfloat16, 4097, 262145)])
+def test_a_large_copy_of_the_weight_does_not_wait_in_the_graph(ft, capi, memory_given_back, dtype, depth, vocabulary):
+    """Three halves for each element of an FP32 weight, or the copy of one that TMA does not take: beyond the 2 GiB they are made again for the gradients."""
+    hidden, _, target = make(100, depth, vocabulary, dtype, seed=99)
+    target[::5] = -100
+    weight = torch.empty(vocabulary, depth, device="cuda", dtype=dtype)
+    for piece in weight.split(65536):
+        piece.copy_(torch.randn(piece.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(piece.shape[0])) * depth ** -0.5)
+    h, w = hidden.requires_grad_(), weight.requires_grad_()
+    before = torch.cuda.memory_allocated()
+    loss = ft.linear_cross_entropy(h, w, target)
+    assert torch.cuda.memory_allocated() - before <= 256 * (vocabulary + 255) * (6 if dtype == torch.float32 else 2) + (16 << 20)
+    grad_hidden, grad_weight = torch.autograd.grad(loss, (h, w))
+    loss2, hidden2, weight2 = split_in_two(capi, hidden.detach(), weight.detach(), target, torch.ones((), device="cuda"))
+    # Either form is off by its slopes' rounding (two of them in the step) and its results' own.
+    tolerance = {torch.float32: 2e-6, torch.bfloat16: 2.0 ** -8}[dtype] * 3
+    assert abs(loss.item() - loss2.item()) <= 2e-6 * loss2.item()
+    assert (grad_hidden - hidden2).float().norm() <= tolerance * hidden2.float().norm() and (grad_weight - weight2).float().norm() <= tolerance * weight2.float().norm()
