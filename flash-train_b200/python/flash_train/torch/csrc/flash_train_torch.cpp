@@ -152,19 +152,13 @@ bool planReuseDisabled() {
     return disabled;
 }
 
-// A size that torch's allocator could not give this thread on a device, and for how many more calls nothing as large is asked
-// for: each refusal makes the allocator synchronise the device and give back all that it caches, which a program near
-// the end of the memory would pay on every call. Not kept with a Plan: such a program's addresses, and with them its Plans, change.
-struct RefusedWorkspace {
-    std::uint64_t bytes = 0;
-    unsigned calls      = 0;
-};
-constexpr unsigned kAskAgainAfter = 64;
+using flash_train_torch::kAskAgainAfter;
+using flash_train_torch::RefusedWorkspace;
 
+// Not kept with a Plan: the addresses of a program near the end of the memory, and with them its Plans, change.
 RefusedWorkspace& refusedWorkspace(std::size_t device) {
     static thread_local std::vector<RefusedWorkspace> refused;
-    if (refused.size() <= device) { refused.resize(device + 1); }
-    return refused[device];
+    return flash_train_torch::ofDevice(refused, device);
 }
 
 // Runs the Plan's first primitive whose workspace torch's allocator can give: the best form of a tensor-core

@@ -133,6 +133,12 @@ class LinearCrossEntropyStep : public torch::autograd::Function<LinearCrossEntro
     }
 };
 
+// What the step form could not be given on a device.
+RefusedWorkspace& refusedStep(std::size_t device) {
+    static thread_local std::vector<RefusedWorkspace> refused;
+    return ofDevice(refused, device);
+}
+
 at::Tensor linearCrossEntropy(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, std::int64_t ignore_index, const std::string& reduction) {
     for (const at::Tensor* operand : {&hidden, &weight}) {
         TORCH_CHECK(operand->is_cuda() && operand->layout() == at::kStrided && !operand->is_neg(), "hidden and weight must be dense device tensors");
@@ -155,7 +161,15 @@ at::Tensor linearCrossEntropy(const at::Tensor& hidden, const at::Tensor& weight
         const FtcudaLinearCrossEntropy q = describe(flat, weight, indices, ignore_index, kind);
         std::uint64_t kept = 0, bytes = 0;
         if (ftcuda_linear_cross_entropy_step_loss_bytes(&q, &kept, &bytes, nullptr, 0) == 0) {
-            return LinearCrossEntropyStep::apply(flat, weight, indices, ignore_index, kind, static_cast<std::int64_t>(kept), static_cast<std::int64_t>(bytes));
+            // Where the allocator has no room for all logits' exponentials, the form that goes through the vocabulary piece by piece takes less.
+            RefusedWorkspace& refused = refusedStep(static_cast<std::size_t>(hidden.device().index()));
+            if (refused.calls != 0 && kept + bytes >= refused.bytes) {
+                --refused.calls;
+            } else {
+                try {
+                    return LinearCrossEntropyStep::apply(flat, weight, indices, ignore_index, kind, static_cast<std::int64_t>(kept), static_cast<std::int64_t>(bytes));
+                } catch (const c10::OutOfMemoryError&) { refused = RefusedWorkspace{kept + bytes, kAskAgainAfter}; }
+            }
         }
     }
     const at::Tensor loss = LinearCrossEntropy::apply(flat, weight, indices, ignore_index, kind);

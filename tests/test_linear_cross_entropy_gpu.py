@@ -768,3 +768,32 @@ def test_a_large_copy_of_the_weight_does_not_wait_in_the_graph(ft, capi, memory_
     tolerance = {torch.float32: 2e-6, torch.bfloat16: 2.0 ** -8}[dtype] * 3
     assert abs(loss.item() - loss2.item()) <= 2e-6 * loss2.item()
     assert (grad_hidden - hidden2).float().norm() <= tolerance * hidden2.float().norm() and (grad_weight - weight2).float().norm() <= tolerance * weight2.float().norm()
+
+
+@pytest.mark.parametrize("dtype, tokens, vocabulary", [(torch.bfloat16, 8192, 131072), (torch.float32, 3072, 65536)])
+def test_where_there_is_no_room_for_the_exponentials(ft, memory_given_back, dtype, tokens, vocabulary):
+    """With less memory left than the step wants, the gradients come from the form that goes through the vocabulary piece by piece."""
+    hidden, weight, target = make(tokens, 64, vocabulary, dtype, seed=97)
+    target[::5] = -100
+    expected = run(ft, hidden, weight, target)
+    torch.cuda.synchronize()
+    gc.collect()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    total = torch.cuda.get_device_properties(0).total_memory
+    before = torch.cuda.memory_reserved()
+    torch.cuda.set_per_process_memory_fraction((before + 1.25 * 2 ** 30) / total)
+    try:
+        for _ in range(3):  # the first of these asks for the room, the others remember
+            got = run(ft, hidden, weight, target)
+            assert torch.cuda.max_memory_reserved() <= before + 1.25 * 2 ** 30
+            tolerance = 2e-6 if dtype == torch.float32 else torch.finfo(dtype).eps
+            assert abs(got[0].item() - expected[0].item()) <= 1e-6 * expected[0].item()
+            assert all((a.double() - b.double()).norm() <= 2 * tolerance * b.double().norm() for a, b in zip(got[1:], expected[1:]))
+            del got
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    # With the memory back, the step is asked for again in the end: equal bits.
+    for _ in range(70):
+        got = run(ft, hidden, weight, target)
+    assert all(torch.equal(a, b) for a, b in zip(got, expected))
