@@ -111,6 +111,7 @@ at::Tensor normOf(const TensorList& gradients, const TensorList* outs, double no
         const at::Tensor& gradient = gradients[i];
         const at::Tensor& out      = outs != nullptr ? (*outs)[i] : gradient;
         checkGradient(gradient, first, "gradient", i);
+        TORCH_CHECK(!recording || !gradient.requires_grad(), "gradient ", i, " must not require a gradient: the norm is not differentiable (detach it, or use torch.no_grad())");
         if (outs != nullptr) {
             if (!out.is_same(gradient)) {
                 checkGradient(out, first, "out", i);
@@ -153,11 +154,11 @@ at::Tensor clipGrads(const pybind11::object& gradients, double max_norm, double 
 void registerGradientNorm(pybind11::module_& module) {
     module.def("grad_norm", &gradNorm,
                "Norm over all elements of a list of gradients (FP32, FP16, BF16; any sizes), as one FP32 number on their device.\n\n"
-               "norm_type: 2, or infinity for the largest magnitude.",
+               "norm_type: 2, or infinity for the largest magnitude. Not differentiable: tensors that require a gradient are refused outside of torch.no_grad().",
                pybind11::arg("gradients"), pybind11::arg("norm_type") = 2.0);
     module.def("clip_grads", &clipGrads,
                "Multiplies every gradient by min(1, max_norm / (norm + 1e-6)) and returns the norm before that, without waiting for it.\n\n"
-               "In place, or into `out`: tensors of the same shapes in any of the three types.",
+               "In place, or into `out`: tensors of the same shapes in any of the three types. Not differentiable, as grad_norm.",
                pybind11::arg("gradients"), pybind11::arg("max_norm"), pybind11::arg("norm_type") = 2.0, pybind11::arg("out") = pybind11::none());
 }
 

@@ -307,3 +307,19 @@ def test_another_device_than_the_current_one(ft, capi):
     with pytest.raises(capi.FTrainError, match="device 1 must be current"):
         capi.gradient_scale(gradients, out.data_ptr(), device=1)
     assert (g == 1).all()
+
+
+def test_what_would_leave_autograd_is_refused(ft):
+    """A penalty on a gradient's norm would otherwise train on nothing."""
+    x = torch.ones(5, device="cuda", requires_grad=True)
+    gradient, = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+    for call in (lambda: ft.grad_norm([gradient]), lambda: ft.grad_norm([x]), lambda: ft.clip_grads([gradient], 1.0), lambda: ft.clip_grads([gradient], 1.0, out=[torch.empty(5, device="cuda")])):
+        with pytest.raises(RuntimeError, match="must not require a gradient: the norm is not differentiable"):
+            call()
+    with torch.no_grad():
+        check_norm(ft.grad_norm([gradient, x]), exact_norm([gradient.detach(), x.detach()]))
+    check_norm(ft.grad_norm([gradient.detach()]), exact_norm([gradient.detach()]))
+    loss = (x * 2).sum()
+    loss.backward()
+    x.grad.requires_grad_()  # clip_grad_norm_ works in place and records nothing
+    check_norm(ft.clip_grad_norm_([x], 1.0), math.sqrt(20.0))
