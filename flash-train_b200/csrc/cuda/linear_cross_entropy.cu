@@ -138,6 +138,13 @@ template<bool kScales> __global__ void __launch_bounds__(kListThreads) listToken
             }
             p.rows.scale[i] = scale;
             p.rows.lse2[i]  = lse2;
+            if (p.rows.own_scale != nullptr) {
+                // The same with the row's own |scale| for the largest one.
+                const float own        = i < count ? p.grad_loss[p.rows.token[i]] : 0.0F;
+                const std::int32_t by  = p.scale_bits - (own != 0.0F && fabsf(own) <= FLT_MAX ? max(-100, ilogbf(own)) : 0);
+                p.rows.own_scale[i]    = i < count && p.rows.target[i] == loss::kBadTarget ? scale : ldexpf(own, by);
+                p.rows.own_unit[i]     = ldexpf(1.0F, -by);
+            }
         }
     }
     for (std::uint32_t i = count + threadIdx.x; i < padded; i += kListThreads) {
@@ -492,7 +499,7 @@ __global__ void __launch_bounds__(kGatherThreads) spreadHidden(const LiveRows ro
     gridDependencyLaunchDependents();
     // (Never beyond, whatever stands there. Without slots every row is its own: the weight's gradient.)
     const std::int32_t row = slot != nullptr ? min(slot[blockIdx.x], static_cast<std::int32_t>(capacity) - 1) : static_cast<std::int32_t>(blockIdx.x);
-    const float unit       = *rows.unit * (upstream != nullptr ? *upstream : 1.0F);
+    const float unit       = (slot != nullptr && row >= 0 && rows.own_unit != nullptr ? rows.own_unit[row] : *rows.unit) * (upstream != nullptr ? *upstream : 1.0F);
     T* const to            = out + static_cast<std::int64_t>(blockIdx.x) * stride;
     const float* const from = sums + static_cast<std::uint64_t>(max(row, 0)) * pitch;
 #pragma unroll 2
@@ -529,6 +536,7 @@ struct Layout {
     std::uint64_t count, unit, slot, hidden, piece;  // kept
     std::uint64_t weight;
     std::uint64_t token, target, scale, lse2, picked, row_loss, partials, exponentials, sums, weight_sums, product, product_bytes;
+    std::uint64_t own_scale, own_unit, own_piece;  // where rows have scales of their own
     std::uint64_t kept_bytes, bytes;
 };
 
@@ -654,10 +662,16 @@ bool libraryPays(const FtcudaLinearCrossEntropy& q, Form form) {
     return large || q.tokens <= 8 || (q.tokens <= 64 && q.depth >= 1024);
 }
 
+// Whether the hidden states' gradient needs slopes of its own: with one scale for all rows, those whose upstream gradient is 2^-16 of the largest would keep four bits of a probability
+// of 2^-17 in FP16, and nothing of one of 2^-22. (Both slopes come out of one product: 2000 x 2048 x 50257 1.23 -> 1.26 ms, 4096 x 1024 x 32000 0.84 -> 0.92.)
+bool rowsHaveScales(const FtcudaLinearCrossEntropy& q, Form form) {
+    return form == Form::kGradients && q.element == FTCUDA_ELEMENT_FP16 && q.reduction == FTCUDA_REDUCTION_NONE;
+}
+
 // What a logit takes of the workspace while it is there, in bytes: its slope, and in the step call its exponential as well where that cannot
 // be in the same place.
 std::uint64_t logitBytes(const FtcudaLinearCrossEntropy& q, Form form) {
-    if (!isFp32(q)) { return 2; }
+    if (!isFp32(q)) { return rowsHaveScales(q, form) ? 4 : 2; }
     return libraryPays(q, form) ? 4 : isStep(form) ? 2 * loss::kPlanes + 4 : 2 * loss::kPlanes;
 }
 
@@ -739,6 +753,11 @@ int layOut(const FtcudaLinearCrossEntropy& q, Form form, std::uint64_t kept_byte
     if (l.planes && isStep(form) && statistics) { l.exponentials = own.take(4 * l.capacity * l.piece_pitch); }
     if (gradients) {
         l.sums = own.take(4 * l.capacity * l.sums_pitch * l.splits);
+        if (rowsHaveScales(q, form)) {
+            l.own_scale = own.take(4 * l.capacity);
+            l.own_unit  = own.take(4 * l.capacity);
+            l.own_piece = own.take(element * l.capacity * l.piece_pitch);
+        }
         if (l.weight_splits > 1) { l.weight_sums = own.take(4 * static_cast<std::uint64_t>(l.weight_rows) * l.sums_pitch * l.weight_splits); }
     }
     if (l.library && q.tokens != 0) {
@@ -820,6 +839,11 @@ class Call final {
         rows_.scale  = own<float>(l_.scale);
         rows_.lse2   = own<float>(l_.lse2);
         rows_.picked = own<float>(l_.picked);
+        own_scales_  = rowsHaveScales(q_, form);
+        if (own_scales_) {
+            rows_.own_scale = own<float>(l_.own_scale);
+            rows_.own_unit  = own<float>(l_.own_unit);
+        }
         products_    = loss::ProductCall{l_.planes || q_.element == FTCUDA_ELEMENT_BF16, l_.planes, static_cast<std::uint32_t>(l_.capacity), static_cast<std::uint32_t>(q_.depth), rows_,
                                       {memory_.kept + l_.hidden, l_.copy_pitch, l_.capacity * l_.copy_pitch}, status, sms_, stream_, message_, capacity_, false};
         if (message_ != nullptr && capacity_ != 0) { message_[0] = '\0'; }
@@ -906,7 +930,7 @@ class Call final {
         if (error == cudaSuccess) { error = gather(); }
         for (std::uint64_t first = 0; first < q_.vocabulary && error == cudaSuccess; first += l_.columns) {
             const std::uint64_t columns = std::min(l_.columns, q_.vocabulary - first);
-            error                       = slopes(first, columns);
+            error                       = slopes(first, columns, grad_hidden != nullptr, grad_weight != nullptr);
             if (error == cudaSuccess) { error = multiplySlopes(first, columns, grad_hidden != nullptr, grad_weight, weight_stride, q_.element, nullptr); }
         }
         return error == cudaSuccess && grad_hidden != nullptr ? spreadTyped(hiddenParts(hidden_stride, nullptr), grad_hidden, q_.element) : error;
@@ -1024,9 +1048,12 @@ class Call final {
     }
 
     // dZ of a piece of the vocabulary, to the workspace.
-    cudaError_t slopes(std::uint64_t first, std::uint64_t columns) const {
+    cudaError_t slopes(std::uint64_t first, std::uint64_t columns, bool for_hidden, bool for_weight) const {
         const std::uint32_t first32 = static_cast<std::uint32_t>(first), columns32 = static_cast<std::uint32_t>(columns);
-        if (!l_.library) { return loss::launchSlopes(products_, weight(first), first32, columns32, memory_.kept + l_.piece, l_.piece_pitch, slopesPlane()); }
+        if (!l_.library) {
+            return loss::launchSlopes(products_, weight(first), first32, columns32, own_scales_ && !for_weight ? nullptr : memory_.kept + l_.piece,
+                                      own_scales_ && for_hidden ? memory_.own + l_.own_piece : nullptr, l_.piece_pitch, slopesPlane());
+        }
         const cudaError_t error = multiply(describeLogits(q_, l_, memory_, first, columns), false);
         if (error != cudaSuccess) { return error; }
         return training::launchOverlapped(rowSlopes, dim3(static_cast<unsigned>(q_.tokens)), dim3(kRowThreads), 0, stream_, rowParams(first, columns, nullptr));
@@ -1039,6 +1066,7 @@ class Call final {
             loss::Gradients gradients{};
             gradients.sums                  = hidden ? own<float>(l_.sums) : nullptr;
             gradients.sums_pitch            = l_.sums_pitch;
+            gradients.own_slopes            = own_scales_ ? memory_.own + l_.own_piece : nullptr;
             gradients.splits                = l_.splits;
             gradients.accumulate            = first != 0;
             gradients.weight_gradient_fp32  = grad_element == FTCUDA_ELEMENT_FP32;
@@ -1101,6 +1129,7 @@ class Call final {
     Memory memory_{};
     cudaStream_t stream_ = nullptr;
     LiveRows rows_{};
+    bool own_scales_ = false;
     loss::ProductCall products_{};
 };
 

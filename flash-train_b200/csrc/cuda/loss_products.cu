@@ -8,7 +8,8 @@
 //
 // dZ is rounded to 16 bits because the tensor cores take it as an operand of the type that W and H have; half a step (2^-9, 2^-12
 // of each value) is what the gradients' own rounding comes to as well. Its scale brings the largest possible value near 1 (BF16) or 2^14 (FP16, whose
-// exponents would not hold the small probabilities otherwise).
+// exponents would not hold the small probabilities otherwise). With an upstream gradient for each token FP16's range holds only those near the largest at one
+// scale, which dW's sums over tokens need; dH's rows have a scale each, and a dZ of their own.
 //
 // One kernel does all four. A pair of CTAs (tcgen05 cta_group::2, a cluster of two) takes tiles of 256 rows and up to 256 columns, K in
 // blocks of 64; a CTA brings its 128 rows of A and its half of B, each as the matrix lies in memory: an operand whose
@@ -120,6 +121,7 @@ struct ProductParams {
     LiveRows rows;
     float2* partials;
     void* slopes;               // or what is kept
+    void* own_slopes;
     std::uint64_t slopes_pitch, slopes_plane;
     float* sums;
     float* weight_sums;         // NULL: the weight's gradient is written as it is
@@ -271,9 +273,9 @@ __device__ __forceinline__ void storePlanes(const ProductParams& p, std::uint32_
 }
 
 // This thread's row of a 16-bit matrix that has room for whole tiles; what lies beyond the columns is never fetched.
-__device__ __forceinline__ void storeRow(const ProductParams& p, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, float scale, bool on, bool bf16,
+__device__ __forceinline__ void storeRow(const ProductParams& p, void* to, std::uint32_t row, std::uint32_t col, std::uint32_t pieces, float scale, bool on, bool bf16,
                                          const float (&v)[128]) {
-    unsigned char* const out = static_cast<unsigned char*>(p.slopes) + (static_cast<std::uint64_t>(row) * p.slopes_pitch + col) * 2;
+    unsigned char* const out = static_cast<unsigned char*>(to) + (static_cast<std::uint64_t>(row) * p.slopes_pitch + col) * 2;
 #pragma unroll
     for (int j = 0; j < 128; j += 16) {
         if (j < 64 || pieces == 4) {
@@ -323,7 +325,7 @@ __device__ __forceinline__ void finishStatistics(const ProductParams& p, const I
     }
     const std::uint32_t piece = 2 * (w.col / p.problem[0].tile_n) + half;
     p.partials[static_cast<std::uint64_t>(piece) * p.capacity + row] = make_float2(none ? -INFINITY : base, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-    if (kKeep && p.terms == 1) { storeRow(p, row, col, pieces, kKeptScale, true, false, v); }
+    if (kKeep && p.terms == 1) { storeRow(p, p.slopes, row, col, pieces, kKeptScale, true, false, v); }
     if (kKeep && p.terms != 1) {
         float* const out = static_cast<float*>(p.slopes) + static_cast<std::uint64_t>(row) * p.slopes_pitch + col;
 #pragma unroll
@@ -352,7 +354,8 @@ __device__ __forceinline__ void finishSlopes(const ProductParams& p, std::uint32
         for (int j = 0; j < 128; ++j) { v[j] = j == at ? v[j] - 1.0F : v[j]; }
     }
     if (p.terms == 1) {
-        storeRow(p, row, col, pieces, scale, on, p.bf16 != 0, v);
+        if (p.slopes != nullptr) { storeRow(p, p.slopes, row, col, pieces, scale, on, p.bf16 != 0, v); }
+        if (p.own_slopes != nullptr) { storeRow(p, p.own_slopes, row, col, pieces, on ? p.rows.own_scale[row] : 0.0F, on, p.bf16 != 0, v); }
     } else {
         storePlanes(p, row, col, pieces, scale, on, v);
     }
@@ -753,12 +756,13 @@ cudaError_t launchKept(const ProductCall& call, Matrix16 weight, std::uint32_t v
     return launch<kKept>(call, maps, p, static_cast<std::uint64_t>(call.capacity / kTileRows) * p.problem[0].tiles_n);
 }
 
-cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, std::uint64_t slopes_pitch,
+cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, void* own_slopes, std::uint64_t slopes_pitch,
                          std::uint64_t slopes_plane) {
     ProductMaps maps;
     ProductParams p = paramsFor(call);
     p.first         = first;
     p.slopes        = slopes;
+    p.own_slopes    = own_slopes;
     p.slopes_pitch  = slopes_pitch;
     p.slopes_plane  = slopes_plane;
     if (!describeLogits(call, weight, columns, maps, p)) { return cudaErrorInvalidValue; }
@@ -826,7 +830,8 @@ cudaError_t launchGradients(const ProductCall& call, Matrix16 weight, std::uint3
         p.sums                    = gradients.sums;
         p.sums_pitch              = gradients.sums_pitch;
         p.accumulate              = gradients.accumulate ? 1 : 0;
-        encoded = encodeOperand(&maps.a[p.problems], call, slopes, false, call.capacity, columns, 128) &&
+        const Matrix16 own = gradients.own_slopes != nullptr ? Matrix16{gradients.own_slopes, slopes.pitch, slopes.plane} : slopes;
+        encoded = encodeOperand(&maps.a[p.problems], call, own, false, call.capacity, columns, 128) &&
                   encodeOperand(&maps.b[p.problems], call, weight, true, call.depth, columns, 64);
         items += static_cast<std::uint64_t>(call.capacity / kTileRows) * tiles_n * problem.splits;
         ++p.problems;

@@ -24,6 +24,8 @@ struct LiveRows {
     float* scale;           // upstream gradient of the row's loss over `unit`
     float* lse2;            // log2 of the row's sum of exponentials
     float* picked;          // the logit of the target
+    float* own_scale;       // FP16, an upstream gradient for each token: the row's scale for the hidden states' gradient, and ...
+    float* own_unit;        // ... what its sum is multiplied by in the end; NULL where `scale` and `unit` do for both gradients
 };
 constexpr std::int32_t kBadTarget = -2;
 
@@ -67,8 +69,8 @@ constexpr float kKeptScale = 8192.0F;
 cudaError_t launchKept(const ProductCall& call, Matrix16 weight, std::uint32_t vocabulary, float2* partials, void* kept, std::uint64_t kept_pitch);
 
 // slopes[row][column - first] = scale (2^(logit log2 e - lse2) - [column is the target]) for `columns` columns from `first` on;
-// `weight` starts at row `first`. The pitch is a multiple of 256.
-cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, std::uint64_t slopes_pitch,
+// `weight` starts at row `first`. The pitch is a multiple of 256. own_slopes: the same with rows.own_scale. Either may be NULL.
+cudaError_t launchSlopes(const ProductCall& call, Matrix16 weight, std::uint32_t first, std::uint32_t columns, void* slopes, void* own_slopes, std::uint64_t slopes_pitch,
                          std::uint64_t slopes_plane);
 
 // How many parts the sums are cut into: over `columns` columns for the gradient of the hidden states (over fewer columns
@@ -79,8 +81,9 @@ struct GradientSplits {
 GradientSplits gradientSplits(std::uint32_t tokens, std::uint32_t depth, std::uint32_t columns, bool planes, int sms);
 
 struct Gradients {
-    // hidden: sums[split][capacity][pitch] (+)= slopes times weight; NULL when not wanted.
+    // hidden: sums[split][capacity][pitch] (+)= slopes (own_slopes, where there are some) times weight; NULL when not wanted.
     float* sums;
+    const void* own_slopes;
     std::uint64_t sums_pitch;  // a multiple of 8
     std::uint32_t splits;
     bool accumulate;

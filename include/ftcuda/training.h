@@ -45,7 +45,8 @@ enum {
  *     NaN, and the gradients too.
  *   - infinities and NaN in what takes part reach the token's loss and the gradients as NaN (a logit of -inf is a probability of 0).
  *   - a gradient's rounding: with BF16 and FP16 operands the logits' gradients are rounded to that type before they are
- *     multiplied, at a scale that keeps FP16's range, and the products' sums once at the end. In the step call their exponentials are FP16 before that,
+ *     multiplied, at a scale that keeps FP16's range, and the products' sums once at the end. Without reduction that scale is each token's own for its row of the hidden states'
+ *     gradient; the weight's gradient, a sum over tokens, has one for all of them, at which a logit's gradient is off by up to 2^-38 of the largest upstream one in FP16. In the step call their exponentials are FP16 before that,
  *     against the largest of 64 or 128 neighbours.
  * Sums are in an order that depends on the sizes and on which tokens take part alone: equal calls give equal bits.
  */

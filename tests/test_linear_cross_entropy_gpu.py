@@ -797,3 +797,25 @@ def test_where_there_is_no_room_for_the_exponentials(ft, memory_given_back, dtyp
     for _ in range(70):
         got = run(ft, hidden, weight, target)
     assert all(torch.equal(a, b) for a, b in zip(got, expected))
+
+
+@pytest.mark.parametrize("tokens, depth, vocabulary", [(200, 96, 700), (300, 200, 5001)])
+def test_fp16_rows_of_small_upstream_gradients(ft, tokens, depth, vocabulary):
+    """A token's row of the hidden states' gradient is as exact beside upstream gradients that are 2^22 times larger as it is alone: against its own bound, which has
+    no part of any other token's."""
+    hidden, weight, target = make(tokens, depth, vocabulary, torch.float16, seed=95)
+    target[::9] = -100
+    oracle = Oracle(hidden, weight, target)
+    upstream = torch.randn(tokens, device="cuda").sign() * torch.exp2(14.0 - torch.arange(tokens, device="cuda") % 23)
+    upstream[3], upstream[4] = 0.0, 2.0 ** -30
+    _, grad_hidden, grad_weight = run(ft, hidden, weight, target, "none", upstream)
+    dh, dh_bound, dw, dw_bound = oracle.gradients(upstream, torch.float16, step=False)
+    # oracle's bound allows 2^-38 of the largest upstream gradient in every slope; of the token's own it is 2^-38 as well.
+    extra = ((upstream.abs().max() - upstream.abs()) * 2.0 ** -38).double()[:, None] * oracle.w.abs().sum(0)[None, :]
+    check(grad_hidden, dh, dh_bound - extra, "hidden's gradient")
+    check(grad_weight, dw, dw_bound, "weight's gradient")
+    assert not grad_hidden[3].any()
+    h, w = hidden.clone().requires_grad_(), weight.clone().requires_grad_()
+    loss = ft.linear_cross_entropy(h, w, target, reduction="none")
+    for alone, both in ((h, grad_hidden), (w, grad_weight)):
+        assert torch.equal(torch.autograd.grad(loss, alone, upstream, retain_graph=True)[0], both)
