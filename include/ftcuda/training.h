@@ -147,8 +147,8 @@ FTCUDA_API int ftcuda_linear_cross_entropy_step(const FtcudaLinearCrossEntropy* 
                                                 size_t message_capacity);
 
 /*
- * The step call in two: the loss first, and the gradients when the upstream gradient (*grad_loss, FP32 on the device) is known, of the operands' type and
- * rounded once. In between the workspace keeps what they are made of, for the same problem, and so does the weight; the hidden states and the targets are not looked at again.
+ * The step call in two: the loss first, and the gradients when the upstream gradient (*grad_loss, FP32 on the device) is known, of the operands' type: FP32
+ * sums times the upstream gradient, rounded to 16 bits once, behind that. In between the workspace keeps what they are made of, for the same problem, and so does the weight; the hidden states and the targets are not looked at again.
  * The second call may be made any number of times, with the workspace_bytes that ftcuda_linear_cross_entropy_step_workspace_bytes says, no more and no less.
  */
 FTCUDA_API int ftcuda_linear_cross_entropy_step_loss(const FtcudaLinearCrossEntropy* problem, float* loss, void* workspace, uint64_t workspace_bytes,

@@ -819,3 +819,39 @@ def test_fp16_rows_of_small_upstream_gradients(ft, tokens, depth, vocabulary):
     loss = ft.linear_cross_entropy(h, w, target, reduction="none")
     for alone, both in ((h, grad_hidden), (w, grad_weight)):
         assert torch.equal(torch.autograd.grad(loss, alone, upstream, retain_graph=True)[0], both)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("factor", [2.0 ** -3, 0.3, 1e-20, 700.0])
+def test_an_upstream_gradient_is_multiplied_in_before_the_rounding(ft, dtype, factor):
+    """One rounding to the results' type, whatever the factor. (FP32 as three BF16 matrices: the factor and the sum, a step each, are in the bound for sums.)"""
+    hidden, weight, target = make(200, 96, 700, dtype, seed=20)
+    _, grad_hidden, grad_weight = run(ft, hidden, weight, target, upstream=torch.tensor(factor, device="cuda"))
+    oracle = Oracle(hidden, weight, target)
+    dh, dh_bound, dw, dw_bound = oracle.gradients(torch.full((200,), factor / 200, device="cuda", dtype=torch.float64), dtype)
+    check(grad_hidden, dh, dh_bound, "hidden's gradient")
+    check(grad_weight, dw, dw_bound, "weight's gradient")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens, depth, vocabulary", [(1, 64, 128), (300, 96, 1500), (70, 1025, 300), (1537, 200, 4001), (3000, 72, 300), (2000, 257, 129)])
+def test_fp32_gradients_of_16_bit_operands(ft, capi, tokens, depth, vocabulary, dtype):
+    """The step in one with gradients in FP32: an odd depth, sums in parts over the tokens, rows apart; nothing is rounded to 16 bits."""
+    hidden, weight, target = make(tokens, depth, vocabulary, dtype, seed=96)
+    target[2::5] = -100
+    q = capi.LinearCrossEntropy(hidden=hidden.data_ptr(), weight=weight.data_ptr(), target=target.data_ptr(), tokens=tokens, vocabulary=vocabulary, depth=depth,
+                                hidden_row_stride=depth, weight_row_stride=depth, ignore_index=-100, element=7 if dtype == torch.float16 else 8, reduction=2, device=0)
+    size = capi.linear_cross_entropy_step_workspace_bytes(q)
+    workspace = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    loss = torch.empty((), device="cuda")
+    grad_hidden, grad_weight = (torch.full((rows, depth + 3), 7.0, device="cuda") for rows in (tokens, vocabulary))
+    capi.linear_cross_entropy_step(q, loss.data_ptr(), capi.ELEMENT_FP32, grad_hidden.data_ptr(), depth + 3, grad_weight.data_ptr(), depth + 3, workspace.data_ptr(), size,
+                                   torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    oracle = Oracle(hidden, weight, target)
+    dh, dh_bound, dw, dw_bound = oracle.gradients(torch.ones(tokens, device="cuda", dtype=torch.float64), dtype)
+    # The bounds but for the results' rounding to 16 bits, in whose place comes FP32's; (the smallest FP16 number is in them, and matters to none of these).
+    half_step = torch.finfo(dtype).eps / 2
+    check(grad_hidden[:, :depth], dh, dh_bound - (1.01 * half_step - STEP) * dh.abs(), "hidden's gradient")
+    check(grad_weight[:, :depth], dw, dw_bound - (1.01 * half_step - STEP) * dw.abs(), "weight's gradient")
+    assert (grad_hidden[:, depth:] == 7).all() and (grad_weight[:, depth:] == 7).all()
