@@ -560,6 +560,17 @@ const char* check(const FtcudaRouting& r) {
     return nullptr;
 }
 
+// Whether the gradient is written where the backward call reads: but over the logits themselves, which a warp reads before it writes them.
+bool overInputs(const FtcudaRouting& r, const float* weights, const std::int32_t* chosen, const std::int32_t* counts, const std::int32_t* routed, const float* grad_weights,
+                const float* grad_loss, const void* out, std::int64_t out_stride) {
+    const std::uint64_t bytes   = training::elementBytes(r.element), slots = r.tokens * r.top_k;
+    const training::Range range = training::rangeOf(out, r.tokens, r.experts, out_stride, bytes);
+    const auto met = [&](const void* at, std::uint64_t words) { return at != nullptr && training::meet(range, training::rangeOf(at, 1, words, 0, 4)); };
+    if (met(weights, slots) || met(chosen, slots) || met(counts, r.experts) || met(routed, 1) || met(grad_weights, slots) || met(grad_loss, 1)) { return true; }
+    const bool same = out == r.logits && (r.tokens == 1 || out_stride == r.row_stride);
+    return !same && training::meet(range, training::rangeOf(r.logits, r.tokens, r.experts, r.row_stride, bytes));
+}
+
 bool wordAligned(const void* pointer) { return pointer != nullptr && training::aligned(pointer, 4); }
 
 // CTAs of the forward kernel: a warp's worth of tokens at least, the SMs filled at most. 32 tokens and fewer stay in one.
@@ -670,6 +681,9 @@ extern "C" int ftcuda_expert_routing_backward(const FtcudaRouting* routing, cons
     }
     if (r.tokens > 1 && (grad_row_stride < static_cast<std::int64_t>(r.experts) || grad_row_stride >= (1LL << 31))) {
         return fail(message, message_capacity, 1, "the gradient's rows overlap, or lie too far apart");
+    }
+    if (overInputs(r, weights, experts, counts, routed, grad_weights, grad_loss, grad_logits, grad_row_stride)) {
+        return fail(message, message_capacity, 1, "the gradient lies across something that the call reads");
     }
     int sms = 0;
     if (!training::deviceIsCurrent(r.device, message, message_capacity) || !deviceSmCount(r.device, &sms, message, message_capacity)) { return 1; }

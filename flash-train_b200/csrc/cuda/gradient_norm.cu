@@ -29,6 +29,9 @@ namespace ftcuda {
 namespace {
 
 using training::Element;
+using training::Range;
+using training::rangeOf;
+using training::sideBySide;
 
 constexpr int kThreads            = 256;
 constexpr int kSumCtasPerSm       = 4;
@@ -454,29 +457,8 @@ const char* checkGradient(const FtcudaGradient& g, bool clip) {
     return nullptr;
 }
 
-// Memory of one operand: `rows` windows of `width` bytes, `stride` bytes apart.
-struct Range {
-    std::uint64_t begin, end, width, stride;
-};
-
-Range rangeOf(const void* address, std::uint64_t rows, std::uint64_t cols, std::int64_t row_stride, std::uint64_t bytes) {
-    Range r;
-    r.begin  = reinterpret_cast<std::uintptr_t>(address);
-    r.width  = cols * bytes;
-    r.stride = rows > 1 ? static_cast<std::uint64_t>(row_stride) * bytes : 0;
-    r.end    = r.begin + (rows - 1) * r.stride + r.width;
-    return r;
-}
 Range inputOf(const FtcudaGradient& g) { return rangeOf(g.data, g.rows, g.cols, g.row_stride, training::elementBytes(g.element)); }
 Range outputOf(const FtcudaGradient& g) { return rangeOf(g.out, g.rows, g.cols, g.out_row_stride, training::elementBytes(g.out_element)); }
-
-// Whether two ranges whose hulls meet, the second beginning no earlier, share no byte as far as their strides show: windows of one matrix, side by side.
-bool sideBySide(const Range& a, const Range& b) {
-    const std::uint64_t stride = a.stride != 0 ? a.stride : b.stride;
-    if (stride == 0 || (a.stride != 0 && b.stride != 0 && a.stride != b.stride) || a.width > stride || b.width > stride) { return false; }
-    const std::uint64_t offset = (b.begin - a.begin) % stride;
-    return offset >= a.width && offset + b.width <= stride;
-}
 
 // An operand by where it begins, and which: gradient 2 i is read, 2 i + 1 written.
 struct Operand {

@@ -53,6 +53,33 @@ inline std::uint64_t elementBytes(std::int32_t element) {
 
 inline bool aligned(const void* pointer, std::uint64_t bytes) { return reinterpret_cast<std::uintptr_t>(pointer) % bytes == 0; }
 
+// Memory of one operand: `rows` windows of `width` bytes, `stride` bytes apart.
+struct Range {
+    std::uint64_t begin, end, width, stride;
+};
+
+inline Range rangeOf(const void* address, std::uint64_t rows, std::uint64_t cols, std::int64_t row_stride, std::uint64_t bytes) {
+    Range r;
+    r.begin  = reinterpret_cast<std::uintptr_t>(address);
+    r.width  = cols * bytes;
+    r.stride = rows > 1 ? static_cast<std::uint64_t>(row_stride) * bytes : 0;
+    r.end    = r.begin + (rows - 1) * r.stride + r.width;
+    return r;
+}
+
+// Whether two ranges whose hulls meet, the second beginning no earlier, share no byte as far as their strides show: windows of one matrix, side by side.
+inline bool sideBySide(const Range& a, const Range& b) {
+    const std::uint64_t stride = a.stride != 0 ? a.stride : b.stride;
+    if (stride == 0 || (a.stride != 0 && b.stride != 0 && a.stride != b.stride) || a.width > stride || b.width > stride) { return false; }
+    const std::uint64_t offset = (b.begin - a.begin) % stride;
+    return offset >= a.width && offset + b.width <= stride;
+}
+
+// Whether they may share one, whichever begins earlier.
+inline bool meet(const Range& a, const Range& b) {
+    return a.begin < b.end && b.begin < a.end && !(a.begin <= b.begin ? sideBySide(a, b) : sideBySide(b, a));
+}
+
 // The device exists and is the calling thread's current one.
 inline bool deviceIsCurrent(std::int32_t device, char* message, std::size_t capacity) {
     int current             = -1;

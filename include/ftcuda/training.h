@@ -213,7 +213,7 @@ FTCUDA_API int ftcuda_expert_routing(const FtcudaRouting* routing, float* weight
 /*
  * grad_logits (of the logits' type, grad_row_stride elements between tokens) from grad_weights (FP32 [tokens][top_k], dense) and *grad_loss (one FP32 on the
  * device), either of which may be NULL, meaning zero; the other arguments as the forward call took and left them (an expert's number beyond the last one
- * is taken for the last one). grad_logits may be the logits themselves, with their stride; otherwise it may not meet what the call reads. Needs no workspace.
+ * is taken for the last one). grad_logits may be the logits themselves, with their stride; otherwise it may not meet what the call reads (refused). Needs no workspace.
  */
 FTCUDA_API int ftcuda_expert_routing_backward(const FtcudaRouting* routing, const float* weights, const int32_t* experts, const int32_t* counts,
                                               const int32_t* routed, const float* grad_weights, const float* grad_loss,

@@ -47,3 +47,28 @@ def test_addresses_that_cannot_be(capi):
 def test_the_workspace_is_bounded(capi):
     assert capi.expert_routing_workspace_bytes(routing(capi, tokens=0)) > 0
     assert capi.expert_routing_workspace_bytes(routing(capi, tokens=(1 << 31) - 1, experts=1024, row_stride=1024)) <= 5 << 20
+
+
+def test_a_gradient_across_what_is_read(capi):
+    r, wide = routing(capi, element=8), routing(capi, row_stride=192)
+    across = [(r, OUTPUTS[:4], 0, 0, 0x10000000 + 2, 64), (r, OUTPUTS[:4], 0, 0, 0x10000000 - 12798, 64), (r, OUTPUTS[:4], 0, 0, 0x10000000, 65),
+              (r, OUTPUTS[:4], 0, 0, 0x10000000 + 128 * 99 + 126, 64), (wide, OUTPUTS[:4], 0, 0, 0x10000000 + 4 * 63, 192), (wide, OUTPUTS[:4], 0, 0, 0x10000000 + 4 * 129, 192),
+              (wide, OUTPUTS[:4], 0, 0, 0x10000000 + 4 * 64, 191)]
+    for i in range(4):  # the last byte of an input, and one in the gradient's middle
+        across += [(r, OUTPUTS[:4], 0, 0, OUTPUTS[i] + (3200, 3200, 256, 4)[i] - 2, 64), (r, OUTPUTS[:4], 0, 0, OUTPUTS[i] - 6400, 64)]
+    across += [(r, OUTPUTS[:4], 0x6000000, 0, 0x6000000 + 3198, 64), (r, OUTPUTS[:4], 0, 0x6000000, 0x6000000 - 12798, 64)]
+    for problem, inputs, grad_weights, grad_loss, out, stride in across:
+        refuse(capi, "lies across", capi.expert_routing_backward, problem, *inputs, grad_weights, grad_loss, out, stride)
+
+
+def test_a_gradient_over_or_beside_the_logits_reaches_the_device_check(capi):
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("would launch on made-up addresses")
+    r, wide = routing(capi, element=8), routing(capi, row_stride=192)
+    for problem, out, stride in ((r, 0x10000000, 64), (r, 0x10000000 + 12800, 64), (r, 0x10000000 - 12800, 64), (wide, 0x10000000, 192), (wide, 0x10000000 + 4 * 64, 192),
+                                 (wide, 0x10000000 + 4 * 128, 192), (wide, 0x10000000 - 4 * 64, 192), (routing(capi, tokens=1), 0x10000000, 7)):
+        with pytest.raises(capi.FTrainError) as info:
+            capi.expert_routing_backward(problem, *OUTPUTS[:4], 0, 0, out, stride)
+        assert "across" not in info.value.message
