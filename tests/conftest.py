@@ -1,4 +1,5 @@
 """Shared test plumbing: import paths, the `gpu` marker, and in-tree builds."""
+import gc
 import importlib.util
 import sys
 from pathlib import Path
@@ -21,6 +22,17 @@ def load_build_module():
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
     return module
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device_memory_between_modules():
+    """What a module's tests leave in torch's cache goes back to the device: a tensor of the next module that lands in a large cached block would keep the rest of it, and
+    tests that leave the allocator little room count on there being none."""
+    yield
+    torch = sys.modules.get("torch")
+    if torch is not None and torch.cuda.is_initialized():
+        gc.collect()
+        torch.cuda.empty_cache()
 
 
 @pytest.fixture(scope="session")
