@@ -11,9 +11,9 @@
 // warp's tokens, a CTA joins its warps and leaves one row of partial sums, and a cluster of eight CTAs adds the rows up; the counts are whole
 // numbers in shared memory. One CTA alone (few tokens) finishes by itself, without the second launch.
 //
-// What bounds it: with few experts latency and HBM (16384 x 64 FP32, top 8: 21.5 us forward, 12.3 backward, 1.5 us of bytes), with many the forward kernel's
-// whole-number instructions (65535 x 256 BF16, top 8: 52 us forward at 0.69 TB/s, the ALU pipe busy for 70 % of the time), the backward one's latency
-// (32.8 us, 2.2 TB/s).
+// What bounds it: with few experts latency (16384 x 64 FP32, top 8, as captured graphs: 20.8 us forward, 26.7 with the backward pass, where a kernel that does next to nothing takes 6.2;
+// 1.5 us of bytes), with many the forward kernel's chains of dependent whole-number instructions (65535 x 256 BF16, top 8: 45 to 52 us forward at 0.7 TB/s, 66 % of the issue slots used and
+// the ALU pipe busy for 62 % of the time), the backward one's latency (31 to 33 us, 2.2 TB/s).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 

@@ -8,6 +8,7 @@
 // the passes over dH (one for each piece) and the launches weigh little. The step call does both without
 // computing Z twice, 6 T V D in all, where kStepBytes have room for all of Z's exponentials, 16 bits each (FP32: for Z):
 // a pass over them, two bytes read and two written for each, makes them dZ for an upstream gradient of 1, and what comes from it is multiplied by the one there is.
+// dZ waits for that in a memory of its own, with the gathered hidden states and, where the limit has room for it, the weight's copy or planes.
 //
 // Tokens without a target are left out first: the others' hidden states are gathered into the workspace, which costs one pass over H,
 // makes what the padding holds irrelevant (a NaN there would reach dW through 0 * NaN), spares the products those rows, and gives

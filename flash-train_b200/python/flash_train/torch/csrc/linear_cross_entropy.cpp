@@ -180,7 +180,9 @@ at::Tensor linearCrossEntropy(const at::Tensor& hidden, const at::Tensor& weight
 
 void registerLinearCrossEntropy(pybind11::module_& module) {
     module.def("linear_cross_entropy", &linearCrossEntropy,
-               "Cross entropy of the logits hidden @ weight.T, which are never all in memory, against `target`; an FP32 tensor.\n\n"
+               "Cross entropy of the logits hidden @ weight.T against `target`; an FP32 tensor.\n\n"
+               "The logits are not kept. With a reduction and gradients wanted, their gradients wait for the backward pass where they take at most 2 GiB;\n"
+               "otherwise, or where there is no room for them, the backward pass computes the logits again, a piece of the vocabulary at a time.\n"
                "hidden (..., depth) and weight (vocabulary, depth): FP32, FP16 or BF16, one type; target (...): INT64. Tokens whose target is\n"
                "ignore_index take no part, whatever their hidden state holds; any other target outside of the vocabulary gives NaN.\n"
                "reduction: 'mean' over the tokens that have a target (0 where none has), 'sum', or 'none' for a loss of target's shape.\n"

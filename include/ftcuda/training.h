@@ -35,8 +35,9 @@ enum {
 
 /*
  * logits[t][v] = hidden[t] . weight[v],  loss[t] = log(sum_v exp(logits[t][v])) - logits[t][target[t]].
- * The logits are never all in memory: a piece of the vocabulary's gradients of them at a time is in the backward call (and a piece of FP32 logits in the forward
- * call where FP32 operands go through the library's products), or, in a step call, their exponentials, at most 2 GiB of them.
+ * The two calls below never have all logits in memory: a piece of the vocabulary's gradients of them at a time is in the backward call, and a piece of FP32 logits in the forward
+ * call where FP32 operands go through the library's products. A step call has a number for each logit: its exponential, then its gradient (FP32 operands that go through the library's
+ * products: the logit, then its gradient), which are kept from the loss to the gradients; at most 2 GiB.
  *   - hidden [tokens][depth], weight [vocabulary][depth]: unit stride along the depth, the others any that keep rows apart; both
  *     of one type. BF16 and FP16 are multiplied by the tensor cores with FP32 sums; FP32 to FP32's precision, as sums of three BF16 matrices (which
  *     the workspace then holds, six bytes an element of the weight) or by the library's FP32 products, whichever is faster for the sizes.
@@ -117,7 +118,8 @@ FTCUDA_API int ftcuda_gradient_norm(const FtcudaGradient* gradients, uint64_t co
 /*
  * The norm as above, and out = data * min(1, max_norm / (norm + 1e-6)), the factor rounded to FP32 once and the product rounded
  * once to the output's type. Where that factor is 1, gradients that are their own `out` are left alone, without being
- * written. A norm that is not a number makes every element NaN; an infinite one makes the finite elements 0 and the others NaN. max_norm >= 0.
+ * written. A norm that is not a number makes every element NaN; an infinite one makes the finite elements 0 and the others NaN (all of them NaN where
+ * max_norm is infinite too). max_norm >= 0.
  * No element may be written that another gradient reads or writes (refused where addresses, sizes and strides
  * show it).
  */
