@@ -855,3 +855,28 @@ def test_fp32_gradients_of_16_bit_operands(ft, capi, tokens, depth, vocabulary, 
     check(grad_hidden[:, :depth], dh, dh_bound - (1.01 * half_step - STEP) * dh.abs(), "hidden's gradient")
     check(grad_weight[:, :depth], dw, dw_bound - (1.01 * half_step - STEP) * dw.abs(), "weight's gradient")
     assert (grad_hidden[:, depth:] == 7).all() and (grad_weight[:, depth:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens, depth, vocabulary", [(5, 131, 90), (70, 1025, 300), (300, 127, 1501)])
+def test_the_step_in_two_over_a_weight_that_is_copied(ft, capi, tokens, depth, vocabulary, dtype):
+    """One workspace, a weight at an odd address with rows at an odd distance, gradients twice: as torch's graph makes them."""
+    hidden, weight, target = make(tokens, depth, vocabulary, dtype, seed=100)
+    target[2::5] = -100
+    buffer = torch.full((3 + vocabulary * (depth + 1),), math.nan, device="cuda", dtype=dtype)
+    view = buffer[3:].view(vocabulary, depth + 1)[:, :depth]
+    view.copy_(weight)
+    loss, expected_hidden, expected_weight = run(ft, hidden, view, target, upstream=torch.tensor(37.5, device="cuda"))
+    q = capi.LinearCrossEntropy(hidden=hidden.data_ptr(), weight=view.data_ptr(), target=target.data_ptr(), tokens=tokens, vocabulary=vocabulary, depth=depth,
+                                hidden_row_stride=depth, weight_row_stride=depth + 1, ignore_index=-100, element={torch.float32: 4, torch.float16: 7, torch.bfloat16: 8}[dtype],
+                                reduction=1, device=0)
+    stream = torch.cuda.current_stream().cuda_stream
+    size = capi.linear_cross_entropy_step_workspace_bytes(q)
+    workspace = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    numbers = torch.tensor([math.nan, 37.5], device="cuda")
+    capi.linear_cross_entropy_step_loss(q, numbers.data_ptr(), workspace.data_ptr(), size, stream)
+    for _ in range(2):
+        grad_hidden, grad_weight = torch.full_like(hidden, math.nan), torch.full_like(weight, math.nan)
+        capi.linear_cross_entropy_step_gradients(q, numbers.data_ptr() + 4, grad_hidden.data_ptr(), depth, grad_weight.data_ptr(), depth, workspace.data_ptr(), size, stream)
+        torch.cuda.synchronize()
+        assert torch.equal(numbers[0], loss) and torch.equal(grad_hidden, expected_hidden) and torch.equal(grad_weight, expected_weight)
