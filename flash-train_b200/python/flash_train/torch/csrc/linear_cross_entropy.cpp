@@ -139,7 +139,8 @@ RefusedWorkspace& refusedStep(std::size_t device) {
     return ofDevice(refused, device);
 }
 
-at::Tensor linearCrossEntropy(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, std::int64_t ignore_index, const std::string& reduction) {
+at::Tensor linearCrossEntropy(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, std::int64_t ignore_index, const std::string& reduction,
+                              bool recompute) {
     for (const at::Tensor* operand : {&hidden, &weight}) {
         TORCH_CHECK(operand->is_cuda() && operand->layout() == at::kStrided && !operand->is_neg(), "hidden and weight must be dense device tensors");
         TORCH_CHECK(elementOf(*operand) != 0, "hidden and weight must be FP32, FP16 or BF16");
@@ -157,7 +158,7 @@ at::Tensor linearCrossEntropy(const at::Tensor& hidden, const at::Tensor& weight
     const at::Tensor flat = hidden.dim() == 2 ? hidden : hidden.reshape({hidden.numel() / depth, depth});
     TORCH_CHECK((flat.stride(1) == 1 && weight.stride(1) == 1) || depth == 1, "hidden and weight must be contiguous along their last dimension");
     const at::Tensor indices = target.reshape({-1}).contiguous();
-    if (at::GradMode::is_enabled() && (flat.requires_grad() || weight.requires_grad())) {
+    if (!recompute && at::GradMode::is_enabled() && (flat.requires_grad() || weight.requires_grad())) {
         const FtcudaLinearCrossEntropy q = describe(flat, weight, indices, ignore_index, kind);
         std::uint64_t kept = 0, bytes = 0;
         if (ftcuda_linear_cross_entropy_step_loss_bytes(&q, &kept, &bytes, nullptr, 0) == 0) {
@@ -182,13 +183,14 @@ void registerLinearCrossEntropy(pybind11::module_& module) {
     module.def("linear_cross_entropy", &linearCrossEntropy,
                "Cross entropy of the logits hidden @ weight.T against `target`; an FP32 tensor.\n\n"
                "The logits are not kept. With a reduction and gradients wanted, their gradients wait for the backward pass where they take at most 2 GiB;\n"
-               "otherwise, or where there is no room for them, the backward pass computes the logits again, a piece of the vocabulary at a time.\n"
+               "otherwise, with recompute=True, or where there is no room for them, the backward pass computes the logits again, a piece of the vocabulary\n"
+               "at a time, for a third more operations.\n"
                "hidden (..., depth) and weight (vocabulary, depth): FP32, FP16 or BF16, one type; target (...): INT64. Tokens whose target is\n"
                "ignore_index take no part, whatever their hidden state holds; any other target outside of the vocabulary gives NaN.\n"
                "reduction: 'mean' over the tokens that have a target (0 where none has), 'sum', or 'none' for a loss of target's shape.\n"
                "Differentiable once in hidden and weight; the gradients have their types.",
                pybind11::arg("hidden"), pybind11::arg("weight"), pybind11::arg("target"), pybind11::kw_only(), pybind11::arg("ignore_index") = -100,
-               pybind11::arg("reduction") = "mean");
+               pybind11::arg("reduction") = "mean", pybind11::arg("recompute") = false);
 }
 
 }  // namespace flash_train_torch

@@ -880,3 +880,21 @@ def test_the_step_in_two_over_a_weight_that_is_copied(ft, capi, tokens, depth, v
         capi.linear_cross_entropy_step_gradients(q, numbers.data_ptr() + 4, grad_hidden.data_ptr(), depth, grad_weight.data_ptr(), depth, workspace.data_ptr(), size, stream)
         torch.cuda.synchronize()
         assert torch.equal(numbers[0], loss) and torch.equal(grad_hidden, expected_hidden) and torch.equal(grad_weight, expected_weight)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_logits_computed_again_on_demand(ft, memory_given_back, dtype):
+    """recompute=True keeps one number a token, and gives the gradients that a definition of its own bounds."""
+    hidden, weight, target = make(1000, 128, 9001, dtype, seed=101)
+    target[::6] = -100
+    h, w = hidden.clone().requires_grad_(), weight.clone().requires_grad_()
+    before = torch.cuda.memory_allocated()
+    loss = ft.linear_cross_entropy(h, w, target, reduction="sum", recompute=True)
+    assert torch.cuda.memory_allocated() - before <= 4 * 1000 + 4096
+    grad_hidden, grad_weight = torch.autograd.grad(loss, (h, w), torch.tensor(3.0, device="cuda"))
+    oracle = Oracle(hidden, weight, target)
+    dh, dh_bound, dw, dw_bound = oracle.gradients(torch.full((1000,), 3.0, device="cuda", dtype=torch.float64), dtype, step=False)
+    check(loss.detach(), oracle.loss.sum(), oracle.loss_error.sum() + 2 * STEP * oracle.loss.sum(), "loss")
+    check(grad_hidden, dh, dh_bound, "hidden's gradient")
+    check(grad_weight, dw, dw_bound, "weight's gradient")
+    assert torch.equal(ft.linear_cross_entropy(hidden, weight, target, recompute=True), ft.linear_cross_entropy(hidden, weight, target))
