@@ -770,7 +770,7 @@ def test_a_large_copy_of_the_weight_does_not_wait_in_the_graph(ft, capi, memory_
     assert (grad_hidden - hidden2).float().norm() <= tolerance * hidden2.float().norm() and (grad_weight - weight2).float().norm() <= tolerance * weight2.float().norm()
 
 
-@pytest.mark.parametrize("dtype, tokens, vocabulary", [(torch.bfloat16, 8192, 131072), (torch.float32, 3072, 65536)])
+@pytest.mark.parametrize("dtype, tokens, vocabulary", [(torch.bfloat16, 8192, 131072), (torch.float32, 3000, 65536)])
 def test_where_there_is_no_room_for_the_exponentials(ft, memory_given_back, dtype, tokens, vocabulary):
     """With less memory left than the step wants, the gradients come from the form that goes through the vocabulary piece by piece."""
     hidden, weight, target = make(tokens, 64, vocabulary, dtype, seed=97)
